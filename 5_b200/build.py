@@ -37,6 +37,7 @@ SOURCES = [
     LIB_DIR / "Kernels" / "map_elementwise_sm100a.cu",
     LIB_DIR / "Kernels" / "pairwise_distance_sm100a.cu",
     LIB_DIR / "Kernels" / "row_reduce_sm100a.cu",
+    LIB_DIR / "Kernels" / "layer_norm_sm100a.cu",
     LIB_DIR / "Kernels" / "gemm_skinny_static_sm100a.cu",
     LIB_DIR / "Kernels" / "selftest_sm100a.cu",
     LIB_DIR / "CAPI" / "Cuda.cpp",

@@ -39,7 +39,7 @@ F16, BF16, F8E4M3, F8E5M2 = 0, 1, 2, 3  # HcCudaDType
 VARIANT_AUTO, VARIANT_DENSE, VARIANT_SKINNY, VARIANT_NOOP, VARIANT_ZERO_FILL, VARIANT_ELEMENTWISE = 0, 1, 2, 3, 4, 5
 VARIANT_TINY = 6  # float32 pipes, bit-identical to the reference simulator; AUTO picks it for m, n <= 64, k <= 128
 VARIANT_NAMES = {0: "auto", 1: "dense", 2: "skinny", 3: "noop", 4: "zero_fill", 5: "elementwise", 6: "tiny"}
-API_VERSION = 8
+API_VERSION = 9
 # Element-wise operations fused into the store of C: ("scale", x), ("add", x), ("max", x),
 # ("min", x) and ("bias",) -- the last adds bias[column].
 EPILOGUE_KINDS = {"scale": 1, "add": 2, "max": 3, "min": 4, "bias": 5}
@@ -58,6 +58,7 @@ EXPORTS = (
     "hcCudaCommInitRank", "hcCudaCommAllGather", "hcCudaCommDestroy", "hcCudaGemmSkinnyStatic", "hcCudaSelfTestDeviceTimeout", "hcCudaGemmPush", "hcCudaIpcExport",
     "hcCudaIpcOpen", "hcCudaIpcClose", "hcCudaMap", "hcCudaMapHost",
     "hcCudaGemmHostDeviceA", "hcCudaPairwise", "hcCudaPairwiseHost", "hcCudaRowSum", "hcCudaRowSumHost", "hcCudaBuildFlags", "hcCudaSelfTestDeviceCheck",
+    "hcCudaLayerNorm", "hcCudaLayerNormPlan", "hcCudaLayerNormBackward", "hcCudaLayerNormBackwardPlan",
 )
 
 
@@ -130,6 +131,28 @@ class _RowSumArgs(ctypes.Structure):
 
 
 ROW_SUM_SQUARE, ROW_SUM_SQRT = 1, 2
+
+
+class _LayerNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_int64), ("cols", ctypes.c_int64), ("dtype", ctypes.c_int32), ("param_dtype", ctypes.c_int32),
+        ("x", ctypes.c_void_p), ("ldx", ctypes.c_int64), ("weight", ctypes.c_void_p), ("bias", ctypes.c_void_p),
+        ("y", ctypes.c_void_p), ("ldy", ctypes.c_int64), ("mean", ctypes.c_void_p), ("rstd", ctypes.c_void_p),
+        ("eps", ctypes.c_float),
+    ]
+
+
+class _LayerNormBackwardArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_int64), ("cols", ctypes.c_int64), ("dtype", ctypes.c_int32), ("param_dtype", ctypes.c_int32),
+        ("dy", ctypes.c_void_p), ("lddy", ctypes.c_int64), ("x", ctypes.c_void_p), ("ldx", ctypes.c_int64),
+        ("weight", ctypes.c_void_p), ("mean", ctypes.c_void_p), ("rstd", ctypes.c_void_p), ("dx", ctypes.c_void_p),
+        ("lddx", ctypes.c_int64), ("dweight", ctypes.c_void_p), ("dbias", ctypes.c_void_p),
+    ]
+
+
+class _OperatorPlanInfo(ctypes.Structure):
+    _fields_ = [("kernel_launches", ctypes.c_int32), ("pieces", ctypes.c_int32), ("scratch_bytes", ctypes.c_int64)]
 
 
 class _DeviceInfo(ctypes.Structure):
@@ -213,6 +236,11 @@ def library() -> ctypes.CDLL:
         lib.hcCudaPairwiseHost.argtypes = [vp, ctypes.POINTER(_PairwiseArgs)]
         lib.hcCudaRowSum.argtypes = [vp, ctypes.POINTER(_RowSumArgs)]
         lib.hcCudaRowSumHost.argtypes = [vp, ctypes.POINTER(_RowSumArgs)]
+        lib.hcCudaLayerNorm.argtypes = [vp, ctypes.POINTER(_LayerNormArgs)]
+        lib.hcCudaLayerNormBackward.argtypes = [vp, ctypes.POINTER(_LayerNormBackwardArgs)]
+        plan_info = ctypes.POINTER(_OperatorPlanInfo)
+        lib.hcCudaLayerNormPlan.argtypes = [ctypes.POINTER(_LayerNormArgs), i, plan_info]
+        lib.hcCudaLayerNormBackwardPlan.argtypes = [ctypes.POINTER(_LayerNormBackwardArgs), i, plan_info]
         for name in EXPORTS:
             getattr(lib, name)  # AttributeError here means a stale or foreign library
         _LIB = lib
@@ -256,6 +284,25 @@ def c_dtype_code(dtype: Any) -> int:
     if name not in codes:
         raise ValueError(f"C must be float32, float16 or bfloat16, got {name}")
     return codes[name]
+
+
+def _numpy_dtype(dtype: Any) -> np.dtype:
+    """`np.dtype(dtype)`, also for the names of the ml_dtypes types ("bfloat16", "float8_e4m3fn", ...)."""
+    if isinstance(dtype, str) and dtype.startswith(("bfloat", "float8_")):
+        import ml_dtypes
+
+        return np.dtype(getattr(ml_dtypes, dtype))
+    return np.dtype(dtype)
+
+
+def _vector(name: str, buf: "DeviceBuffer | None", length: int, *dtypes: Any) -> int | None:
+    """The address of an optional vector argument of `length` elements of one of `dtypes`."""
+    if buf is None:
+        return None
+    if buf.shape != (length,) or buf.dtype not in dtypes:
+        raise ValueError(f"{name} must be a vector of {length} elements of {' or '.join(np.dtype(d).name for d in dtypes)}, "
+                         f"got {buf.shape} of {buf.dtype.name}")
+    return buf.ptr
 
 
 class GemmPlan:
@@ -548,6 +595,50 @@ class Context:
         args = _RowSumArgs(w, h, x.ctypes.data, pitch, out.ctypes.data, flags)
         self._check(self._lib.hcCudaRowSumHost(self._handle, ctypes.byref(args)))
 
+    def layer_norm(self, x: "DeviceBuffer", y: "DeviceBuffer", *, weight: "DeviceBuffer | None" = None,
+                   bias: "DeviceBuffer | None" = None, eps: float = 1e-5, mean: "DeviceBuffer | None" = None,
+                   rstd: "DeviceBuffer | None" = None) -> None:
+        """Enqueues y = (x - mean) * rstd * weight + bias with the mean and 1 / sqrt(variance + eps) of
+        each row (asynchronous; see `synchronize`). `x`, `y`: float32, float16 or bfloat16 device
+        matrices (rows, cols) of one type; `weight`, `bias`: vectors of `cols` values, float32 or of
+        that type (without them: 1 and 0). `mean`, `rstd`: float32 vectors of `rows` values that
+        receive the statistics `layer_norm_backward` needs. `y` may be `x` itself."""
+        rows, cols = self._norm_shape("layer_norm", x, y)
+        params = self._norm_params("layer_norm", x.dtype, weight, bias)
+        args = _LayerNormArgs(rows, cols, c_dtype_code(x.dtype), c_dtype_code(params), x.ptr, x.ld,
+                              _vector("weight", weight, cols, params), _vector("bias", bias, cols, params), y.ptr, y.ld,
+                              _vector("mean", mean, rows, np.float32), _vector("rstd", rstd, rows, np.float32), eps)
+        self._check(self._lib.hcCudaLayerNorm(self._handle, ctypes.byref(args)))
+
+    def layer_norm_backward(self, dy: "DeviceBuffer", x: "DeviceBuffer", dx: "DeviceBuffer", *, mean: "DeviceBuffer",
+                            rstd: "DeviceBuffer", weight: "DeviceBuffer | None" = None,
+                            dweight: "DeviceBuffer | None" = None, dbias: "DeviceBuffer | None" = None) -> None:
+        """Enqueues the gradients of `layer_norm` (asynchronous): `dx` from the gradient `dy` of its
+        output, its input `x` and the `mean` and `rstd` it stored, and, where given, `dweight` and `dbias`
+        (overwritten; the type of `weight`). `dx` may be `dy` or `x` itself."""
+        rows, cols = self._norm_shape("layer_norm_backward", x, dy, dx)
+        params = self._norm_params("layer_norm_backward", x.dtype, weight, dweight, dbias)
+        args = _LayerNormBackwardArgs(rows, cols, c_dtype_code(x.dtype), c_dtype_code(params), dy.ptr, dy.ld, x.ptr, x.ld,
+                                      _vector("weight", weight, cols, params), _vector("mean", mean, rows, np.float32),
+                                      _vector("rstd", rstd, rows, np.float32), dx.ptr, dx.ld,
+                                      _vector("dweight", dweight, cols, params), _vector("dbias", dbias, cols, params))
+        self._check(self._lib.hcCudaLayerNormBackward(self._handle, ctypes.byref(args)))
+
+    @staticmethod
+    def _norm_shape(call: str, x: "DeviceBuffer", *others: "DeviceBuffer") -> tuple[int, int]:
+        for buf in (x, *others):
+            if buf.ndim != 2 or buf.shape != x.shape or buf.dtype != x.dtype:
+                raise ValueError(f"{call}() takes device matrices of one shape and type")
+        return x.shape
+
+    @staticmethod
+    def _norm_params(call: str, dtype: np.dtype, *vectors: "DeviceBuffer | None") -> np.dtype:
+        """The type the weight and bias vectors share: float32, or that of the matrices."""
+        kinds = {v.dtype for v in vectors if v is not None}
+        if len(kinds) > 1:
+            raise ValueError(f"{call}() takes weight and bias vectors (and their gradients) of one type")
+        return kinds.pop() if kinds else np.dtype(np.float32)
+
     def gemm_host(self, a: np.ndarray, b: np.ndarray, c: np.ndarray, *,
                   variant: int = VARIANT_AUTO, b_transposed: bool = False, accumulate: bool = False,
                   epilogue: Sequence[tuple] = (), bias: np.ndarray | None = None) -> None:
@@ -659,7 +750,7 @@ class DeviceBuffer:
     def __init__(self, ctx: Context, shape: tuple[int, ...], dtype: Any, *, ld: int | None = None) -> None:
         self.ctx = ctx
         self.shape = tuple(int(s) for s in shape)
-        self.dtype = np.dtype(dtype)
+        self.dtype = _numpy_dtype(dtype)
         self.ndim = len(self.shape)
         cols = self.shape[-1] if self.shape else 1
         self.ld = int(cols if ld is None else ld)
@@ -678,7 +769,7 @@ class DeviceBuffer:
         self = cls.__new__(cls)
         self.ctx = ctx
         self.shape = tuple(int(s) for s in shape)
-        self.dtype = np.dtype(dtype)
+        self.dtype = _numpy_dtype(dtype)
         self.ndim = len(self.shape)
         cols = self.shape[-1] if self.shape else 1
         self.ld = int(cols if ld is None else ld)

@@ -1867,6 +1867,212 @@ int hcCudaRowSumHost(HcCudaContext *ctx, const HcCudaRowSumArgs *args) {
   return synchronize_locked(ctx);
 }
 
+namespace {
+
+size_t float_bytes(int c_type) { return c_type == HC_CUDA_C_F32 ? 4 : 2; }
+
+bool is_c_type(int t) { return t == HC_CUDA_C_F32 || t == HC_CUDA_C_F16 || t == HC_CUDA_C_BF16; }
+
+// A row-major matrix or vector argument as a named range of memory, for the checks below.
+struct Operand {
+  const char *name;
+  const void *ptr;
+  int64_t rows, cols, ld;
+  size_t elem;
+  size_t bytes() const { return (static_cast<size_t>(rows - 1) * static_cast<size_t>(ld) + static_cast<size_t>(cols)) * elem; }
+};
+
+// Non-null, aligned to its element, a pitch of at least its columns.
+int check_operand(const HcCudaContext *ctx, const Operand &o) {
+  if (o.ptr == nullptr)
+    return fail(ctx, HC_CUDA_ERR_INVALID_ARGUMENT, "%s must not be null", o.name);
+  if ((reinterpret_cast<uintptr_t>(o.ptr) & (o.elem - 1)) != 0)
+    return fail(ctx, HC_CUDA_ERR_INVALID_ARGUMENT, "%s must be %zu-byte aligned", o.name, o.elem);
+  if (o.ld < o.cols || o.ld > kMaxPitch)
+    return fail(ctx, HC_CUDA_ERR_INVALID_ARGUMENT, "the pitch of %s (%lld) must be at least its columns (%lld)", o.name,
+                (long long)o.ld, (long long)o.cols);
+  return HC_CUDA_OK;
+}
+
+// An output may not overlap `other`, except that with `same_ok` it may be the very same matrix.
+int check_apart(const HcCudaContext *ctx, const Operand &out, const Operand &other, bool same_ok = false) {
+  if (out.ptr == nullptr || other.ptr == nullptr || !ranges_overlap(out.ptr, out.bytes(), other.ptr, other.bytes()))
+    return HC_CUDA_OK;
+  if (same_ok && out.ptr == other.ptr && out.ld == other.ld)
+    return HC_CUDA_OK;
+  return fail(ctx, HC_CUDA_ERR_INVALID_ARGUMENT, "%s must not %soverlap %s", out.name, same_ok ? "partially " : "",
+              other.name);
+}
+
+int check_norm_shape(const HcCudaContext *ctx, int64_t rows, int64_t cols, int dtype, int param_dtype) {
+  if (rows < 0 || cols < 0)
+    return fail(ctx, HC_CUDA_ERR_INVALID_ARGUMENT, "rows and cols must be non-negative (got %lld, %lld)",
+                (long long)rows, (long long)cols);
+  if (rows > 0x7fffffffLL || cols > kMaxDim)
+    return fail(ctx, HC_CUDA_ERR_UNSUPPORTED, "rows must be below 2^31 and cols at most 2^30");
+  if (!is_c_type(dtype))
+    return fail(ctx, HC_CUDA_ERR_INVALID_ARGUMENT, "dtype must be an HcCudaCType (got %d)", dtype);
+  if (param_dtype != HC_CUDA_C_F32 && param_dtype != dtype)
+    return fail(ctx, HC_CUDA_ERR_INVALID_ARGUMENT, "param_dtype must be float32 or the dtype of x (got %d)", param_dtype);
+  return HC_CUDA_OK;
+}
+
+int check_layer_norm_args(const HcCudaContext *ctx, const HcCudaLayerNormArgs *args) {
+  if (args == nullptr)
+    return fail(ctx, HC_CUDA_ERR_INVALID_ARGUMENT, "args must not be null");
+  if (int rc = check_norm_shape(ctx, args->rows, args->cols, args->dtype, args->param_dtype))
+    return rc;
+  if (!(args->eps >= 0.0f) || args->eps > 3.402823466e38f)
+    return fail(ctx, HC_CUDA_ERR_INVALID_ARGUMENT, "eps must be finite and not negative");
+  if (args->rows == 0 || args->cols == 0)
+    return HC_CUDA_OK;
+  const size_t es = float_bytes(args->dtype), ps = float_bytes(args->param_dtype);
+  const Operand x{"x", args->x, args->rows, args->cols, args->ldx, es};
+  const Operand y{"y", args->y, args->rows, args->cols, args->ldy, es};
+  const Operand weight{"weight", args->weight, 1, args->cols, args->cols, ps};
+  const Operand bias{"bias", args->bias, 1, args->cols, args->cols, ps};
+  const Operand mean{"mean", args->mean, 1, args->rows, args->rows, 4};
+  const Operand rstd{"rstd", args->rstd, 1, args->rows, args->rows, 4};
+  for (const Operand *o : {&x, &y, &weight, &bias, &mean, &rstd})
+    if (o == &x || o == &y || o->ptr != nullptr)
+      if (int rc = check_operand(ctx, *o))
+        return rc;
+  if (int rc = check_apart(ctx, y, x, /*same_ok=*/true))
+    return rc;
+  for (const Operand *o : {&weight, &bias, &mean, &rstd})
+    if (int rc = check_apart(ctx, y, *o))
+      return rc;
+  for (const Operand *out : {&mean, &rstd})
+    for (const Operand *o : {&x, &weight, &bias})
+      if (int rc = check_apart(ctx, *out, *o))
+        return rc;
+  return check_apart(ctx, mean, rstd);
+}
+
+int check_layer_norm_backward_args(const HcCudaContext *ctx, const HcCudaLayerNormBackwardArgs *args) {
+  if (args == nullptr)
+    return fail(ctx, HC_CUDA_ERR_INVALID_ARGUMENT, "args must not be null");
+  if (int rc = check_norm_shape(ctx, args->rows, args->cols, args->dtype, args->param_dtype))
+    return rc;
+  if (args->cols == 0)
+    return HC_CUDA_OK;
+  const size_t es = float_bytes(args->dtype), ps = float_bytes(args->param_dtype);
+  const Operand dweight{"dweight", args->dweight, 1, args->cols, args->cols, ps};
+  const Operand dbias{"dbias", args->dbias, 1, args->cols, args->cols, ps};
+  for (const Operand *o : {&dweight, &dbias})
+    if (o->ptr != nullptr)
+      if (int rc = check_operand(ctx, *o))
+        return rc;
+  if (int rc = check_apart(ctx, dweight, dbias))
+    return rc;
+  if (args->rows == 0)
+    return HC_CUDA_OK;
+  const Operand dy{"dy", args->dy, args->rows, args->cols, args->lddy, es};
+  const Operand x{"x", args->x, args->rows, args->cols, args->ldx, es};
+  const Operand dx{"dx", args->dx, args->rows, args->cols, args->lddx, es};
+  const Operand weight{"weight", args->weight, 1, args->cols, args->cols, ps};
+  const Operand mean{"mean", args->mean, 1, args->rows, args->rows, 4};
+  const Operand rstd{"rstd", args->rstd, 1, args->rows, args->rows, 4};
+  for (const Operand *o : {&dy, &x, &dx, &weight, &mean, &rstd})
+    if (o != &weight || o->ptr != nullptr)
+      if (int rc = check_operand(ctx, *o))
+        return rc;
+  for (const Operand *o : {&dy, &x})
+    if (int rc = check_apart(ctx, dx, *o, /*same_ok=*/true))
+      return rc;
+  for (const Operand *o : {&weight, &mean, &rstd, &dweight, &dbias})
+    if (int rc = check_apart(ctx, dx, *o))
+      return rc;
+  for (const Operand *out : {&dweight, &dbias})
+    for (const Operand *o : {&dy, &x, &weight, &mean, &rstd})
+      if (int rc = check_apart(ctx, *out, *o))
+        return rc;
+  return HC_CUDA_OK;
+}
+
+// Validation and launch plan of the two calls; `ctx` only receives the error text (null: per thread).
+int plan_layer_norm(const HcCudaContext *ctx, const HcCudaLayerNormArgs *args, HcCudaOperatorPlanInfo *plan) {
+  if (int rc = check_layer_norm_args(ctx, args))
+    return rc;
+  const bool empty = args->rows == 0 || args->cols == 0;
+  *plan = HcCudaOperatorPlanInfo{empty ? 0 : 1, empty ? 0 : 1, 0};
+  return HC_CUDA_OK;
+}
+
+int plan_layer_norm_backward(const HcCudaContext *ctx, const HcCudaLayerNormBackwardArgs *args, int sm_count,
+                             HcCudaOperatorPlanInfo *plan) {
+  if (int rc = check_layer_norm_backward_args(ctx, args))
+    return rc;
+  *plan = HcCudaOperatorPlanInfo{0, 0, 0};
+  if (args->rows == 0 || args->cols == 0)
+    return HC_CUDA_OK;
+  const int vec = hc::sm100::layer_norm_vector(args->dtype, args->dy, args->lddy, args->x, args->ldx, args->dx, args->lddx);
+  const bool params = args->dweight != nullptr || args->dbias != nullptr;
+  plan->pieces = 1;
+  plan->kernel_launches = hc::sm100::layer_norm_backward_launches(args->rows, args->cols, vec, params);
+  if (params)
+    plan->scratch_bytes =
+        static_cast<int64_t>(hc::sm100::layer_norm_backward_scratch(args->rows, args->cols, vec, sm_count));
+  return HC_CUDA_OK;
+}
+
+} // namespace
+
+int hcCudaLayerNormPlan(const HcCudaLayerNormArgs *args, int sm_count, HcCudaOperatorPlanInfo *out) {
+  (void)sm_count;
+  if (out == nullptr)
+    return fail(nullptr, HC_CUDA_ERR_INVALID_ARGUMENT, "out must not be null");
+  return plan_layer_norm(nullptr, args, out);
+}
+
+int hcCudaLayerNormBackwardPlan(const HcCudaLayerNormBackwardArgs *args, int sm_count, HcCudaOperatorPlanInfo *out) {
+  if (out == nullptr)
+    return fail(nullptr, HC_CUDA_ERR_INVALID_ARGUMENT, "out must not be null");
+  return plan_layer_norm_backward(nullptr, args, sm_count > 0 ? sm_count : kDefaultSmCount, out);
+}
+
+int hcCudaLayerNorm(HcCudaContext *ctx, const HcCudaLayerNormArgs *args) {
+  if (ctx == nullptr)
+    return fail(ctx, HC_CUDA_ERR_INVALID_ARGUMENT, "ctx must not be null");
+  std::lock_guard<std::mutex> lock(ctx->mu);
+  HcCudaOperatorPlanInfo plan;
+  if (int rc = plan_layer_norm(ctx, args, &plan))
+    return rc;
+  if (plan.kernel_launches == 0)
+    return HC_CUDA_OK;
+  HC_TRY_CUDA(ctx, cudaSetDevice(ctx->device));
+  HC_TRY_CUDA(ctx, hc::sm100::launch_layer_norm(args->x, args->ldx, args->weight, args->bias, args->y, args->ldy,
+                                                args->mean, args->rstd, args->rows, args->cols, args->eps, args->dtype,
+                                                args->param_dtype, ctx->prop.multiProcessorCount, ctx->stream));
+  return HC_CUDA_OK;
+}
+
+int hcCudaLayerNormBackward(HcCudaContext *ctx, const HcCudaLayerNormBackwardArgs *args) {
+  if (ctx == nullptr)
+    return fail(ctx, HC_CUDA_ERR_INVALID_ARGUMENT, "ctx must not be null");
+  std::lock_guard<std::mutex> lock(ctx->mu);
+  const int sm_count = ctx->prop.multiProcessorCount;
+  HcCudaOperatorPlanInfo plan;
+  if (int rc = plan_layer_norm_backward(ctx, args, sm_count, &plan))
+    return rc;
+  if (args->cols == 0)
+    return HC_CUDA_OK;
+  HC_TRY_CUDA(ctx, cudaSetDevice(ctx->device));
+  if (args->rows == 0) {  // sums over no rows
+    for (void *p : {args->dweight, args->dbias})
+      if (p != nullptr)
+        HC_TRY_CUDA(ctx, cudaMemsetAsync(p, 0, static_cast<size_t>(args->cols) * float_bytes(args->param_dtype), ctx->stream));
+    return HC_CUDA_OK;
+  }
+  if (int rc = ensure_scratch(ctx, static_cast<size_t>(plan.scratch_bytes)))
+    return rc;
+  HC_TRY_CUDA(ctx, hc::sm100::launch_layer_norm_backward(
+                       args->dy, args->lddy, args->x, args->ldx, args->weight, args->mean, args->rstd, args->dx, args->lddx,
+                       args->dweight, args->dbias, static_cast<float *>(ctx->scratch), args->rows, args->cols, args->dtype,
+                       args->param_dtype, sm_count, ctx->stream));
+  return HC_CUDA_OK;
+}
+
 int hcCudaSelfTestDeviceTimeout(HcCudaContext *ctx, int64_t budget_cycles) {
   if (ctx == nullptr)
     return fail(ctx, HC_CUDA_ERR_INVALID_ARGUMENT, "ctx must not be null");

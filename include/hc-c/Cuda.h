@@ -39,7 +39,7 @@
 extern "C" {
 #endif
 
-#define HC_CUDA_API_VERSION 8
+#define HC_CUDA_API_VERSION 9
 
 typedef enum HcCudaStatus {
   HC_CUDA_OK = 0,
@@ -414,6 +414,76 @@ HC_CUDA_CAPI_EXPORTED int hcCudaRowSum(HcCudaContext *ctx, const HcCudaRowSumArg
 /* Synchronous; x and out are host pointers (NumPy buffers): the in-place, synchronous behaviour of
  * `hc.simulator.launch` (hc/simulator.py:165-186). */
 HC_CUDA_CAPI_EXPORTED int hcCudaRowSumHost(HcCudaContext *ctx, const HcCudaRowSumArgs *args);
+
+/* ---- layer norm over the rows of a matrix -------------------------------------------------- */
+
+/* What one call of an operator below does; computed on the host without touching a device. */
+typedef struct HcCudaOperatorPlanInfo {
+  int32_t kernel_launches; /* kernels the call enqueues (0: nothing to compute) */
+  int32_t pieces;          /* parts the work is done in one after the other (1, or 0 when there is none) */
+  int64_t scratch_bytes;   /* context scratch the call needs */
+} HcCudaOperatorPlanInfo;
+
+/* With mean_r and rstd_r = 1 / sqrt(variance_r + eps) of the `cols` values of row r,
+ * y = (x - mean_r) * rstd_r * weight + bias. No counterpart in the reference, whose kernels reduce rows
+ * one value at a time (hc/_sim_types.py:1050-1102); the operator stands beside hcCudaRowSum.
+ * x and y: HcCudaCType `dtype`; weight and bias (each may be NULL: 1 and 0): `param_dtype`, which is
+ * float32 or `dtype`. Sums are float32, the variance is that of the differences from the mean, and y is
+ * rounded once. Matrices are row-major with element pitches, aligned to their element size; rows that
+ * start on 16-byte boundaries are accessed 16 bytes at a time. y may be the very same matrix as x (same
+ * pointer and pitch) but must not overlap anything else. rows == 0 or cols == 0 writes nothing. */
+typedef struct HcCudaLayerNormArgs {
+  int64_t rows, cols;
+  int32_t dtype;       /* HcCudaCType of x and y */
+  int32_t param_dtype; /* HcCudaCType of weight and bias */
+  const void *x;
+  int64_t ldx;
+  const void *weight;
+  const void *bias;
+  void *y;
+  int64_t ldy;
+  float *mean; /* rows floats each, or NULL: what the backward pass needs */
+  float *rstd;
+  float eps;   /* finite, not negative */
+} HcCudaLayerNormArgs;
+
+/* Asynchronous; device pointers on the context's device. */
+HC_CUDA_CAPI_EXPORTED int hcCudaLayerNorm(HcCudaContext *ctx, const HcCudaLayerNormArgs *args);
+/* Validates `args` exactly as hcCudaLayerNorm does (pointers are checked but never dereferenced) and
+ * reports what would run on a device with `sm_count` SMs. Needs no device. */
+HC_CUDA_CAPI_EXPORTED int hcCudaLayerNormPlan(const HcCudaLayerNormArgs *args, int sm_count,
+                                              HcCudaOperatorPlanInfo *out);
+
+/* The gradients of sum(y * dy): with n = (x - mean_r) * rstd_r and a = dy * weight,
+ *   dx = rstd_r * (a - sum_c(a) / cols - n * sum_c(a * n) / cols)
+ *   dweight = sum_r(dy * n),  dbias = sum_r(dy)
+ * mean and rstd are those that hcCudaLayerNorm stored. dweight and dbias (param_dtype, `cols` values, each
+ * may be NULL) are overwritten; their sums over rows are float32, added in an order that depends only on
+ * the sizes, alignment and the device, so a call gives the same bits every time. dx may be the very same
+ * matrix as dy or x (same pointer and pitch). rows == 0 sets dweight and dbias to zero; cols == 0 writes
+ * nothing. Uses context scratch. */
+typedef struct HcCudaLayerNormBackwardArgs {
+  int64_t rows, cols;
+  int32_t dtype;       /* HcCudaCType of dy, x and dx */
+  int32_t param_dtype; /* HcCudaCType of weight, dweight and dbias */
+  const void *dy;
+  int64_t lddy;
+  const void *x;
+  int64_t ldx;
+  const void *weight; /* NULL: 1 */
+  const float *mean;
+  const float *rstd;
+  void *dx;
+  int64_t lddx;
+  void *dweight;
+  void *dbias;
+} HcCudaLayerNormBackwardArgs;
+
+/* Asynchronous; device pointers on the context's device. */
+HC_CUDA_CAPI_EXPORTED int hcCudaLayerNormBackward(HcCudaContext *ctx, const HcCudaLayerNormBackwardArgs *args);
+/* The same validation and report for the backward pass, without a device. */
+HC_CUDA_CAPI_EXPORTED int hcCudaLayerNormBackwardPlan(const HcCudaLayerNormBackwardArgs *args, int sm_count,
+                                                      HcCudaOperatorPlanInfo *out);
 
 /* ---- the product fused with its gather (N-sharded GEMM, one process per GPU) ------------- */
 
