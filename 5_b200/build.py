@@ -38,6 +38,7 @@ SOURCES = [
     LIB_DIR / "Kernels" / "pairwise_distance_sm100a.cu",
     LIB_DIR / "Kernels" / "row_reduce_sm100a.cu",
     LIB_DIR / "Kernels" / "layer_norm_sm100a.cu",
+    LIB_DIR / "Kernels" / "linear_loss_sm100a.cu",
     LIB_DIR / "Kernels" / "gemm_skinny_static_sm100a.cu",
     LIB_DIR / "Kernels" / "selftest_sm100a.cu",
     LIB_DIR / "CAPI" / "Cuda.cpp",

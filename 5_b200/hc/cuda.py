@@ -59,6 +59,7 @@ EXPORTS = (
     "hcCudaIpcOpen", "hcCudaIpcClose", "hcCudaMap", "hcCudaMapHost",
     "hcCudaGemmHostDeviceA", "hcCudaPairwise", "hcCudaPairwiseHost", "hcCudaRowSum", "hcCudaRowSumHost", "hcCudaBuildFlags", "hcCudaSelfTestDeviceCheck",
     "hcCudaLayerNorm", "hcCudaLayerNormPlan", "hcCudaLayerNormBackward", "hcCudaLayerNormBackwardPlan",
+    "hcCudaLinearLoss", "hcCudaLinearLossPlan", "hcCudaLinearLossBackward", "hcCudaLinearLossBackwardPlan",
 )
 
 
@@ -151,6 +152,22 @@ class _LayerNormBackwardArgs(ctypes.Structure):
     ]
 
 
+_LOSS_FIELDS = [
+    ("rows", ctypes.c_int64), ("vocab", ctypes.c_int64), ("width", ctypes.c_int64), ("dtype", ctypes.c_int32),
+    ("targets_64", ctypes.c_int32), ("h", ctypes.c_void_p), ("ldh", ctypes.c_int64), ("w", ctypes.c_void_p),
+    ("ldw", ctypes.c_int64), ("targets", ctypes.c_void_p), ("ignore_index", ctypes.c_int64),
+]
+
+
+class _LinearLossArgs(ctypes.Structure):
+    _fields_ = [*_LOSS_FIELDS, ("loss", ctypes.c_void_p), ("lse", ctypes.c_void_p)]
+
+
+class _LinearLossBackwardArgs(ctypes.Structure):
+    _fields_ = [*_LOSS_FIELDS, ("lse", ctypes.c_void_p), ("dloss", ctypes.c_void_p), ("dh", ctypes.c_void_p),
+                ("lddh", ctypes.c_int64), ("dw", ctypes.c_void_p), ("lddw", ctypes.c_int64)]
+
+
 class _OperatorPlanInfo(ctypes.Structure):
     _fields_ = [("kernel_launches", ctypes.c_int32), ("pieces", ctypes.c_int32), ("scratch_bytes", ctypes.c_int64)]
 
@@ -238,7 +255,11 @@ def library() -> ctypes.CDLL:
         lib.hcCudaRowSumHost.argtypes = [vp, ctypes.POINTER(_RowSumArgs)]
         lib.hcCudaLayerNorm.argtypes = [vp, ctypes.POINTER(_LayerNormArgs)]
         lib.hcCudaLayerNormBackward.argtypes = [vp, ctypes.POINTER(_LayerNormBackwardArgs)]
+        lib.hcCudaLinearLoss.argtypes = [vp, ctypes.POINTER(_LinearLossArgs)]
+        lib.hcCudaLinearLossBackward.argtypes = [vp, ctypes.POINTER(_LinearLossBackwardArgs)]
         plan_info = ctypes.POINTER(_OperatorPlanInfo)
+        lib.hcCudaLinearLossPlan.argtypes = [ctypes.POINTER(_LinearLossArgs), i, plan_info]
+        lib.hcCudaLinearLossBackwardPlan.argtypes = [ctypes.POINTER(_LinearLossBackwardArgs), i, plan_info]
         lib.hcCudaLayerNormPlan.argtypes = [ctypes.POINTER(_LayerNormArgs), i, plan_info]
         lib.hcCudaLayerNormBackwardPlan.argtypes = [ctypes.POINTER(_LayerNormBackwardArgs), i, plan_info]
         for name in EXPORTS:
@@ -638,6 +659,42 @@ class Context:
         if len(kinds) > 1:
             raise ValueError(f"{call}() takes weight and bias vectors (and their gradients) of one type")
         return kinds.pop() if kinds else np.dtype(np.float32)
+
+    def linear_cross_entropy(self, h: "DeviceBuffer", w: "DeviceBuffer", targets: "DeviceBuffer", loss: "DeviceBuffer",
+                             lse: "DeviceBuffer", *, ignore_index: int = -100) -> None:
+        """Enqueues the softmax cross entropy of the logits `h @ w.T` against `targets` (asynchronous; see
+        `synchronize`): per row, `lse` = log(sum(exp(logits))) and `loss` = lse - logits[target], float32
+        vectors. `h` (rows, width) and `w` (vocab, width): float16 or bfloat16 device matrices of one
+        type; `targets`: int64 or int32. Rows whose target is `ignore_index` have loss 0; any other target
+        outside the vocabulary gives NaN. The logits are not stored."""
+        args = _LinearLossArgs(*self._loss_call("linear_cross_entropy", h, w, targets, ignore_index),
+                               _vector("loss", loss, h.shape[0], np.float32), _vector("lse", lse, h.shape[0], np.float32))
+        self._check(self._lib.hcCudaLinearLoss(self._handle, ctypes.byref(args)))
+
+    def linear_cross_entropy_backward(self, h: "DeviceBuffer", w: "DeviceBuffer", targets: "DeviceBuffer",
+                                      lse: "DeviceBuffer", dloss: "DeviceBuffer", *, dh: "DeviceBuffer | None" = None,
+                                      dw: "DeviceBuffer | None" = None, ignore_index: int = -100) -> None:
+        """Enqueues the gradients of sum(loss * dloss) (asynchronous): `dh` and `dw`, shaped and typed like `h` and
+        `w`, each optional and overwritten. `lse` is what `linear_cross_entropy` stored, `dloss` a float32
+        vector. Rows that `linear_cross_entropy` leaves out have no gradient. The logits are computed
+        again, a piece of the vocabulary at a time."""
+        for name, grad, like in (("dh", dh, h), ("dw", dw, w)):
+            if grad is not None and (grad.shape != like.shape or grad.dtype != like.dtype):
+                raise ValueError(f"{name} must have the shape and type of {name[1:]}")
+        args = _LinearLossBackwardArgs(
+            *self._loss_call("linear_cross_entropy_backward", h, w, targets, ignore_index),
+            _vector("lse", lse, h.shape[0], np.float32), _vector("dloss", dloss, h.shape[0], np.float32),
+            None if dh is None else dh.ptr, 0 if dh is None else dh.ld, None if dw is None else dw.ptr,
+            0 if dw is None else dw.ld)
+        self._check(self._lib.hcCudaLinearLossBackward(self._handle, ctypes.byref(args)))
+
+    @staticmethod
+    def _loss_call(call: str, h: "DeviceBuffer", w: "DeviceBuffer", targets: "DeviceBuffer", ignore_index: int) -> tuple:
+        if h.ndim != 2 or w.ndim != 2 or h.shape[1] != w.shape[1] or h.dtype != w.dtype:
+            raise ValueError(f"{call}() takes h (rows, width) and w (vocab, width) of one type, got {h.shape} of "
+                             f"{h.dtype.name} and {w.shape} of {w.dtype.name}")
+        return (h.shape[0], w.shape[0], h.shape[1], dtype_code(h.dtype), int(targets.dtype == np.int64), h.ptr, h.ld, w.ptr,
+                w.ld, _vector("targets", targets, h.shape[0], np.int64, np.int32), ignore_index)
 
     def gemm_host(self, a: np.ndarray, b: np.ndarray, c: np.ndarray, *,
                   variant: int = VARIANT_AUTO, b_transposed: bool = False, accumulate: bool = False,

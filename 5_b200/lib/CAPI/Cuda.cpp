@@ -109,6 +109,8 @@ struct HcCudaContext {
   int *status_host = nullptr;  // pinned
   void *scratch = nullptr;
   size_t scratch_bytes = 0;
+  void *work = nullptr;  // what an operator keeps between the launches of one call (its products use `scratch`)
+  size_t work_bytes = 0;
   unsigned *counters = nullptr;
   size_t counters_bytes = 0;
   int4 *pairwise_leaves = nullptr;  // summation schedule of the pairwise kernel for `pairwise_h`
@@ -465,6 +467,21 @@ int ensure_scratch(HcCudaContext *ctx, size_t bytes) {
   const size_t grown = static_cast<size_t>(round_up(static_cast<int64_t>(bytes), 1 << 20));
   HC_TRY_CUDA(ctx, cudaMalloc(&ctx->scratch, grown));
   ctx->scratch_bytes = grown;
+  return HC_CUDA_OK;
+}
+
+int ensure_work(HcCudaContext *ctx, size_t bytes) {
+  if (bytes <= ctx->work_bytes)
+    return HC_CUDA_OK;
+  if (ctx->work != nullptr) {
+    HC_TRY_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
+    HC_TRY_CUDA(ctx, cudaFree(ctx->work));
+    ctx->work = nullptr;
+    ctx->work_bytes = 0;
+  }
+  const size_t grown = static_cast<size_t>(round_up(static_cast<int64_t>(bytes), 1 << 20));
+  HC_TRY_CUDA(ctx, cudaMalloc(&ctx->work, grown));
+  ctx->work_bytes = grown;
   return HC_CUDA_OK;
 }
 
@@ -927,6 +944,8 @@ int hcCudaContextDestroy(HcCudaContext *ctx) {
       cudaStreamDestroy(ctx->copy_out);
     if (ctx->scratch != nullptr)
       cudaFree(ctx->scratch);
+    if (ctx->work != nullptr)
+      cudaFree(ctx->work);
     if (ctx->counters != nullptr)
       cudaFree(ctx->counters);
     if (ctx->pairwise_leaves != nullptr)
@@ -2070,6 +2089,430 @@ int hcCudaLayerNormBackward(HcCudaContext *ctx, const HcCudaLayerNormBackwardArg
                        args->dy, args->lddy, args->x, args->ldx, args->weight, args->mean, args->rstd, args->dx, args->lddx,
                        args->dweight, args->dbias, static_cast<float *>(ctx->scratch), args->rows, args->cols, args->dtype,
                        args->param_dtype, sm_count, ctx->stream));
+  return HC_CUDA_OK;
+}
+
+namespace {
+
+// What both passes over the logits share: arguments by one name, then where things lie in `work`.
+struct LossCall {
+  int64_t rows, vocab, width;
+  int32_t dtype, targets_64;
+  const void *h;
+  int64_t ldh;
+  const void *w;
+  int64_t ldw;
+  const void *targets;
+  int64_t ignore_index;
+};
+
+extern "C++" template <typename Args>
+LossCall loss_call(const Args &a) {
+  return LossCall{a.rows, a.vocab, a.width, a.dtype, a.targets_64, a.h, a.ldh, a.w, a.ldw, a.targets, a.ignore_index};
+}
+
+Operand operand_h(const LossCall &c) { return {"h", c.h, c.rows, c.width, c.ldh, 2}; }
+Operand operand_w(const LossCall &c) { return {"w", c.w, c.vocab, c.width, c.ldw, 2}; }
+Operand operand_targets(const LossCall &c) {
+  return {"targets", c.targets, 1, c.rows, c.rows, static_cast<size_t>(c.targets_64 ? 8 : 4)};
+}
+
+int check_loss_sizes(const HcCudaContext *ctx, const LossCall &c) {
+  if (c.rows < 0 || c.vocab < 1 || c.width < 1)
+    return fail(ctx, HC_CUDA_ERR_INVALID_ARGUMENT, "rows must be non-negative, vocab and width at least 1 (got %lld, %lld, %lld)",
+                (long long)c.rows, (long long)c.vocab, (long long)c.width);
+  if (c.rows > kMaxDim || c.vocab > kMaxDim || c.width > kMaxDim)
+    return fail(ctx, HC_CUDA_ERR_UNSUPPORTED, "rows, vocab and width must each be at most 2^30");
+  if (((c.rows + 255) / 256) * ((c.vocab + 255) / 256) > 0x3fffffffLL)
+    return fail(ctx, HC_CUDA_ERR_UNSUPPORTED, "too many tiles of logits");
+  if (c.dtype != HC_CUDA_F16 && c.dtype != HC_CUDA_BF16)
+    return fail(ctx, HC_CUDA_ERR_INVALID_ARGUMENT, "dtype must be HC_CUDA_F16 or HC_CUDA_BF16 (got %d)", c.dtype);
+  if (c.targets_64 != 0 && c.targets_64 != 1)
+    return fail(ctx, HC_CUDA_ERR_INVALID_ARGUMENT, "targets_64 must be 0 or 1 (got %d)", c.targets_64);
+  return HC_CUDA_OK;
+}
+
+bool needs_repack(const void *p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0 || (ld * 2) % 16 != 0; }
+
+// Bytes of the copies of h and w that TMA can address, and the places of things behind them in `work`.
+struct LossWork {
+  int64_t h_copy = -1, w_copy = -1;  // offsets, -1: read where they stand
+  int64_t copy_ld = 0;
+  int64_t bytes = 0;
+  int64_t take(int64_t n) {
+    const int64_t at = bytes;
+    bytes += round_up(n, 1024);
+    return at;
+  }
+};
+
+LossWork loss_copies(const LossCall &c, bool copy_h) {
+  LossWork work;
+  work.copy_ld = round_up(c.width, kRepackPitchBytes / 2);
+  if (copy_h || needs_repack(c.h, c.ldh))
+    work.h_copy = work.take(c.rows * work.copy_ld * 2);
+  if (needs_repack(c.w, c.ldw))
+    work.w_copy = work.take(c.vocab * work.copy_ld * 2);
+  return work;
+}
+
+// The launch over columns [first, first + count) of the logits; h and w are aligned for TMA here.
+hc::sm100::LinearLoss loss_launch(const LossCall &c, int64_t first, int64_t count) {
+  hc::sm100::LinearLoss p{};
+  p.rows = static_cast<int>(c.rows);
+  p.vocab = static_cast<int>(count);
+  p.width = static_cast<int>(c.width);
+  p.first_column = first;
+  p.vocab_total = c.vocab;
+  p.targets = c.targets;
+  p.targets_64 = c.targets_64;
+  p.ignore_index = c.ignore_index;
+  p.c_dtype = c.dtype == HC_CUDA_BF16 ? hc::sm100::kCTypeBF16 : hc::sm100::kCTypeF16;
+  return p;
+}
+
+// Enqueues the copies and points `c` at them. `counting_rows`: the copy of h has zeros in the rows that do
+// not count.
+int enqueue_loss_copies(HcCudaContext *ctx, const LossWork &work, bool counting_rows, LossCall *c) {
+  char *base = static_cast<char *>(ctx->work);
+  if (counting_rows)
+    HC_TRY_CUDA(ctx, hc::sm100::launch_linear_loss_rows(loss_launch(*c, 0, c->vocab), c->h, c->ldh, base + work.h_copy,
+                                                        work.copy_ld, ctx->stream));
+  const bool repack_h = work.h_copy >= 0 && !counting_rows;
+  if (repack_h || work.w_copy >= 0)
+    HC_TRY_CUDA(ctx, hc::sm100::launch_repack_pitch_two(
+                         c->h, c->ldh, base + (repack_h ? work.h_copy : 0), work.copy_ld,
+                         repack_h ? static_cast<int>(c->rows) : 0, static_cast<int>(c->width), c->w, c->ldw,
+                         base + (work.w_copy < 0 ? 0 : work.w_copy), work.copy_ld,
+                         work.w_copy < 0 ? 0 : static_cast<int>(c->vocab), static_cast<int>(c->width), ctx->stream));
+  if (work.h_copy >= 0) {
+    c->h = base + work.h_copy;
+    c->ldh = work.copy_ld;
+  }
+  if (work.w_copy >= 0) {
+    c->w = base + work.w_copy;
+    c->ldw = work.copy_ld;
+  }
+  return HC_CUDA_OK;
+}
+
+int enqueue_loss_tiles(HcCudaContext *ctx, const LossCall &c, const hc::sm100::LinearLoss &p, bool grad) {
+  CUtensorMap tmap_h, tmap_w;
+  if (int rc = encode_map(ctx, &tmap_h, c.dtype, c.h, static_cast<uint64_t>(c.width), static_cast<uint64_t>(c.rows),
+                          static_cast<uint64_t>(c.ldh) * 2, 64, 128))
+    return rc;
+  const char *w = static_cast<const char *>(c.w) + static_cast<size_t>(p.first_column) * static_cast<size_t>(c.ldw) * 2;
+  if (int rc = encode_map(ctx, &tmap_w, c.dtype, w, static_cast<uint64_t>(c.width), static_cast<uint64_t>(p.vocab),
+                          static_cast<uint64_t>(c.ldw) * 2, 64, 128))
+    return rc;
+  HC_TRY_CUDA(ctx, hc::sm100::launch_linear_loss(tmap_h, tmap_w, p, grad, ctx->prop.multiProcessorCount, ctx->status_dev,
+                                                 ctx->stream));
+  return HC_CUDA_OK;
+}
+
+struct LossForwardPlan {
+  LossWork work;
+  int64_t partials = 0, target_logit = 0;
+};
+
+int plan_linear_loss(const HcCudaContext *ctx, const HcCudaLinearLossArgs *args, LossForwardPlan *plan,
+                     HcCudaOperatorPlanInfo *info) {
+  if (args == nullptr)
+    return fail(ctx, HC_CUDA_ERR_INVALID_ARGUMENT, "args must not be null");
+  const LossCall c = loss_call(*args);
+  if (int rc = check_loss_sizes(ctx, c))
+    return rc;
+  *info = HcCudaOperatorPlanInfo{0, 0, 0};
+  if (c.rows == 0)
+    return HC_CUDA_OK;
+  const Operand h = operand_h(c), w = operand_w(c), targets = operand_targets(c);
+  const Operand loss{"loss", args->loss, 1, c.rows, c.rows, 4}, lse{"lse", args->lse, 1, c.rows, c.rows, 4};
+  for (const Operand *o : {&h, &w, &targets, &loss, &lse})
+    if (int rc = check_operand(ctx, *o))
+      return rc;
+  for (const Operand *out : {&loss, &lse})
+    for (const Operand *in : {&h, &w, &targets})
+      if (int rc = check_apart(ctx, *out, *in))
+        return rc;
+  if (int rc = check_apart(ctx, loss, lse))
+    return rc;
+  plan->work = loss_copies(c, /*copy_h=*/false);
+  plan->partials = plan->work.take(static_cast<int64_t>(hc::sm100::linear_loss_parts(static_cast<int>(c.vocab))) * c.rows * 8);
+  plan->target_logit = plan->work.take(c.rows * 4);
+  const bool copies = plan->work.h_copy >= 0 || plan->work.w_copy >= 0;
+  *info = HcCudaOperatorPlanInfo{copies ? 3 : 2, 1, plan->work.bytes};
+  return HC_CUDA_OK;
+}
+
+// Bytes that g and its transpose may take together; more only where a piece of 256 columns needs it.
+constexpr int64_t kLossPieceBytes = int64_t(1) << 29;
+
+struct LossBackwardPlan {
+  LossWork work;
+  int64_t piece = 0;  // columns of the vocabulary per piece, a multiple of 256
+  int64_t pieces = 0;
+  int64_t g = 0, gt = 0, ldg = 0, ldgt = 0;
+  int64_t dh_sums = -1, dw_sums = -1;  // float32, where a product cannot write its result's type at once
+  int64_t sums_ld = 0;
+  int64_t scales = -1;
+};
+
+// The two products of a piece as GEMM arguments; `c` is already aligned, `base` the start of `work`.
+HcCudaGemmArgs loss_dh_product(const LossCall &c, const LossBackwardPlan &plan, char *base, int64_t first, int64_t count,
+                               const HcCudaLinearLossBackwardArgs &args) {
+  HcCudaGemmArgs g{};
+  g.m = c.rows;
+  g.n = c.width;
+  g.k = count;
+  g.dtype = c.dtype;
+  g.a = base + plan.g;
+  g.lda = plan.ldg;
+  g.b = static_cast<const char *>(c.w) + static_cast<size_t>(first) * static_cast<size_t>(c.ldw) * 2;
+  g.ldb = c.ldw;
+  g.b_layout = HC_CUDA_B_KN;
+  if (plan.dh_sums >= 0) {
+    g.c = base + plan.dh_sums;
+    g.ldc = plan.sums_ld;
+    g.accumulate = first != 0 ? 1 : 0;
+    g.c_dtype = HC_CUDA_C_F32;
+  } else {
+    g.c = args.dh;
+    g.ldc = args.lddh;
+    g.c_dtype = c.dtype == HC_CUDA_BF16 ? HC_CUDA_C_BF16 : HC_CUDA_C_F16;
+  }
+  return g;
+}
+
+HcCudaGemmArgs loss_dw_product(const LossCall &c, const LossBackwardPlan &plan, char *base, int64_t first, int64_t count,
+                               const HcCudaLinearLossBackwardArgs &args) {
+  HcCudaGemmArgs g{};
+  g.m = count;
+  g.n = c.width;
+  g.k = c.rows;
+  g.dtype = c.dtype;
+  g.a = base + plan.gt;
+  g.lda = plan.ldgt;
+  g.b = c.h;
+  g.ldb = c.ldh;
+  g.b_layout = HC_CUDA_B_KN;
+  if (plan.dw_sums >= 0) {
+    g.c = base + plan.dw_sums;
+    g.ldc = plan.sums_ld;
+    g.c_dtype = HC_CUDA_C_F32;
+  } else {
+    g.c = static_cast<char *>(args.dw) + static_cast<size_t>(first) * static_cast<size_t>(args.lddw) * 2;
+    g.ldc = args.lddw;
+    g.c_dtype = c.dtype == HC_CUDA_BF16 ? HC_CUDA_C_BF16 : HC_CUDA_C_F16;
+  }
+  return g;
+}
+
+int plan_linear_loss_backward(const HcCudaContext *ctx, const HcCudaLinearLossBackwardArgs *args, int sm_count,
+                              LossBackwardPlan *plan, HcCudaOperatorPlanInfo *info) {
+  if (args == nullptr)
+    return fail(ctx, HC_CUDA_ERR_INVALID_ARGUMENT, "args must not be null");
+  const LossCall c = loss_call(*args);
+  if (int rc = check_loss_sizes(ctx, c))
+    return rc;
+  *info = HcCudaOperatorPlanInfo{0, 0, 0};
+  const Operand dw{"dw", args->dw, c.vocab, c.width, args->lddw, 2};
+  if (args->dw != nullptr)
+    if (int rc = check_operand(ctx, dw))
+      return rc;
+  if (c.rows == 0 || (args->dh == nullptr && args->dw == nullptr))
+    return HC_CUDA_OK;
+  const Operand dh{"dh", args->dh, c.rows, c.width, args->lddh, 2};
+  if (args->dh != nullptr)
+    if (int rc = check_operand(ctx, dh))
+      return rc;
+  const Operand h = operand_h(c), w = operand_w(c), targets = operand_targets(c);
+  const Operand lse{"lse", args->lse, 1, c.rows, c.rows, 4}, dloss{"dloss", args->dloss, 1, c.rows, c.rows, 4};
+  for (const Operand *o : {&h, &w, &targets, &lse, &dloss})
+    if (int rc = check_operand(ctx, *o))
+      return rc;
+  for (const Operand *out : {&dh, &dw})
+    for (const Operand *in : {&h, &w, &targets, &lse, &dloss})
+      if (int rc = check_apart(ctx, *out, *in))
+        return rc;
+  if (int rc = check_apart(ctx, dh, dw))
+    return rc;
+
+  plan->work = loss_copies(c, /*copy_h=*/args->dw != nullptr);
+  plan->ldgt = round_up(c.rows, 64);
+  int64_t piece = kLossPieceBytes / (4 * plan->ldgt) / 256 * 256;
+  if (const char *forced = std::getenv("HC_CUDA_LOSS_PIECE"))  // tuning aid: columns per piece
+    piece = std::atoll(forced) / 256 * 256;
+  if (piece < 256)
+    piece = 256;
+  plan->pieces = (c.vocab + piece - 1) / piece;
+  plan->piece = round_up((c.vocab + plan->pieces - 1) / plan->pieces, 256);  // pieces of one size, but for the last
+  plan->pieces = (c.vocab + plan->piece - 1) / plan->piece;
+  const int64_t columns = c.vocab < plan->piece ? c.vocab : plan->piece;
+  plan->ldg = round_up(columns, 64);
+  plan->g = plan->work.take(args->dh != nullptr ? c.rows * plan->ldg * 2 : 0);
+  plan->gt = plan->work.take(args->dw != nullptr ? columns * plan->ldgt * 2 : 0);
+  plan->sums_ld = round_up(c.width, 4);
+  const bool scaled = c.dtype == HC_CUDA_F16;
+  if (args->dh != nullptr && (plan->pieces > 1 || scaled))
+    plan->dh_sums = plan->work.take(c.rows * plan->sums_ld * 4);
+  if (args->dw != nullptr && scaled)
+    plan->dw_sums = plan->work.take(columns * plan->sums_ld * 4);
+  if (scaled)
+    plan->scales = plan->work.take(8);
+
+  // Launches, and the scratch of the products.
+  LossCall aligned = c;
+  char *const base = reinterpret_cast<char *>(uintptr_t(1) << 40);  // stands for `work`, which is aligned
+  const bool counting_rows = args->dw != nullptr;
+  const bool repacks = (plan->work.h_copy >= 0 && !counting_rows) || plan->work.w_copy >= 0;
+  if (plan->work.h_copy >= 0) {
+    aligned.h = base + plan->work.h_copy;
+    aligned.ldh = plan->work.copy_ld;
+  }
+  if (plan->work.w_copy >= 0) {
+    aligned.w = base + plan->work.w_copy;
+    aligned.ldw = plan->work.copy_ld;
+  }
+  int launches = (counting_rows ? 1 : 0) + (repacks ? 1 : 0) + (scaled ? 1 : 0) + (plan->dh_sums >= 0 ? 1 : 0);
+  int64_t scratch = 0;
+  for (int64_t first = 0; first < c.vocab; first += plan->piece) {
+    const int64_t count = c.vocab - first < plan->piece ? c.vocab - first : plan->piece;
+    ++launches;
+    HcCudaGemmPlanInfo product;
+    if (args->dh != nullptr) {
+      const HcCudaGemmArgs g = loss_dh_product(aligned, *plan, base, first, count, *args);
+      if (int rc = plan_gemm(ctx, &g, sm_count, false, &product))
+        return rc;
+      launches += product.kernel_launches;
+      scratch = product.scratch_bytes > scratch ? product.scratch_bytes : scratch;
+    }
+    if (args->dw != nullptr) {
+      const HcCudaGemmArgs g = loss_dw_product(aligned, *plan, base, first, count, *args);
+      if (int rc = plan_gemm(ctx, &g, sm_count, false, &product))
+        return rc;
+      launches += product.kernel_launches + (plan->dw_sums >= 0 ? 1 : 0);
+      scratch = product.scratch_bytes > scratch ? product.scratch_bytes : scratch;
+    }
+  }
+  *info = HcCudaOperatorPlanInfo{launches, static_cast<int32_t>(plan->pieces), plan->work.bytes + scratch};
+  return HC_CUDA_OK;
+}
+
+} // namespace
+
+int hcCudaLinearLossPlan(const HcCudaLinearLossArgs *args, int sm_count, HcCudaOperatorPlanInfo *out) {
+  (void)sm_count;
+  if (out == nullptr)
+    return fail(nullptr, HC_CUDA_ERR_INVALID_ARGUMENT, "out must not be null");
+  LossForwardPlan plan;
+  return plan_linear_loss(nullptr, args, &plan, out);
+}
+
+int hcCudaLinearLoss(HcCudaContext *ctx, const HcCudaLinearLossArgs *args) {
+  if (ctx == nullptr)
+    return fail(ctx, HC_CUDA_ERR_INVALID_ARGUMENT, "ctx must not be null");
+  std::lock_guard<std::mutex> lock(ctx->mu);
+  LossForwardPlan plan;
+  HcCudaOperatorPlanInfo info;
+  if (int rc = plan_linear_loss(ctx, args, &plan, &info))
+    return rc;
+  if (info.kernel_launches == 0)
+    return HC_CUDA_OK;
+  HC_TRY_CUDA(ctx, cudaSetDevice(ctx->device));
+  if (int rc = ensure_work(ctx, static_cast<size_t>(plan.work.bytes)))
+    return rc;
+  LossCall c = loss_call(*args);
+  if (int rc = enqueue_loss_copies(ctx, plan.work, /*counting_rows=*/false, &c))
+    return rc;
+  char *const base = static_cast<char *>(ctx->work);
+  hc::sm100::LinearLoss p = loss_launch(c, 0, c.vocab);
+  p.partials = reinterpret_cast<float2 *>(base + plan.partials);
+  p.target_logit = reinterpret_cast<float *>(base + plan.target_logit);
+  p.loss_out = args->loss;
+  p.lse_out = args->lse;
+  if (int rc = enqueue_loss_tiles(ctx, c, p, /*grad=*/false))
+    return rc;
+  HC_TRY_CUDA(ctx, hc::sm100::launch_linear_loss_join(p, ctx->stream));
+  return HC_CUDA_OK;
+}
+
+int hcCudaLinearLossBackwardPlan(const HcCudaLinearLossBackwardArgs *args, int sm_count, HcCudaOperatorPlanInfo *out) {
+  if (out == nullptr)
+    return fail(nullptr, HC_CUDA_ERR_INVALID_ARGUMENT, "out must not be null");
+  LossBackwardPlan plan;
+  return plan_linear_loss_backward(nullptr, args, sm_count > 0 ? sm_count : kDefaultSmCount, &plan, out);
+}
+
+int hcCudaLinearLossBackward(HcCudaContext *ctx, const HcCudaLinearLossBackwardArgs *args) {
+  if (ctx == nullptr)
+    return fail(ctx, HC_CUDA_ERR_INVALID_ARGUMENT, "ctx must not be null");
+  std::lock_guard<std::mutex> lock(ctx->mu);
+  const int sm_count = ctx->prop.multiProcessorCount;
+  LossBackwardPlan plan;
+  HcCudaOperatorPlanInfo info;
+  if (int rc = plan_linear_loss_backward(ctx, args, sm_count, &plan, &info))
+    return rc;
+  if (info.kernel_launches == 0) {
+    if (args->rows == 0 && args->dw != nullptr) {  // a sum over no rows
+      HC_TRY_CUDA(ctx, cudaSetDevice(ctx->device));
+      HC_TRY_CUDA(ctx, cudaMemset2DAsync(args->dw, static_cast<size_t>(args->lddw) * 2, 0, static_cast<size_t>(args->width) * 2,
+                                         static_cast<size_t>(args->vocab), ctx->stream));
+    }
+    return HC_CUDA_OK;
+  }
+  HC_TRY_CUDA(ctx, cudaSetDevice(ctx->device));
+  if (int rc = ensure_work(ctx, static_cast<size_t>(plan.work.bytes)))
+    return rc;
+  LossCall c = loss_call(*args);
+  if (int rc = enqueue_loss_copies(ctx, plan.work, /*counting_rows=*/args->dw != nullptr, &c))
+    return rc;
+  char *const base = static_cast<char *>(ctx->work);
+  float *const scales = plan.scales >= 0 ? reinterpret_cast<float *>(base + plan.scales) : nullptr;
+  const int narrow_type = c.dtype == HC_CUDA_BF16 ? hc::sm100::kCTypeBF16 : hc::sm100::kCTypeF16;
+  const float *const factor = scales != nullptr ? scales + 1 : nullptr;
+  for (int64_t first = 0; first < c.vocab; first += plan.piece) {
+    const int64_t count = c.vocab - first < plan.piece ? c.vocab - first : plan.piece;
+    hc::sm100::LinearLoss p = loss_launch(c, first, count);
+    p.lse = args->lse;
+    p.dloss = args->dloss;
+    p.scale = scales;
+    if (args->dh != nullptr) {
+      p.g = base + plan.g;
+      p.ldg = plan.ldg;
+    }
+    if (args->dw != nullptr) {
+      p.gt = base + plan.gt;
+      p.ldgt = plan.ldgt;
+    }
+    if (first == 0 && scales != nullptr)
+      HC_TRY_CUDA(ctx, hc::sm100::launch_linear_loss_scale(p, scales, ctx->stream));
+    if (int rc = enqueue_loss_tiles(ctx, c, p, /*grad=*/true))
+      return rc;
+    HcCudaGemmPlanInfo product;
+    if (args->dh != nullptr) {
+      const HcCudaGemmArgs g = loss_dh_product(c, plan, base, first, count, *args);
+      if (int rc = plan_gemm(ctx, &g, sm_count, false, &product))
+        return rc;
+      if (int rc = enqueue_gemm(ctx, &g, product))
+        return rc;
+    }
+    if (args->dw != nullptr) {
+      const HcCudaGemmArgs g = loss_dw_product(c, plan, base, first, count, *args);
+      if (int rc = plan_gemm(ctx, &g, sm_count, false, &product))
+        return rc;
+      if (int rc = enqueue_gemm(ctx, &g, product))
+        return rc;
+      if (plan.dw_sums >= 0)
+        HC_TRY_CUDA(ctx, hc::sm100::launch_narrow(reinterpret_cast<const float *>(base + plan.dw_sums), plan.sums_ld,
+                                                  static_cast<char *>(args->dw) + static_cast<size_t>(first) * args->lddw * 2,
+                                                  args->lddw, static_cast<int>(count), static_cast<int>(c.width), factor,
+                                                  narrow_type, ctx->stream));
+    }
+  }
+  if (plan.dh_sums >= 0)
+    HC_TRY_CUDA(ctx, hc::sm100::launch_narrow(reinterpret_cast<const float *>(base + plan.dh_sums), plan.sums_ld, args->dh,
+                                              args->lddh, static_cast<int>(c.rows), static_cast<int>(c.width), factor,
+                                              narrow_type, ctx->stream));
   return HC_CUDA_OK;
 }
 

@@ -318,5 +318,41 @@ cudaError_t launch_layer_norm_backward(const void *dy, long long lddy, const voi
                                        void *dbias, float *partials, long long rows, long long cols, int dtype,
                                        int param_dtype, int sm_count, cudaStream_t stream);
 
+// ---- softmax cross entropy of a linear layer ------------------------------------------------------
+// One launch over the logits H W^T of `rows` rows of H and `vocab` rows of W (the tensor maps: H as
+// {width inner, rows}, W as {width inner, vocab}, boxes {64, 128}, 128-byte swizzle), which are the
+// columns first_column .. of a vocabulary of vocab_total.
+struct LinearLoss {
+  int rows, vocab, width;
+  long long first_column, vocab_total;
+  const void *targets;  // rows int64 (targets_64) or int32
+  int targets_64;
+  long long ignore_index;
+  int c_dtype;  // kCTypeF16 or kCTypeBF16: the type of H and W, and of g
+  // Forward: linear_loss_parts(vocab) x rows partial pairs, the logit of each row's target, the results.
+  float2 *partials;
+  float *target_logit, *loss_out, *lse_out;
+  // Gradient: the upstream factors, times *scale when there is one; g [rows, ldg] with ldg a multiple of
+  // 32 not below vocab, and its transpose gt [vocab, ldgt]; either may be null.
+  const float *lse, *dloss, *scale;
+  void *g;
+  long long ldg;
+  void *gt;
+  long long ldgt;
+};
+int linear_loss_parts(int vocab);
+cudaError_t launch_linear_loss(const CUtensorMap &tmap_h, const CUtensorMap &tmap_w, const LinearLoss &p, bool grad,
+                               int sm_count, int *status, cudaStream_t stream);
+// Joins the partial pairs into lse_out and loss_out.
+cudaError_t launch_linear_loss_join(const LinearLoss &p, cudaStream_t stream);
+// scales[0]: the power of two for float16's g, scales[1]: its inverse.
+cudaError_t launch_linear_loss_scale(const LinearLoss &p, float *scales, cudaStream_t stream);
+// copy (16-byte aligned, ldc a multiple of 8) = the rows of h, with zeros for those that do not count.
+cudaError_t launch_linear_loss_rows(const LinearLoss &p, const void *h, long long ldh, void *copy, long long ldc,
+                                    cudaStream_t stream);
+// dst[r, c] = src[r, c] * (*factor, or 1), rounded to 16 bits; src 16-byte aligned with lds a multiple of 4.
+cudaError_t launch_narrow(const float *src, long long lds, void *dst, long long ldd, int rows, int cols,
+                          const float *factor, int c_dtype, cudaStream_t stream);
+
 } // namespace sm100
 } // namespace hc

@@ -1,0 +1,544 @@
+// Softmax cross entropy of a linear layer over a vocabulary, without the matrix of its logits.
+//
+//   l = H W^T            (H: rows x width, W: vocab x width, float32 accumulation)
+//   lse_r = log sum_v exp(l[r, v]),   loss_r = lse_r - l[r, target_r]
+//   g[r, v] = dloss_r (exp(l[r, v] - lse_r) - [v == target_r]),   dH = g W,   dW = g^T H
+//
+// Forward: the product's tiles never leave the SM. A pair of CTAs computes a 256 x 256 tile of l as the
+// dense kernel does (TMA ring, tcgen05.mma.cta_group::2, two accumulators in tensor memory); its epilogue,
+// in which a lane holds a row, keeps the running maximum and the sum of exponentials of the row over the
+// columns of the tile, and writes those two numbers per row and half tile instead of 256 logits. The tile
+// that holds a row's target also writes that logit. A second kernel joins the partial pairs of each row.
+//
+// Gradient: the logits are computed again with the same kernel, whose epilogue now turns them into g,
+// rounded to the operands' type, for one piece of the vocabulary at a time -- stored both as it stands and
+// transposed, so that both products with it, dH += g W_piece and dW_piece = g^T H, read it along their
+// inner dimension. Those products are the dense kernels' (lib/CAPI/Cuda.cpp enqueues them).
+//
+// Bound: the tensor pipe, 2 rows vocab width operations forward and 8 for forward and gradient (6 if the
+// logits were kept). The exponentials, one per logit, run in the epilogue warps under the next tile's
+// products: 65536 of them per tile and pair take 2048 cycles of the two SMs' special function units
+// against 8 width cycles of products.
+//
+// float16: g = p - 1 or p times dloss, and with a mean over many rows it would fall below the type's
+// normal range. The rows' factors are therefore multiplied by a power of two that brings the largest of
+// |dloss| to 2^14 (found on the device), and the products are divided by it in float32 before they are
+// rounded. bfloat16 has the range of float32 and takes the factors as they are.
+#include "gemm_epilogue.cuh"
+#include "device_checks.cuh"
+#include "gemm_launch.h"
+#include "sm100_ptx.cuh"
+
+#include <cfloat>
+
+namespace hc {
+namespace sm100 {
+
+namespace loss {
+
+constexpr int kTileM = 256;  // rows of H per pair, 128 per CTA
+constexpr int kTileN = 256;  // rows of W per pair, 128 loaded by each CTA
+constexpr int kCtaRows = 128;
+constexpr int kBlockK = 128;  // of the width per ring stage: two 64-wide boxes per operand
+constexpr int kUmmaK = 16;
+constexpr int kStages = 3;
+constexpr int kEpilogueWarps = 8;  // two per quarter of the tensor-memory lanes, half of the columns each
+constexpr int kThreads = 64 + 32 * kEpilogueWarps;
+constexpr int kTmemColumns = 512;  // two accumulators
+constexpr int kColumnsPerWarp = kTileN / 2;
+constexpr uint32_t kBoxBytes = kCtaRows * 64 * 2;
+constexpr uint32_t kOperandBytes = 2 * kBoxBytes;
+constexpr uint32_t kStageBytes = 2 * kOperandBytes;  // per CTA
+constexpr uint32_t kBarrierBytes = 256;
+constexpr uint32_t kSmemBytes = kStages * kStageBytes + kBarrierBytes + 1024;
+static_assert(kSmemBytes <= 227 * 1024, "dynamic shared memory of one CTA");
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ long long target_of(const LinearLoss &p, long long row) {
+  return p.targets_64 ? static_cast<const long long *>(p.targets)[row] : static_cast<const int *>(p.targets)[row];
+}
+
+// Walks the tiles down the rows of H within groups of `group_n` tile columns (see gemm_dense_pair_kernel).
+__device__ __forceinline__ int2 tile_of(int tile, int tiles_m, int tiles_n, int group_n) {
+  const int per_group = group_n * tiles_m;
+  const int group = tile / per_group, first_n = group * group_n;
+  const int width = min(group_n, tiles_n - first_n), inside = tile - group * per_group;
+  return make_int2(inside / width, first_n + inside % width);
+}
+
+// ---------------------------------------------------------------- epilogues ---------
+
+// Running maximum (times log2 e) and sum of exponentials of one row.
+struct Running {
+  float top;  // max l * log2(e), -inf before the first finite value
+  float sum;  // sum exp2(l * log2(e) - top)
+};
+
+// 32 logits of this lane's row, the first at column `col0` of `vocab`.
+__device__ __forceinline__ void take_chunk(const uint32_t (&r)[32], int col0, int vocab, Running &run) {
+  float top = -INFINITY;
+  if (col0 + 32 <= vocab) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      top = fmaxf(top, __uint_as_float(r[j]));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (col0 + j < vocab)
+        top = fmaxf(top, __uint_as_float(r[j]));
+  }
+  top = fmaxf(run.top, top * kLog2e);
+  const float base = top == -INFINITY ? 0.0f : top;  // nothing finite yet: exp2(-inf - 0) = 0
+  float sum = run.sum * exp2_fast(run.top - base);
+  float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    const float e = exp2_fast(fmaf(__uint_as_float(r[j]), kLog2e, -base));
+    part[j & 3] += (col0 + 32 <= vocab || col0 + j < vocab) ? e : 0.0f;
+  }
+  run.top = top;
+  run.sum = sum + ((part[0] + part[1]) + (part[2] + part[3]));
+}
+
+// The logit of a row's target, if it is among these 32.
+__device__ __forceinline__ void take_target(const uint32_t (&r)[32], int offset, float *out) {
+  if (static_cast<unsigned>(offset) < 32u) {
+    float v = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      v = j == offset ? __uint_as_float(r[j]) : v;
+    *out = v;
+  }
+}
+
+template <bool kGrad>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+linear_loss_kernel(const __grid_constant__ CUtensorMap tmap_h, const __grid_constant__ CUtensorMap tmap_w,
+                   const LinearLoss p, uint32_t idesc, int tiles_m, int tiles_n, int group_n, int *status) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  const uint32_t smem_base = (raw_addr + 1023u) & ~1023u;
+  uint8_t *smem_gen = smem_raw + (smem_base - raw_addr);
+  const uint32_t bar_base = smem_base + kStages * kStageBytes;
+  auto full_bar = [&](uint32_t s) { return bar_base + 8u * s; };
+  auto empty_bar = [&](uint32_t s) { return bar_base + 8u * (kStages + s); };
+  auto tmem_full_bar = [&](uint32_t a) { return bar_base + 8u * (2 * kStages + a); };
+  auto tmem_empty_bar = [&](uint32_t a) { return bar_base + 8u * (2 * kStages + 2 + a); };
+  const uint32_t misc_off = (bar_base - smem_base) + 8u * (2 * kStages + 4);
+  volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(smem_gen + misc_off);
+  volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(smem_gen + misc_off + 4);
+
+  const int warp = static_cast<int>(threadIdx.x >> 5), lane = static_cast<int>(threadIdx.x & 31);
+  const uint32_t cta_rank = cluster_cta_rank();  // 0: issues the MMAs, 1: partner
+
+  if (threadIdx.x == 0) {
+    for (uint32_t s = 0; s < kStages; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    for (uint32_t a = 0; a < 2; ++a) {
+      mbar_init(tmem_full_bar(a), 1);
+      mbar_init(tmem_empty_bar(a), 2 * kEpilogueWarps);
+    }
+    *abort_flag = 0;
+    mbar_fence_init();
+    tma_prefetch_descriptor(&tmap_h);
+    tma_prefetch_descriptor(&tmap_w);
+  }
+  cluster_sync_all();  // both CTAs' barriers exist before either signals across the pair
+  if (warp == 1) {
+    tmem_alloc_pair(smem_u32(const_cast<uint32_t *>(tmem_slot)), kTmemColumns);
+    tmem_relinquish_alloc_permit_pair();
+  }
+  tcgen05_fence_before_sync();
+  __syncthreads();
+  tcgen05_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+
+  const int num_tiles = tiles_m * tiles_n;
+  const int num_kb = (p.width + kBlockK - 1) / kBlockK;
+  const int first_tile = static_cast<int>(blockIdx.x >> 1), tile_step = static_cast<int>(gridDim.x >> 1);
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer ------
+    if (lane == 0) {
+      // The tile columns of a group are read again by every tile row: keep W, let H pass (as measured
+      // for the dense kernel).
+      const uint64_t pol_h = l2_policy_evict_normal(), pol_w = l2_policy_evict_last();
+      uint32_t stage = 0, phase = 0;
+      bool ok = true;
+      for (int tile = first_tile; ok && tile < num_tiles; tile += tile_step) {
+        const int2 at = tile_of(tile, tiles_m, tiles_n, group_n);
+        const int m0 = at.x * kTileM + static_cast<int>(cta_rank) * kCtaRows;
+        const int n0 = at.y * kTileN + static_cast<int>(cta_rank) * kCtaRows;
+        if (!HC_CHECK(status, abort_flag, HC_CHECK_TILE_COORDINATES,
+                      at.x >= 0 && at.x < tiles_m && at.y >= 0 && at.y < tiles_n))
+          break;
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag)) {
+            ok = false;
+            break;
+          }
+          const uint32_t h_dst = smem_base + stage * kStageBytes, w_dst = h_dst + kOperandBytes;
+          const uint32_t leader_full = map_to_cta(full_bar(stage), 0);
+          if (cta_rank == 0)
+            mbar_arrive_expect_tx(full_bar(stage), 2 * kStageBytes);
+#pragma unroll
+          for (int sub = 0; sub < kBlockK / 64; ++sub) {
+            const int k0 = kb * kBlockK + sub * 64;  // (past the width: zeros)
+            tma_load_2d_pair_hint(h_dst + sub * kBoxBytes, &tmap_h, leader_full, k0, m0, pol_h);
+            tma_load_2d_pair_hint(w_dst + sub * kBoxBytes, &tmap_w, leader_full, k0, n0, pol_w);
+          }
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer (CTA 0) -
+    if (lane == 0 && cta_rank == 0) {
+      uint32_t stage = 0, phase = 0, iter = 0;
+      bool ok = true;
+      for (int tile = first_tile; ok && tile < num_tiles; tile += tile_step, ++iter) {
+        const uint32_t acc = iter & 1u;
+        if (!mbar_wait(tmem_empty_bar(acc), ((iter >> 1) & 1u) ^ 1u, abort_flag))
+          break;
+        tcgen05_fence_after_sync();
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!mbar_wait(full_bar(stage), phase, abort_flag)) {
+            ok = false;
+            break;
+          }
+          tcgen05_fence_after_sync();
+          const uint32_t h_addr = smem_base + stage * kStageBytes, w_addr = h_addr + kOperandBytes;
+#pragma unroll
+          for (int kk = 0; kk < kBlockK / kUmmaK; ++kk) {
+            const uint64_t advance = static_cast<uint64_t>((kk % 4) * 2);  // 32 bytes inside the swizzle row
+            umma_ss_pair<false>(tmem_base + acc * kTileN,
+                                make_smem_desc_sw128(h_addr + (kk / 4) * kBoxBytes, 16, 1024) + advance,
+                                make_smem_desc_sw128(w_addr + (kk / 4) * kBoxBytes, 16, 1024) + advance, idesc,
+                                (kb != 0 || kk != 0) ? 1u : 0u);
+          }
+          umma_commit_pair(map_to_cta(empty_bar(stage), 0));
+          umma_commit_pair(map_to_cta(empty_bar(stage), 1));
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (ok) {
+          umma_commit_pair(map_to_cta(tmem_full_bar(acc), 0));
+          umma_commit_pair(map_to_cta(tmem_full_bar(acc), 1));
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue ----------
+    const int quarter = warp & 3, part = (warp - 2) >> 2;
+    uint32_t iter = 0;
+    for (int tile = first_tile; tile < num_tiles; tile += tile_step, ++iter) {
+      const int2 at = tile_of(tile, tiles_m, tiles_n, group_n);
+      const uint32_t acc = iter & 1u;
+      const int row = at.x * kTileM + static_cast<int>(cta_rank) * kCtaRows + quarter * 32 + lane;
+      const int col_base = at.y * kTileN + part * kColumnsPerWarp;
+      const bool live = row < p.rows;
+      // What the row needs is fetched while its products are still running.
+      long long target = -1;
+      float scale = 0.0f, lse2 = 0.0f;
+      if (live) {
+        target = target_of(p, row);
+        if (kGrad) {
+          // A row that does not count has no gradient, whatever its dloss and lse hold.
+          const bool counts = target != p.ignore_index && target >= 0 && target < p.vocab_total;
+          scale = counts ? p.dloss[row] * (p.scale != nullptr ? *p.scale : 1.0f) : 0.0f;
+          lse2 = counts ? p.lse[row] * kLog2e : INFINITY;
+        }
+        target = target == p.ignore_index ? -1 : target - p.first_column;
+      }
+      const int target_col =
+          target >= 0 && target < p.vocab ? static_cast<int>(target) - col_base : -1;  // within this warp's columns
+      const bool ready = mbar_wait(tmem_full_bar(acc), (iter >> 1) & 1u, abort_flag);
+      if (!__all_sync(0xffffffffu, ready))
+        break;
+      tcgen05_fence_after_sync();
+      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * kTileN + part * kColumnsPerWarp;
+      uint32_t ra[32], rb[32];
+      Running run{-INFINITY, 0.0f};
+
+      auto finish = [&](uint32_t (&r)[32], int chunk) {
+        const int col0 = col_base + chunk * 32;
+        if (col0 >= p.vocab)
+          return;  // the same for the whole warp
+        if constexpr (!kGrad) {
+          take_chunk(r, col0, p.vocab, run);
+          take_target(r, live ? target_col - chunk * 32 : -1, p.target_logit + row);
+        } else {
+          // g, rounded to the operands' type; two neighbouring columns per word.
+          uint32_t w[16];
+          const int hit = target_col - chunk * 32;
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            float a = exp2_fast(fmaf(__uint_as_float(r[j]), kLog2e, -lse2));
+            float b = exp2_fast(fmaf(__uint_as_float(r[j + 1]), kLog2e, -lse2));
+            a = (j == hit ? a - 1.0f : a) * scale;
+            b = (j + 1 == hit ? b - 1.0f : b) * scale;
+            w[j / 2] = pack_pair(a, b, p.c_dtype);
+          }
+          if (scale == 0.0f) {  // exactly nothing, also where the logits are not finite
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              w[j] = 0u;
+          }
+          // Transposed: 32 lanes write 32 neighbouring rows of a column.
+          if (live && p.gt != nullptr) {
+            uint16_t *gt = static_cast<uint16_t *>(p.gt) + static_cast<long long>(col0) * p.ldgt + row;
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (col0 + j < p.vocab)
+                gt[static_cast<long long>(j) * p.ldgt] = static_cast<uint16_t>(w[j / 2] >> (16 * (j & 1)));
+          }
+          // As it stands: a lane writes 64 bytes of its row (the pitch holds whole chunks of 32 columns).
+          if (live && p.g != nullptr) {
+            uint4 *g = reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.g) + static_cast<long long>(row) * p.ldg + col0);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              g[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+          }
+        }
+      };
+
+      tmem_load_32x32b_x32(taddr, ra);
+#pragma unroll 1
+      for (int chunk = 0; chunk < kColumnsPerWarp / 32; chunk += 2) {
+        tmem_load_wait_for(ra);
+        tmem_load_32x32b_x32(taddr + (chunk + 1) * 32, rb);
+        finish(ra, chunk);
+        tmem_load_wait_for(rb);
+        if (chunk + 2 < kColumnsPerWarp / 32) {
+          tmem_load_32x32b_x32(taddr + (chunk + 2) * 32, ra);
+        } else {  // the accumulator has been read: back to the MMA issuer
+          tcgen05_fence_before_sync();
+          __syncwarp();
+          if (lane == 0)
+            mbar_arrive_cluster(map_to_cta(tmem_empty_bar(acc), 0));
+        }
+        finish(rb, chunk + 1);
+      }
+      if (!kGrad && live)
+        p.partials[static_cast<long long>(at.y * 2 + part) * p.rows + row] = make_float2(run.top, run.sum);
+    }
+  }
+
+  // Neither CTA leaves (or frees tensor memory) while its partner can still use it.
+  tcgen05_fence_before_sync();
+  __syncthreads();
+  if (*abort_flag != 0) {
+    if (threadIdx.x == 0)
+      atomicCAS(status, 0, kStatusDeviceWaitTimeout);
+    const long long start = clock64();
+    while (clock64() - start < 2000000LL) {
+    }
+  }
+  cluster_sync_all();
+  tcgen05_fence_after_sync();
+  if (warp == 1)
+    tmem_dealloc_pair(tmem_base, kTmemColumns);
+}
+
+// Joins the partial pairs of each row: 32 rows per CTA (a lane each), eight warps that share the parts.
+constexpr int kJoinWarps = 8;
+
+__global__ void __launch_bounds__(32 * kJoinWarps)
+join_kernel(const LinearLoss p, int parts) {
+  __shared__ float2 shared[kJoinWarps][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int row = static_cast<int>(blockIdx.x) * 32 + lane;
+  Running run{-INFINITY, 0.0f};
+  bool poisoned = false;
+  auto add = [&](float2 v) {
+    if (v.y == 0.0f)
+      return;  // no value above -inf in that part
+    poisoned |= v.y != v.y;
+    const float top = fmaxf(run.top, v.x);
+    run.sum = run.sum * exp2_fast(run.top - top) + v.y * exp2_fast(v.x - top);
+    run.top = top;
+  };
+  if (row < p.rows)
+    for (int k = warp; k < parts; k += kJoinWarps)
+      add(p.partials[static_cast<long long>(k) * p.rows + row]);
+  shared[warp][lane] = make_float2(run.top, poisoned ? NAN : run.sum);
+  __syncthreads();
+  if (warp != 0 || row >= p.rows)
+    return;
+  run = Running{-INFINITY, 0.0f};
+  poisoned = false;
+  for (int k = 0; k < kJoinWarps; ++k)
+    add(shared[k][lane]);
+  const float lse = poisoned ? NAN : run.sum == 0.0f ? -INFINITY : run.top * kLn2 + logf(run.sum);
+  const long long target = target_of(p, row);
+  p.lse_out[row] = lse;
+  p.loss_out[row] = target == p.ignore_index                   ? 0.0f
+                    : (target < 0 || target >= p.vocab_total) ? NAN
+                                                              : lse - p.target_logit[row];
+}
+
+// float16: the power of two that brings the largest |dloss| of the rows that count to 2^14, and its inverse.
+__global__ void __launch_bounds__(1024)
+scale_kernel(const LinearLoss p, float *scales) {
+  __shared__ float shared[32];
+  float top = 0.0f;
+  for (int row = threadIdx.x; row < p.rows; row += 1024) {
+    const long long target = target_of(p, row);
+    const float d = fabsf(p.dloss[row]);
+    if (target != p.ignore_index && target >= 0 && target < p.vocab_total && d < INFINITY)
+      top = fmaxf(top, d);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if ((threadIdx.x & 31) == 0)
+    shared[threadIdx.x >> 5] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int k = 1; k < 32; ++k)
+      top = fmaxf(top, shared[k]);
+    int e = 0;
+    if (top > 0.0f) {
+      frexpf(top, &e);               // top = f 2^e, f in [1/2, 1)
+      e = max(-100, min(100, 14 - e));  // the factor and its inverse stay normal numbers
+    }
+    scales[0] = ldexpf(1.0f, e);
+    scales[1] = ldexpf(1.0f, -e);
+  }
+}
+
+// The rows of H with zeros in place of those that do not count: their g is zero, but the product g^T H
+// would still make a NaN of a zero times an infinity or a NaN that such a row (padding, say) may hold.
+template <typename Word>
+__global__ void __launch_bounds__(256)
+counting_rows_kernel(const LinearLoss p, const uint16_t *src, long long lds, uint16_t *dst, long long ldd) {
+  constexpr int kPer = sizeof(Word) / 2;
+  const int words = (p.width + kPer - 1) / kPer;
+  for (int row = blockIdx.y; row < p.rows; row += gridDim.y) {
+    const long long target = target_of(p, row);
+    const bool counts = target != p.ignore_index && target >= 0 && target < p.vocab_total;
+    for (int i = blockIdx.x * 256 + threadIdx.x; i < words; i += gridDim.x * 256) {
+      const uint16_t *s = src + static_cast<long long>(row) * lds + i * kPer;
+      uint16_t *d = dst + static_cast<long long>(row) * ldd + i * kPer;
+      if (i * kPer + kPer <= p.width) {
+        *reinterpret_cast<Word *>(d) = counts ? *reinterpret_cast<const Word *>(s) : Word{};
+      } else {
+        for (int e = 0; e < p.width - i * kPer; ++e)
+          d[e] = counts ? s[e] : uint16_t{0};
+      }
+    }
+  }
+}
+
+// dst = src * factor rounded to 16 bits, for a matrix of rows x cols.
+template <typename Pair>
+__global__ void __launch_bounds__(256)
+narrow_kernel(const float *src, long long lds, void *dst, long long ldd, int rows, int cols, const float *factor, int c_dtype) {
+  const float f = factor != nullptr ? *factor : 1.0f;
+  for (int row = blockIdx.y; row < rows; row += gridDim.y) {
+    const float *s = src + static_cast<long long>(row) * lds;
+    uint16_t *d = static_cast<uint16_t *>(dst) + static_cast<long long>(row) * ldd;
+    const int c = (blockIdx.x * 256 + threadIdx.x) * 4;
+    if (c >= cols)
+      continue;
+    const float4 v = *reinterpret_cast<const float4 *>(s + c);  // (lds is a multiple of 4)
+    if (sizeof(Pair) == 8 && c + 4 <= cols) {
+      *reinterpret_cast<uint2 *>(d + c) = make_uint2(pack_pair(v.x * f, v.y * f, c_dtype), pack_pair(v.z * f, v.w * f, c_dtype));
+    } else {
+      const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (c + i < cols)
+          d[c + i] = round_to_16(e[i] * f, c_dtype);
+    }
+  }
+}
+
+}  // namespace loss
+
+int linear_loss_parts(int vocab) { return 2 * ((vocab + loss::kTileN - 1) / loss::kTileN); }
+
+cudaError_t launch_linear_loss(const CUtensorMap &tmap_h, const CUtensorMap &tmap_w, const LinearLoss &p, bool grad,
+                               int sm_count, int *status, cudaStream_t stream) {
+  using namespace loss;
+  static thread_local int configured_device = -1;
+  int device = 0;
+  cudaError_t err = cudaGetDevice(&device);
+  if (err != cudaSuccess)
+    return err;
+  if (configured_device != device) {
+    err = cudaFuncSetAttribute(linear_loss_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    if (err == cudaSuccess)
+      err = cudaFuncSetAttribute(linear_loss_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    if (err != cudaSuccess)
+      return err;
+    configured_device = device;
+  }
+  const int tiles_m = (p.rows + kTileM - 1) / kTileM, tiles_n = (p.vocab + kTileN - 1) / kTileN;
+  const long long tiles = static_cast<long long>(tiles_m) * tiles_n;
+  if (tiles <= 0 || tiles > 0x3fffffffLL)
+    return cudaErrorInvalidValue;
+  const long long clusters = tiles < sm_count / 2 ? tiles : sm_count / 2;
+  const uint32_t idesc = make_idesc_f16(p.c_dtype == kCTypeBF16 ? 1u : 0u, false, false, kTileM, kTileN);
+  const unsigned grid = static_cast<unsigned>(2 * clusters);
+  if (grad)
+    linear_loss_kernel<true><<<grid, kThreads, kSmemBytes, stream>>>(tmap_h, tmap_w, p, idesc, tiles_m, tiles_n, 8, status);
+  else
+    linear_loss_kernel<false><<<grid, kThreads, kSmemBytes, stream>>>(tmap_h, tmap_w, p, idesc, tiles_m, tiles_n, 8, status);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_linear_loss_join(const LinearLoss &p, cudaStream_t stream) {
+  loss::join_kernel<<<(p.rows + 31) / 32, 32 * loss::kJoinWarps, 0, stream>>>(p, linear_loss_parts(p.vocab));
+  return cudaGetLastError();
+}
+
+cudaError_t launch_linear_loss_scale(const LinearLoss &p, float *scales, cudaStream_t stream) {
+  loss::scale_kernel<<<1, 1024, 0, stream>>>(p, scales);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_linear_loss_rows(const LinearLoss &p, const void *h, long long ldh, void *copy, long long ldc,
+                                    cudaStream_t stream) {
+  const bool wide = (reinterpret_cast<uintptr_t>(h) & 15) == 0 && (ldh & 7) == 0;
+  const int words = wide ? (p.width + 7) / 8 : p.width;
+  const dim3 grid(static_cast<unsigned>(words < 4096 ? (words + 255) / 256 : 16),
+                  static_cast<unsigned>(p.rows < 65535 ? p.rows : 65535));
+  const uint16_t *src = static_cast<const uint16_t *>(h);
+  uint16_t *dst = static_cast<uint16_t *>(copy);
+  if (wide)
+    loss::counting_rows_kernel<uint4><<<grid, 256, 0, stream>>>(p, src, ldh, dst, ldc);
+  else
+    loss::counting_rows_kernel<uint16_t><<<grid, 256, 0, stream>>>(p, src, ldh, dst, ldc);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_narrow(const float *src, long long lds, void *dst, long long ldd, int rows, int cols,
+                          const float *factor, int c_dtype, cudaStream_t stream) {
+  if (rows == 0 || cols == 0)
+    return cudaSuccess;
+  const dim3 grid(static_cast<unsigned>((cols + 1023) / 1024), static_cast<unsigned>(rows < 65535 ? rows : 65535));
+  if ((ldd & 3) == 0 && (reinterpret_cast<uintptr_t>(dst) & 7) == 0)
+    loss::narrow_kernel<uint2><<<grid, 256, 0, stream>>>(src, lds, dst, ldd, rows, cols, factor, c_dtype);
+  else
+    loss::narrow_kernel<uint16_t><<<grid, 256, 0, stream>>>(src, lds, dst, ldd, rows, cols, factor, c_dtype);
+  return cudaGetLastError();
+}
+
+}  // namespace sm100
+}  // namespace hc

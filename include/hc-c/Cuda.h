@@ -485,6 +485,70 @@ HC_CUDA_CAPI_EXPORTED int hcCudaLayerNormBackward(HcCudaContext *ctx, const HcCu
 HC_CUDA_CAPI_EXPORTED int hcCudaLayerNormBackwardPlan(const HcCudaLayerNormBackwardArgs *args, int sm_count,
                                                       HcCudaOperatorPlanInfo *out);
 
+/* ---- softmax cross entropy of a linear layer over a vocabulary ----------------------------- */
+
+/* With the logits l = H W^T (H: rows x width, W: vocab x width, row-major, float16 or bfloat16; products
+ * accumulated in float32):
+ *   lse_r = log(sum_v exp(l[r, v])),   loss_r = lse_r - l[r, targets[r]]
+ * A row whose target is `ignore_index` has loss 0 (its lse is still stored). Any other target outside
+ * [0, vocab) has loss NaN and no gradient. The logits are never stored: each tile of them is reduced to
+ * two numbers per row where it is computed. Matrices aligned to their element size; a base or pitch
+ * that is not a multiple of 16 bytes costs a repack through context scratch. vocab and width at least 1;
+ * rows == 0 writes nothing. No counterpart in the reference; the operator stands beside hcCudaGemm. */
+typedef struct HcCudaLinearLossArgs {
+  int64_t rows, vocab, width;
+  int32_t dtype;      /* HC_CUDA_F16 or HC_CUDA_BF16, of h and w */
+  int32_t targets_64; /* 1: targets are int64; 0: int32 */
+  const void *h;
+  int64_t ldh;
+  const void *w;
+  int64_t ldw;
+  const void *targets;
+  int64_t ignore_index;
+  float *loss; /* rows floats */
+  float *lse;  /* rows floats */
+} HcCudaLinearLossArgs;
+
+/* Asynchronous; device pointers on the context's device. */
+HC_CUDA_CAPI_EXPORTED int hcCudaLinearLoss(HcCudaContext *ctx, const HcCudaLinearLossArgs *args);
+/* The same validation, and what would run, without a device. */
+HC_CUDA_CAPI_EXPORTED int hcCudaLinearLossPlan(const HcCudaLinearLossArgs *args, int sm_count,
+                                               HcCudaOperatorPlanInfo *out);
+
+/* The gradients of sum_r(loss_r * dloss_r): with g[r, v] = dloss_r * (exp(l[r, v] - lse_r) - [v == targets[r]])
+ * and rows that do not count (ignored, or a target outside the vocabulary) left out whatever they and their
+ * dloss hold,
+ *   dh = g W,   dw = g^T H
+ * both overwritten, in the type of h and w, each optional (NULL). lse is what hcCudaLinearLoss stored. The
+ * logits are computed again, one piece of the vocabulary at a time; g is rounded to the operands' type for
+ * the two products, whose sums are float32. For float16 a power of two found on the device keeps g inside
+ * the type's normal range. A call gives the same bits every time. rows == 0 sets dw to zero. Uses context
+ * scratch: a copy of h (for dw), g and its transpose for one piece of the vocabulary (together 512 MiB at
+ * most, or 1 KiB per row where that is more), and float32 sums of dh when there is more than one piece. */
+typedef struct HcCudaLinearLossBackwardArgs {
+  int64_t rows, vocab, width;
+  int32_t dtype;
+  int32_t targets_64;
+  const void *h;
+  int64_t ldh;
+  const void *w;
+  int64_t ldw;
+  const void *targets;
+  int64_t ignore_index;
+  const float *lse;
+  const float *dloss; /* rows floats */
+  void *dh;           /* rows x width, or NULL */
+  int64_t lddh;
+  void *dw;           /* vocab x width, or NULL */
+  int64_t lddw;
+} HcCudaLinearLossBackwardArgs;
+
+/* Asynchronous; device pointers on the context's device. */
+HC_CUDA_CAPI_EXPORTED int hcCudaLinearLossBackward(HcCudaContext *ctx, const HcCudaLinearLossBackwardArgs *args);
+/* The same validation, and what would run, without a device. */
+HC_CUDA_CAPI_EXPORTED int hcCudaLinearLossBackwardPlan(const HcCudaLinearLossBackwardArgs *args, int sm_count,
+                                                       HcCudaOperatorPlanInfo *out);
+
 /* ---- the product fused with its gather (N-sharded GEMM, one process per GPU) ------------- */
 
 #define HC_CUDA_MAX_PUSH_TARGETS 7
