@@ -39,6 +39,8 @@ SOURCES = [
     LIB_DIR / "Kernels" / "row_reduce_sm100a.cu",
     LIB_DIR / "Kernels" / "layer_norm_sm100a.cu",
     LIB_DIR / "Kernels" / "linear_loss_sm100a.cu",
+    LIB_DIR / "Kernels" / "gemm_w4_f16_sm100a.cu",
+    LIB_DIR / "Kernels" / "gemm_w4_bf16_sm100a.cu",
     LIB_DIR / "Kernels" / "gemm_skinny_static_sm100a.cu",
     LIB_DIR / "Kernels" / "selftest_sm100a.cu",
     LIB_DIR / "CAPI" / "Cuda.cpp",
@@ -47,6 +49,7 @@ HEADERS = [
     LIB_DIR / "Kernels" / "gemm_launch.h",
     LIB_DIR / "Kernels" / "sm100_ptx.cuh",
     LIB_DIR / "Kernels" / "gemm_epilogue.cuh",
+    LIB_DIR / "Kernels" / "gemm_w4.cuh",
     LIB_DIR / "Kernels" / "device_checks.cuh",
     REPO_ROOT / "include" / "hc-c" / "Cuda.h",
 ]

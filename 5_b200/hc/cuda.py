@@ -60,6 +60,7 @@ EXPORTS = (
     "hcCudaGemmHostDeviceA", "hcCudaPairwise", "hcCudaPairwiseHost", "hcCudaRowSum", "hcCudaRowSumHost", "hcCudaBuildFlags", "hcCudaSelfTestDeviceCheck",
     "hcCudaLayerNorm", "hcCudaLayerNormPlan", "hcCudaLayerNormBackward", "hcCudaLayerNormBackwardPlan",
     "hcCudaLinearLoss", "hcCudaLinearLossPlan", "hcCudaLinearLossBackward", "hcCudaLinearLossBackwardPlan",
+    "hcCudaGemmW4", "hcCudaGemmW4Plan",
 )
 
 
@@ -168,6 +169,15 @@ class _LinearLossBackwardArgs(ctypes.Structure):
                 ("lddh", ctypes.c_int64), ("dw", ctypes.c_void_p), ("lddw", ctypes.c_int64)]
 
 
+class _GemmW4Args(ctypes.Structure):
+    _fields_ = [
+        ("m", ctypes.c_int64), ("n", ctypes.c_int64), ("k", ctypes.c_int64), ("dtype", ctypes.c_int32),
+        ("c_dtype", ctypes.c_int32), ("a", ctypes.c_void_p), ("lda", ctypes.c_int64), ("q", ctypes.c_void_p),
+        ("ldq", ctypes.c_int64), ("scales", ctypes.c_void_p), ("lds", ctypes.c_int64), ("zeros", ctypes.c_void_p),
+        ("ldz", ctypes.c_int64), ("group", ctypes.c_int64), ("c", ctypes.c_void_p), ("ldc", ctypes.c_int64),
+    ]
+
+
 class _OperatorPlanInfo(ctypes.Structure):
     _fields_ = [("kernel_launches", ctypes.c_int32), ("pieces", ctypes.c_int32), ("scratch_bytes", ctypes.c_int64)]
 
@@ -257,7 +267,9 @@ def library() -> ctypes.CDLL:
         lib.hcCudaLayerNormBackward.argtypes = [vp, ctypes.POINTER(_LayerNormBackwardArgs)]
         lib.hcCudaLinearLoss.argtypes = [vp, ctypes.POINTER(_LinearLossArgs)]
         lib.hcCudaLinearLossBackward.argtypes = [vp, ctypes.POINTER(_LinearLossBackwardArgs)]
+        lib.hcCudaGemmW4.argtypes = [vp, ctypes.POINTER(_GemmW4Args)]
         plan_info = ctypes.POINTER(_OperatorPlanInfo)
+        lib.hcCudaGemmW4Plan.argtypes = [ctypes.POINTER(_GemmW4Args), i, plan_info]
         lib.hcCudaLinearLossPlan.argtypes = [ctypes.POINTER(_LinearLossArgs), i, plan_info]
         lib.hcCudaLinearLossBackwardPlan.argtypes = [ctypes.POINTER(_LinearLossBackwardArgs), i, plan_info]
         lib.hcCudaLayerNormPlan.argtypes = [ctypes.POINTER(_LayerNormArgs), i, plan_info]
@@ -695,6 +707,30 @@ class Context:
                              f"{h.dtype.name} and {w.shape} of {w.dtype.name}")
         return (h.shape[0], w.shape[0], h.shape[1], dtype_code(h.dtype), int(targets.dtype == np.int64), h.ptr, h.ld, w.ptr,
                 w.ld, _vector("targets", targets, h.shape[0], np.int64, np.int32), ignore_index)
+
+    def gemm_w4(self, a: "DeviceBuffer", q: "DeviceBuffer", scales: "DeviceBuffer", c: "DeviceBuffer", *, group: int,
+                zeros: "DeviceBuffer | None" = None) -> None:
+        """Enqueues C = A @ W.T for W[j, k] = scales[j, k // group] * (q[j, k] - zeros[j, k // group])
+        (asynchronous; see `synchronize`). `a`: up to 64 rows (m, k) of float16 or bfloat16; `q`: 4-bit
+        weights, uint8 (n, ceil(k / 2)) with the even k in the low half of a byte; `scales` (n, ceil(k / group))
+        of A's type; `zeros`: uint8 of that shape, values 0..15, or 8 throughout; `group`: 32, 64 or a
+        multiple of 128; `c` (m, n): float32 or A's type. Sums are float32, rounded once."""
+        for name, buf in (("a", a), ("q", q), ("scales", scales), ("c", c), ("zeros", zeros)):
+            if buf is not None and buf.ndim != 2:
+                raise ValueError(f"gemm_w4(): {name} must be a device matrix")
+        (m, k), n = a.shape, q.shape[0]
+        groups = -(-k // group) if group > 0 else 0
+        if q.dtype != np.uint8 or q.shape != (n, (k + 1) // 2) or c.shape != (m, n):
+            raise ValueError(f"gemm_w4(): a {a.shape} and c {c.shape} take q as uint8 of shape (n, {(k + 1) // 2}), got "
+                             f"{q.shape} of {q.dtype.name}")
+        if scales.dtype != a.dtype or (group > 0 and scales.shape != (n, groups)):
+            raise ValueError(f"gemm_w4(): scales must be {a.dtype.name} of shape {(n, groups)}, got {scales.shape} of "
+                             f"{scales.dtype.name}")
+        if zeros is not None and (zeros.dtype != np.uint8 or zeros.shape != scales.shape):
+            raise ValueError("gemm_w4(): zeros must be uint8 with the shape of scales")
+        args = _GemmW4Args(m, n, k, dtype_code(a.dtype), c_dtype_code(c.dtype), a.ptr, a.ld, q.ptr, q.ld, scales.ptr, scales.ld,
+                           None if zeros is None else zeros.ptr, 0 if zeros is None else zeros.ld, group, c.ptr, c.ld)
+        self._check(self._lib.hcCudaGemmW4(self._handle, ctypes.byref(args)))
 
     def gemm_host(self, a: np.ndarray, b: np.ndarray, c: np.ndarray, *,
                   variant: int = VARIANT_AUTO, b_transposed: bool = False, accumulate: bool = False,

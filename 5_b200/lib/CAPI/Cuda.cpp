@@ -2516,6 +2516,140 @@ int hcCudaLinearLossBackward(HcCudaContext *ctx, const HcCudaLinearLossBackwardA
   return HC_CUDA_OK;
 }
 
+namespace {
+
+struct W4Plan {
+  bool repack_a = false;
+  int64_t copy_ld = 0;
+  int64_t partials = 0;  // offset in scratch, behind the copy of A
+  int64_t units = 0;
+  int grid = 0;
+};
+
+int plan_gemm_w4(const HcCudaContext *ctx, const HcCudaGemmW4Args *args, int sm_count, W4Plan *plan,
+                 HcCudaOperatorPlanInfo *info) {
+  if (args == nullptr)
+    return fail(ctx, HC_CUDA_ERR_INVALID_ARGUMENT, "args must not be null");
+  const int64_t m = args->m, n = args->n, k = args->k;
+  if (m < 0 || n < 0 || k < 0)
+    return fail(ctx, HC_CUDA_ERR_INVALID_ARGUMENT, "m, n, k must be non-negative (got %lld, %lld, %lld)", (long long)m,
+                (long long)n, (long long)k);
+  if (m > hc::sm100::w4_max_m() || n > kMaxDim || k > kMaxDim)
+    return fail(ctx, HC_CUDA_ERR_UNSUPPORTED, "4-bit weights take m <= %d, n and k at most 2^30 (got %lld, %lld, %lld)",
+                hc::sm100::w4_max_m(), (long long)m, (long long)n, (long long)k);
+  if (args->dtype != HC_CUDA_F16 && args->dtype != HC_CUDA_BF16)
+    return fail(ctx, HC_CUDA_ERR_INVALID_ARGUMENT, "dtype must be HC_CUDA_F16 or HC_CUDA_BF16 (got %d)", args->dtype);
+  const int own_type = args->dtype == HC_CUDA_BF16 ? HC_CUDA_C_BF16 : HC_CUDA_C_F16;
+  if (args->c_dtype != HC_CUDA_C_F32 && args->c_dtype != own_type)
+    return fail(ctx, HC_CUDA_ERR_INVALID_ARGUMENT, "c_dtype must be float32 or the type of a (got %d)", args->c_dtype);
+  if (args->group != 32 && args->group != 64 && (args->group < 128 || args->group % 128 != 0 || args->group > kMaxDim))
+    return fail(ctx, HC_CUDA_ERR_INVALID_ARGUMENT, "group must be 32, 64 or a multiple of 128 (got %lld)",
+                (long long)args->group);
+  *info = HcCudaOperatorPlanInfo{0, 0, 0};
+  if (m == 0 || n == 0)
+    return HC_CUDA_OK;
+  const Operand c{"c", args->c, m, n, args->ldc, float_bytes(args->c_dtype)};
+  if (int rc = check_operand(ctx, c))
+    return rc;
+  if (k == 0)
+    return HC_CUDA_OK;
+  const int64_t row_bytes = (k + 1) / 2, groups = (k + args->group - 1) / args->group;
+  const Operand a{"a", args->a, m, k, args->lda, 2}, q{"q", args->q, n, row_bytes, args->ldq, 1};
+  const Operand scales{"scales", args->scales, n, groups, args->lds, 2}, zeros{"zeros", args->zeros, n, groups, args->ldz, 1};
+  for (const Operand *o : {&a, &q, &scales, &zeros})
+    if (o != &zeros || o->ptr != nullptr)
+      if (int rc = check_operand(ctx, *o))
+        return rc;
+  for (const Operand *o : {&a, &q, &scales, &zeros})
+    if (int rc = check_apart(ctx, c, *o))
+      return rc;
+  plan->repack_a = needs_repack(args->a, args->lda);
+  plan->copy_ld = round_up(k, kRepackPitchBytes / 2);
+  plan->partials = plan->repack_a ? round_up(m * plan->copy_ld * 2, 1024) : 0;
+  plan->units = hc::sm100::w4_blocks(n) * hc::sm100::w4_stages(k);
+  plan->grid = hc::sm100::w4_grid(plan->units, static_cast<int>(m), sm_count);
+  *info = HcCudaOperatorPlanInfo{
+      plan->repack_a ? 2 : 1, 1,
+      plan->partials + static_cast<int64_t>(hc::sm100::w4_partials_bytes(plan->grid, static_cast<int>(m)))};
+  return HC_CUDA_OK;
+}
+
+} // namespace
+
+int hcCudaGemmW4Plan(const HcCudaGemmW4Args *args, int sm_count, HcCudaOperatorPlanInfo *out) {
+  if (out == nullptr)
+    return fail(nullptr, HC_CUDA_ERR_INVALID_ARGUMENT, "out must not be null");
+  W4Plan plan;
+  return plan_gemm_w4(nullptr, args, sm_count > 0 ? sm_count : kDefaultSmCount, &plan, out);
+}
+
+int hcCudaGemmW4(HcCudaContext *ctx, const HcCudaGemmW4Args *args) {
+  if (ctx == nullptr)
+    return fail(ctx, HC_CUDA_ERR_INVALID_ARGUMENT, "ctx must not be null");
+  std::lock_guard<std::mutex> lock(ctx->mu);
+  W4Plan plan;
+  HcCudaOperatorPlanInfo info;
+  if (int rc = plan_gemm_w4(ctx, args, ctx->prop.multiProcessorCount, &plan, &info))
+    return rc;
+  if (args->m == 0 || args->n == 0)
+    return HC_CUDA_OK;
+  HC_TRY_CUDA(ctx, cudaSetDevice(ctx->device));
+  if (args->k == 0) {
+    const size_t elem = float_bytes(args->c_dtype);
+    HC_TRY_CUDA(ctx, cudaMemset2DAsync(args->c, static_cast<size_t>(args->ldc) * elem, 0, static_cast<size_t>(args->n) * elem,
+                                       static_cast<size_t>(args->m), ctx->stream));
+    return HC_CUDA_OK;
+  }
+  if (int rc = ensure_scratch(ctx, static_cast<size_t>(info.scratch_bytes)))
+    return rc;
+  if (int rc = ensure_counters(ctx, static_cast<size_t>(hc::sm100::w4_blocks(args->n)) * sizeof(unsigned)))
+    return rc;
+  const int m = static_cast<int>(args->m), n = static_cast<int>(args->n), k = static_cast<int>(args->k);
+  const void *a = args->a;
+  int64_t lda = args->lda;
+  if (plan.repack_a) {
+    HC_TRY_CUDA(ctx, hc::sm100::launch_repack_pitch_two(a, lda, ctx->scratch, plan.copy_ld, m, k, nullptr, 0, nullptr, 0, 0, 0,
+                                                        ctx->stream));
+    a = ctx->scratch;
+    lda = plan.copy_ld;
+  }
+  hc::sm100::W4 p{};
+  p.m = m;
+  p.n = n;
+  p.row_bytes = (k + 1) / 2;
+  p.groups = static_cast<int>((args->k + args->group - 1) / args->group);
+  p.group = args->group < 128 ? static_cast<int>(args->group) : 128;
+  p.span = args->group < 128 ? 1 : static_cast<int>(args->group / 128);
+  p.stages_k = static_cast<int>(hc::sm100::w4_stages(k));
+  p.phase = (reinterpret_cast<uintptr_t>(args->q) & 15) != 0 || (args->ldq & 15) != 0 ? 1 : 0;
+  p.grid = plan.grid;
+  p.units = plan.units;
+  p.q = static_cast<const uint8_t *>(args->q);
+  p.ldq = args->ldq;
+  p.scales = static_cast<const uint16_t *>(args->scales);
+  p.lds = args->lds;
+  p.zeros = static_cast<const uint8_t *>(args->zeros);
+  p.ldz = args->ldz;
+  p.c = args->c;
+  p.ldc = args->ldc;
+  p.c_dtype = args->c_dtype;
+  p.partials = reinterpret_cast<float *>(static_cast<char *>(ctx->scratch) + plan.partials);
+  p.counters = ctx->counters;
+  CUtensorMap tmap_a, tmap_q;
+  if (int rc = encode_map(ctx, &tmap_a, args->dtype, a, static_cast<uint64_t>(k), static_cast<uint64_t>(m),
+                          static_cast<uint64_t>(lda) * 2, 64, 8 * static_cast<uint32_t>(hc::sm100::w4_tiles(m))))
+    return rc;
+  if (p.phase)
+    tmap_q = tmap_a;  // not used
+  else if (int rc = encode_map(ctx, &tmap_q, HC_CUDA_F8E4M3, args->q, static_cast<uint64_t>(p.row_bytes), static_cast<uint64_t>(n),
+                               static_cast<uint64_t>(args->ldq), 128, 128))
+    return rc;
+  HC_TRY_CUDA(ctx, args->dtype == HC_CUDA_BF16
+                       ? hc::sm100::launch_gemm_w4_bf16(tmap_q, tmap_a, p, ctx->status_dev, ctx->stream)
+                       : hc::sm100::launch_gemm_w4_f16(tmap_q, tmap_a, p, ctx->status_dev, ctx->stream));
+  return HC_CUDA_OK;
+}
+
 int hcCudaSelfTestDeviceTimeout(HcCudaContext *ctx, int64_t budget_cycles) {
   if (ctx == nullptr)
     return fail(ctx, HC_CUDA_ERR_INVALID_ARGUMENT, "ctx must not be null");

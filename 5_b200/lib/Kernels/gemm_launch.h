@@ -354,5 +354,45 @@ cudaError_t launch_linear_loss_rows(const LinearLoss &p, const void *h, long lon
 cudaError_t launch_narrow(const float *src, long long lds, void *dst, long long ldd, int rows, int cols,
                           const float *factor, int c_dtype, cudaStream_t stream);
 
+// ---- products with 4-bit weights -------------------------------------------------------------------
+struct W4 {
+  int m, n;       // rows of A (1..64), rows of q
+  int row_bytes;  // of q that count: ceil(k / 2)
+  int groups;     // scales per row
+  int group;      // 32, 64 or 128: the kernel's group ...
+  int span;       // ... and how many of them share a scale
+  int stages_k;   // w4_stages(k)
+  int phase;      // q's rows do not all start on 16-byte boundaries: tmap_q is not used
+  int grid;       // CTAs, at most `units`
+  long long units;  // row blocks x stages_k
+  const uint8_t *q;
+  long long ldq;  // bytes
+  const uint16_t *scales;
+  long long lds;
+  const uint8_t *zeros;  // or null: 8
+  long long ldz;
+  void *c;
+  long long ldc;
+  int c_dtype;
+  float *partials;     // w4_partials_bytes
+  unsigned *counters;  // one per row block, zero before and after
+};
+// n-tiles of 8 rows of A a launch is made for: 1, 2, 4 or 8.
+inline int w4_tiles(int m) { return m <= 8 ? 1 : m <= 16 ? 2 : m <= 32 ? 4 : 8; }
+inline int w4_max_m() { return 64; }
+inline long long w4_blocks(long long n) { return (n + 127) / 128; }
+inline long long w4_stages(long long k) { return (k + 255) / 256; }
+inline int w4_grid(long long units, int m, int sm_count) {
+  const long long slots = static_cast<long long>(sm_count) * (w4_tiles(m) <= 2 ? 2 : 1);
+  return static_cast<int>(units < slots ? units : slots);
+}
+inline size_t w4_partials_bytes(int grid, int m) { return static_cast<size_t>(grid) * 2 * 128 * 8 * w4_tiles(m) * 4; }
+// tmap_q: q as bytes {row_bytes inner, n}, box {128, 128}; tmap_a: A as {k inner, m}, box {64, 8 w4_tiles(m)};
+// both 128-byte swizzle.
+cudaError_t launch_gemm_w4_bf16(const CUtensorMap &tmap_q, const CUtensorMap &tmap_a, const W4 &p, int *status,
+                                cudaStream_t stream);
+cudaError_t launch_gemm_w4_f16(const CUtensorMap &tmap_q, const CUtensorMap &tmap_a, const W4 &p, int *status,
+                               cudaStream_t stream);
+
 } // namespace sm100
 } // namespace hc

@@ -549,6 +549,40 @@ HC_CUDA_CAPI_EXPORTED int hcCudaLinearLossBackward(HcCudaContext *ctx, const HcC
 HC_CUDA_CAPI_EXPORTED int hcCudaLinearLossBackwardPlan(const HcCudaLinearLossBackwardArgs *args, int sm_count,
                                                        HcCudaOperatorPlanInfo *out);
 
+/* ---- products with 4-bit weights and group scales ------------------------------------------ */
+
+/* C[i, j] = sum over groups g of scales[j, g] * sum over k in g of (q[j, k] - zeros[j, g]) * A[i, k]
+ * for m <= 64 rows of A (float16 or bfloat16) and n rows of 4-bit weights: q holds two to a byte, the even k
+ * in the low half, rows of ceil(k / 2) bytes at a pitch of ldq bytes; scales, n x ceil(k / group), in A's type;
+ * zeros, n x ceil(k / group) bytes of 0..15 each, or NULL for 8 throughout. group: 32, 64 or a multiple of
+ * 128; the last group of a row may be shorter. Everything is summed in float32 (the weights enter as integers,
+ * the scales multiply the sums of their groups) and rounded once into C: float32, or A's type. The same bits
+ * every call. It is to a matrix of 4-bit weights what the skinny variant of hcCudaGemm is to one of 16 bits:
+ * HBM bound up to about 16 rows. A whose base or pitch is not a multiple of 16 bytes costs a repack launch; q
+ * is read where it stands, fastest when its rows start on 16-byte boundaries. m == 0 or n == 0 writes
+ * nothing; k == 0 sets C to zero. No counterpart in the reference. */
+typedef struct HcCudaGemmW4Args {
+  int64_t m, n, k;
+  int32_t dtype;   /* HC_CUDA_F16 or HC_CUDA_BF16, of A and scales */
+  int32_t c_dtype; /* HC_CUDA_C_F32, or the HcCudaCType of `dtype` */
+  const void *a;
+  int64_t lda;
+  const void *q;
+  int64_t ldq;
+  const void *scales;
+  int64_t lds;
+  const void *zeros; /* or NULL */
+  int64_t ldz;
+  int64_t group;
+  void *c;
+  int64_t ldc;
+} HcCudaGemmW4Args;
+
+/* Asynchronous; device pointers on the context's device. */
+HC_CUDA_CAPI_EXPORTED int hcCudaGemmW4(HcCudaContext *ctx, const HcCudaGemmW4Args *args);
+/* The same validation, and what would run, without a device. */
+HC_CUDA_CAPI_EXPORTED int hcCudaGemmW4Plan(const HcCudaGemmW4Args *args, int sm_count, HcCudaOperatorPlanInfo *out);
+
 /* ---- the product fused with its gather (N-sharded GEMM, one process per GPU) ------------- */
 
 #define HC_CUDA_MAX_PUSH_TARGETS 7
