@@ -98,6 +98,7 @@ struct MapCacheEntry {
   const void *base = nullptr;
   uint64_t inner = 0, outer = 0, pitch_bytes = 0;
   uint32_t box_inner = 0, box_outer = 0;
+  CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B;
   CUtensorMap map;
 };
 
@@ -519,12 +520,13 @@ int ensure_stage(HcCudaContext *ctx, int which, size_t bytes) {
 constexpr int kMapFloat32 = -1;  // encode_map's dtype for C; otherwise an HcCudaDType
 
 int encode_map(HcCudaContext *ctx, CUtensorMap *map, int dtype, const void *base, uint64_t inner,
-               uint64_t outer, uint64_t pitch_bytes, uint32_t box_inner, uint32_t box_outer) {
+               uint64_t outer, uint64_t pitch_bytes, uint32_t box_inner, uint32_t box_outer,
+               CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
   // A tensor map is a pure function of these arguments, and callers launch the same product on
   // the same buffers over and over: keep the last few (the caller holds ctx->mu).
   for (MapCacheEntry &e : ctx->map_cache) {
     if (e.valid && e.base == base && e.inner == inner && e.outer == outer && e.pitch_bytes == pitch_bytes &&
-        e.box_inner == box_inner && e.box_outer == box_outer && e.dtype == dtype) {
+        e.box_inner == box_inner && e.box_outer == box_outer && e.dtype == dtype && e.swizzle == swizzle) {
       *map = e.map;
       return HC_CUDA_OK;
     }
@@ -539,7 +541,7 @@ int encode_map(HcCudaContext *ctx, CUtensorMap *map, int dtype, const void *base
                                                                      : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   const CUresult res = ctx->encode(map, type, 2, const_cast<void *>(base), dims, strides, box,
                                    elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                   swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (res != CUDA_SUCCESS)
     return fail(ctx, HC_CUDA_ERR_CUDA,
@@ -548,7 +550,7 @@ int encode_map(HcCudaContext *ctx, CUtensorMap *map, int dtype, const void *base
                 (unsigned long long)pitch_bytes);
   MapCacheEntry &slot = ctx->map_cache[ctx->map_cache_next];
   ctx->map_cache_next = (ctx->map_cache_next + 1) % kMapCacheEntries;
-  slot = MapCacheEntry{true, dtype, base, inner, outer, pitch_bytes, box_inner, box_outer, *map};
+  slot = MapCacheEntry{true, dtype, base, inner, outer, pitch_bytes, box_inner, box_outer, swizzle, *map};
   return HC_CUDA_OK;
 }
 
@@ -2520,7 +2522,8 @@ namespace {
 
 struct W4Plan {
   bool repack_a = false;
-  int64_t copy_ld = 0;
+  bool phase = false;    // q's rows do not all start on 16-byte boundaries
+  int64_t a_ld = 0;      // pitch of A where the kernel reads it
   int64_t partials = 0;  // offset in scratch, behind the copy of A
   int64_t units = 0;
   int grid = 0;
@@ -2563,10 +2566,15 @@ int plan_gemm_w4(const HcCudaContext *ctx, const HcCudaGemmW4Args *args, int sm_
   for (const Operand *o : {&a, &q, &scales, &zeros})
     if (int rc = check_apart(ctx, c, *o))
       return rc;
-  plan->repack_a = needs_repack(args->a, args->lda);
-  plan->copy_ld = round_up(k, kRepackPitchBytes / 2);
-  plan->partials = plan->repack_a ? round_up(m * plan->copy_ld * 2, 1024) : 0;
+  // (The pitch of a single row does not matter.)
+  const bool one_row = m == 1 && (reinterpret_cast<uintptr_t>(args->a) & 15) == 0;
+  plan->repack_a = !one_row && needs_repack(args->a, args->lda);
+  plan->a_ld = plan->repack_a || one_row ? round_up(k, kRepackPitchBytes / 2) : args->lda;
+  plan->partials = plan->repack_a ? round_up(m * plan->a_ld * 2, 1024) : 0;
   plan->units = hc::sm100::w4_blocks(n) * hc::sm100::w4_stages(k);
+  if (plan->units > 0x3fffffff)
+    return fail(ctx, HC_CUDA_ERR_UNSUPPORTED, "n x k is too large: at most 2^30 blocks of 128 x 256 weights");
+  plan->phase = (reinterpret_cast<uintptr_t>(args->q) & 15) != 0 || (args->ldq & 15) != 0;
   plan->grid = hc::sm100::w4_grid(plan->units, static_cast<int>(m), sm_count);
   *info = HcCudaOperatorPlanInfo{
       plan->repack_a ? 2 : 1, 1,
@@ -2606,12 +2614,10 @@ int hcCudaGemmW4(HcCudaContext *ctx, const HcCudaGemmW4Args *args) {
     return rc;
   const int m = static_cast<int>(args->m), n = static_cast<int>(args->n), k = static_cast<int>(args->k);
   const void *a = args->a;
-  int64_t lda = args->lda;
   if (plan.repack_a) {
-    HC_TRY_CUDA(ctx, hc::sm100::launch_repack_pitch_two(a, lda, ctx->scratch, plan.copy_ld, m, k, nullptr, 0, nullptr, 0, 0, 0,
-                                                        ctx->stream));
+    HC_TRY_CUDA(ctx, hc::sm100::launch_repack_pitch_two(a, args->lda, ctx->scratch, plan.a_ld, m, k, nullptr, 0, nullptr, 0, 0,
+                                                        0, ctx->stream));
     a = ctx->scratch;
-    lda = plan.copy_ld;
   }
   hc::sm100::W4 p{};
   p.m = m;
@@ -2621,23 +2627,33 @@ int hcCudaGemmW4(HcCudaContext *ctx, const HcCudaGemmW4Args *args) {
   p.group = args->group < 128 ? static_cast<int>(args->group) : 128;
   p.span = args->group < 128 ? 1 : static_cast<int>(args->group / 128);
   p.stages_k = static_cast<int>(hc::sm100::w4_stages(k));
-  p.phase = (reinterpret_cast<uintptr_t>(args->q) & 15) != 0 || (args->ldq & 15) != 0 ? 1 : 0;
+  p.phase = plan.phase ? 1 : 0;
   p.grid = plan.grid;
-  p.units = plan.units;
+  p.share = static_cast<int>(plan.units / plan.grid);
+  p.extra = static_cast<int>(plan.units % plan.grid);
   p.q = static_cast<const uint8_t *>(args->q);
   p.ldq = args->ldq;
   p.scales = static_cast<const uint16_t *>(args->scales);
   p.lds = args->lds;
   p.zeros = static_cast<const uint8_t *>(args->zeros);
   p.ldz = args->ldz;
+  const int per_stage = 256 / p.group;  // groups of a stage
+  p.vector_scales = p.span == 1 && p.groups % per_stage == 0 && args->lds % per_stage == 0 &&
+                    (reinterpret_cast<uintptr_t>(args->scales) & (2 * per_stage - 1)) == 0 &&
+                    (args->zeros == nullptr || (args->ldz % per_stage == 0 &&
+                                                (reinterpret_cast<uintptr_t>(args->zeros) & (per_stage - 1)) == 0));
   p.c = args->c;
   p.ldc = args->ldc;
   p.c_dtype = args->c_dtype;
   p.partials = reinterpret_cast<float *>(static_cast<char *>(ctx->scratch) + plan.partials);
   p.counters = ctx->counters;
   CUtensorMap tmap_a, tmap_q;
+  // Up to 16 rows: whole stages of k, as they lie in memory; more: boxes for the tensor cores.
+  const bool few = m <= 16;
   if (int rc = encode_map(ctx, &tmap_a, args->dtype, a, static_cast<uint64_t>(k), static_cast<uint64_t>(m),
-                          static_cast<uint64_t>(lda) * 2, 64, 8 * static_cast<uint32_t>(hc::sm100::w4_tiles(m))))
+                          static_cast<uint64_t>(plan.a_ld) * 2, few ? 256 : 64,
+                          static_cast<uint32_t>(hc::sm100::w4_tokens(m)),
+                          few ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B))
     return rc;
   if (p.phase)
     tmap_q = tmap_a;  // not used

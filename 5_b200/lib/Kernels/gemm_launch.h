@@ -363,32 +363,36 @@ struct W4 {
   int span;       // ... and how many of them share a scale
   int stages_k;   // w4_stages(k)
   int phase;      // q's rows do not all start on 16-byte boundaries: tmap_q is not used
-  int grid;       // CTAs, at most `units`
-  long long units;  // row blocks x stages_k
+  int grid;       // CTAs, at most as many as there are (row block, stage of k) units
+  int share;      // units of a CTA; the first `extra` CTAs have one more
+  int extra;
   const uint8_t *q;
   long long ldq;  // bytes
   const uint16_t *scales;
   long long lds;
   const uint8_t *zeros;  // or null: 8
   long long ldz;
+  int vector_scales;  // a stage's scales (and zero points) of a row can be read with one access each
   void *c;
   long long ldc;
   int c_dtype;
   float *partials;     // w4_partials_bytes
   unsigned *counters;  // one per row block, zero before and after
 };
-// n-tiles of 8 rows of A a launch is made for: 1, 2, 4 or 8.
-inline int w4_tiles(int m) { return m <= 8 ? 1 : m <= 16 ? 2 : m <= 32 ? 4 : 8; }
+// Rows of A a launch is made for: 8, 16, 32 or 64.
+inline int w4_tokens(int m) { return m <= 8 ? 8 : m <= 16 ? 16 : m <= 32 ? 32 : 64; }
 inline int w4_max_m() { return 64; }
 inline long long w4_blocks(long long n) { return (n + 127) / 128; }
 inline long long w4_stages(long long k) { return (k + 255) / 256; }
+// CTAs of the kernel for up to 16 rows that fit on an SM.
+constexpr int w4_few_ctas() { return 3; }
 inline int w4_grid(long long units, int m, int sm_count) {
-  const long long slots = static_cast<long long>(sm_count) * (w4_tiles(m) <= 2 ? 2 : 1);
+  const long long slots = static_cast<long long>(sm_count) * (m <= 16 ? w4_few_ctas() : 1);
   return static_cast<int>(units < slots ? units : slots);
 }
-inline size_t w4_partials_bytes(int grid, int m) { return static_cast<size_t>(grid) * 2 * 128 * 8 * w4_tiles(m) * 4; }
-// tmap_q: q as bytes {row_bytes inner, n}, box {128, 128}; tmap_a: A as {k inner, m}, box {64, 8 w4_tiles(m)};
-// both 128-byte swizzle.
+inline size_t w4_partials_bytes(int grid, int m) { return static_cast<size_t>(grid) * 2 * 128 * w4_tokens(m) * 4; }
+// tmap_q: q as bytes {row_bytes inner, n}, box {128, 128}, 128-byte swizzle; tmap_a: A as {k inner, m}, for
+// more than 16 rows box {64, w4_tokens(m)} and 128-byte swizzle, else box {256, w4_tokens(m)} without swizzle.
 cudaError_t launch_gemm_w4_bf16(const CUtensorMap &tmap_q, const CUtensorMap &tmap_a, const W4 &p, int *status,
                                 cudaStream_t stream);
 cudaError_t launch_gemm_w4_f16(const CUtensorMap &tmap_q, const CUtensorMap &tmap_a, const W4 &p, int *status,

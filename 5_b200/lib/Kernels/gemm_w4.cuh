@@ -3,29 +3,40 @@
 //   C[i, j] = sum_groups s[j, g] sum_{k in group g} (q[j, k] - z[j, g]) A[i, k]
 //
 // q: 0..15, two to a byte (even k in the low half), rows of ceil(k / 2) bytes; s: one scale per row of q and
-// group of 32, 64 or a multiple of 128 consecutive k, in A's type; z: one byte each, or 8 throughout. A: m <= 64 rows of
-// float16 or bfloat16.
+// group of 32, 64 or a multiple of 128 consecutive k, in A's type; z: one byte each, or 8 throughout. A:
+// m <= 64 rows of float16 or bfloat16.
 //
-// Bound: HBM reads of q, half a byte per weight, as long as the work per weight hides under them: at the
-// copy bandwidth an SM receives about 45 weights per cycle, so a warp may spend under three instructions
-// per 32 of them. The weights therefore go to the tensor cores as integers: a nibble becomes a 16-bit float by
-// being put under the exponent of 1024 (128 for bfloat16), one subtraction of 1024 + z -- exact -- serves two of
-// them, and mma.sync (16 weights rows x 16 of k x 8 rows of A, float32 sums) does the rest. The group's
-// scale multiplies the float32 sums of the group, so the only roundings are those of float32 sums and of the
-// result: nothing is lost to a 16-bit product of scale and weight. (tcgen05 would want the weights expanded
-// in shared memory and its sums drained from tensor memory at every group; with at most 8 columns in use
-// the tensor work is a twentieth of the unpacking.)
+// Bound: HBM reads of q, half a byte per weight. At the copy bandwidth an SM receives 45 weights per cycle, and
+// turning them into 16-bit floats is integer work (masks and shifts, at half the issue rate): 5 to 7 such
+// instructions per 8 weights leave little room for anything else.
 //
-// Layout of the work. A stage is 128 rows of q x 256 of k (16 KiB) and the m rows of A for them, brought by
-// TMA into a ring of 128-byte-swizzled buffers (out-of-range rows, bytes and k read as zeros), so bytes in
-// flight do not depend on registers. Eight warps take it: 4 of 32 rows x 2 of 128 k. In a 32-bit word of q
-// sit 8 consecutive k; a lane reads the word its quad position names, and the four pairs (0,4) (1,5) (2,6)
-// (3,7) that masks and shifts produce are used as the fragment's k pairs -- sums do not care in which order
-// k runs, A's fragment is permuted alike.
+// The weights enter the product as integers: a nibble becomes a float by being put under the exponent of 1024
+// (128 for bfloat16), and one subtraction of 1024 + z, exact, serves two of them. The group's scale
+// multiplies the float32 sums of the group. So nothing is lost to a 16-bit product of scale and weight: the
+// only roundings are those of float32 sums and of the result.
 //
-// Rows of q that do not start on 16-byte boundaries (an odd k) cannot be addressed by a tensor map: a
-// producer warp then copies each row's bytes with cp.async.bulk from the boundary below its start, and the
-// consumers read at the row's own phase with a funnel shift.
+// q and A arrive by TMA in a ring of 128-byte-swizzled stages of 128 rows x 256 of k (out-of-range rows, bytes
+// and k read as zeros), computed as C^T = W A^T. In a 32-bit word of q sit 8 consecutive k; masks and shifts
+// pair them as (0,4) (1,5) (2,6) (3,7). Sums do not care in which order k runs, so A's pairs are formed alike.
+//
+// Up to 16 rows of A: mma.sync with 16 rows of q by 16 of k by 8 rows of A. The tensor work is small whatever
+// the instruction, and a warp that expands weights into its own fragments and keeps its own sums hands nothing
+// on: it only waits for stages. What is the same for several of them is done once: one more warp starts the loads
+// and lays out scales and zero points ready to use, another forms A's pairs in shared memory. Four consumer warps
+// of 32 rows make a CTA with these two, three CTAs share an SM. (1 x 16384 x 8192 in bfloat16: 24.7 us; with the
+// scales fetched by every consumer a stage ahead 30.8, with one warp for loads, scales and pairs 26.8.)
+//
+// 17 to 64 rows: tcgen05.mma with M = 128 rows of q, N = 32 or 64. The expanded weights go to the tensor cores
+// through tensor memory, not through shared memory (the expanded form is four times q's bytes, which shared
+// memory would have to take and give back): a lane of an expanding warp owns a row of q, which is the lane its
+// operand has to lie in. Two sets of four warps take one half of a stage's k each, in steps of 64 of k. A set
+// has two operand buffers, so that a step's products run while the next step is expanded, and two places for
+// sums, so that a group's sums are read -- and added, times the group's scale, to the running ones -- only when
+// they are long done. A's pairs are formed by two helper warps.
+//
+// Rows of q that do not start on 16-byte boundaries (an odd k) cannot be addressed by a tensor map: warps of
+// their own then copy each row's 16-byte pieces from the boundary below its start with cp.async, and the
+// readers take words at the row's own phase with a funnel shift.
 //
 // The (row block, stage of k) units are dealt out as one sequence, an equal share to every CTA, so that the GPU
 // is evenly loaded whatever n and k are; a CTA whose share begins or ends inside a row block leaves float32
@@ -44,41 +55,10 @@ namespace w4 {
 
 constexpr int kRows = 128;        // rows of q per block
 constexpr int kStageK = 256;      // of k per stage: 128 bytes of q
-constexpr int kConsumers = 8;     // warps: 4 (rows) x 2 (k)
-constexpr int kThreads = 32 * (kConsumers + 1);
-constexpr int kQuarterRows = 32;  // rows per consumer warp: two fragments of 16
 constexpr uint32_t kQBytes = kRows * 128;
-constexpr uint32_t kPhasePitch = 144;  // bytes per row of a stage copied at its own phase
+constexpr int kPhasePieces = 9;   // 16-byte pieces of a row of a stage copied at its own phase
+constexpr uint32_t kPhasePitch = 16 * kPhasePieces;
 constexpr uint32_t kQPhaseBytes = kRows * kPhasePitch;
-
-// The ring: as many stages as fit with `kTiles` n-tiles of 8 rows of A.
-template <int kTiles, bool kPhase>
-struct Ring {
-  static constexpr uint32_t kABoxBytes = 8 * kTiles * 128;      // 64 of k x padded m
-  static constexpr uint32_t kABytes = (kStageK / 64) * kABoxBytes;
-  static constexpr uint32_t kQStageBytes = kPhase ? (kQPhaseBytes + 1023) / 1024 * 1024 : kQBytes;
-  static constexpr uint32_t kStageBytes = kQStageBytes + kABytes;
-  // Two CTAs per SM for up to 16 rows of A, one beyond.
-  static constexpr uint32_t kBudget = kTiles <= 2 ? 100 * 1024 : 192 * 1024;
-  static constexpr int kStages = kBudget / kStageBytes < 8 ? static_cast<int>(kBudget / kStageBytes) : 8;
-  // Behind the ring: barriers, then the place where the sums of the two k halves meet.
-  static constexpr uint32_t kMeetBytes = kRows * 8 * kTiles * 4;
-  static constexpr uint32_t kSmemBytes = kStages * kStageBytes + 256 + kMeetBytes + 1024;
-  static_assert(kStages >= 2 && kSmemBytes <= (kTiles <= 2 ? 113 : 227) * 1024, "shared memory of a CTA");
-};
-
-template <bool kBf16>
-__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (kBf16)
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
 // (x & mask) | magic
 __device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t magic) {
   uint32_t r;
@@ -89,22 +69,27 @@ __device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t m
 // What a row's zero point subtracts from the expanded nibbles.
 template <bool kBf16>
 struct Zero {
-  __nv_bfloat162 low;
-  __device__ explicit Zero(int z) { low = __float2bfloat162_rn(128.0f + static_cast<float>(z)); }
-  __device__ Zero() {}
+  __nv_bfloat162 low;  // 128 + z
+  __device__ void set(int z) { low = __float2bfloat162_rn(128.0f + static_cast<float>(z)); }
+  // From the pair that StageScales stores.
+  __device__ void set_pair(uint32_t pair) { low = *reinterpret_cast<const __nv_bfloat162 *>(&pair); }
 };
 template <>
 struct Zero<false> {
-  __half2 low, high;  // 1024 + z, and 64 + z for nibbles left four bits up
-  __device__ explicit Zero(int z) {
+  __half2 low, high;  // 1024 + z, and -(64 + z) for nibbles left four bits up
+  __device__ void set(int z) {
     low = __float2half2_rn(1024.0f + static_cast<float>(z));
     high = __float2half2_rn(-64.0f - static_cast<float>(z));
   }
-  __device__ Zero() {}
+  __device__ void set_pair(uint32_t pair) {
+    low = *reinterpret_cast<const __half2 *>(&pair);
+    const uint32_t up = and_or(pair << 4, 0x00f000f0u, 0xd400d400u);
+    high = *reinterpret_cast<const __half2 *>(&up);
+  }
 };
 
 // Eight nibbles of a word as four pairs (0,4) (1,5) (2,6) (3,7) of exact 16-bit floats q - z.
-__device__ __forceinline__ void expand(uint32_t w, const Zero<true> &z, uint32_t (&out)[4]) {
+__device__ __forceinline__ void expand(uint32_t w, const Zero<true> &z, uint32_t *out) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const uint32_t v = and_or(w >> (4 * i), 0x000f000fu, 0x43004300u);
@@ -112,7 +97,7 @@ __device__ __forceinline__ void expand(uint32_t w, const Zero<true> &z, uint32_t
     out[i] = *reinterpret_cast<const uint32_t *>(&d);
   }
 }
-__device__ __forceinline__ void expand(uint32_t w, const Zero<false> &z, uint32_t (&out)[4]) {
+__device__ __forceinline__ void expand(uint32_t w, const Zero<false> &z, uint32_t *out) {
   const __half2 sixteenth = __float2half2_rn(0.0625f);
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -145,47 +130,331 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   return v;
 }
 
-// Bulk copy, global -> shared; both addresses and the size multiples of 16 bytes.
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-               :: "r"(dst), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar)
-               : "memory");
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ void sts128(uint32_t addr, const uint4 &v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" :: "r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
-// The units (row block, stage of k) of CTA `cta` are [first_unit(cta), first_unit(cta + 1)); owner_of is the
-// CTA of a unit. There are at least as many units as CTAs.
-__device__ __forceinline__ long long first_unit(long long cta, long long units, long long grid) { return cta * units / grid; }
-__device__ __forceinline__ long long owner_of(long long unit, long long units, long long grid) {
-  return ((unit + 1) * grid - 1) / units;
+// 16 bytes global -> shared, of which `bytes` are read and the rest are zeros.
+__device__ __forceinline__ void copy_16(uint32_t dst, const void *src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+// One arrival on `bar` when this thread's copies so far have landed.
+__device__ __forceinline__ void copies_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" :: "r"(bar) : "memory");
 }
 
-// Barriers of the consumer warps, and of the four of them that hold a block's sums.
+// 32 columns of this warp's lanes of tensor memory.
+__device__ __forceinline__ void tmem_store_x32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+      :: "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+         "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
+         "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
+         "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// D[tmem] (+)= A[tmem] * B[smem]: 16-bit operands, the first from tensor memory (a lane per row, two of k
+// per column).
+__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+      "}\n"
+      :
+      : "r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// The units (row block, stage of k) of CTA `cta` are [first_unit(cta), first_unit(cta + 1)); owner_of is the CTA
+// of a unit.
+__device__ __forceinline__ int first_unit(const W4 &p, int cta) { return cta * p.share + min(cta, p.extra); }
+__device__ __forceinline__ int owner_of(const W4 &p, int unit) {
+  const int long_ones = p.extra * (p.share + 1);
+  return unit < long_ones ? unit / (p.share + 1) : p.extra + (unit - long_ones) / p.share;
+}
+
+// A CTA that did part of a row block leaves its sums in a slot of its own: its first if the block is the first
+// it touches, else its second. Of the CTAs `first` .. that share a block only `first` may have begun before it.
+__device__ __forceinline__ float *part_slot(const W4 &p, int cta, int first, int block, int slot_floats) {
+  const int second = cta == first && first_unit(p, first) < block * p.stages_k ? 1 : 0;
+  return p.partials + static_cast<size_t>(2 * cta + second) * slot_floats;
+}
+
+// After the slot is written: counts the part in and tells whether this CTA's is the last of the block's `parts`
+// (which then adds all of them in their order). `sync` is a barrier of the threads that hold the sums, thread 0
+// among them; its atomic operation releases what they wrote and acquires what the other CTAs' released.
+template <typename Sync>
+__device__ __forceinline__ bool count_part(const W4 &p, int block, int parts, volatile uint32_t *last_flag, Sync sync) {
+  sync();
+  if (threadIdx.x == 0) {
+    unsigned before;
+    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(p.counters + block) : "memory");
+    const bool all = before + 1 == static_cast<unsigned>(parts);
+    if (all)
+      p.counters[block] = 0u;  // as it was found
+    *last_flag = all ? 1u : 0u;
+  }
+  sync();
+  const bool all = *last_flag != 0;
+  sync();  // the flag may be written again
+  return all;
+}
+
+// The work of the warps that bring rows of q from odd places: `warps` of them share a stage, 16-byte piece by
+// piece, from the boundary at or below each row's first byte.
+__device__ __forceinline__ void copy_stage(const W4 &p, uint32_t q_dst, uint32_t full, int block, int ks, int index,
+                                           int warps, int lane) {
+  const uint8_t *const q_end = p.q + (static_cast<long long>(p.n) - 1) * p.ldq + p.row_bytes;
+  const int wanted = min(128, p.row_bytes - ks * 128);  // bytes of a row in this stage, at least 1
+#pragma unroll 6
+  for (int i = index * 32 + lane; i < kRows * kPhasePieces; i += 32 * warps) {
+    const int local = i / kPhasePieces, piece = i - local * kPhasePieces;
+    const long long row = static_cast<long long>(block) * kRows + local;
+    if (row >= p.n)
+      break;
+    const uint8_t *begin = p.q + row * p.ldq + ks * 128ll;
+    const int at = static_cast<int>(reinterpret_cast<uintptr_t>(begin) & 15);
+    const uint8_t *src = begin - at + piece * 16;
+    // Nothing is read behind q; what precedes a row in its first piece belongs to the same allocation.
+    const long long inside = q_end - src;
+    if (piece * 16 < at + wanted && inside > 0)
+      copy_16(q_dst + static_cast<uint32_t>(i) * 16, src, inside < 16 ? static_cast<uint32_t>(inside) : 16u);
+  }
+  copies_arrive(full);
+}
+
+// 32-bit words, or bytes packed into words, from an address aligned to all of them.
+__device__ __forceinline__ void load_words(const void *src, uint32_t (&out)[1]) {
+  out[0] = __ldg(static_cast<const uint32_t *>(src));
+}
+__device__ __forceinline__ void load_words(const void *src, uint32_t (&out)[2]) {
+  const uint2 v = __ldg(static_cast<const uint2 *>(src));
+  out[0] = v.x, out[1] = v.y;
+}
+__device__ __forceinline__ void load_words(const void *src, uint32_t (&out)[4]) {
+  const uint4 v = __ldg(static_cast<const uint4 *>(src));
+  out[0] = v.x, out[1] = v.y, out[2] = v.z, out[3] = v.w;
+}
+template <int kBytes>
+__device__ __forceinline__ void load_bytes(const uint8_t *src, uint32_t (&out)[(kBytes + 3) / 4]) {
+  if constexpr (kBytes == 2)
+    out[0] = __ldg(reinterpret_cast<const uint16_t *>(src));
+  else
+    load_words(src, out);
+}
+
+// Eight consecutive 16-bit k of A in the order (0,4) (1,5) (2,6) (3,7).
+__device__ __forceinline__ uint4 in_pairs(const uint4 &v) {
+  return make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
+                    __byte_perm(v.y, v.w, 0x7632));
+}
+
+// Rows first, first + step, ... below m of a stage of A, in place: element 8 j + 2 i + h becomes what was 8 j + i +
+// 4 h. A lane takes the same 16-byte piece of every row.
+__device__ __forceinline__ void arrange_rows(uint32_t a_addr, uint32_t box_bytes, int first, int step, int m, int lane) {
+  const uint32_t at = a_addr + static_cast<uint32_t>(lane >> 3) * box_bytes;
+  auto place = [&](int t) {
+    return at + static_cast<uint32_t>(t) * 128 + ((static_cast<uint32_t>(lane & 7) ^ static_cast<uint32_t>(t & 7)) << 4);
+  };
+  int t = first;
+  for (; t + 7 * step < m; t += 8 * step) {  // eight loads in flight
+    uint4 v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      v[i] = lds128(place(t + i * step));
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      sts128(place(t + i * step), in_pairs(v[i]));
+  }
+  for (; t < m; t += step)
+    sts128(place(t), in_pairs(lds128(place(t))));
+  fence_proxy_async_smem();  // the tensor cores read it next
+}
+
+// The scales and zero points on their way from memory to the stages, four rows of q per lane of the warp that
+// brings them: fetched as they lie in memory, kAhead stages early, and stored as pairs (the scale as a float,
+// what the zero point subtracts as two 16-bit floats), [group of the stage][row].
+template <bool kBf16, int kGroup>
+struct ScaleStream {
+  static constexpr int kGroups = kStageK / kGroup;  // of a stage: 2, 4 or 8
+  static constexpr int kAhead = 2;
+  static constexpr int kZeroWords = (kGroups + 3) / 4;
+  uint32_t scale[kAhead][kRows / 32][kGroups / 2], zero[kAhead][kRows / 32][kZeroWords];
+  const uint16_t *scale_row[kRows / 32];
+  const uint8_t *zero_row[kRows / 32];
+  int left, ks;    // units still to be fetched; the stage of k of the next
+  long long block;  // of the next
+
+  __device__ __forceinline__ ScaleStream(const W4 &p, int unit_begin, int unit_end, int lane) {
+    left = unit_end - unit_begin;
+    block = unit_begin / p.stages_k;
+    ks = unit_begin - static_cast<int>(block) * p.stages_k;
+    point(p, lane);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      fetch(p, i, lane);
+  }
+  __device__ __forceinline__ void point(const W4 &p, int lane) {
+#pragma unroll
+    for (int i = 0; i < kRows / 32; ++i) {
+      // Rows past the end take the last row's scales; their results are not stored.
+      const long long at = block * kRows + i * 32 + lane, row = at < p.n ? at : p.n - 1;
+      scale_row[i] = p.scales + row * p.lds;
+      zero_row[i] = p.zeros + row * p.ldz;
+    }
+  }
+  __device__ __forceinline__ void fetch(const W4 &p, int to, int lane) {
+    if (--left < 0)
+      return;
+    const int first = ks * kGroups;
+#pragma unroll
+    for (int i = 0; i < kRows / 32; ++i) {
+#pragma unroll
+      for (int j = 0; j < kZeroWords; ++j)
+        zero[to][i][j] = p.zeros == nullptr ? 0x08080808u : 0u;
+      if (p.vector_scales) {  // whole groups of whole stages, on boundaries of as many
+        load_words(scale_row[i] + first, scale[to][i]);
+        if (p.zeros != nullptr)
+          load_bytes<kGroups>(zero_row[i] + first, zero[to][i]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kGroups; ++j) {
+          // (p.span: how many of the kernel's groups share a scale, for groups of several times 128.)
+          const int group = min(p.span == 1 ? first + j : (first + j) / p.span, p.groups - 1);
+          const uint32_t v = scale_row[i][group];
+          scale[to][i][j / 2] = j % 2 == 0 ? v : scale[to][i][j / 2] | v << 16;
+          if (p.zeros != nullptr)
+            zero[to][i][j / 4] |= static_cast<uint32_t>(zero_row[i][group]) << (8 * (j % 4));
+        }
+      }
+    }
+    if (++ks == p.stages_k) {
+      ks = 0;
+      ++block;
+      if (left > 0)
+        point(p, lane);
+    }
+  }
+  // The oldest stage fetched goes to `at`, another is fetched.
+  __device__ __forceinline__ void advance(const W4 &p, uint32_t at, int lane) {
+#pragma unroll
+    for (int j = 0; j < kGroups; ++j)
+#pragma unroll
+      for (int i = 0; i < kRows / 32; ++i) {
+        const uint32_t bits = j % 2 == 0 ? scale[0][i][j / 2] & 0xffffu : scale[0][i][j / 2] >> 16;
+        const uint32_t pair = __byte_perm(zero[0][i][j / 4], kBf16 ? 0x43434343u : 0x64646464u, 0x4040u | (0x101u * (j % 4)));
+        asm volatile("st.shared.v2.u32 [%0], {%1, %2};"
+                     :: "r"(at + static_cast<uint32_t>((j * kRows + i * 32 + lane) * 8)),
+                        "r"(__float_as_uint(scale_value<kBf16>(static_cast<uint16_t>(bits)))), "r"(pair)
+                     : "memory");
+      }
+#pragma unroll
+    for (int i = 0; i < kRows / 32; ++i) {
+#pragma unroll
+      for (int j = 0; j < kGroups / 2; ++j)
+        scale[0][i][j] = scale[1][i][j];
+#pragma unroll
+      for (int j = 0; j < kZeroWords; ++j)
+        zero[0][i][j] = zero[1][i][j];
+    }
+    fetch(p, 1, lane);
+  }
+};
+
+// A's pairs for mma.sync: rows of 512 bytes, of every other one the two halves of each 128 bytes change places
+// too, so that the consumers' loads of a pair of rows fall into different banks.
+__device__ __forceinline__ void arrange_plain_rows(uint32_t a_addr, int m, int lane) {
+  for (int t = 0; t < m; t += 4) {
+    uint4 v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      v[u] = lds128(a_addr + static_cast<uint32_t>(t + u) * 512 + static_cast<uint32_t>(lane) * 16);
+    __syncwarp();
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      sts128(a_addr + static_cast<uint32_t>(t + u) * 512 + ((static_cast<uint32_t>(lane) ^ ((t + u) & 1 ? 4u : 0u)) << 4),
+             in_pairs(v[u]));
+  }
+  fence_proxy_async_smem();  // TMA writes here next
+}
+
+// ---------------------------------------------------------------- up to 16 rows of A ------------
+
+namespace few {
+
+constexpr int kConsumers = 4;  // warps, 32 rows of q each
+constexpr int kLoadWarp = kConsumers, kHelperWarp = kConsumers + 1;
+constexpr int kThreads = 32 * (kConsumers + 2);
+
+// Two n-tiles of 8 rows of A at most. A stage also holds, for each of its groups and rows of q, the scale as a
+// float and what the zero point subtracts, ready to use. Several CTAs share an SM; the ring is as long as
+// that leaves room for.
+template <int kTiles, bool kPhase, int kGroup>
+struct Shape {
+  static constexpr int kTokens = 8 * kTiles;
+  static constexpr int kCtasPerSm = w4_few_ctas();
+  static constexpr int kGroups = kStageK / kGroup;  // of a stage: 2, 4 or 8
+  static constexpr uint32_t kABytes = kTokens * kStageK * 2;
+  static constexpr uint32_t kQStageBytes = kPhase ? kQPhaseBytes : kQBytes;
+  static constexpr uint32_t kScaleBytes = kGroups * kRows * 8;
+  static constexpr uint32_t kStageBytes = kQStageBytes + kABytes + kScaleBytes;
+  static constexpr uint32_t kBudget = (228 / kCtasPerSm - 1) * 1024 - 1024 - 128;
+  static constexpr int kStages = kBudget / kStageBytes < 4 ? static_cast<int>(kBudget / kStageBytes) : 4;
+  static constexpr uint32_t kSmemBytes = kStages * kStageBytes + 128 + 1024;
+  static_assert(kStages >= 2 && kStageBytes % 1024 == 0, "ring");
+};
+
+// d = a b (+ d)
+template <bool kBf16>
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, bool first) {
+  const float c0 = first ? 0.0f : d[0], c1 = first ? 0.0f : d[1], c2 = first ? 0.0f : d[2], c3 = first ? 0.0f : d[3];
+  if constexpr (kBf16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+}
+
 __device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kConsumers) : "memory"); }
-__device__ __forceinline__ void half_sync() { asm volatile("bar.sync 2, %0;" ::"n"(16 * kConsumers) : "memory"); }
 
 template <bool kBf16, int kTiles, bool kPhase, int kGroup>
-__global__ void __launch_bounds__(kThreads, kTiles <= 2 ? 2 : 1)
-gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_a, const W4 p,
-               int *status) {
-  using R = Ring<kTiles, kPhase>;
-  constexpr int kGroupsPerStage = kStageK / kGroup;        // 2, 4 or 8
-  constexpr int kGroupsPerHalf = kGroupsPerStage / 2;      // of a warp's 128 of k: 1, 2 or 4
+__global__ void __launch_bounds__(kThreads, Shape<kTiles, kPhase, kGroup>::kCtasPerSm)
+gemm_w4_few_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_a, const W4 p,
+                   int *status) {
+  using S = Shape<kTiles, kPhase, kGroup>;
   constexpr int kChunksPerGroup = kGroup / 32;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   const uint32_t smem_base = (raw_addr + 1023u) & ~1023u;
   uint8_t *smem_gen = smem_raw + (smem_base - raw_addr);
-  const uint32_t bar_base = smem_base + R::kStages * R::kStageBytes;
+  const uint32_t bar_base = smem_base + S::kStages * S::kStageBytes;
   auto full_bar = [&](uint32_t s) { return bar_base + 8u * s; };
-  auto empty_bar = [&](uint32_t s) { return bar_base + 8u * (R::kStages + s); };
+  auto empty_bar = [&](uint32_t s) { return bar_base + 8u * (S::kStages + s); };
+  auto ready_bar = [&](uint32_t s) { return bar_base + 8u * (2 * S::kStages + s); };  // arrived, and made ready
   volatile uint32_t *abort_flag =
-      reinterpret_cast<volatile uint32_t *>(smem_gen + R::kStages * R::kStageBytes + 8u * 2 * R::kStages);
+      reinterpret_cast<volatile uint32_t *>(smem_gen + S::kStages * S::kStageBytes + 8u * 3 * S::kStages);
   volatile uint32_t *last_flag = abort_flag + 1;
   const int warp = static_cast<int>(threadIdx.x >> 5), lane = static_cast<int>(threadIdx.x & 31);
   if (threadIdx.x == 0) {
-    for (uint32_t s = 0; s < R::kStages; ++s) {
-      mbar_init(full_bar(s), 1);
+    for (uint32_t s = 0; s < S::kStages; ++s) {
+      mbar_init(full_bar(s), 1 + (kPhase ? 32 : 0));
       mbar_init(empty_bar(s), kConsumers);
+      mbar_init(ready_bar(s), kPhase ? 1 : 2);
     }
     *abort_flag = 0;
     mbar_fence_init();
@@ -195,80 +464,37 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant
   }
   __syncthreads();
 
-  const long long grid = gridDim.x;
-  const long long unit_begin = first_unit(blockIdx.x, p.units, grid), unit_end = first_unit(blockIdx.x + 1, p.units, grid);
+  const int cta = static_cast<int>(blockIdx.x);
+  const int unit_begin = first_unit(p, cta), unit_end = first_unit(p, cta + 1);
   const int stages_k = p.stages_k;
 
-  if (warp == kConsumers) {
-    // ------------------------------------------------------------ producer ----------
+  if (warp == kLoadWarp) {
+    // ------------------------------------------------------------ loads -------------
+    // One lane issues the TMA loads. The others bring the scales, or the rows of q at odd places.
+    ScaleStream<kBf16, kGroup> scales(p, unit_begin, kPhase ? unit_begin : unit_end, lane);
     uint32_t stage = 0, phase = 0;
-    long long block = unit_begin / stages_k;
-    int ks = static_cast<int>(unit_begin - block * stages_k);
-    for (long long unit = unit_begin; unit < unit_end; ++unit) {
-      const bool free = mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag);
+    int block = unit_begin / stages_k, ks = unit_begin - block * stages_k;
+    for (int unit = unit_begin; unit < unit_end; ++unit) {
+      const bool free = mbar_wait_asleep(empty_bar(stage), phase ^ 1u, abort_flag);
       if (!__all_sync(0xffffffffu, free))
         break;
-      const uint32_t q_dst = smem_base + stage * R::kStageBytes, a_dst = q_dst + R::kQStageBytes;
-      if constexpr (!kPhase) {
-        if (lane == 0) {
-          mbar_arrive_expect_tx(full_bar(stage), R::kStageBytes);
-          tma_load_2d(q_dst, &tmap_q, full_bar(stage), ks * 128, static_cast<int>(block) * kRows);
-#pragma unroll
-          for (int j = 0; j < kStageK / 64; ++j)
-            tma_load_2d(a_dst + j * R::kABoxBytes, &tmap_a, full_bar(stage), ks * kStageK + j * 64, 0);
-        }
+      const uint32_t at = smem_base + stage * S::kStageBytes;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(full_bar(stage), kPhase ? S::kABytes : S::kStageBytes - S::kScaleBytes);
+        if (!kPhase)
+          tma_load_2d(at, &tmap_q, full_bar(stage), ks * 128, block * kRows);
+        tma_load_2d(at + S::kQStageBytes, &tmap_a, full_bar(stage), ks * kStageK, 0);
+      }
+      __syncwarp();
+      if (kPhase) {
+        copy_stage(p, at, full_bar(stage), block, ks, 0, 1, lane);
       } else {
-        // Each lane brings four rows: the 16-byte pieces from the boundary at or below the row's first
-        // byte of this stage up to the last one that lies wholly inside q; what is left of q's very end
-        // goes byte by byte.
-        uint32_t bytes[kRows / 32], total = 0;
-        const uint8_t *source[kRows / 32];
-        const uint8_t *const q_end = p.q + (static_cast<long long>(p.n) - 1) * p.ldq + p.row_bytes;
-#pragma unroll
-        for (int i = 0; i < kRows / 32; ++i) {
-          const long long row = block * kRows + i * 32 + lane;
-          bytes[i] = 0;
-          source[i] = nullptr;
-          if (row < p.n) {
-            const uint8_t *begin = p.q + row * p.ldq + ks * 128ll;
-            const int wanted = min(128, p.row_bytes - ks * 128);  // at least 1
-            const uint8_t *low = reinterpret_cast<const uint8_t *>(reinterpret_cast<uintptr_t>(begin) & ~uintptr_t{15});
-            const uint8_t *high = reinterpret_cast<const uint8_t *>(
-                (reinterpret_cast<uintptr_t>(begin + wanted) + 15) & ~uintptr_t{15});
-            const uint32_t dst = q_dst + static_cast<uint32_t>(i * 32 + lane) * kPhasePitch;
-            if (high > q_end) {
-              const uint8_t *whole = reinterpret_cast<const uint8_t *>(reinterpret_cast<uintptr_t>(q_end) & ~uintptr_t{15});
-              if (whole < low)
-                whole = low;
-              for (const uint8_t *b = whole < begin ? begin : whole; b < begin + wanted; ++b)
-                smem_gen[dst - smem_base + static_cast<uint32_t>(b - low)] = *b;
-              fence_proxy_async_smem();
-              high = whole;
-            }
-            source[i] = low;
-            bytes[i] = static_cast<uint32_t>(high - low);
-          }
-          total += bytes[i];
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1)
-          total += __shfl_xor_sync(0xffffffffu, total, o);
-        // The bytes stored above are ordered before the consumers' reads by lane 0's arrival.
+        scales.advance(p, at + S::kQStageBytes + S::kABytes, lane);
         __syncwarp();
         if (lane == 0)
-          mbar_arrive_expect_tx(full_bar(stage), total + R::kABytes);
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < kRows / 32; ++i)
-          if (bytes[i] != 0)
-            bulk_load(q_dst + static_cast<uint32_t>(i * 32 + lane) * kPhasePitch, source[i], bytes[i], full_bar(stage));
-        if (lane == 0) {
-#pragma unroll
-          for (int j = 0; j < kStageK / 64; ++j)
-            tma_load_2d(a_dst + j * R::kABoxBytes, &tmap_a, full_bar(stage), ks * kStageK + j * 64, 0);
-        }
+          mbar_arrive(ready_bar(stage));
       }
-      if (++stage == R::kStages) {
+      if (++stage == S::kStages) {
         stage = 0;
         phase ^= 1u;
       }
@@ -277,210 +503,147 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant
         ++block;
       }
     }
-  }
-
-  // ---------------------------------------------------------------- consumers ----------
-  const int row_warp = warp & 3, k_half = (warp >> 2) & 1;
-  const int g = lane >> 2, q4 = lane & 3;  // fragment row (or row of A), position in the quad
-  float *const meet = reinterpret_cast<float *>(smem_gen + R::kStages * R::kStageBytes + 256);
-  uint32_t stage = 0, phase = 0;
-  long long unit = unit_begin;
-  bool ok = true;  // (a wait that ran out: the barriers below are still met)
-  while (warp < kConsumers && unit < unit_end) {
-    const long long block = unit / stages_k;
-    const int ks_begin = static_cast<int>(unit - block * stages_k);
-    const long long left = unit_end - unit;
-    const int ks_end = left < stages_k - ks_begin ? ks_begin + static_cast<int>(left) : stages_k;
-    float total[2][kTiles][4];
+    if (kPhase)
+      asm volatile("cp.async.wait_all;" ::: "memory");
+  } else if (warp == kHelperWarp) {
+    // ------------------------------------------------------------ helper ------------
+    // Forms A's pairs; brings the scales where the load warp copies q.
+    ScaleStream<kBf16, kGroup> scales(p, unit_begin, kPhase ? unit_end : unit_begin, lane);
+    uint32_t stage = 0, phase = 0;
+    for (int unit = unit_begin; unit < unit_end; ++unit) {
+      const uint32_t at = smem_base + stage * S::kStageBytes;
+      if (kPhase) {
+        const bool free = mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag);
+        if (!__all_sync(0xffffffffu, free))
+          break;
+        scales.advance(p, at + S::kQStageBytes + S::kABytes, lane);
+      }
+      const bool arrived = mbar_wait(full_bar(stage), phase, abort_flag);
+      if (!__all_sync(0xffffffffu, arrived))
+        break;
+      arrange_plain_rows(at + S::kQStageBytes, p.m, lane);
+      __syncwarp();
+      if (lane == 0)
+        mbar_arrive(ready_bar(stage));
+      if (++stage == S::kStages) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ consumers ---------
+    const int g = lane >> 2, q4 = lane & 3;  // fragment row (or row of A), position in the quad
+    // Row g of A, of which odd rows have the halves of 128 bytes exchanged.
+    const uint32_t a_lane = S::kQStageBytes + static_cast<uint32_t>(g) * 512 + static_cast<uint32_t>(q4) * 16;
+    const uint32_t a_swap = (g & 1) != 0 ? 64u : 0u;
+    uint32_t stage = 0, phase = 0;
+    int unit = unit_begin;
+    while (unit < unit_end) {
+      const int block = unit / stages_k, ks_begin = unit - block * stages_k;
+      const int ks_end = min(stages_k, ks_begin + (unit_end - unit));
+      float total[2][kTiles][4];
 #pragma unroll
-    for (int f = 0; f < 2; ++f)
+      for (int f = 0; f < 2; ++f)
 #pragma unroll
-      for (int t = 0; t < kTiles; ++t)
+        for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          total[f][t][e] = 0.0f;
-    if (ok) {
+          for (int e = 0; e < 4; ++e)
+            total[f][t][e] = 0.0f;
       // This lane's four rows of q: two fragments, rows g and g + 8 of each.
-      long long row[4];
       uint32_t row_at[4], row_shift[4];
+      if constexpr (kPhase) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int local = row_warp * kQuarterRows + i * 8 + g;
-        row[i] = block * kRows + local;
-        if (row[i] >= p.n)
-          row[i] = p.n - 1;  // computed and not stored
-        if constexpr (kPhase) {
-          const uint32_t at = static_cast<uint32_t>((reinterpret_cast<uintptr_t>(p.q) + (block * kRows + local) * p.ldq) & 15);
-          row_at[i] = static_cast<uint32_t>(local) * kPhasePitch + (at & ~3u);
-          row_shift[i] = 8 * (at & 3u);
-        } else {
-          row_at[i] = static_cast<uint32_t>(local) * 128;
-          row_shift[i] = 0;
+        for (int i = 0; i < 4; ++i) {
+          const int local = warp * 32 + i * 8 + g;
+          const uint32_t shift = static_cast<uint32_t>(
+              (reinterpret_cast<uintptr_t>(p.q) + (static_cast<long long>(block) * kRows + local) * p.ldq) & 15);
+          row_at[i] = static_cast<uint32_t>(local) * kPhasePitch + (shift & ~3u) + static_cast<uint32_t>(q4) * 4;
+          row_shift[i] = 8 * (shift & 3u);
         }
       }
-      // Scales and zero points of the warp's groups of a stage: group j of row i is held by quad position j.
-      uint16_t next_scale[4];
-      uint8_t next_zero[4];
-      auto fetch = [&](int ks) {
-        // (p.span: how many of the kernel's groups share a scale, for groups of several times 128.)
-        const int group =
-            min((ks * kGroupsPerStage + k_half * kGroupsPerHalf + (q4 % kGroupsPerHalf)) / p.span, p.groups - 1);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          next_scale[i] = p.scales[row[i] * p.lds + group];
-          next_zero[i] = p.zeros != nullptr ? p.zeros[row[i] * p.ldz + group] : uint8_t{8};
-        }
-      };
-      fetch(ks_begin);
+      const uint32_t q_lane = static_cast<uint32_t>(warp * 32 + g) * 128 + (static_cast<uint32_t>(g) << 4) + static_cast<uint32_t>(q4) * 4;
+      const uint32_t scale_lane = S::kQStageBytes + S::kABytes + static_cast<uint32_t>(warp * 32 + g) * 8;
       for (int ks = ks_begin; ks < ks_end; ++ks) {
-        uint32_t scale_bits[4], zero_bits[4];
+        // (A wait that runs out raises the abort flag: what follows then computes on whatever the ring holds,
+        // in bounds, and the launch is reported as failed.)
+        mbar_wait(ready_bar(stage), phase, abort_flag);
+        __syncwarp();
+        const uint32_t q_addr = smem_base + stage * S::kStageBytes, a_even = q_addr + a_lane + a_swap, a_odd = q_addr + a_lane + 64 - a_swap;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          scale_bits[i] = next_scale[i];
-          zero_bits[i] = next_zero[i];
-        }
-        if (ks + 1 < ks_end)
-          fetch(ks + 1);
-        const bool ready = mbar_wait(full_bar(stage), phase, abort_flag);
-        if (!__all_sync(0xffffffffu, ready)) {
-          ok = false;
-          break;
-        }
-        const uint32_t q_addr = smem_base + stage * R::kStageBytes, a_addr = q_addr + R::kQStageBytes;
-#pragma unroll
-        for (int gi = 0; gi < kGroupsPerHalf; ++gi) {
+        for (int gi = 0; gi < S::kGroups; ++gi) {
           float scale[4];
           Zero<kBf16> zero[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const uint32_t both = __shfl_sync(0xffffffffu, scale_bits[i] | (zero_bits[i] << 16), (lane & ~3) | gi);
-            scale[i] = scale_value<kBf16>(static_cast<uint16_t>(both));
-            zero[i] = Zero<kBf16>(static_cast<int>(both >> 16));
+            const uint2 v = lds64(q_addr + scale_lane + static_cast<uint32_t>(gi * kRows * 8 + i * 64));
+            scale[i] = __uint_as_float(v.x);
+            zero[i].set_pair(v.y);
           }
           float sum[2][kTiles][4];
 #pragma unroll
-          for (int f = 0; f < 2; ++f)
+          for (int ci = 0; ci < kChunksPerGroup; ++ci) {
+            const int chunk = gi * kChunksPerGroup + ci;  // 32 of k, 16 bytes of q
+            uint4 b[kTiles];  // 8 of k of one row of A, paired as expand() pairs the weights
 #pragma unroll
             for (int t = 0; t < kTiles; ++t)
+              b[t] = lds128((chunk % 2 == 0 ? a_even : a_odd) + static_cast<uint32_t>((chunk / 2) * 128 + t * 4096));
+            uint32_t word[4];
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                sum[f][t][e] = 0.0f;
-#pragma unroll
-          for (int ci = 0; ci < kChunksPerGroup; ++ci) {
-            const int chunk = k_half * 4 + gi * kChunksPerGroup + ci;  // 32 of k, 16 bytes of q
-            // A: 8 consecutive k of one row per lane, paired as expand() pairs the weights.
-            uint32_t b[kTiles][4];
-#pragma unroll
-            for (int t = 0; t < kTiles; ++t) {
-              const uint32_t box = a_addr + static_cast<uint32_t>(chunk >> 1) * R::kABoxBytes;
-              const uint32_t piece = static_cast<uint32_t>((chunk & 1) * 4 + q4);
-              const uint4 v = lds128(box + static_cast<uint32_t>(t * 8 + g) * 128 + ((piece ^ static_cast<uint32_t>(g)) << 4));
-              b[t][0] = __byte_perm(v.x, v.z, 0x5410);
-              b[t][1] = __byte_perm(v.x, v.z, 0x7632);
-              b[t][2] = __byte_perm(v.y, v.w, 0x5410);
-              b[t][3] = __byte_perm(v.y, v.w, 0x7632);
+            for (int i = 0; i < 4; ++i) {
+              if constexpr (kPhase) {
+                const uint32_t at = q_addr + row_at[i] + static_cast<uint32_t>(chunk * 16);
+                word[i] = __funnelshift_r(lds32(at), lds32(at + 4), row_shift[i]);
+              } else {
+                word[i] = lds32(((q_addr + q_lane) ^ static_cast<uint32_t>(chunk << 4)) + static_cast<uint32_t>(i) * 1024);
+              }
             }
 #pragma unroll
             for (int f = 0; f < 2; ++f) {
-              uint32_t word[2], lo[4], hi[4];
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const int i = 2 * f + h;
-                if constexpr (kPhase) {
-                  const uint32_t at = q_addr + row_at[i] + static_cast<uint32_t>(chunk * 16 + q4 * 4);
-                  word[h] = __funnelshift_r(lds32(at), lds32(at + 4), row_shift[i]);
-                } else {
-                  word[h] = lds32(q_addr + row_at[i] + ((static_cast<uint32_t>(chunk) ^ static_cast<uint32_t>(g)) << 4) +
-                                  static_cast<uint32_t>(q4 * 4));
-                }
-              }
-              expand(word[0], zero[2 * f], lo);
-              expand(word[1], zero[2 * f + 1], hi);
+              uint32_t lo[4], hi[4];
+              expand(word[2 * f], zero[2 * f], lo);
+              expand(word[2 * f + 1], zero[2 * f + 1], hi);
               const uint32_t a0[4] = {lo[0], hi[0], lo[1], hi[1]}, a1[4] = {lo[2], hi[2], lo[3], hi[3]};
 #pragma unroll
               for (int t = 0; t < kTiles; ++t) {
-                mma<kBf16>(sum[f][t], a0, b[t][0], b[t][1]);
-                mma<kBf16>(sum[f][t], a1, b[t][2], b[t][3]);
+                mma<kBf16>(sum[f][t], a0, b[t].x, b[t].y, ci == 0);
+                mma<kBf16>(sum[f][t], a1, b[t].z, b[t].w, false);
               }
             }
           }
 #pragma unroll
-          for (int f = 0; f < 2; ++f)
+          for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int t = 0; t < kTiles; ++t) {
-              total[f][t][0] = fmaf(scale[2 * f], sum[f][t][0], total[f][t][0]);
-              total[f][t][1] = fmaf(scale[2 * f], sum[f][t][1], total[f][t][1]);
-              total[f][t][2] = fmaf(scale[2 * f + 1], sum[f][t][2], total[f][t][2]);
-              total[f][t][3] = fmaf(scale[2 * f + 1], sum[f][t][3], total[f][t][3]);
-            }
+            for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                float &to = total[i / 2][t][2 * (i % 2) + e];
+                to = fmaf(scale[i], sum[i / 2][t][2 * (i % 2) + e], to);
+              }
         }
         __syncwarp();
         if (lane == 0)
           mbar_arrive(empty_bar(stage));
-        if (++stage == R::kStages) {
+        if (++stage == S::kStages) {
           stage = 0;
           phase ^= 1u;
         }
       }
-    }
-    unit += ks_end - ks_begin;
+      unit += ks_end - ks_begin;
 
-    // The two k halves meet in shared memory; lane (g, q4) of a fragment holds rows g and g + 8 and the
-    // rows 2 q4, 2 q4 + 1 of A.
-    auto place = [&](int f, int h, int t) {
-      return (row_warp * kQuarterRows + f * 16 + h * 8 + g) * (8 * kTiles) + t * 8 + 2 * q4;
-    };
-    if (k_half == 1) {
-#pragma unroll
-      for (int f = 0; f < 2; ++f)
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            *reinterpret_cast<float2 *>(meet + place(f, h, t)) = make_float2(total[f][t][2 * h], total[f][t][2 * h + 1]);
-    }
-    consumers_sync();
-    if (k_half == 0) {
-#pragma unroll
-      for (int f = 0; f < 2; ++f)
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float2 v = *reinterpret_cast<const float2 *>(meet + place(f, h, t));
-            total[f][t][2 * h] += v.x;
-            total[f][t][2 * h + 1] += v.y;
-          }
+      // Lane (g, q4) holds rows g and g + 8 of its fragments and the rows 2 q4, 2 q4 + 1 of A.
+      auto place = [&](int i, int t) { return (warp * 32 + i * 8 + g) * S::kTokens + t * 8 + 2 * q4; };
       bool store = true;
       if (ks_begin != 0 || ks_end != stages_k) {
-        // Part of a block: leave the sums in this CTA's slot and count it in. The CTAs that share the
-        // block are consecutive; the one that counts last adds all parts in their order.
-        constexpr int kSlot = kRows * 8 * kTiles;
-        const long long first = owner_of(block * stages_k, p.units, grid);
-        const long long last = owner_of((block + 1) * stages_k - 1, p.units, grid);
-        auto slot_of = [&](long long cta) {
-          return p.partials + (2 * cta + (first_unit(cta, p.units, grid) / stages_k == block ? 0 : 1)) * kSlot;
-        };
-        float *mine = slot_of(blockIdx.x);
+        constexpr int kSlot = kRows * S::kTokens;
+        const int first = owner_of(p, block * stages_k), last = owner_of(p, (block + 1) * stages_k - 1);
+        float *mine = part_slot(p, cta, first, block, kSlot);
 #pragma unroll
-        for (int f = 0; f < 2; ++f)
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-              __stcg(reinterpret_cast<float2 *>(mine + place(f, h, t)), make_float2(total[f][t][2 * h], total[f][t][2 * h + 1]));
-        __threadfence();
-        half_sync();
-        if (threadIdx.x == 0) {
-          const unsigned parts = static_cast<unsigned>(last - first + 1);
-          const unsigned before = atomicAdd(p.counters + block, 1u);
-          *last_flag = before + 1 == parts ? 1u : 0u;
-          if (before + 1 == parts)
-            p.counters[block] = 0u;  // as it was found
-          __threadfence();
-        }
-        half_sync();
-        store = *last_flag != 0;
+            __stcg(reinterpret_cast<float2 *>(mine + place(i, t)),
+                   make_float2(total[i / 2][t][2 * (i % 2)], total[i / 2][t][2 * (i % 2) + 1]));
+        store = count_part(p, block, last - first + 1, last_flag, [] { consumers_sync(); });
         if (store) {
 #pragma unroll
           for (int f = 0; f < 2; ++f)
@@ -489,37 +652,47 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant
 #pragma unroll
               for (int e = 0; e < 4; ++e)
                 total[f][t][e] = 0.0f;
-          for (long long cta = first; cta <= last; ++cta) {
-            const float *part = slot_of(cta);
+          constexpr int kAhead = 4 / kTiles;  // parts whose loads are in flight together
+          for (int part = first; part <= last; part += kAhead) {
+            float2 v[kAhead][4][kTiles];
 #pragma unroll
-            for (int f = 0; f < 2; ++f)
+            for (int u = 0; u < kAhead; ++u) {
+              const float *from = part_slot(p, min(part + u, last), first, block, kSlot);
 #pragma unroll
-              for (int t = 0; t < kTiles; ++t)
+              for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                  const float2 v = __ldcg(reinterpret_cast<const float2 *>(part + place(f, h, t)));
-                  total[f][t][2 * h] += v.x;
-                  total[f][t][2 * h + 1] += v.y;
-                }
+                for (int t = 0; t < kTiles; ++t)
+                  v[u][i][t] = __ldcg(reinterpret_cast<const float2 *>(from + place(i, t)));
+            }
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int t = 0; t < kTiles; ++t)
+                  if (part + u <= last) {
+                    total[i / 2][t][2 * (i % 2)] += v[u][i][t].x;
+                    total[i / 2][t][2 * (i % 2) + 1] += v[u][i][t].y;
+                  }
           }
         }
       }
       if (store) {
 #pragma unroll
-        for (int f = 0; f < 2; ++f)
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const long long column = block * kRows + row_warp * kQuarterRows + f * 16 + (e >> 1) * 8 + g;
-              const int i = t * 8 + 2 * q4 + (e & 1);
-              if (i < p.m && column < p.n)
-                store_c_element(p.c, static_cast<long long>(i) * p.ldc + column, total[f][t][e], p.c_dtype);
+            for (int e = 0; e < 2; ++e) {
+              const long long column = static_cast<long long>(block) * kRows + warp * 32 + i * 8 + g;
+              const int token = t * 8 + 2 * q4 + e;
+              if (token < p.m && column < p.n)
+                store_c_element(p.c, token * p.ldc + column, total[i / 2][t][2 * (i % 2) + e], p.c_dtype);
             }
       }
     }
-    consumers_sync();  // `meet` is free again
   }
+
   __syncthreads();
   if (*abort_flag != 0) {
     if (threadIdx.x == 0)
@@ -530,47 +703,497 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant
   }
 }
 
-template <bool kBf16, int kTiles, bool kPhase, int kGroup>
-cudaError_t launch(const CUtensorMap &tmap_q, const CUtensorMap &tmap_a, const W4 &p, int *status, cudaStream_t stream) {
-  using R = Ring<kTiles, kPhase>;
-  static thread_local int configured_device = -1;
+}  // namespace few
+
+// ---------------------------------------------------------------- 17 to 64 rows of A ------------
+
+namespace many {
+
+constexpr int kHalfK = 128;    // of a stage, for each of the two sets
+constexpr int kStepK = 64;     // of k between two hand-overs of a set, two per stage
+constexpr int kExpanders = 8;  // warps: 2 sets x 4 quarters of the tensor-memory lanes
+constexpr int kProducerWarp = kExpanders, kMmaWarp = kExpanders + 1, kFirstHelper = kExpanders + 2;
+constexpr int kHelpers = 2;    // warps that put A in order, and copy rows of q at odd places
+constexpr int kThreads = 32 * (kExpanders + 2 + kHelpers);
+constexpr uint32_t kOperandColumns = kStepK / 2;  // 32-bit columns of tensor memory per operand buffer
+constexpr uint32_t kSumsAt = 4 * kOperandColumns;
+
+// What follows from the rows of A a launch is made for (kTokens = 32 or 64, also N of the instruction), the group
+// and q's alignment.
+template <int kTokens, bool kPhase, int kGroup>
+struct Shape {
+  static constexpr int kGroupsPerHalf = kHalfK / kGroup;  // 1, 2 or 4
+  static constexpr int kAccs = kGroup == 32 ? 2 : 1;      // groups of a step, each with sums of its own
+  static constexpr int kSlots = kAccs * kTokens == 128 ? 1 : 2;  // places for sums per set
+  static constexpr uint32_t kUsedColumns = kSumsAt + 2 * kSlots * kAccs * kTokens;
+  static constexpr uint32_t kTmemColumns = kUsedColumns <= 256 ? 256 : 512;
+  static_assert(kUsedColumns <= 512, "tensor memory");
+  static constexpr uint32_t kABoxBytes = kTokens * 128;    // 64 of k x kTokens rows of A
+  static constexpr uint32_t kABytes = (kStageK / 64) * kABoxBytes;
+  static constexpr uint32_t kQStageBytes = kPhase ? kQPhaseBytes : kQBytes;
+  static constexpr uint32_t kStageBytes = kQStageBytes + kABytes;
+  static constexpr int kStages = 192 * 1024 / kStageBytes < 6 ? static_cast<int>(192 * 1024 / kStageBytes) : 6;
+  // Behind the ring: barriers, then the place where the sums of the two sets meet.
+  static constexpr uint32_t kMeetBytes = kRows * kTokens * 4;
+  static constexpr uint32_t kSmemBytes = kStages * kStageBytes + 256 + kMeetBytes + 1024;
+  static_assert(kStages >= 3 && kSmemBytes <= 227 * 1024, "shared memory of a CTA");
+  static_assert(kStageBytes % 1024 == 0 && kQStageBytes % 1024 == 0, "swizzled boxes are 1 KiB aligned");
+};
+
+// Barriers of the expanding warps, and of the first set of them, which finishes a block.
+__device__ __forceinline__ void expanders_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kExpanders) : "memory"); }
+__device__ __forceinline__ void first_set_sync() { asm volatile("bar.sync 2, %0;" ::"n"(16 * kExpanders) : "memory"); }
+
+template <bool kBf16, int kTokens, bool kPhase, int kGroup>
+__global__ void __launch_bounds__(kThreads, 1)
+gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_a, const W4 p,
+               uint32_t idesc, int *status) {
+  using S = Shape<kTokens, kPhase, kGroup>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  const uint32_t smem_base = (raw_addr + 1023u) & ~1023u;
+  uint8_t *smem_gen = smem_raw + (smem_base - raw_addr);
+  const uint32_t bar_base = smem_base + S::kStages * S::kStageBytes;
+  auto full_bar = [&](uint32_t s) { return bar_base + 8u * s; };                    // q and A have arrived
+  auto empty_bar = [&](uint32_t s) { return bar_base + 8u * (S::kStages + s); };    // both have been read
+  auto order_bar = [&](uint32_t s) { return bar_base + 8u * (2 * S::kStages + s); };  // A is in order (arrangers)
+  auto operand_bar = [&](uint32_t set, uint32_t b) { return bar_base + 8u * (3 * S::kStages + 2 * set + b); };  // expanded
+  auto done_bar = [&](uint32_t set, uint32_t b) { return bar_base + 8u * (3 * S::kStages + 4 + 2 * set + b); };  // multiplied
+  constexpr uint32_t kMiscOff = S::kStages * S::kStageBytes + 8u * (3 * S::kStages + 8);
+  static_assert(8 * (3 * S::kStages + 8) + 12 <= 256, "barriers");
+  volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(smem_gen + kMiscOff);
+  volatile uint32_t *last_flag = abort_flag + 1;
+  volatile uint32_t *tmem_slot = abort_flag + 2;
+  const int warp = static_cast<int>(threadIdx.x >> 5), lane = static_cast<int>(threadIdx.x & 31);
+  if (threadIdx.x == 0) {
+    for (uint32_t s = 0; s < S::kStages; ++s) {
+      mbar_init(full_bar(s), 1 + (kPhase ? 32 * kHelpers : 0));
+      mbar_init(empty_bar(s), kExpanders + 2);  // every expanding warp, and the products of each half
+      mbar_init(order_bar(s), kHelpers);
+    }
+    for (uint32_t i = 0; i < 4; ++i) {
+      mbar_init(operand_bar(i >> 1, i & 1), kExpanders / 2);
+      mbar_init(done_bar(i >> 1, i & 1), 1);
+    }
+    *abort_flag = 0;
+    mbar_fence_init();
+    if (!kPhase)
+      tma_prefetch_descriptor(&tmap_q);
+    tma_prefetch_descriptor(&tmap_a);
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(smem_u32(const_cast<uint32_t *>(tmem_slot)), S::kTmemColumns);
+    tmem_relinquish_alloc_permit();
+  }
+  tcgen05_fence_before_sync();
+  __syncthreads();
+  tcgen05_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+
+  const int cta = static_cast<int>(blockIdx.x);
+  const int unit_begin = first_unit(p, cta), unit_end = first_unit(p, cta + 1);
+  const int stages_k = p.stages_k;
+
+  if (warp == kProducerWarp) {
+    // ------------------------------------------------------------ producer ----------
+    uint32_t stage = 0, phase = 0;
+    int block = unit_begin / stages_k, ks = unit_begin - block * stages_k;
+    for (int unit = unit_begin; unit < unit_end; ++unit) {
+      const bool free = mbar_wait_asleep(empty_bar(stage), phase ^ 1u, abort_flag);
+      if (!__all_sync(0xffffffffu, free))
+        break;
+      if (lane == 0) {
+        const uint32_t q_dst = smem_base + stage * S::kStageBytes, a_dst = q_dst + S::kQStageBytes;
+        mbar_arrive_expect_tx(full_bar(stage), kPhase ? S::kABytes : S::kStageBytes);
+        if (!kPhase)
+          tma_load_2d(q_dst, &tmap_q, full_bar(stage), ks * 128, block * kRows);
+#pragma unroll
+        for (int j = 0; j < kStageK / 64; ++j)
+          tma_load_2d(a_dst + j * S::kABoxBytes, &tmap_a, full_bar(stage), ks * kStageK + j * 64, 0);
+      }
+      __syncwarp();
+      if (++stage == S::kStages) {
+        stage = 0;
+        phase ^= 1u;
+      }
+      if (++ks == stages_k) {
+        ks = 0;
+        ++block;
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    // ------------------------------------------------------------ MMA issuer --------
+    uint32_t stage = 0, phase = 0, turn = 0;  // turn: stages done so far, modulo 2
+    bool ok = true;
+    for (int unit = unit_begin; ok && unit < unit_end; ++unit) {
+      const uint32_t a_addr = smem_base + stage * S::kStageBytes + S::kQStageBytes;
+      const bool ready = mbar_wait(order_bar(stage), phase, abort_flag);
+      if (!__all_sync(0xffffffffu, ready))
+        break;
+      if (lane == 0) {
+#pragma unroll
+        for (uint32_t step = 0; step < 2; ++step) {
+#pragma unroll
+          for (uint32_t set = 0; set < 2; ++set) {
+            if (ok && !mbar_wait(operand_bar(set, step), turn, abort_flag))
+              ok = false;
+            if (!ok)
+              continue;
+            tcgen05_fence_after_sync();
+            const uint32_t slot = kGroup == 128 ? turn : S::kSlots == 2 ? step : 0u;
+            const uint32_t sums = tmem_base + kSumsAt + (set * S::kSlots + slot) * (S::kAccs * kTokens);
+            const uint32_t operand = tmem_base + (2 * set + step) * kOperandColumns;
+            // 64 of k are one box of A.
+            const uint64_t desc = make_smem_desc_sw128(a_addr + (2 * set + step) * S::kABoxBytes, 16, 1024);
+#pragma unroll
+            for (uint32_t kk = 0; kk < kStepK / 16; ++kk) {
+              const bool first = kGroup == 128 ? step == 0 && kk == 0 : (kk * 16) % kGroup == 0;
+              umma_f16_ts(sums + (kGroup == 32 ? kk / 2 : 0) * kTokens, operand + kk * 8, desc + kk * 2, idesc, first ? 0u : 1u);
+            }
+            umma_commit(done_bar(set, step));
+            if (step == 1)
+              umma_commit(empty_bar(stage));  // this half of A's stage has been read
+          }
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+      turn ^= 1u;
+      if (++stage == S::kStages) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    }
+  } else if (warp >= kFirstHelper) {
+    // ------------------------------------------------------------ helpers -----------
+    const int helper = warp - kFirstHelper;
+    // A is put in order so many units behind the copies (fewer than the ring holds): by then they have mostly
+    // landed, and the copies stay ahead.
+    constexpr int kBehind = kPhase ? 2 : 0;
+    uint32_t stage = 0, phase = 0, arrange_stage = 0, arrange_phase = 0;
+    int block = unit_begin / stages_k, ks = unit_begin - block * stages_k;
+    for (int unit = unit_begin; unit < unit_end + kBehind; ++unit) {
+      if (kPhase && unit < unit_end) {
+        const bool free = mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag);
+        if (!__all_sync(0xffffffffu, free))
+          break;
+        copy_stage(p, smem_base + stage * S::kStageBytes, full_bar(stage), block, ks, helper, kHelpers, lane);
+        if (++stage == S::kStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+        if (++ks == stages_k) {
+          ks = 0;
+          ++block;
+        }
+      }
+      if (unit >= unit_begin + kBehind) {
+        const bool ready = mbar_wait(full_bar(arrange_stage), arrange_phase, abort_flag);
+        if (!__all_sync(0xffffffffu, ready))
+          break;
+        arrange_rows(smem_base + arrange_stage * S::kStageBytes + S::kQStageBytes, S::kABoxBytes, helper, kHelpers, p.m, lane);
+        __syncwarp();
+        if (lane == 0)
+          mbar_arrive(order_bar(arrange_stage));
+        if (++arrange_stage == S::kStages) {
+          arrange_stage = 0;
+          arrange_phase ^= 1u;
+        }
+      }
+    }
+    if (kPhase)
+      asm volatile("cp.async.wait_all;" ::: "memory");
+  } else {
+    // ------------------------------------------------------------ expanding warps ---
+    const uint32_t set = static_cast<uint32_t>(warp >> 2);
+    const int local = (warp & 3) * 32 + lane;  // this lane's row of the block, and its tensor-memory lane
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t operands = tmem_base + lanes + 2 * set * kOperandColumns;
+    const uint32_t sums = tmem_base + lanes + kSumsAt + set * (S::kSlots * S::kAccs * kTokens);
+    float *const meet = reinterpret_cast<float *>(smem_gen + S::kStages * S::kStageBytes + 256);
+    uint32_t stage = 0, phase = 0, turn = 0;
+    bool used = false;  // whether the operand buffers hold an earlier stage's steps
+    int unit = unit_begin;
+    bool ok = true;  // (a wait that ran out: the barriers below are still met)
+    while (unit < unit_end) {
+      const int block = unit / stages_k, ks_begin = unit - block * stages_k;
+      const int ks_end = min(stages_k, ks_begin + (unit_end - unit));
+      float total[kTokens];
+#pragma unroll
+      for (int t = 0; t < kTokens; ++t)
+        total[t] = 0.0f;
+      // Adds the sums at `slot`, times their groups' scales.
+      auto collect = [&](uint32_t slot, const float *scale) {
+#pragma unroll
+        for (int j = 0; j < S::kAccs; ++j) {
+          const uint32_t at = sums + (slot * S::kAccs + j) * kTokens;
+#pragma unroll
+          for (int t0 = 0; t0 < kTokens; t0 += 16) {
+            uint32_t r[16];
+            tmem_load_32x32b_x16(at + t0, r);
+            tmem_load_wait();
+#pragma unroll
+            for (int t = 0; t < 16; ++t)
+              total[t0 + t] = fmaf(scale[j], __uint_as_float(r[t]), total[t0 + t]);
+          }
+        }
+      };
+      // Waits until the products of this set's step in buffer `b` of the stage with that turn are done.
+      auto wait_done = [&](uint32_t b, uint32_t of_turn) {
+        const bool done = mbar_wait(done_bar(set, b), of_turn, abort_flag);
+        if (!__all_sync(0xffffffffu, done))
+          ok = false;
+        tcgen05_fence_after_sync();
+      };
+      if (ok) {
+        // Rows past the end are computed on the last row's scales and not stored.
+        const long long row = static_cast<long long>(block) * kRows + local < p.n ? static_cast<long long>(block) * kRows + local : p.n - 1;
+        const uint16_t *const scales = p.scales + row * p.lds;
+        const uint8_t *const zeros = p.zeros != nullptr ? p.zeros + row * p.ldz : nullptr;
+        uint32_t row_at, row_shift = 0;
+        if constexpr (kPhase) {
+          const uint32_t at = static_cast<uint32_t>(
+              (reinterpret_cast<uintptr_t>(p.q) + (static_cast<long long>(block) * kRows + local) * p.ldq) & 15);
+          row_at = static_cast<uint32_t>(local) * kPhasePitch + set * 64 + (at & ~3u);
+          row_shift = 8 * (at & 3u);
+        } else {
+          row_at = static_cast<uint32_t>(local) * 128;
+        }
+        // Raw scales and zero points of this stage and the next two (a sector of them that is not in the cache
+        // yet takes longer to arrive than a stage takes to expand).
+        uint32_t raw[2][S::kGroupsPerHalf];
+        auto fetch = [&](int ks, uint32_t (&into)[S::kGroupsPerHalf]) {
+          // (p.span: how many of the kernel's groups share a scale, for groups of several times 128.)
+          const int first = (ks * 2 + static_cast<int>(set)) * S::kGroupsPerHalf;
+#pragma unroll
+          for (int j = 0; j < S::kGroupsPerHalf; ++j) {
+            const int group = min(p.span == 1 ? first + j : (first + j) / p.span, p.groups - 1);
+            into[j] = scales[group] | (zeros != nullptr ? zeros[group] : 8u) << 16;
+          }
+        };
+        fetch(ks_begin, raw[0]);
+        if (ks_begin + 1 < ks_end)
+          fetch(ks_begin + 1, raw[1]);
+        float before[S::kGroupsPerHalf];  // scales of the stage whose sums are not yet collected
+        bool pending = false;
+        for (int ks = ks_begin; ok && ks < ks_end; ++ks) {
+          float scale[S::kGroupsPerHalf];
+          Zero<kBf16> zero[S::kGroupsPerHalf];
+#pragma unroll
+          for (int j = 0; j < S::kGroupsPerHalf; ++j) {
+            scale[j] = scale_value<kBf16>(static_cast<uint16_t>(raw[0][j]));
+            zero[j].set(static_cast<int>(raw[0][j] >> 16));
+            raw[0][j] = raw[1][j];
+          }
+          if (ks + 2 < ks_end)
+            fetch(ks + 2, raw[1]);
+          const bool ready = mbar_wait(full_bar(stage), phase, abort_flag);
+          if (!__all_sync(0xffffffffu, ready)) {
+            ok = false;
+            break;
+          }
+          const uint32_t q_addr = smem_base + stage * S::kStageBytes + row_at;
+#pragma unroll
+          for (int step = 0; step < 2; ++step) {
+            if (!ok)
+              break;
+            uint32_t w[8], r[32];
+            if constexpr (kPhase) {
+              uint32_t low = lds32(q_addr + step * 32);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const uint32_t high = lds32(q_addr + step * 32 + i * 4 + 4);
+                w[i] = __funnelshift_r(low, high, row_shift);
+                low = high;
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const uint32_t piece = set * 4 + static_cast<uint32_t>(2 * step + i);
+                const uint4 v = lds128(q_addr + ((piece ^ (static_cast<uint32_t>(lane) & 7u)) << 4));
+                w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              expand(w[i], zero[(step * 8 + i) * 8 / kGroup], r + 4 * i);
+            if (step == 1) {
+              __syncwarp();
+              if (lane == 0)
+                mbar_arrive(empty_bar(stage));  // this warp's rows of q have been read
+            }
+            if (used)
+              wait_done(static_cast<uint32_t>(step), turn ^ 1u);  // the step that had this buffer a stage ago
+            tmem_store_x32(operands + static_cast<uint32_t>(step) * kOperandColumns, r);
+            // Sums that this step's products overwrite are collected first; they are done, by the wait above
+            // (with one place only, they are those of the step before, which are waited for here).
+            if constexpr (kGroup != 128 && S::kSlots == 2) {
+              if (pending)
+                collect(static_cast<uint32_t>(step), before + step * S::kAccs);
+            }
+            if constexpr (S::kSlots == 1) {
+              if (step == 0 ? pending : true) {
+                wait_done(static_cast<uint32_t>(step ^ 1), step == 0 ? turn ^ 1u : turn);
+                collect(0, step == 0 ? before + S::kAccs : scale);
+              }
+            }
+            tmem_store_wait();
+            tcgen05_fence_before_sync();
+            __syncwarp();
+            if (lane == 0)
+              mbar_arrive(operand_bar(set, static_cast<uint32_t>(step)));
+          }
+          // Groups of a whole stage half: the stage before is done, both its buffers having been waited for.
+          if constexpr (kGroup == 128) {
+            if (pending)
+              collect(turn ^ 1u, before);
+          }
+#pragma unroll
+          for (int j = 0; j < S::kGroupsPerHalf; ++j)
+            before[j] = scale[j];
+          pending = used = true;
+          turn ^= 1u;
+          if (++stage == S::kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (ok && pending) {  // the last stage of the segment
+          wait_done(0, turn ^ 1u);
+          wait_done(1, turn ^ 1u);
+          if constexpr (kGroup == 128) {
+            collect(turn ^ 1u, before);
+          } else if constexpr (S::kSlots == 2) {
+            collect(0, before);
+            collect(1, before + S::kAccs);
+          } else {
+            collect(0, before + S::kAccs);
+          }
+          tcgen05_fence_before_sync();
+        }
+      }
+      unit += ks_end - ks_begin;
+
+      // The two sets meet in shared memory; a lane holds a row of q, i.e. a column of C.
+      if (set == 1) {
+#pragma unroll
+        for (int t = 0; t < kTokens; ++t)
+          meet[t * kRows + local] = total[t];
+      }
+      expanders_sync();
+      if (set == 0) {
+#pragma unroll
+        for (int t = 0; t < kTokens; ++t)
+          total[t] += meet[t * kRows + local];
+        bool store = true;
+        if (ks_begin != 0 || ks_end != stages_k) {
+          constexpr int kSlot = kRows * kTokens;
+          const int first = owner_of(p, block * stages_k), last = owner_of(p, (block + 1) * stages_k - 1);
+          float *mine = part_slot(p, cta, first, block, kSlot) + local;
+#pragma unroll
+          for (int t = 0; t < kTokens; ++t)
+            if (t < p.m)
+              __stcg(mine + t * kRows, total[t]);
+          store = count_part(p, block, last - first + 1, last_flag, [] { first_set_sync(); });
+          if (store) {
+#pragma unroll
+            for (int t = 0; t < kTokens; ++t)
+              total[t] = 0.0f;
+            for (int part = first; part <= last; ++part) {
+              const float *from = part_slot(p, part, first, block, kSlot) + local;
+#pragma unroll
+              for (int t = 0; t < kTokens; ++t)
+                if (t < p.m)
+                  total[t] += __ldcg(from + t * kRows);
+            }
+          }
+        }
+        const long long column = static_cast<long long>(block) * kRows + local;
+        if (store && column < p.n) {
+#pragma unroll
+          for (int t = 0; t < kTokens; ++t)
+            if (t < p.m)
+              store_c_element(p.c, t * p.ldc + column, total[t], p.c_dtype);
+        }
+      }
+      expanders_sync();  // `meet` is free again
+    }
+  }
+
+  tcgen05_fence_before_sync();
+  __syncthreads();
+  tcgen05_fence_after_sync();
+  if (*abort_flag != 0) {
+    if (threadIdx.x == 0)
+      atomicCAS(status, 0, kStatusDeviceWaitTimeout);
+    const long long start = clock64();
+    while (clock64() - start < 2000000LL) {
+    }
+    __syncthreads();
+  }
+  if (warp == kMmaWarp)
+    tmem_dealloc(tmem_base, S::kTmemColumns);
+}
+
+}  // namespace many
+
+// ---------------------------------------------------------------- launch ------------------------
+
+template <typename Kernel>
+cudaError_t allow_shared(Kernel kernel, uint32_t bytes, int *configured_device) {
   int device = 0;
   cudaError_t err = cudaGetDevice(&device);
-  if (err != cudaSuccess)
-    return err;
-  if (configured_device != device) {
-    err = cudaFuncSetAttribute(gemm_w4_kernel<kBf16, kTiles, kPhase, kGroup>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               static_cast<int>(R::kSmemBytes));
+  if (err == cudaSuccess && *configured_device != device) {
+    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+    if (err == cudaSuccess)
+      *configured_device = device;
+  }
+  return err;
+}
+
+template <bool kBf16, int kTokens, bool kPhase, int kGroup>
+cudaError_t launch(const CUtensorMap &tmap_q, const CUtensorMap &tmap_a, const W4 &p, int *status, cudaStream_t stream) {
+  static thread_local int configured_device = -1;
+  if constexpr (kTokens <= 16) {
+    using S = few::Shape<kTokens / 8, kPhase, kGroup>;
+    auto kernel = few::gemm_w4_few_kernel<kBf16, kTokens / 8, kPhase, kGroup>;
+    const cudaError_t err = allow_shared(kernel, S::kSmemBytes, &configured_device);
     if (err != cudaSuccess)
       return err;
-    configured_device = device;
+    kernel<<<static_cast<unsigned>(p.grid), few::kThreads, S::kSmemBytes, stream>>>(tmap_q, tmap_a, p, status);
+  } else {
+    using S = many::Shape<kTokens, kPhase, kGroup>;
+    auto kernel = many::gemm_w4_kernel<kBf16, kTokens, kPhase, kGroup>;
+    const cudaError_t err = allow_shared(kernel, S::kSmemBytes, &configured_device);
+    if (err != cudaSuccess)
+      return err;
+    const uint32_t idesc = make_idesc_f16(kBf16 ? 1u : 0u, false, false, kRows, kTokens);
+    kernel<<<static_cast<unsigned>(p.grid), many::kThreads, S::kSmemBytes, stream>>>(tmap_q, tmap_a, p, idesc, status);
   }
-  gemm_w4_kernel<kBf16, kTiles, kPhase, kGroup><<<p.grid, kThreads, R::kSmemBytes, stream>>>(tmap_q, tmap_a, p, status);
   return cudaGetLastError();
 }
 
 template <bool kBf16>
 cudaError_t launch_w4(const CUtensorMap &tmap_q, const CUtensorMap &tmap_a, const W4 &p, int *status, cudaStream_t stream) {
-  const int tiles = w4_tiles(p.m);
+  const int tokens = w4_tokens(p.m);
   const bool phase = p.phase != 0;
-#define HC_W4(TILES, GROUP)                                                               \
-  return phase ? launch<kBf16, TILES, true, GROUP>(tmap_q, tmap_a, p, status, stream)     \
-               : launch<kBf16, TILES, false, GROUP>(tmap_q, tmap_a, p, status, stream)
-#define HC_W4_GROUPS(TILES) \
-  {                         \
-    if (p.group == 32)      \
-      HC_W4(TILES, 32);     \
-    if (p.group == 64)      \
-      HC_W4(TILES, 64);     \
-    HC_W4(TILES, 128);      \
+#define HC_W4(TOKENS, GROUP)                                                               \
+  return phase ? launch<kBf16, TOKENS, true, GROUP>(tmap_q, tmap_a, p, status, stream)     \
+               : launch<kBf16, TOKENS, false, GROUP>(tmap_q, tmap_a, p, status, stream)
+#define HC_W4_GROUPS(TOKENS) \
+  {                          \
+    if (p.group == 32)       \
+      HC_W4(TOKENS, 32);     \
+    if (p.group == 64)       \
+      HC_W4(TOKENS, 64);     \
+    HC_W4(TOKENS, 128);      \
   }
-  if (tiles == 1)
-    HC_W4_GROUPS(1)
-  if (tiles == 2)
-    HC_W4_GROUPS(2)
-  if (tiles == 4)
-    HC_W4_GROUPS(4)
-  HC_W4_GROUPS(8)
+  if (tokens == 8)
+    HC_W4_GROUPS(8)
+  if (tokens == 16)
+    HC_W4_GROUPS(16)
+  if (tokens == 32)
+    HC_W4_GROUPS(32)
+  HC_W4_GROUPS(64)
 #undef HC_W4_GROUPS
 #undef HC_W4
 }

@@ -75,6 +75,37 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
   return true;
 }
 
+// The same wait for kernels whose other warps are short of issue slots: the thread sleeps in the
+// hardware, for up to about 4 us at a time, instead of polling.
+__device__ __forceinline__ bool mbar_wait_asleep(uint32_t bar, uint32_t parity, volatile uint32_t *abort_flag,
+                                                 long long timeout_cycles = kWaitTimeoutCycles) {
+  auto asleep = [&]() {
+    uint32_t done;
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
+        "selp.u32 %0, 1, 0, p;\n"
+        "}\n"
+        : "=r"(done)
+        : "r"(bar), "r"(parity), "r"(4000u)
+        : "memory");
+    return done != 0;
+  };
+  if (asleep())
+    return true;
+  const long long start = clock64();
+  while (!asleep()) {
+    if (*abort_flag != 0)
+      return false;
+    if (clock64() - start > timeout_cycles) {
+      *abort_flag = 1;
+      return false;
+    }
+  }
+  return true;
+}
+
 // ---------------------------------------------------------------- TMA ---------------
 
 __device__ __forceinline__ void tma_prefetch_descriptor(const CUtensorMap *map) {

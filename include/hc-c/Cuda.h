@@ -558,8 +558,8 @@ HC_CUDA_CAPI_EXPORTED int hcCudaLinearLossBackwardPlan(const HcCudaLinearLossBac
  * 128; the last group of a row may be shorter. Everything is summed in float32 (the weights enter as integers,
  * the scales multiply the sums of their groups) and rounded once into C: float32, or A's type. The same bits
  * every call. It is to a matrix of 4-bit weights what the skinny variant of hcCudaGemm is to one of 16 bits:
- * HBM bound up to about 16 rows. A whose base or pitch is not a multiple of 16 bytes costs a repack launch; q
- * is read where it stands, fastest when its rows start on 16-byte boundaries. m == 0 or n == 0 writes
+ * HBM bound for few rows. An A of several rows whose base or pitch is not a multiple of 16 bytes costs a
+ * repack launch; q is read where it stands, fastest when its rows start on 16-byte boundaries. m == 0 or n == 0 writes
  * nothing; k == 0 sets C to zero. No counterpart in the reference. */
 typedef struct HcCudaGemmW4Args {
   int64_t m, n, k;

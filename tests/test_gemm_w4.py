@@ -28,8 +28,9 @@ def test_plans() -> None:
     assert (status, info.kernel_launches, info.pieces) == (OK, 1, 1) and info.scratch_bytes > 0
     assert plan(zeros=None)[0] == OK
     assert plan(lda=513)[1].kernel_launches == 2 and plan(a=A + 2)[1].kernel_launches == 2  # one repack of A
-    assert plan(k=513)[1].kernel_launches == 2
-    assert plan(q=Q + 1)[1].kernel_launches == 1 and plan(ldq=257)[1].kernel_launches == 1  # q stays where it is
+    assert plan(k=513)[1].kernel_launches == 2 and plan(m=1, k=513)[1].kernel_launches == 1  # one row has no pitch
+    assert plan(m=1, a=A + 2)[1].kernel_launches == 2
+    assert plan(q=Q + 1)[1].kernel_launches == 1 and plan(ldq=257)[1].kernel_launches == 1   # q stays where it is
     for group in (32, 64, 128, 256, 384, 4096):
         assert plan(k=4096, group=group)[0] == OK
     for empty in ({"m": 0}, {"n": 0}):
@@ -43,6 +44,8 @@ def test_plans() -> None:
     ({"m": -1}, INVALID, "m, n, k must be non-negative"),
     ({"m": 65}, UNSUPPORTED, "m <= 64"),
     ({"n": (1 << 30) + 1}, UNSUPPORTED, "at most 2^30"),
+    ({"n": 1 << 30, "k": 1 << 30, "lda": 1 << 30, "ldq": 1 << 29, "lds": 1 << 23, "ldz": 1 << 23, "ldc": 1 << 30,
+      "a": 1 << 62, "q": 1 << 63, "scales": 1 << 60, "zeros": 1 << 61, "c": 4096}, UNSUPPORTED, "too large"),
     ({"dtype": cuda.F8E4M3}, INVALID, "dtype"),
     ({"c_dtype": cuda.C_F16}, INVALID, "c_dtype"),
     ({"group": 0}, INVALID, "group"),
