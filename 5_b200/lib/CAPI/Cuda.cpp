@@ -2027,13 +2027,13 @@ int plan_layer_norm_backward(const HcCudaContext *ctx, const HcCudaLayerNormBack
   *plan = HcCudaOperatorPlanInfo{0, 0, 0};
   if (args->rows == 0 || args->cols == 0)
     return HC_CUDA_OK;
-  const int vec = hc::sm100::layer_norm_vector(args->dtype, args->dy, args->lddy, args->x, args->ldx, args->dx, args->lddx);
+  const int vec = hc::sm100::layer_norm_vector(args->dtype, args->cols, args->dy, args->lddy, args->x, args->ldx, args->dx, args->lddx);
   const bool params = args->dweight != nullptr || args->dbias != nullptr;
   plan->pieces = 1;
-  plan->kernel_launches = hc::sm100::layer_norm_backward_launches(args->rows, args->cols, vec, params);
+  plan->kernel_launches = hc::sm100::layer_norm_backward_launches(args->rows, args->cols, vec, args->dtype, params);
   if (params)
     plan->scratch_bytes =
-        static_cast<int64_t>(hc::sm100::layer_norm_backward_scratch(args->rows, args->cols, vec, sm_count));
+        static_cast<int64_t>(hc::sm100::layer_norm_backward_scratch(args->rows, args->cols, vec, args->dtype, sm_count));
   return HC_CUDA_OK;
 }
 
@@ -2064,7 +2064,7 @@ int hcCudaLayerNorm(HcCudaContext *ctx, const HcCudaLayerNormArgs *args) {
   HC_TRY_CUDA(ctx, cudaSetDevice(ctx->device));
   HC_TRY_CUDA(ctx, hc::sm100::launch_layer_norm(args->x, args->ldx, args->weight, args->bias, args->y, args->ldy,
                                                 args->mean, args->rstd, args->rows, args->cols, args->eps, args->dtype,
-                                                args->param_dtype, ctx->prop.multiProcessorCount, ctx->stream));
+                                                args->param_dtype, ctx->prop.multiProcessorCount, ctx->status_dev, ctx->stream));
   return HC_CUDA_OK;
 }
 
@@ -2090,7 +2090,7 @@ int hcCudaLayerNormBackward(HcCudaContext *ctx, const HcCudaLayerNormBackwardArg
   HC_TRY_CUDA(ctx, hc::sm100::launch_layer_norm_backward(
                        args->dy, args->lddy, args->x, args->ldx, args->weight, args->mean, args->rstd, args->dx, args->lddx,
                        args->dweight, args->dbias, static_cast<float *>(ctx->scratch), args->rows, args->cols, args->dtype,
-                       args->param_dtype, sm_count, ctx->stream));
+                       args->param_dtype, sm_count, ctx->status_dev, ctx->stream));
   return HC_CUDA_OK;
 }
 

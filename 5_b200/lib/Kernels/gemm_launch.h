@@ -302,21 +302,21 @@ cudaError_t launch_map_f32(const float *x, const float *y, float *out, long long
 
 // ---- layer norm --------------------------------------------------------------------------------
 // dtype and param_dtype: kCTypeF32, kCTypeF16 or kCTypeBF16; param_dtype is float32 or dtype.
-// layer_norm_vector: elements per access for three matrices (16 bytes' worth, or 1 when a base or pitch
-// rules that out).
-int layer_norm_vector(int dtype, const void *a, long long lda, const void *b, long long ldb, const void *c,
+// layer_norm_vector: elements per access for three matrices (16 bytes' worth, or 1 when a base, a pitch
+// or the number of columns rules that out).
+int layer_norm_vector(int dtype, long long cols, const void *a, long long lda, const void *b, long long ldb, const void *c,
                       long long ldc);
 cudaError_t launch_layer_norm(const void *x, long long ldx, const void *weight, const void *bias, void *y,
                               long long ldy, float *mean, float *rstd, long long rows, long long cols, float eps,
-                              int dtype, int param_dtype, int sm_count, cudaStream_t stream);
+                              int dtype, int param_dtype, int sm_count, int *status, cudaStream_t stream);
 // `partials`: layer_norm_backward_scratch bytes (with vec = layer_norm_vector of dy, x and dx), used when
 // dweight or dbias is wanted.
-int layer_norm_backward_launches(long long rows, long long cols, int vec, bool params);
-size_t layer_norm_backward_scratch(long long rows, long long cols, int vec, int sm_count);
+int layer_norm_backward_launches(long long rows, long long cols, int vec, int dtype, bool params);
+size_t layer_norm_backward_scratch(long long rows, long long cols, int vec, int dtype, int sm_count);
 cudaError_t launch_layer_norm_backward(const void *dy, long long lddy, const void *x, long long ldx, const void *weight,
                                        const float *mean, const float *rstd, void *dx, long long lddx, void *dweight,
                                        void *dbias, float *partials, long long rows, long long cols, int dtype,
-                                       int param_dtype, int sm_count, cudaStream_t stream);
+                                       int param_dtype, int sm_count, int *status, cudaStream_t stream);
 
 // ---- softmax cross entropy of a linear layer ------------------------------------------------------
 // One launch over the logits H W^T of `rows` rows of H and `vocab` rows of W (the tensor maps: H as

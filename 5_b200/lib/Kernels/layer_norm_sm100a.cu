@@ -21,7 +21,14 @@
 //
 // Rows that are too long for the registers of a CTA are walked several times (the later walks mostly
 // hit the L2); dw and db then come from a kernel of their own that walks columns.
+//
+// Large matrices go through persistent kernels whose rows arrive in shared memory by bulk copies some rows
+// ahead (below). Measured: 16384 x 4096 bfloat16 forward 54.5 us (4.9 TB/s), backward 115 us (3.5 TB/s); 4000 x
+// 8192 float32 49.4 us (5.3 TB/s) and 91 us (4.3 TB/s). What holds the 16-bit ones back is no longer memory
+// but arithmetic and its latency (0.6 instructions a cycle and scheduler with four warps, the registers being
+// full), which is why the sums and the scaling work on pairs of floats in one instruction.
 #include "gemm_launch.h"
+#include "sm100_ptx.cuh"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -140,6 +147,13 @@ __device__ __forceinline__ float row_sum(float v, float *shared) {
   if (lane == 0)
     shared[warp] = v;
   __syncthreads();
+  if (warps <= 8) {  // (the same for the whole CTA)
+    v = lane < warps ? shared[lane] : 0.0f;
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1)
+      v += __shfl_xor_sync(0xffffffffu, v, o);
+    return __shfl_sync(0xffffffffu, v, 0);
+  }
   return warp_sum(lane < warps ? shared[lane] : 0.0f);
 }
 
@@ -188,7 +202,7 @@ layer_norm_kernel(const Forward f) {
         square = fmaf(v[j][i], v[j][i], square);
     }
   }
-  const float rstd = 1.0f / sqrtf(row_sum<kWarpRow>(square, sums[1]) * inv + f.eps);
+  const float rstd = rsqrtf(row_sum<kWarpRow>(square, sums[1]) * inv + f.eps);
   T *y = static_cast<T *>(f.y) + r * f.ldy;
 #pragma unroll
   for (int j = 0; j < kPacks; ++j) {
@@ -244,7 +258,7 @@ layer_norm_long_kernel(const Forward f) {
     }
     square += part;
   }
-  const float rstd = 1.0f / sqrtf(row_sum<false>(square, sums[1]) * inv + f.eps);
+  const float rstd = rsqrtf(row_sum<false>(square, sums[1]) * inv + f.eps);
   for (long long c = first; c < cols; c += step) {
     const Pack<T, kVec> p = load_pack<T, kVec>(x, c, cols);
     float w[kVec], b[kVec];
@@ -500,86 +514,628 @@ layer_norm_partials_kernel(const float *partials, int count, long long cols, P *
     out[column] = from_float<P>(total);
 }
 
+// ---------------------------------------------------------------- rows through a ring in shared memory ------
+//
+// For many rows: a CTA is persistent and its rows arrive by cp.async.bulk a few rows ahead, so that the bytes
+// in flight depend neither on registers nor on how far the arithmetic has got. Rows at odd places are copied
+// from the 16-byte boundary below their first element to the one above their last (never behind the matrix:
+// there the last few elements are read where they stand) and read element by element.
+
+// How a thread's kPer elements lie: packs of kVec, a pack of every thread after another.
+template <int kVec>
+__device__ __forceinline__ int element_of(int t, int j, int threads) {
+  return (t + j / kVec * threads) * kVec + j % kVec;
+}
+
+__device__ __forceinline__ float2 splat(float v) { return make_float2(v, v); }
+
+// A row's copy: where it starts in memory, how many bytes come by the bulk copy.
+struct RowCopy {
+  uintptr_t low;
+  uint32_t bytes;
+  __device__ __forceinline__ RowCopy(const void *base, long long row, long long ld, long long cols, long long rows, int size) {
+    const uintptr_t first = reinterpret_cast<uintptr_t>(base) + static_cast<uintptr_t>(row * ld * size);
+    const uintptr_t end = reinterpret_cast<uintptr_t>(base) + static_cast<uintptr_t>(((rows - 1) * ld + cols) * size);
+    low = first & ~uintptr_t{15};
+    uintptr_t high = (first + static_cast<uintptr_t>(cols * size) + 15) & ~uintptr_t{15};
+    if (high > end)
+      high = end & ~uintptr_t{15};
+    bytes = high > low ? static_cast<uint32_t>(high - low) : 0u;
+  }
+};
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, uintptr_t src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               :: "r"(dst), "l"(static_cast<uint64_t>(src)), "r"(bytes), "r"(bar)
+               : "memory");
+}
+
+// A thread's elements of a row in the ring as floats, zeros past its end. `place`: the row's slot; only the
+// matrix's last row may have elements that were not copied. (Packs are whole: kVec > 1 divides cols.)
+template <typename T, int kVec, int kPer>
+__device__ __forceinline__ void read_row(float2 (&pairs)[kPer / 2], const uint8_t *place, const T *row, int cols, const RowCopy &copy,
+                                         bool last, int t, int threads) {
+  float v[kPer];
+  const int lead = kVec > 1 ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(row) - copy.low);  // bytes
+  if (kVec == 1 && last) {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const int c = t + j * threads, at = lead + c * static_cast<int>(sizeof(T));
+      v[j] = c >= cols ? 0.0f
+             : at + static_cast<int>(sizeof(T)) <= static_cast<int>(copy.bytes) ? to_float(*reinterpret_cast<const T *>(place + at))
+                                                                                : to_float(row[c]);
+    }
+  } else {
+#pragma unroll
+    for (int q = 0; q < kPer / kVec; ++q) {
+      const int c = (t + q * threads) * kVec;
+      Pack<T, kVec> p = zero_pack<T, kVec>();
+      if (c < cols)
+        p = *reinterpret_cast<const Pack<T, kVec> *>(place + lead + c * static_cast<int>(sizeof(T)));
+#pragma unroll
+      for (int i = 0; i < kVec; ++i)
+        v[q * kVec + i] = to_float(p.v[i]);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kPer / 2; ++j)
+    pairs[j] = make_float2(v[2 * j], v[2 * j + 1]);
+}
+
+// A thread's share of a weight or bias vector, kept for all rows as it lies in memory.
+template <typename P, int kVec, int kPer>
+struct Params {
+  Pack<P, kVec> v[kPer / kVec];
+  __device__ __forceinline__ Params(const P *p, int cols, int t, int threads, float fallback) {
+#pragma unroll
+    for (int q = 0; q < kPer / kVec; ++q) {
+      const int c = (t + q * threads) * kVec;
+#pragma unroll
+      for (int i = 0; i < kVec; ++i)
+        v[q].v[i] = p != nullptr && c < cols ? p[c + i] : from_float<P>(fallback);
+    }
+  }
+  __device__ __forceinline__ float operator[](int j) const { return to_float(v[j / kVec].v[j % kVec]); }
+  __device__ __forceinline__ float2 pair(int j) const { return make_float2((*this)[2 * j], (*this)[2 * j + 1]); }
+};
+
+// kVec elements from column c of a row or, one by one, those at c and c + step; nothing past the end.
+template <typename T, int kVec>
+__device__ __forceinline__ void store_unit(T *row, int c, int step, int cols, const T (&v)[kVec > 1 ? kVec : 2]) {
+  if constexpr (kVec > 1) {
+    if (c < cols) {
+      Pack<T, kVec> p;
+#pragma unroll
+      for (int i = 0; i < kVec; ++i)
+        p.v[i] = v[i];
+      *reinterpret_cast<Pack<T, kVec> *>(row + c) = p;
+    }
+  } else {
+    if (c < cols)
+      row[c] = v[0];
+    if (c + step < cols)
+      row[c + step] = v[1];
+  }
+}
+
+struct Ring {
+  int stages;
+  uint32_t slot;    // bytes of one matrix's row in a stage, a multiple of 16
+  int rows, parts;  // backward: rows of a tile, warps that share one (rows x parts warps in all)
+};
+
+template <typename T, typename P, int kVec, int kPer, int kThreads, int kCtas>
+__global__ void __launch_bounds__(kThreads, kCtas)
+layer_norm_ring_kernel(const Forward f, const Ring ring, int *status) {
+  extern __shared__ __align__(128) uint8_t shared[];
+  __shared__ float sums[2][2][32];
+  __shared__ uint32_t abort_word;
+  volatile uint32_t *abort_flag = &abort_word;
+  const int t = threadIdx.x, threads = blockDim.x, cols = static_cast<int>(f.cols);
+  const uint32_t bars = smem_u32(shared), slots = bars + 128;
+  const uint8_t *const slots_gen = shared + 128;
+  const T *x = static_cast<const T *>(f.x);
+  auto load = [&](long long row, int stage) {
+    const RowCopy copy(x, row, f.ldx, f.cols, f.rows, sizeof(T));
+    mbar_arrive_expect_tx(bars + 8u * stage, copy.bytes);
+    if (copy.bytes != 0)
+      bulk_load(slots + stage * ring.slot, copy.low, copy.bytes, bars + 8u * stage);
+  };
+  if (t == 0) {
+    for (int s = 0; s < ring.stages; ++s)
+      mbar_init(bars + 8u * s, 1);
+    abort_word = 0;
+    mbar_fence_init();
+    for (int s = 0; s < ring.stages; ++s)
+      if (blockIdx.x + static_cast<long long>(s) * gridDim.x < f.rows)
+        load(blockIdx.x + static_cast<long long>(s) * gridDim.x, s);
+  }
+  const Params<P, kVec, kPer> weight(static_cast<const P *>(f.weight), cols, t, threads, 1.0f);
+  const Params<P, kVec, kPer> bias(static_cast<const P *>(f.bias), cols, t, threads, 0.0f);
+  __syncthreads();
+  const float inv = 1.0f / static_cast<float>(cols);
+  int stage = 0, turn = 0;
+  uint32_t parity = 0;
+  for (long long r = blockIdx.x; r < f.rows; r += gridDim.x, turn ^= 1) {
+    const T *row = x + r * f.ldx;
+    float2 v[kPer / 2];
+    mbar_wait(bars + 8u * stage, parity, abort_flag);
+    read_row<T, kVec, kPer>(v, slots_gen + stage * ring.slot, row, cols,
+                            RowCopy(x, r, f.ldx, f.cols, f.rows, sizeof(T)), r == f.rows - 1, t, threads);
+    float2 two = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int j = 0; j < kPer / 2; ++j)
+      two = __fadd2_rn(two, v[j]);
+    const float sum = two.x + two.y;
+    const float mean = row_sum<false>(sum, sums[turn][0]) * inv;
+    if (t == 0 && r + static_cast<long long>(ring.stages) * gridDim.x < f.rows)
+      load(r + static_cast<long long>(ring.stages) * gridDim.x, stage);  // every thread has read the slot
+    if (++stage == ring.stages) {
+      stage = 0;
+      parity ^= 1u;
+    }
+    two = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int j = 0; j < kPer / 2; ++j) {
+      if (element_of<kVec>(t, 2 * j, threads) < cols) {
+        v[j] = __fadd2_rn(v[j], splat(-mean));
+        if (kVec == 1 && element_of<kVec>(t, 2 * j + 1, threads) >= cols)
+          v[j].y = 0.0f;
+        two = __ffma2_rn(v[j], v[j], two);
+      }
+    }
+    const float square = two.x + two.y;
+    const float rstd = rsqrtf(row_sum<false>(square, sums[turn][1]) * inv + f.eps);
+    T *y = static_cast<T *>(f.y) + r * f.ldy;
+    constexpr int kUnit = kVec > 1 ? kVec : 2;
+#pragma unroll
+    for (int u = 0; u < kPer / kUnit; ++u) {
+      T out[kUnit];
+#pragma unroll
+      for (int i = 0; i < kUnit / 2; ++i) {
+        const int j = u * (kUnit / 2) + i;
+        const float2 o = __ffma2_rn(__fmul2_rn(v[j], splat(rstd)), weight.pair(j), bias.pair(j));
+        out[2 * i] = from_float<T>(o.x);
+        out[2 * i + 1] = from_float<T>(o.y);
+      }
+      store_unit<T, kVec>(y, element_of<kVec>(t, u * kUnit, threads), threads, cols, out);
+    }
+    if (t == 0) {
+      if (f.mean != nullptr)
+        f.mean[r] = mean;
+      if (f.rstd != nullptr)
+        f.rstd[r] = rstd;
+    }
+  }
+  __syncthreads();
+  if (t == 0 && abort_word != 0)
+    atomicCAS(status, 0, kStatusDeviceWaitTimeout);
+}
+
+// Backward: a stage holds a tile of ring.rows rows of x and dy, and a tile is gone through twice. First the warps
+// share its rows, ring.parts warps a row, and find the two sums of each; then, with one barrier between, every
+// thread takes its own kPer columns of all rows, writes dx and adds to dw and db, which stay in registers. What
+// a row costs besides its elements (shuffles, barrier, addresses) is thus paid by few warps or for several
+// rows at once.
+template <typename T, typename P, int kVec, int kPer, int kThreads, int kCtas>
+__global__ void __launch_bounds__(kThreads, kCtas)
+layer_norm_backward_ring_kernel(const Backward g, const Ring ring, int *status) {
+  extern __shared__ __align__(128) uint8_t shared[];
+  __shared__ float4 sums[2][32];  // [row * parts + part]: sum a, sum a n, mean, rstd
+  __shared__ uint32_t abort_word;
+  volatile uint32_t *abort_flag = &abort_word;
+  const int t = threadIdx.x, threads = blockDim.x, cols = static_cast<int>(g.cols), lane = t & 31, warp = t >> 5;
+  const int rows = ring.rows, parts = ring.parts;
+  const uint32_t bars = smem_u32(shared), slots = bars + 128, stage_bytes = 2u * rows * ring.slot;
+  const uint8_t *const slots_gen = shared + 128;
+  const T *x = static_cast<const T *>(g.x), *dy = static_cast<const T *>(g.dy);
+  const long long tiles = (g.rows + rows - 1) / rows;
+  auto load = [&](long long tile, int stage) {
+    const int live = static_cast<int>(min(static_cast<long long>(rows), g.rows - tile * rows));
+    uint32_t total = 0;
+    for (int r = 0; r < live; ++r)
+      total += RowCopy(x, tile * rows + r, g.ldx, g.cols, g.rows, sizeof(T)).bytes +
+               RowCopy(dy, tile * rows + r, g.lddy, g.cols, g.rows, sizeof(T)).bytes;
+    mbar_arrive_expect_tx(bars + 8u * stage, total);
+    for (int r = 0; r < live; ++r) {
+      const RowCopy cx(x, tile * rows + r, g.ldx, g.cols, g.rows, sizeof(T)), cd(dy, tile * rows + r, g.lddy, g.cols, g.rows, sizeof(T));
+      const uint32_t at = slots + stage * stage_bytes + 2u * r * ring.slot;
+      if (cx.bytes != 0)
+        bulk_load(at, cx.low, cx.bytes, bars + 8u * stage);
+      if (cd.bytes != 0)
+        bulk_load(at + ring.slot, cd.low, cd.bytes, bars + 8u * stage);
+    }
+  };
+  if (t == 0) {
+    for (int s = 0; s < ring.stages; ++s)
+      mbar_init(bars + 8u * s, 1);
+    abort_word = 0;
+    mbar_fence_init();
+    for (int s = 0; s < ring.stages; ++s)
+      if (blockIdx.x + static_cast<long long>(s) * gridDim.x < tiles)
+        load(blockIdx.x + static_cast<long long>(s) * gridDim.x, s);
+  }
+  constexpr int kUnit = kVec > 1 ? kVec : 2, kPairs = kUnit / 2;
+  constexpr bool kKeep = kPer <= 16;  // the weights stay in registers between the rows (else dw and db fill them)
+  const P *const w = static_cast<const P *>(g.weight);
+  // The weights of the unit of elements at column c (with kVec == 1: at c and c + step).
+  auto weights = [&](float2 (&out)[kPairs], int c, int step) {
+    if constexpr (kVec > 1) {
+      float v[kVec];
+      load_params<P, kVec>(v, w, c, cols, g.params_aligned != 0, 1.0f);
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i)
+        out[i] = make_float2(v[2 * i], v[2 * i + 1]);
+    } else {
+      out[0].x = w != nullptr && c < cols ? to_float(w[c]) : 1.0f;
+      out[0].y = w != nullptr && c + step < cols ? to_float(w[c + step]) : 1.0f;
+    }
+  };
+  float2 dw[kPer / 2], db[kPer / 2], weight[kKeep ? kPer / kUnit : 1][kPairs];
+#pragma unroll
+  for (int j = 0; j < kPer / 2; ++j)
+    dw[j] = db[j] = make_float2(0.0f, 0.0f);
+  if constexpr (kKeep) {
+#pragma unroll
+    for (int u = 0; u < kPer / kUnit; ++u)
+      weights(weight[u], element_of<kVec>(t, u * kUnit, threads), threads);
+  }
+  __syncthreads();
+  const float inv = 1.0f / static_cast<float>(cols);
+  const int my_row = warp / parts, my_part = warp - my_row * parts;
+  float next_mean = 0.0f, next_rstd = 0.0f;  // of this warp's row of the tile to come
+  auto fetch_statistics = [&](long long tile) {
+    const long long r = tile * rows + my_row;
+    if (r < g.rows) {
+      next_mean = g.mean[r];
+      next_rstd = g.rstd[r];
+    }
+  };
+  fetch_statistics(blockIdx.x);
+  int stage = 0, turn = 0, before = 0;
+  uint32_t parity = 0;
+  for (long long tile = blockIdx.x; tile < tiles; tile += gridDim.x, turn ^= 1) {
+    const long long row0 = tile * rows;
+    const int live = static_cast<int>(min(static_cast<long long>(rows), g.rows - row0));
+    const uint8_t *const place = slots_gen + stage * stage_bytes;
+    // A unit of a row of the tile; at odd places, in the matrix's last row, what was not copied comes from memory.
+    auto unit = [&](float2 (&out)[kPairs], const T *base, long long ld, int r, int which, int c, int step) {
+      const uint8_t *const at = place + (2u * r + which) * ring.slot;
+      if constexpr (kVec > 1) {
+        const Pack<T, kVec> p = *reinterpret_cast<const Pack<T, kVec> *>(at + c * static_cast<int>(sizeof(T)));
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i)
+          out[i] = make_float2(to_float(p.v[2 * i]), to_float(p.v[2 * i + 1]));
+      } else {
+        const T *const row = base + (row0 + r) * ld;
+        const int lead = static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15);
+        const int copied = row0 + r == g.rows - 1 ? static_cast<int>(RowCopy(base, row0 + r, ld, g.cols, g.rows, sizeof(T)).bytes)
+                                                  : static_cast<int>(ring.slot);
+        auto one = [&](int k) {
+          const int place_of = lead + k * static_cast<int>(sizeof(T));
+          return k >= cols ? 0.0f
+                 : place_of + static_cast<int>(sizeof(T)) <= copied ? to_float(*reinterpret_cast<const T *>(at + place_of))
+                                                                    : to_float(row[k]);
+        };
+        out[0] = make_float2(one(c), one(c + step));
+      }
+    };
+    const float mean = next_mean, rstd = next_rstd;
+    fetch_statistics(tile + gridDim.x);
+    mbar_wait(bars + 8u * stage, parity, abort_flag);
+    if (my_row < live) {
+      // sum of a, and of a (x - mean): rstd is multiplied in once at the end.
+      float2 s = make_float2(0.0f, 0.0f), sn = s;
+      const float2 minus = splat(-mean);
+#pragma unroll 4
+      for (int c = (my_part * 32 + lane) * kVec; c < cols; c += parts * 32 * kUnit) {
+        float2 vx[kPairs], vd[kPairs], vw[kPairs];
+        unit(vx, x, g.ldx, my_row, 0, c, parts * 32);
+        unit(vd, dy, g.lddy, my_row, 1, c, parts * 32);
+        weights(vw, c, parts * 32);
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+          const float2 a = __fmul2_rn(vd[i], vw[i]);
+          s = __fadd2_rn(s, a);
+          sn = __ffma2_rn(a, __fadd2_rn(vx[i], minus), sn);
+        }
+      }
+      const float s1 = warp_sum(s.x + s.y), sn1 = warp_sum(sn.x + sn.y) * rstd;
+      if (lane == 0)
+        sums[turn][warp] = make_float4(s1, sn1, mean, rstd);
+    }
+    __syncthreads();
+    // Every thread is through with the tile before: its stage takes another.
+    const long long next = tile + static_cast<long long>(ring.stages - 1) * gridDim.x;
+    if (t == 0 && tile != blockIdx.x && next < tiles)
+      load(next, before);
+    for (int r = 0; r < live; ++r) {
+      float4 total = sums[turn][r * parts];
+      if (parts <= 4) {
+        for (int k = 1; k < parts; ++k) {
+          total.x += sums[turn][r * parts + k].x;
+          total.y += sums[turn][r * parts + k].y;
+        }
+      } else {
+        const float4 v = lane < parts ? sums[turn][r * parts + lane] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        total.x = warp_sum(v.x);
+        total.y = warp_sum(v.y);
+      }
+      const float2 minus_ms = splat(-total.x * inv), minus_msn = splat(-total.y * inv), minus_mean = splat(-total.z),
+                   rs = splat(total.w);
+      T *dx = static_cast<T *>(g.dx) + (row0 + r) * g.lddx;
+#pragma unroll
+      for (int u = 0; u < kPer / kUnit; ++u) {
+        const int c = element_of<kVec>(t, u * kUnit, threads);
+        if (c < cols) {
+          float2 vx[kPairs], vd[kPairs], vw[kPairs];
+          unit(vx, x, g.ldx, r, 0, c, threads);
+          unit(vd, dy, g.lddy, r, 1, c, threads);
+          if constexpr (!kKeep)
+            weights(vw, c, threads);
+          T out[kUnit];
+#pragma unroll
+          for (int i = 0; i < kPairs; ++i) {
+            const int j = u * kPairs + i;
+            const float2 n = __fmul2_rn(__fadd2_rn(vx[i], minus_mean), rs), d = vd[i];
+            dw[j] = __ffma2_rn(d, n, dw[j]);
+            db[j] = __fadd2_rn(db[j], d);
+            const float2 o = __fmul2_rn(__ffma2_rn(n, minus_msn, __ffma2_rn(d, kKeep ? weight[kKeep ? u : 0][i] : vw[i], minus_ms)), rs);
+            out[2 * i] = from_float<T>(o.x);
+            out[2 * i + 1] = from_float<T>(o.y);
+          }
+          store_unit<T, kVec>(dx, c, threads, cols, out);
+        }
+      }
+    }
+    before = stage;
+    if (++stage == ring.stages) {
+      stage = 0;
+      parity ^= 1u;
+    }
+  }
+  if (g.partials != nullptr) {
+    float *mine = g.partials + static_cast<long long>(blockIdx.x) * 2 * cols;
+    if constexpr (kVec > 1) {  // four at a time: cols is a multiple of four, and so is every row of partials
+#pragma unroll
+      for (int j = 0; j < kPer; j += 4) {
+        const int c = element_of<kVec>(t, j, threads);
+        if (c < cols) {
+          *reinterpret_cast<float4 *>(mine + c) = make_float4(dw[j / 2].x, dw[j / 2].y, dw[j / 2 + 1].x, dw[j / 2 + 1].y);
+          *reinterpret_cast<float4 *>(mine + cols + c) = make_float4(db[j / 2].x, db[j / 2].y, db[j / 2 + 1].x, db[j / 2 + 1].y);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        const int c = element_of<kVec>(t, j, threads);
+        if (c < cols) {
+          mine[c] = j % 2 != 0 ? dw[j / 2].y : dw[j / 2].x;
+          mine[cols + c] = j % 2 != 0 ? db[j / 2].y : db[j / 2].x;
+        }
+      }
+    }
+  }
+  __syncthreads();
+  if (t == 0 && abort_word != 0)
+    atomicCAS(status, 0, kStatusDeviceWaitTimeout);
+}
+
 // ---------------------------------------------------------------- launch ------------
 
-template <typename T, typename P, int kVec>
-cudaError_t launch_forward(const Forward &f, int sm_count, cudaStream_t stream) {
-  const long long packs = (f.cols + kVec - 1) / kVec;
+// How a call is laid out; for the kernels and for the scratch they need.
+struct Plan {
+  enum Kind { kWarpRows, kDirect, kRing, kLong } kind;
+  int threads, per;  // per: elements per thread (ring) or packs per thread (direct, warp rows)
+  int grid;          // CTAs of the kernel that walks rows; of a long backward pass, the row chunks of dw and db
+  Ring ring;
+  size_t shared;
+};
+
+constexpr long long kMostRingCols = 16 * kMaxThreads;
+constexpr int kMostStages = 8;
+
+int threads_for(long long cols, int per) { return static_cast<int>((cols + per - 1) / per + 31) / 32 * 32; }
+
+// CTAs that share an SM: as many as its registers hold, at most eight.
+int ring_ctas(int threads_per_sm, int threads) {
+  const int ctas = threads_per_sm / threads;
+  return ctas < 8 ? ctas : 8;
+}
+
+// Forward. What a row costs besides its elements is per warp, so few warps with 32 elements a thread (and the
+// registers of 512 threads) suit long rows: 16384 x 2048 bfloat16 takes 33.0 us so and 38.2 us with 8 elements
+// a thread; 16384 x 1024 takes 24.9 and 22.7 us. At odd places (vec == 1) 8 elements are better up to 2048
+// columns: 16384 x 1503 float16 takes 64 us, with 32 elements 84 us; beyond, a row is dearer to read from
+// shared memory element by element than it is worth (1024 x 4095: 18.7 us, without the ring 16.6 us).
+bool forward_ring(Plan *plan, long long rows, long long cols, int vec, int size, int sm_count) {
+  if (cols > (vec > 1 ? kMostRingCols : 2048))
+    return false;
+  plan->kind = Plan::kRing;
+  plan->per = cols <= (vec > 1 ? 1024 : 2048) ? 8 : 32;
+  plan->threads = threads_for(cols, plan->per);
+  plan->ring.slot = static_cast<uint32_t>((cols * size + 15) / 16 * 16 + 16);  // a row at an odd place needs 16 more
+  const int most = ring_ctas(plan->per == 8 ? 1024 : 512, plan->threads);
+  const long long stages = (200 * 1024 / most - 256) / plan->ring.slot;
+  if (stages < 2)
+    return false;
+  plan->ring.stages = static_cast<int>(stages < kMostStages ? stages : kMostStages);
+  plan->shared = 128 + static_cast<size_t>(plan->ring.stages) * plan->ring.slot;
+  const long long ctas = static_cast<long long>(sm_count) * most;
+  plan->grid = static_cast<int>(rows < ctas ? rows : ctas);
+  return true;
+}
+
+// Backward: 16 elements a thread up to 8192 columns (16384 x 4096 bfloat16 takes 115 us so, with 8 elements
+// 143 us, with 32 elements 136 us), 32 beyond, where dw and db of 512 threads fill the registers. Tiles of as
+// many rows as leave three stages and give every CTA four tiles, and warps to share them.
+bool backward_ring(Plan *plan, long long rows, long long cols, int vec, int size, int sm_count) {
+  if (cols > (vec > 1 ? kMostRingCols : 2048))
+    return false;
+  plan->kind = Plan::kRing;
+  plan->per = cols <= 8192 ? 16 : 32;
+  plan->threads = threads_for(cols, plan->per);
+  plan->ring.slot = static_cast<uint32_t>((cols * size + 15) / 16 * 16 + 16);
+  const int most = ring_ctas(512, plan->threads);
+  const long long budget = 200 * 1024 / most - 256, pair = 2LL * plan->ring.slot;
+  const int warps = plan->threads / 32;
+  int tile = 1;
+  while (tile < 8 && warps % (2 * tile) == 0 && 3 * 2 * tile * pair <= budget && rows >= 4LL * tile * most * sm_count)
+    tile *= 2;
+  const long long stages = budget / (tile * pair);
+  if (stages < 2)
+    return false;
+  plan->ring.rows = tile;
+  plan->ring.parts = warps / tile;
+  plan->ring.stages = static_cast<int>(stages < kMostStages ? stages : kMostStages);
+  plan->shared = 128 + static_cast<size_t>(plan->ring.stages) * tile * pair;
+  const long long ctas = static_cast<long long>(sm_count) * most, tiles = (rows + tile - 1) / tile;
+  plan->grid = static_cast<int>(tiles < ctas ? tiles : ctas);
+  return true;
+}
+
+Plan forward_plan(long long rows, long long cols, int vec, int size, int sm_count) {
+  Plan plan{};
+  const long long packs = (cols + vec - 1) / vec;
+  // The ring pays for rows of more than 1 KiB (16384 x 512 float32: 18.7 us either way; 65536 x 512 bfloat16
+  // 53 us, without it 47 us) in matrices of 4 MiB and more, which give every CTA several rows (592 x 4096
+  // bfloat16: 7.5 us, without it 7.9 us; 296 x 4096: 7.6 and 6.9 us).
+  if (cols * size > 1024 && rows * cols * size >= 4LL << 20 && forward_ring(&plan, rows, cols, vec, size, sm_count))
+    return plan;
   if (packs <= 64) {  // a warp holds a row in at most two packs per lane
-    const unsigned grid = static_cast<unsigned>((f.rows + kWarpRowWarps - 1) / kWarpRowWarps);
-    if (packs <= 32)
-      layer_norm_kernel<T, P, kVec, 1, true><<<grid, 32 * kWarpRowWarps, 0, stream>>>(f);
-    else
-      layer_norm_kernel<T, P, kVec, 2, true><<<grid, 32 * kWarpRowWarps, 0, stream>>>(f);
-    return cudaGetLastError();
+    plan.kind = Plan::kWarpRows;
+    plan.threads = 32 * kWarpRowWarps;
+    plan.per = packs <= 32 ? 1 : 2;
+    plan.grid = static_cast<int>((rows + kWarpRowWarps - 1) / kWarpRowWarps);
+    return plan;
   }
+  plan.grid = static_cast<int>(rows);
   if (packs > 4 * kMaxThreads) {
-    layer_norm_long_kernel<T, P, kVec><<<static_cast<unsigned>(f.rows), kMaxThreads, 0, stream>>>(f);
-    return cudaGetLastError();
+    plan.kind = Plan::kLong;
+    plan.threads = kMaxThreads;
+    return plan;
   }
-  // Few rows: as many threads as the row has packs, for the shortest chain of loads. Many rows: CTAs of
-  // at most 256 threads with up to four packs each, so that several CTAs overlap on an SM.
-  const int most = f.rows <= sm_count ? kMaxThreads : 256;
-  int per = packs <= most ? 1 : packs <= 2 * most ? 2 : 4;
-  const int threads = static_cast<int>(((packs + per - 1) / per + 31) / 32 * 32);
-  const unsigned grid = static_cast<unsigned>(f.rows);
-  if (per == 1)
-    layer_norm_kernel<T, P, kVec, 1, false><<<grid, threads, 0, stream>>>(f);
-  else if (per == 2)
-    layer_norm_kernel<T, P, kVec, 2, false><<<grid, threads, 0, stream>>>(f);
-  else
-    layer_norm_kernel<T, P, kVec, 4, false><<<grid, threads, 0, stream>>>(f);
+  // As many threads as the row has packs, for the shortest chain of loads.
+  plan.kind = Plan::kDirect;
+  plan.per = packs <= kMaxThreads ? 1 : packs <= 2 * kMaxThreads ? 2 : 4;
+  plan.threads = static_cast<int>(((packs + plan.per - 1) / plan.per + 31) / 32 * 32);
+  return plan;
+}
+
+Plan backward_plan(long long rows, long long cols, int vec, int size, int sm_count) {
+  Plan plan{};
+  const long long packs = (cols + vec - 1) / vec;
+  if (packs <= 32) {
+    plan.kind = Plan::kWarpRows;
+    plan.threads = 32 * kWarpRowWarps;
+    const long long units = (rows + kWarpRowWarps - 1) / kWarpRowWarps;
+    plan.grid = static_cast<int>(units < 4LL * sm_count ? units : 4LL * sm_count);
+    plan.shared = sizeof(float) * kWarpRowWarps * 2 * static_cast<size_t>(cols);
+    return plan;
+  }
+  // Without the ring a thread holds one pack, which float32 rows of up to 1024 columns do with few enough
+  // threads: 16384 x 512 takes 41.1 us, through the ring 45.2 us, 16384 x 1024 51.6 and 53.9 us (bfloat16: 65.7
+  // and 43.3 us).
+  if (!(vec == 4 && cols <= 1024) && backward_ring(&plan, rows, cols, vec, size, sm_count))
+    return plan;
+  if (packs <= kMaxThreads) {
+    plan.kind = Plan::kDirect;
+    plan.threads = static_cast<int>((packs + 31) / 32 * 32);
+    const long long ctas = static_cast<long long>(sm_count) * (plan.threads > 512 ? 1 : plan.threads > 256 ? 2 : 4);
+    plan.grid = static_cast<int>(rows < ctas ? rows : ctas);
+    return plan;
+  }
+  plan.kind = Plan::kLong;
+  plan.threads = kMaxThreads;
+  // Row chunks of the column kernel: enough CTAs to fill the GPU a few times over.
+  const long long column_blocks = (packs + 255) / 256;
+  const long long chunks = (8LL * sm_count + column_blocks - 1) / column_blocks;
+  plan.grid = static_cast<int>(rows < chunks ? rows : chunks);
+  return plan;
+}
+
+template <typename Kernel, typename... Args>
+cudaError_t launch_ring(Kernel kernel, const Plan &plan, cudaStream_t stream, const Args &...args) {
+  // (Set at every launch: the kernels are many and the call is cheap.)
+  const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(plan.shared));
+  if (err != cudaSuccess)
+    return err;
+  kernel<<<plan.grid, plan.threads, plan.shared, stream>>>(args...);
   return cudaGetLastError();
 }
 
-// CTAs of the backward kernel, which is also the number of partial rows.
-int backward_grid(long long rows, long long cols, int vec, int sm_count, bool *long_rows) {
-  const long long packs = (cols + vec - 1) / vec;
-  *long_rows = packs > kMaxThreads;
-  if (*long_rows) {
-    // Row chunks of the column kernel: enough CTAs to fill the GPU a few times over.
-    const long long column_blocks = (packs + 255) / 256;
-    const long long chunks = (8LL * sm_count + column_blocks - 1) / column_blocks;
-    return static_cast<int>(rows < chunks ? rows : chunks);
+template <typename T, typename P, int kVec>
+cudaError_t launch_forward(const Forward &f, int sm_count, int *status, cudaStream_t stream) {
+  const Plan plan = forward_plan(f.rows, f.cols, kVec, sizeof(T), sm_count);
+  switch (plan.kind) {
+  case Plan::kWarpRows:
+    if (plan.per == 1)
+      layer_norm_kernel<T, P, kVec, 1, true><<<plan.grid, plan.threads, 0, stream>>>(f);
+    else
+      layer_norm_kernel<T, P, kVec, 2, true><<<plan.grid, plan.threads, 0, stream>>>(f);
+    break;
+  case Plan::kRing:
+    if (plan.per == 8)
+      return launch_ring(layer_norm_ring_kernel<T, P, kVec, 8, 256, 4>, plan, stream, f, plan.ring, status);
+    if constexpr (kVec > 1)
+      return launch_ring(layer_norm_ring_kernel<T, P, kVec, 32, 512, 1>, plan, stream, f, plan.ring, status);
+    break;
+  case Plan::kDirect:
+    if (plan.per == 1)
+      layer_norm_kernel<T, P, kVec, 1, false><<<plan.grid, plan.threads, 0, stream>>>(f);
+    else if (plan.per == 2)
+      layer_norm_kernel<T, P, kVec, 2, false><<<plan.grid, plan.threads, 0, stream>>>(f);
+    else
+      layer_norm_kernel<T, P, kVec, 4, false><<<plan.grid, plan.threads, 0, stream>>>(f);
+    break;
+  case Plan::kLong:
+    layer_norm_long_kernel<T, P, kVec><<<plan.grid, plan.threads, 0, stream>>>(f);
+    break;
   }
-  const bool warp_rows = packs <= 32;
-  const long long units = warp_rows ? (rows + kWarpRowWarps - 1) / kWarpRowWarps : rows;
-  const int threads = warp_rows ? 32 * kWarpRowWarps : static_cast<int>((packs + 31) / 32 * 32);
-  const long long ctas = static_cast<long long>(sm_count) * (threads >= 1024 ? 1 : threads > 512 ? 1 : threads > 256 ? 2 : 4);
-  return static_cast<int>(units < ctas ? units : ctas);
+  return cudaGetLastError();
 }
 
 template <typename T, typename P, int kVec>
-cudaError_t launch_backward(const Backward &g, P *dweight, P *dbias, int sm_count, cudaStream_t stream) {
-  const long long packs = (g.cols + kVec - 1) / kVec;
-  bool long_rows = false;
-  const int grid = backward_grid(g.rows, g.cols, kVec, sm_count, &long_rows);
+cudaError_t launch_backward(const Backward &g, P *dweight, P *dbias, int sm_count, int *status, cudaStream_t stream) {
+  const Plan plan = backward_plan(g.rows, g.cols, kVec, sizeof(T), sm_count);
   cudaError_t err = cudaSuccess;
-  if (long_rows) {
+  switch (plan.kind) {
+  case Plan::kWarpRows:
+    layer_norm_backward_kernel<T, P, kVec, 1, true, 32 * kWarpRowWarps>
+        <<<plan.grid, plan.threads, g.partials != nullptr ? plan.shared : 0, stream>>>(g);
+    err = cudaGetLastError();
+    break;
+  case Plan::kRing:
+    if (plan.per == 16) {
+      err = launch_ring(layer_norm_backward_ring_kernel<T, P, kVec, 16, 512, 1>, plan, stream, g, plan.ring, status);
+    } else if constexpr (kVec > 1) {
+      err = launch_ring(layer_norm_backward_ring_kernel<T, P, kVec, 32, 512, 1>, plan, stream, g, plan.ring, status);
+    }
+    break;
+  case Plan::kDirect:
+    if (plan.threads <= 512)
+      layer_norm_backward_kernel<T, P, kVec, 1, false, 512><<<plan.grid, plan.threads, 0, stream>>>(g);
+    else
+      layer_norm_backward_kernel<T, P, kVec, 1, false, kMaxThreads><<<plan.grid, plan.threads, 0, stream>>>(g);
+    err = cudaGetLastError();
+    break;
+  case Plan::kLong:
     if (g.partials != nullptr) {  // before dx, which may be written over dy or x
-      const dim3 blocks(static_cast<unsigned>((packs + 255) / 256), static_cast<unsigned>(grid));
+      const long long packs = (g.cols + kVec - 1) / kVec;
+      const dim3 blocks(static_cast<unsigned>((packs + 255) / 256), static_cast<unsigned>(plan.grid));
       layer_norm_columns_kernel<T, kVec><<<blocks, 256, 0, stream>>>(g);
       err = cudaGetLastError();
       if (err != cudaSuccess)
         return err;
     }
     layer_norm_backward_long_kernel<T, P, kVec><<<static_cast<unsigned>(g.rows), kMaxThreads, 0, stream>>>(g);
-  } else if (packs <= 32) {
-    const size_t shared = g.partials != nullptr ? sizeof(float) * kWarpRowWarps * 2 * static_cast<size_t>(g.cols) : 0;
-    layer_norm_backward_kernel<T, P, kVec, 1, true, 32 * kWarpRowWarps>
-        <<<grid, 32 * kWarpRowWarps, shared, stream>>>(g);
-  } else {
-    const int threads = static_cast<int>((packs + 31) / 32 * 32);
-    if (threads <= 512)
-      layer_norm_backward_kernel<T, P, kVec, 1, false, 512><<<grid, threads, 0, stream>>>(g);
-    else
-      layer_norm_backward_kernel<T, P, kVec, 1, false, kMaxThreads><<<grid, threads, 0, stream>>>(g);
+    err = cudaGetLastError();
+    break;
   }
-  err = cudaGetLastError();
   if (err != cudaSuccess || g.partials == nullptr)
     return err;
   const dim3 blocks(static_cast<unsigned>((g.cols + 31) / 32), 2);
-  layer_norm_partials_kernel<P><<<blocks, 1024, 0, stream>>>(g.partials, grid, g.cols, dweight, dbias);
+  layer_norm_partials_kernel<P><<<blocks, 1024, 0, stream>>>(g.partials, plan.grid, g.cols, dweight, dbias);
   return cudaGetLastError();
 }
 
@@ -587,12 +1143,13 @@ bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 
 }  // namespace norm
 
-// Elements per access: 16 bytes' worth when every row of every matrix starts on a 16-byte boundary.
-int layer_norm_vector(int dtype, const void *a, long long lda, const void *b, long long ldb, const void *c,
+// Elements per access: 16 bytes' worth when every row of every matrix starts on a 16-byte boundary and consists
+// of whole 16-byte pieces.
+int layer_norm_vector(int dtype, long long cols, const void *a, long long lda, const void *b, long long ldb, const void *c,
                       long long ldc) {
   const int size = dtype == kCTypeF32 ? 4 : 2;
   const bool ok = norm::aligned16(a) && norm::aligned16(b) && norm::aligned16(c) && (lda * size) % 16 == 0 &&
-                  (ldb * size) % 16 == 0 && (ldc * size) % 16 == 0;
+                  (ldb * size) % 16 == 0 && (ldc * size) % 16 == 0 && (cols * size) % 16 == 0;
   return ok ? 16 / size : 1;
 }
 
@@ -610,36 +1167,34 @@ int layer_norm_vector(int dtype, const void *a, long long lda, const void *b, lo
 
 cudaError_t launch_layer_norm(const void *x, long long ldx, const void *weight, const void *bias, void *y,
                               long long ldy, float *mean, float *rstd, long long rows, long long cols, float eps,
-                              int dtype, int param_dtype, int sm_count, cudaStream_t stream) {
-  const int vec = layer_norm_vector(dtype, x, ldx, y, ldy, y, ldy);
+                              int dtype, int param_dtype, int sm_count, int *status, cudaStream_t stream) {
+  const int vec = layer_norm_vector(dtype, cols, x, ldx, y, ldy, y, ldy);
   norm::Forward f{x, weight, bias, y, mean, rstd, rows, cols, ldx, ldy, eps,
                   norm::aligned16(weight) && norm::aligned16(bias) ? 1 : 0};
-#define HC_NORM_FORWARD(T, P, V) norm::launch_forward<T, P, V>(f, sm_count, stream)
+#define HC_NORM_FORWARD(T, P, V) norm::launch_forward<T, P, V>(f, sm_count, status, stream)
   HC_NORM_TYPES(HC_NORM_FORWARD);
 #undef HC_NORM_FORWARD
 }
 
-int layer_norm_backward_launches(long long rows, long long cols, int vec, bool params) {
-  bool long_rows = false;
-  norm::backward_grid(rows, cols, vec, 1, &long_rows);
-  return 1 + (params ? (long_rows ? 2 : 1) : 0);
+int layer_norm_backward_launches(long long rows, long long cols, int vec, int dtype, bool params) {
+  const norm::Plan plan = norm::backward_plan(rows, cols, vec, dtype == kCTypeF32 ? 4 : 2, 148);
+  return 1 + (params ? (plan.kind == norm::Plan::kLong ? 2 : 1) : 0);
 }
 
-size_t layer_norm_backward_scratch(long long rows, long long cols, int vec, int sm_count) {
-  bool long_rows = false;
-  return sizeof(float) * 2 * static_cast<size_t>(cols) *
-         static_cast<size_t>(norm::backward_grid(rows, cols, vec, sm_count, &long_rows));
+size_t layer_norm_backward_scratch(long long rows, long long cols, int vec, int dtype, int sm_count) {
+  const norm::Plan plan = norm::backward_plan(rows, cols, vec, dtype == kCTypeF32 ? 4 : 2, sm_count);
+  return sizeof(float) * 2 * static_cast<size_t>(cols) * static_cast<size_t>(plan.grid);
 }
 
 cudaError_t launch_layer_norm_backward(const void *dy, long long lddy, const void *x, long long ldx, const void *weight,
                                        const float *mean, const float *rstd, void *dx, long long lddx, void *dweight,
                                        void *dbias, float *partials, long long rows, long long cols, int dtype,
-                                       int param_dtype, int sm_count, cudaStream_t stream) {
-  const int vec = layer_norm_vector(dtype, dy, lddy, x, ldx, dx, lddx);
+                                       int param_dtype, int sm_count, int *status, cudaStream_t stream) {
+  const int vec = layer_norm_vector(dtype, cols, dy, lddy, x, ldx, dx, lddx);
   norm::Backward g{dy, x, weight, mean, rstd, dx, dweight != nullptr || dbias != nullptr ? partials : nullptr,
                    rows, cols, lddy, ldx, lddx, norm::aligned16(weight) ? 1 : 0};
 #define HC_NORM_BACKWARD(T, P, V) \
-  norm::launch_backward<T, P, V>(g, static_cast<P *>(dweight), static_cast<P *>(dbias), sm_count, stream)
+  norm::launch_backward<T, P, V>(g, static_cast<P *>(dweight), static_cast<P *>(dbias), sm_count, status, stream)
   HC_NORM_TYPES(HC_NORM_BACKWARD);
 #undef HC_NORM_BACKWARD
 }

@@ -206,6 +206,49 @@ def test_many_rows_repeat_bit_for_bit(gpu_ctx) -> None:
         assert np.array_equal(p, q)
 
 
+@pytest.mark.parametrize("dtype, param", [("bfloat16", "bfloat16"), ("float32", "float32"), ("float16", "float32")])
+@pytest.mark.parametrize("rows, cols, pad", [(700, 300, 0), (601, 257, 0), (1500, 513, 3), (650, 1000, 0), (593, 2048, 8),
+                                             (600, 2049, 0), (640, 4096, 0), (600, 5001, 2), (595, 8200, 0), (593, 16383, 0)])
+def test_many_rows(rows, cols, pad, dtype, param, gpu_ctx) -> None:
+    """Enough rows that every CTA walks several: rows on 16-byte boundaries and at every place between them."""
+    x, dy, w, b = inputs(rows, cols, dtype, param, 8)
+    y, mean, rstd = run_forward(gpu_ctx, x, w, b, pad)
+    check_forward(dtype, x, w, b, y, mean, rstd)
+    grads = run_backward(gpu_ctx, dy, x, w, mean, rstd, pad)
+    check_backward(dtype, param, dy, x, w, mean, rstd, *grads)
+    for p, q in zip(grads, run_backward(gpu_ctx, dy, x, w, mean, rstd, pad, in_place="dy")):
+        assert np.array_equal(p, q)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_a_window_of_a_larger_matrix(dtype, gpu_ctx) -> None:
+    """Rows that start inside a 16-byte piece, in a buffer whose other columns are NaN and stay as they are."""
+    rows, cols, left, ld = 700, 1000, 3, 1013
+    x, dy, w, b = inputs(rows, cols, dtype, "float32", 9)
+    t = np_dtype(dtype)
+
+    def window(values):
+        host = np.full((rows, ld), np.nan, t)
+        if values is not None:
+            host[:, left:left + cols] = values
+        buf = make(gpu_ctx, host)
+        return buf, buf.window(0, rows, left, left + cols)
+
+    (bx, vx), (by, vy), (bd, vd), (bg, vg) = window(x), window(None), window(dy), window(None)
+    bw, bb = make(gpu_ctx, w), make(gpu_ctx, b)
+    mean, rstd = empty(gpu_ctx, (rows,), np.float32), empty(gpu_ctx, (rows,), np.float32)
+    dw, db = empty(gpu_ctx, (cols,), np.float32), empty(gpu_ctx, (cols,), np.float32)
+    gpu_ctx.layer_norm(vx, vy, weight=bw, bias=bb, eps=EPS, mean=mean, rstd=rstd)
+    gpu_ctx.layer_norm_backward(vd, vx, vg, mean=mean, rstd=rstd, weight=bw, dweight=dw, dbias=db)
+    gpu_ctx.synchronize()
+    y, dx = by.to_numpy(), bg.to_numpy()
+    check_forward(dtype, x, w, b, y[:, left:left + cols], mean.to_numpy(), rstd.to_numpy())
+    check_backward(dtype, "float32", dy, x, w, mean.to_numpy(), rstd.to_numpy(), dx[:, left:left + cols], dw.to_numpy(),
+                   db.to_numpy())
+    for out in (y, dx):
+        assert np.isnan(out[:, :left].astype(np.float32)).all() and np.isnan(out[:, left + cols:].astype(np.float32)).all()
+
+
 def test_empty_problems(gpu_ctx) -> None:
     w = np.ones(8, np.float32)
     bw, dw = make(gpu_ctx, w), empty(gpu_ctx, (8,), np.float32)
