@@ -2173,13 +2173,9 @@ hc::sm100::LinearLoss loss_launch(const LossCall &c, int64_t first, int64_t coun
   return p;
 }
 
-// Enqueues the copies and points `c` at them. `counting_rows`: the copy of h has zeros in the rows that do
-// not count.
+// Enqueues the copies and points `c` at them. `counting_rows`: h has been copied already.
 int enqueue_loss_copies(HcCudaContext *ctx, const LossWork &work, bool counting_rows, LossCall *c) {
   char *base = static_cast<char *>(ctx->work);
-  if (counting_rows)
-    HC_TRY_CUDA(ctx, hc::sm100::launch_linear_loss_rows(loss_launch(*c, 0, c->vocab), c->h, c->ldh, base + work.h_copy,
-                                                        work.copy_ld, ctx->stream));
   const bool repack_h = work.h_copy >= 0 && !counting_rows;
   if (repack_h || work.w_copy >= 0)
     HC_TRY_CUDA(ctx, hc::sm100::launch_repack_pitch_two(
@@ -2254,12 +2250,12 @@ struct LossBackwardPlan {
   int64_t piece = 0;  // columns of the vocabulary per piece, a multiple of 256
   int64_t pieces = 0;
   int64_t g = 0, gt = 0, ldg = 0, ldgt = 0;
-  int64_t dh_sums = -1, dw_sums = -1;  // float32, where a product cannot write its result's type at once
+  int64_t dh_sums = -1;  // float32, where dh is the sum of several products or their fastest form writes float32
   int64_t sums_ld = 0;
-  int64_t scales = -1;
+  int64_t scales = 0;
 };
 
-// The two products of a piece as GEMM arguments; `c` is already aligned, `base` the start of `work`.
+// The two products of a piece as GEMM arguments, their 16-bit results scaled by scales[1]; `c` is already aligned, `base` the start of `work`.
 HcCudaGemmArgs loss_dh_product(const LossCall &c, const LossBackwardPlan &plan, char *base, int64_t first, int64_t count,
                                const HcCudaLinearLossBackwardArgs &args) {
   HcCudaGemmArgs g{};
@@ -2281,6 +2277,9 @@ HcCudaGemmArgs loss_dh_product(const LossCall &c, const LossBackwardPlan &plan, 
     g.c = args.dh;
     g.ldc = args.lddh;
     g.c_dtype = c.dtype == HC_CUDA_BF16 ? HC_CUDA_C_BF16 : HC_CUDA_C_F16;
+    g.epilogue_count = 1;
+    g.epilogue_kind[0] = HC_CUDA_EPILOGUE_SCALE;
+    g.epilogue_value[0] = 1.0f;
   }
   return g;
 }
@@ -2297,15 +2296,12 @@ HcCudaGemmArgs loss_dw_product(const LossCall &c, const LossBackwardPlan &plan, 
   g.b = c.h;
   g.ldb = c.ldh;
   g.b_layout = HC_CUDA_B_KN;
-  if (plan.dw_sums >= 0) {
-    g.c = base + plan.dw_sums;
-    g.ldc = plan.sums_ld;
-    g.c_dtype = HC_CUDA_C_F32;
-  } else {
-    g.c = static_cast<char *>(args.dw) + static_cast<size_t>(first) * static_cast<size_t>(args.lddw) * 2;
-    g.ldc = args.lddw;
-    g.c_dtype = c.dtype == HC_CUDA_BF16 ? HC_CUDA_C_BF16 : HC_CUDA_C_F16;
-  }
+  g.c = static_cast<char *>(args.dw) + static_cast<size_t>(first) * static_cast<size_t>(args.lddw) * 2;
+  g.ldc = args.lddw;
+  g.c_dtype = c.dtype == HC_CUDA_BF16 ? HC_CUDA_C_BF16 : HC_CUDA_C_F16;
+  g.epilogue_count = 1;
+  g.epilogue_kind[0] = HC_CUDA_EPILOGUE_SCALE;
+  g.epilogue_value[0] = 1.0f;
   return g;
 }
 
@@ -2354,13 +2350,7 @@ int plan_linear_loss_backward(const HcCudaContext *ctx, const HcCudaLinearLossBa
   plan->g = plan->work.take(args->dh != nullptr ? c.rows * plan->ldg * 2 : 0);
   plan->gt = plan->work.take(args->dw != nullptr ? columns * plan->ldgt * 2 : 0);
   plan->sums_ld = round_up(c.width, 4);
-  const bool scaled = c.dtype == HC_CUDA_F16;
-  if (args->dh != nullptr && (plan->pieces > 1 || scaled))
-    plan->dh_sums = plan->work.take(c.rows * plan->sums_ld * 4);
-  if (args->dw != nullptr && scaled)
-    plan->dw_sums = plan->work.take(columns * plan->sums_ld * 4);
-  if (scaled)
-    plan->scales = plan->work.take(8);
+  plan->scales = plan->work.take(8);
 
   // Launches, and the scratch of the products.
   LossCall aligned = c;
@@ -2375,12 +2365,27 @@ int plan_linear_loss_backward(const HcCudaContext *ctx, const HcCudaLinearLossBa
     aligned.w = base + plan->work.w_copy;
     aligned.ldw = plan->work.copy_ld;
   }
-  int launches = (counting_rows ? 1 : 0) + (repacks ? 1 : 0) + (scaled ? 1 : 0) + (plan->dh_sums >= 0 ? 1 : 0);
+  HcCudaGemmPlanInfo product;
+  if (args->dh != nullptr) {
+    // The sums are float32 where there are several products, and where the form that shares one product's k
+    // among clusters, which writes float32, would be taken for it: 128 x 512 x 4099 takes 38 us without it.
+    const int64_t bytes = plan->work.bytes;
+    plan->dh_sums = plan->work.take(c.rows * plan->sums_ld * 4);
+    if (plan->pieces == 1) {
+      const HcCudaGemmArgs g = loss_dh_product(aligned, *plan, base, 0, c.vocab, *args);
+      if (int rc = plan_gemm(ctx, &g, sm_count, false, &product))
+        return rc;
+      if (product.cluster_size <= 1) {
+        plan->dh_sums = -1;
+        plan->work.bytes = bytes;
+      }
+    }
+  }
+  int launches = 1 + (repacks ? 1 : 0) + (plan->dh_sums >= 0 ? 1 : 0);
   int64_t scratch = 0;
   for (int64_t first = 0; first < c.vocab; first += plan->piece) {
     const int64_t count = c.vocab - first < plan->piece ? c.vocab - first : plan->piece;
     ++launches;
-    HcCudaGemmPlanInfo product;
     if (args->dh != nullptr) {
       const HcCudaGemmArgs g = loss_dh_product(aligned, *plan, base, first, count, *args);
       if (int rc = plan_gemm(ctx, &g, sm_count, false, &product))
@@ -2392,7 +2397,7 @@ int plan_linear_loss_backward(const HcCudaContext *ctx, const HcCudaLinearLossBa
       const HcCudaGemmArgs g = loss_dw_product(aligned, *plan, base, first, count, *args);
       if (int rc = plan_gemm(ctx, &g, sm_count, false, &product))
         return rc;
-      launches += product.kernel_launches + (plan->dw_sums >= 0 ? 1 : 0);
+      launches += product.kernel_launches;
       scratch = product.scratch_bytes > scratch ? product.scratch_bytes : scratch;
     }
   }
@@ -2466,18 +2471,24 @@ int hcCudaLinearLossBackward(HcCudaContext *ctx, const HcCudaLinearLossBackwardA
   if (int rc = ensure_work(ctx, static_cast<size_t>(plan.work.bytes)))
     return rc;
   LossCall c = loss_call(*args);
-  if (int rc = enqueue_loss_copies(ctx, plan.work, /*counting_rows=*/args->dw != nullptr, &c))
-    return rc;
   char *const base = static_cast<char *>(ctx->work);
-  float *const scales = plan.scales >= 0 ? reinterpret_cast<float *>(base + plan.scales) : nullptr;
+  float *const scales = reinterpret_cast<float *>(base + plan.scales);
+  const bool copy_h = args->dw != nullptr;
+  hc::sm100::LinearLoss all = loss_launch(c, 0, c.vocab);
+  all.dloss = args->dloss;
+  HC_TRY_CUDA(ctx, hc::sm100::launch_linear_loss_prepare(all, scales, c.h, c.ldh, copy_h ? base + plan.work.h_copy : nullptr,
+                                                         plan.work.copy_ld, ctx->stream));
+  if (int rc = enqueue_loss_copies(ctx, plan.work, copy_h, &c))
+    return rc;
   const int narrow_type = c.dtype == HC_CUDA_BF16 ? hc::sm100::kCTypeBF16 : hc::sm100::kCTypeF16;
-  const float *const factor = scales != nullptr ? scales + 1 : nullptr;
+  hc::sm100::Epilogue scaled{};
+  scaled.device_factor = scales + 1;
   for (int64_t first = 0; first < c.vocab; first += plan.piece) {
     const int64_t count = c.vocab - first < plan.piece ? c.vocab - first : plan.piece;
     hc::sm100::LinearLoss p = loss_launch(c, first, count);
     p.lse = args->lse;
     p.dloss = args->dloss;
-    p.scale = scales;
+    p.scales = scales;
     if (args->dh != nullptr) {
       p.g = base + plan.g;
       p.ldg = plan.ldg;
@@ -2486,8 +2497,6 @@ int hcCudaLinearLossBackward(HcCudaContext *ctx, const HcCudaLinearLossBackwardA
       p.gt = base + plan.gt;
       p.ldgt = plan.ldgt;
     }
-    if (first == 0 && scales != nullptr)
-      HC_TRY_CUDA(ctx, hc::sm100::launch_linear_loss_scale(p, scales, ctx->stream));
     if (int rc = enqueue_loss_tiles(ctx, c, p, /*grad=*/true))
       return rc;
     HcCudaGemmPlanInfo product;
@@ -2495,25 +2504,20 @@ int hcCudaLinearLossBackward(HcCudaContext *ctx, const HcCudaLinearLossBackwardA
       const HcCudaGemmArgs g = loss_dh_product(c, plan, base, first, count, *args);
       if (int rc = plan_gemm(ctx, &g, sm_count, false, &product))
         return rc;
-      if (int rc = enqueue_gemm(ctx, &g, product))
+      if (int rc = enqueue_gemm(ctx, &g, product, plan.dh_sums >= 0 ? hc::sm100::Epilogue{} : scaled))
         return rc;
     }
     if (args->dw != nullptr) {
       const HcCudaGemmArgs g = loss_dw_product(c, plan, base, first, count, *args);
       if (int rc = plan_gemm(ctx, &g, sm_count, false, &product))
         return rc;
-      if (int rc = enqueue_gemm(ctx, &g, product))
+      if (int rc = enqueue_gemm(ctx, &g, product, scaled))
         return rc;
-      if (plan.dw_sums >= 0)
-        HC_TRY_CUDA(ctx, hc::sm100::launch_narrow(reinterpret_cast<const float *>(base + plan.dw_sums), plan.sums_ld,
-                                                  static_cast<char *>(args->dw) + static_cast<size_t>(first) * args->lddw * 2,
-                                                  args->lddw, static_cast<int>(count), static_cast<int>(c.width), factor,
-                                                  narrow_type, ctx->stream));
     }
   }
   if (plan.dh_sums >= 0)
     HC_TRY_CUDA(ctx, hc::sm100::launch_narrow(reinterpret_cast<const float *>(base + plan.dh_sums), plan.sums_ld, args->dh,
-                                              args->lddh, static_cast<int>(c.rows), static_cast<int>(c.width), factor,
+                                              args->lddh, static_cast<int>(c.rows), static_cast<int>(c.width), scales + 1,
                                               narrow_type, ctx->stream));
   return HC_CUDA_OK;
 }

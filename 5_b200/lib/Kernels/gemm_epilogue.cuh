@@ -57,6 +57,11 @@ __device__ __forceinline__ void store_c_element(void *c, long long index, float 
     static_cast<uint16_t *>(c)[index] = round_to_16(v, c_dtype);
 }
 
+// The constant of operation `op`.
+__device__ __forceinline__ float op_constant(const Epilogue &ep, int op) {
+  return ep.device_factor != nullptr ? ep.op_value[op] * __ldg(ep.device_factor) : ep.op_value[op];
+}
+
 // The fused element-wise work on one value that is about to be stored at `dst` (column `col`).
 __device__ __forceinline__ float finish_value(float v, const float *dst, int col, const Epilogue &ep) {
   if (ep.accumulate)
@@ -65,7 +70,7 @@ __device__ __forceinline__ float finish_value(float v, const float *dst, int col
   for (int i = 0; i < kMaxEpilogueOps; ++i) {
     if (i < ep.op_count) {
       const int kind = ep.op_kind[i];
-      const float x = kind == kEpilogueBiasColumn ? __ldg(ep.bias + col) : ep.op_value[i];
+      const float x = kind == kEpilogueBiasColumn ? __ldg(ep.bias + col) : op_constant(ep, i);
       v = kind == kEpilogueScale ? v * x
         : kind == kEpilogueMax   ? max_nan(v, x)
         : kind == kEpilogueMin   ? min_nan(v, x)
@@ -85,7 +90,7 @@ __device__ __forceinline__ void apply_ops_to_groups(float4 (&v)[8], const Epilog
     if (op >= ep.op_count)
       break;
     const int kind = ep.op_kind[op];
-    const float x = ep.op_value[op];
+    const float x = op_constant(ep, op);
     if (kind == kEpilogueScale) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -137,7 +142,7 @@ __device__ __forceinline__ void apply_ops_to_column(float (&v)[N], float bias, c
     if (op >= ep.op_count)
       break;
     const int kind = ep.op_kind[op];
-    const float x = kind == kEpilogueBiasColumn ? bias : ep.op_value[op];
+    const float x = kind == kEpilogueBiasColumn ? bias : op_constant(ep, op);
     if (kind == kEpilogueScale) {
 #pragma unroll
       for (int j = 0; j < N; ++j)
@@ -171,7 +176,7 @@ __device__ __forceinline__ void apply_ops_lane_row(uint32_t (&r)[32], int col0, 
     if (op >= ep.op_count)
       break;
     const int kind = ep.op_kind[op];
-    const float x = ep.op_value[op];
+    const float x = op_constant(ep, op);
     if (kind == kEpilogueScale) {
 #pragma unroll
       for (int j = 0; j < 32; ++j)
@@ -216,7 +221,7 @@ __device__ __forceinline__ float finish_loaded(float v, float previous, float bi
   for (int i = 0; i < kMaxEpilogueOps; ++i) {
     if (i < ep.op_count) {
       const int kind = ep.op_kind[i];
-      const float x = kind == kEpilogueBiasColumn ? bias : ep.op_value[i];
+      const float x = kind == kEpilogueBiasColumn ? bias : op_constant(ep, i);
       v = kind == kEpilogueScale ? v * x
         : kind == kEpilogueMax   ? max_nan(v, x)
         : kind == kEpilogueMin   ? min_nan(v, x)

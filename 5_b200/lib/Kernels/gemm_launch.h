@@ -68,6 +68,9 @@ struct Epilogue {
   int op_kind[kMaxEpilogueOps];
   float op_value[kMaxEpilogueOps];
   const float *bias;
+  // Where a launch's only operation is a scaling by a number that an earlier kernel finds: it is multiplied
+  // into op_value[0]. Null otherwise.
+  const float *device_factor;
   // Element type of C: 0 float32, 1 float16, 2 bfloat16 (the float32 value rounded to nearest
   // even). 16-bit output is written by the kernels that do not read C.
   int c_dtype;
@@ -332,9 +335,9 @@ struct LinearLoss {
   // Forward: linear_loss_parts(vocab) x rows partial pairs, the logit of each row's target, the results.
   float2 *partials;
   float *target_logit, *loss_out, *lse_out;
-  // Gradient: the upstream factors, times *scale when there is one; g [rows, ldg] with ldg a multiple of
+  // Gradient: the upstream factors as fractions of scales[0]; g [rows, ldg] with ldg a multiple of
   // 32 not below vocab, and its transpose gt [vocab, ldgt]; either may be null.
-  const float *lse, *dloss, *scale;
+  const float *lse, *dloss, *scales;
   void *g;
   long long ldg;
   void *gt;
@@ -345,12 +348,12 @@ cudaError_t launch_linear_loss(const CUtensorMap &tmap_h, const CUtensorMap &tma
                                int sm_count, int *status, cudaStream_t stream);
 // Joins the partial pairs into lse_out and loss_out.
 cudaError_t launch_linear_loss_join(const LinearLoss &p, cudaStream_t stream);
-// scales[0]: the power of two for float16's g, scales[1]: its inverse.
-cudaError_t launch_linear_loss_scale(const LinearLoss &p, float *scales, cudaStream_t stream);
-// copy (16-byte aligned, ldc a multiple of 8) = the rows of h, with zeros for those that do not count.
-cudaError_t launch_linear_loss_rows(const LinearLoss &p, const void *h, long long ldh, void *copy, long long ldc,
-                                    cudaStream_t stream);
-// dst[r, c] = src[r, c] * (*factor, or 1), rounded to 16 bits; src 16-byte aligned with lds a multiple of 4.
+// scales[0]: the largest |dloss| of the rows that count (1 when it is zero), scales[1]: what the products of g
+// must be multiplied by. With a copy (16-byte aligned, ldc a multiple of 8): the rows of h, with zeros for those
+// that do not count.
+cudaError_t launch_linear_loss_prepare(const LinearLoss &p, float *scales, const void *h, long long ldh, void *copy,
+                                       long long ldc, cudaStream_t stream);
+// dst[r, c] = src[r, c] * *factor, rounded to 16 bits; src 16-byte aligned with lds a multiple of 4.
 cudaError_t launch_narrow(const float *src, long long lds, void *dst, long long ldd, int rows, int cols,
                           const float *factor, int c_dtype, cudaStream_t stream);
 

@@ -20,10 +20,11 @@
 // products: 65536 of them per tile and pair take 2048 cycles of the two SMs' special function units
 // against 8 width cycles of products.
 //
-// float16: g = p - 1 or p times dloss, and with a mean over many rows it would fall below the type's
-// normal range. The rows' factors are therefore multiplied by a power of two that brings the largest of
-// |dloss| to 2^14 (found on the device), and the products are divided by it in float32 before they are
-// rounded. bfloat16 has the range of float32 and takes the factors as they are.
+// Rounding g: dloss is often the same for all rows (one over their number), and rounding (p - 1) dloss would
+// then be off by the same fraction in every row, which the sums over rows do not average out. The kernel
+// therefore finds the largest |dloss| of the rows that count, uses dloss as a fraction of it, so that g is
+// (p - 1) or p to the type's precision, and the products take the factor back in float32 before they are
+// rounded. float16 also multiplies g by 2^14, because p may lie below the type's normal range.
 #include "gemm_epilogue.cuh"
 #include "device_checks.cuh"
 #include "gemm_launch.h"
@@ -64,6 +65,13 @@ __device__ __forceinline__ float exp2_fast(float x) {
 
 __device__ __forceinline__ long long target_of(const LinearLoss &p, long long row) {
   return p.targets_64 ? static_cast<const long long *>(p.targets)[row] : static_cast<const int *>(p.targets)[row];
+}
+
+// The power of two that g is multiplied by.
+__device__ __forceinline__ float g_scale(int c_dtype) { return c_dtype == kCTypeF16 ? 16384.0f : 1.0f; }
+
+__device__ __forceinline__ bool counts_row(const LinearLoss &p, long long target) {
+  return target != p.ignore_index && target >= 0 && target < p.vocab_total;
 }
 
 // Walks the tiles down the rows of H within groups of `group_n` tile columns (see gemm_dense_pair_kernel).
@@ -259,8 +267,8 @@ linear_loss_kernel(const __grid_constant__ CUtensorMap tmap_h, const __grid_cons
         target = target_of(p, row);
         if (kGrad) {
           // A row that does not count has no gradient, whatever its dloss and lse hold.
-          const bool counts = target != p.ignore_index && target >= 0 && target < p.vocab_total;
-          scale = counts ? p.dloss[row] * (p.scale != nullptr ? *p.scale : 1.0f) : 0.0f;
+          const bool counts = counts_row(p, target);
+          scale = counts ? p.dloss[row] / p.scales[0] * g_scale(p.c_dtype) : 0.0f;
           lse2 = counts ? p.lse[row] * kLog2e : INFINITY;
         }
         target = target == p.ignore_index ? -1 : target - p.first_column;
@@ -355,36 +363,54 @@ linear_loss_kernel(const __grid_constant__ CUtensorMap tmap_h, const __grid_cons
     tmem_dealloc_pair(tmem_base, kTmemColumns);
 }
 
-// Joins the partial pairs of each row: 32 rows per CTA (a lane each), eight warps that share the parts.
-constexpr int kJoinWarps = 8;
+// Joins the partial pairs of each row: 32 rows per CTA, whose warps first share the parts (a lane each row), then
+// the rows (a lane each warp's share). 4096 rows of 256 parts: 5 us.
+constexpr int kJoinWarps = 32;
+
+// A part's sum brought to the scale of `top`; a part without a value above -inf adds nothing.
+__device__ __forceinline__ float joined(float2 v, float top) { return v.y == 0.0f ? 0.0f : v.y * exp2_fast(v.x - top); }
 
 __global__ void __launch_bounds__(32 * kJoinWarps)
 join_kernel(const LinearLoss p, int parts) {
-  __shared__ float2 shared[kJoinWarps][32];
+  __shared__ float2 shared[kJoinWarps][33];
+  constexpr int kAtOnce = 8;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int row = static_cast<int>(blockIdx.x) * 32 + lane;
-  Running run{-INFINITY, 0.0f};
-  bool poisoned = false;
-  auto add = [&](float2 v) {
-    if (v.y == 0.0f)
-      return;  // no value above -inf in that part
-    poisoned |= v.y != v.y;
-    const float top = fmaxf(run.top, v.x);
-    run.sum = run.sum * exp2_fast(run.top - top) + v.y * exp2_fast(v.x - top);
-    run.top = top;
-  };
-  if (row < p.rows)
-    for (int k = warp; k < parts; k += kJoinWarps)
-      add(p.partials[static_cast<long long>(k) * p.rows + row]);
-  shared[warp][lane] = make_float2(run.top, poisoned ? NAN : run.sum);
+  int row = static_cast<int>(blockIdx.x) * 32 + lane;
+  float2 run = make_float2(-INFINITY, 0.0f);
+  for (int k0 = warp; k0 < parts; k0 += kAtOnce * kJoinWarps) {
+    float2 v[kAtOnce];
+    float top = run.x;
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int k = k0 + i * kJoinWarps;
+      v[i] = make_float2(-INFINITY, 0.0f);
+      if (k < parts && row < p.rows)
+        v[i] = p.partials[static_cast<long long>(k) * p.rows + row];
+    }
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i)
+      top = fmaxf(top, v[i].x);
+    float sum = joined(run, top);
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i)
+      sum += joined(v[i], top);
+    run = make_float2(top, sum);
+  }
+  shared[warp][lane] = run;
   __syncthreads();
-  if (warp != 0 || row >= p.rows)
+  run = shared[lane][warp];
+  row = static_cast<int>(blockIdx.x) * 32 + warp;
+  float top = run.x;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  float sum = joined(run, top);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane != 0 || row >= p.rows)
     return;
-  run = Running{-INFINITY, 0.0f};
-  poisoned = false;
-  for (int k = 0; k < kJoinWarps; ++k)
-    add(shared[k][lane]);
-  const float lse = poisoned ? NAN : run.sum == 0.0f ? -INFINITY : run.top * kLn2 + logf(run.sum);
+  const float lse = sum == 0.0f ? -INFINITY : top * kLn2 + logf(sum);  // (a NaN stays one)
   const long long target = target_of(p, row);
   p.lse_out[row] = lse;
   p.loss_out[row] = target == p.ignore_index                   ? 0.0f
@@ -392,46 +418,41 @@ join_kernel(const LinearLoss p, int parts) {
                                                               : lse - p.target_logit[row];
 }
 
-// float16: the power of two that brings the largest |dloss| of the rows that count to 2^14, and its inverse.
-__global__ void __launch_bounds__(1024)
-scale_kernel(const LinearLoss p, float *scales) {
-  __shared__ float shared[32];
-  float top = 0.0f;
-  for (int row = threadIdx.x; row < p.rows; row += 1024) {
-    const long long target = target_of(p, row);
-    const float d = fabsf(p.dloss[row]);
-    if (target != p.ignore_index && target >= 0 && target < p.vocab_total && d < INFINITY)
-      top = fmaxf(top, d);
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if ((threadIdx.x & 31) == 0)
-    shared[threadIdx.x >> 5] = top;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int k = 1; k < 32; ++k)
-      top = fmaxf(top, shared[k]);
-    int e = 0;
-    if (top > 0.0f) {
-      frexpf(top, &e);               // top = f 2^e, f in [1/2, 1)
-      e = max(-100, min(100, 14 - e));  // the factor and its inverse stay normal numbers
-    }
-    scales[0] = ldexpf(1.0f, e);
-    scales[1] = ldexpf(1.0f, -e);
-  }
-}
-
-// The rows of H with zeros in place of those that do not count: their g is zero, but the product g^T H
-// would still make a NaN of a zero times an infinity or a NaN that such a row (padding, say) may hold.
+// Before the gradient: the scales, by the grid's first CTA, and the rows of H with zeros in place of those that
+// do not count, by the others. (Their g is zero, but the product g^T H would still make a NaN of a zero times
+// an infinity or a NaN that such a row, padding say, may hold.)
 template <typename Word>
 __global__ void __launch_bounds__(256)
-counting_rows_kernel(const LinearLoss p, const uint16_t *src, long long lds, uint16_t *dst, long long ldd) {
+prepare_kernel(const LinearLoss p, float *scales, const uint16_t *src, long long lds, uint16_t *dst, long long ldd) {
+  if (blockIdx.y == 0) {
+    __shared__ float shared[8];
+    if (blockIdx.x != 0)
+      return;
+    float top = 0.0f;
+#pragma unroll 8
+    for (int row = threadIdx.x; row < p.rows; row += 256) {
+      const float d = fabsf(p.dloss[row]);
+      if (d < INFINITY && counts_row(p, target_of(p, row)))
+        top = fmaxf(top, d);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if ((threadIdx.x & 31) == 0)
+      shared[threadIdx.x >> 5] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int k = 1; k < 8; ++k)
+        top = fmaxf(top, shared[k]);
+      scales[0] = top > 0.0f ? top : 1.0f;
+      scales[1] = scales[0] / g_scale(p.c_dtype);
+    }
+    return;
+  }
   constexpr int kPer = sizeof(Word) / 2;
   const int words = (p.width + kPer - 1) / kPer;
-  for (int row = blockIdx.y; row < p.rows; row += gridDim.y) {
-    const long long target = target_of(p, row);
-    const bool counts = target != p.ignore_index && target >= 0 && target < p.vocab_total;
+  for (int row = blockIdx.y - 1; row < p.rows; row += gridDim.y - 1) {
+    const bool counts = counts_row(p, target_of(p, row));
     for (int i = blockIdx.x * 256 + threadIdx.x; i < words; i += gridDim.x * 256) {
       const uint16_t *s = src + static_cast<long long>(row) * lds + i * kPer;
       uint16_t *d = dst + static_cast<long long>(row) * ldd + i * kPer;
@@ -449,7 +470,7 @@ counting_rows_kernel(const LinearLoss p, const uint16_t *src, long long lds, uin
 template <typename Pair>
 __global__ void __launch_bounds__(256)
 narrow_kernel(const float *src, long long lds, void *dst, long long ldd, int rows, int cols, const float *factor, int c_dtype) {
-  const float f = factor != nullptr ? *factor : 1.0f;
+  const float f = *factor;
   for (int row = blockIdx.y; row < rows; row += gridDim.y) {
     const float *s = src + static_cast<long long>(row) * lds;
     uint16_t *d = static_cast<uint16_t *>(dst) + static_cast<long long>(row) * ldd;
@@ -508,23 +529,18 @@ cudaError_t launch_linear_loss_join(const LinearLoss &p, cudaStream_t stream) {
   return cudaGetLastError();
 }
 
-cudaError_t launch_linear_loss_scale(const LinearLoss &p, float *scales, cudaStream_t stream) {
-  loss::scale_kernel<<<1, 1024, 0, stream>>>(p, scales);
-  return cudaGetLastError();
-}
-
-cudaError_t launch_linear_loss_rows(const LinearLoss &p, const void *h, long long ldh, void *copy, long long ldc,
-                                    cudaStream_t stream) {
+cudaError_t launch_linear_loss_prepare(const LinearLoss &p, float *scales, const void *h, long long ldh, void *copy,
+                                       long long ldc, cudaStream_t stream) {
   const bool wide = (reinterpret_cast<uintptr_t>(h) & 15) == 0 && (ldh & 7) == 0;
   const int words = wide ? (p.width + 7) / 8 : p.width;
-  const dim3 grid(static_cast<unsigned>(words < 4096 ? (words + 255) / 256 : 16),
-                  static_cast<unsigned>(p.rows < 65535 ? p.rows : 65535));
+  const dim3 grid(copy == nullptr ? 1u : static_cast<unsigned>(words < 4096 ? (words + 255) / 256 : 16),
+                  copy == nullptr ? 1u : static_cast<unsigned>(1 + (p.rows < 65534 ? p.rows : 65534)));
   const uint16_t *src = static_cast<const uint16_t *>(h);
   uint16_t *dst = static_cast<uint16_t *>(copy);
   if (wide)
-    loss::counting_rows_kernel<uint4><<<grid, 256, 0, stream>>>(p, src, ldh, dst, ldc);
+    loss::prepare_kernel<uint4><<<grid, 256, 0, stream>>>(p, scales, src, ldh, dst, ldc);
   else
-    loss::counting_rows_kernel<uint16_t><<<grid, 256, 0, stream>>>(p, src, ldh, dst, ldc);
+    loss::prepare_kernel<uint16_t><<<grid, 256, 0, stream>>>(p, scales, src, ldh, dst, ldc);
   return cudaGetLastError();
 }
 
