@@ -2649,6 +2649,8 @@ int hcCudaGemmW4(HcCudaContext *ctx, const HcCudaGemmW4Args *args) {
   p.c = args->c;
   p.ldc = args->ldc;
   p.c_dtype = args->c_dtype;
+  p.c_vector = args->ldc % 4 == 0 &&
+               (reinterpret_cast<uintptr_t>(args->c) & (args->c_dtype == HC_CUDA_C_F32 ? 15 : 7)) == 0;
   p.partials = reinterpret_cast<float *>(static_cast<char *>(ctx->scratch) + plan.partials);
   p.counters = ctx->counters;
   CUtensorMap tmap_a, tmap_q;

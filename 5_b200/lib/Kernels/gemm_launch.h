@@ -379,6 +379,7 @@ struct W4 {
   void *c;
   long long ldc;
   int c_dtype;
+  int c_vector;        // four consecutive elements of C, from a multiple of four, can be written with one access
   float *partials;     // w4_partials_bytes
   unsigned *counters;  // one per row block, zero before and after
 };

@@ -77,9 +77,11 @@ struct Zero {
 template <>
 struct Zero<false> {
   __half2 low, high;  // 1024 + z, and -(64 + z) for nibbles left four bits up
+  __half2 mixed;      // -(1024 + z), -(64 + z)
   __device__ void set(int z) {
     low = __float2half2_rn(1024.0f + static_cast<float>(z));
     high = __float2half2_rn(-64.0f - static_cast<float>(z));
+    mixed = __floats2half2_rn(-1024.0f - static_cast<float>(z), -64.0f - static_cast<float>(z));
   }
   __device__ void set_pair(uint32_t pair) {
     low = *reinterpret_cast<const __half2 *>(&pair);
@@ -108,6 +110,27 @@ __device__ __forceinline__ void expand(uint32_t w, const Zero<false> &z, uint32_
     const uint32_t u = and_or(x, 0x00f000f0u, 0x64006400u);  // 1024 + 16 q
     const __half2 e = __hfma2(*reinterpret_cast<const __half2 *>(&u), sixteenth, z.high);
     out[2 * i + 1] = *reinterpret_cast<const uint32_t *>(&e);
+  }
+}
+
+// The same in the order of k, pairs (0,1) (2,3) (4,5) (6,7), at two or three instructions more per word: a byte
+// comes into both halves of a word, and of one of them the upper nibble counts (which bfloat16 has no bits for).
+__device__ __forceinline__ void expand_in_order(uint32_t w, const Zero<true> &z, uint32_t *out) {
+  const uint32_t upper = w >> 4;
+#pragma unroll
+  for (uint32_t i = 0; i < 4; ++i) {
+    const uint32_t v = and_or(__byte_perm(w, upper, 0x0400u + 0x1111u * i), 0x000f000fu, 0x43004300u);
+    const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&v), z.low);
+    out[i] = *reinterpret_cast<const uint32_t *>(&d);
+  }
+}
+__device__ __forceinline__ void expand_in_order(uint32_t w, const Zero<false> &z, uint32_t *out) {
+  const __half2 down = __floats2half2_rn(1.0f, 0.0625f);
+#pragma unroll
+  for (uint32_t i = 0; i < 4; ++i) {
+    const uint32_t v = and_or(__byte_perm(w, w, 0x1111u * i), 0x00f0000fu, 0x64006400u);  // 1024 + q, 1024 + 16 q
+    const __half2 d = __hfma2(*reinterpret_cast<const __half2 *>(&v), down, z.mixed);
+    out[i] = *reinterpret_cast<const uint32_t *>(&d);
   }
 }
 
@@ -159,6 +182,12 @@ __device__ __forceinline__ void tmem_store_x32(uint32_t taddr, const uint32_t (&
          "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
          "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
+}
+// True in one lane of the (whole) warp, which the compiler knows to be one.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(one));
+  return one != 0;
 }
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -259,28 +288,6 @@ __device__ __forceinline__ void load_bytes(const uint8_t *src, uint32_t (&out)[(
 __device__ __forceinline__ uint4 in_pairs(const uint4 &v) {
   return make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
                     __byte_perm(v.y, v.w, 0x7632));
-}
-
-// Rows first, first + step, ... below m of a stage of A, in place: element 8 j + 2 i + h becomes what was 8 j + i +
-// 4 h. A lane takes the same 16-byte piece of every row.
-__device__ __forceinline__ void arrange_rows(uint32_t a_addr, uint32_t box_bytes, int first, int step, int m, int lane) {
-  const uint32_t at = a_addr + static_cast<uint32_t>(lane >> 3) * box_bytes;
-  auto place = [&](int t) {
-    return at + static_cast<uint32_t>(t) * 128 + ((static_cast<uint32_t>(lane & 7) ^ static_cast<uint32_t>(t & 7)) << 4);
-  };
-  int t = first;
-  for (; t + 7 * step < m; t += 8 * step) {  // eight loads in flight
-    uint4 v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      v[i] = lds128(place(t + i * step));
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      sts128(place(t + i * step), in_pairs(v[i]));
-  }
-  for (; t < m; t += step)
-    sts128(place(t), in_pairs(lds128(place(t))));
-  fence_proxy_async_smem();  // the tensor cores read it next
 }
 
 // The scales and zero points on their way from memory to the stages, four rows of q per lane of the warp that
@@ -710,21 +717,27 @@ gemm_w4_few_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
 namespace many {
 
 constexpr int kHalfK = 128;    // of a stage, for each of the two sets
-constexpr int kStepK = 64;     // of k between two hand-overs of a set, two per stage
-constexpr int kExpanders = 8;  // warps: 2 sets x 4 quarters of the tensor-memory lanes
-constexpr int kProducerWarp = kExpanders, kMmaWarp = kExpanders + 1, kFirstHelper = kExpanders + 2;
-constexpr int kHelpers = 2;    // warps that put A in order, and copy rows of q at odd places
-constexpr int kThreads = 32 * (kExpanders + 2 + kHelpers);
-constexpr uint32_t kOperandColumns = kStepK / 2;  // 32-bit columns of tensor memory per operand buffer
-constexpr uint32_t kSumsAt = 4 * kOperandColumns;
+constexpr int kCollectors = 4;  // warps, one per quarter of the tensor-memory lanes; the first ones of the CTA
+constexpr int kExpanders = 8;   // warps: 2 sets x 4 quarters
+constexpr int kProducerWarp = kCollectors + kExpanders, kMmaWarp = kProducerWarp + 1, kHelperWarp = kMmaWarp + 2;
+// Rows of q at odd places are copied by the producer and one more warp.
+constexpr int kCopiers = 2;
 
 // What follows from the rows of A a launch is made for (kTokens = 32 or 64, also N of the instruction), the group
 // and q's alignment.
 template <int kTokens, bool kPhase, int kGroup>
 struct Shape {
+  static constexpr int kThreads = 32 * (kCollectors + kExpanders + 3 + (kPhase ? kCopiers - 1 : 0));
   static constexpr int kGroupsPerHalf = kHalfK / kGroup;  // 1, 2 or 4
-  static constexpr int kAccs = kGroup == 32 ? 2 : 1;      // groups of a step, each with sums of its own
-  static constexpr int kSlots = kAccs * kTokens == 128 ? 1 : 2;  // places for sums per set
+  // Of k between two hand-overs of a set. Every hand-over costs the issuing thread a wait and a commit, about as
+  // much as four instructions of this size, so a half is handed over at once where tensor memory has room for
+  // the sums of all its groups (64 x 18944 x 8192: XX us, in halves of it YY us).
+  static constexpr int kStepK = kGroupsPerHalf * kTokens <= 128 ? kHalfK : kHalfK / 2;
+  static constexpr int kSteps = kHalfK / kStepK;
+  static constexpr int kAccs = kStepK / kGroup;  // groups of a step, each with sums of its own
+  static constexpr int kSlots = kAccs * kTokens <= 64 ? 2 : 1;  // places for sums per set
+  static constexpr uint32_t kOperandColumns = kStepK / 2;       // 32-bit columns of tensor memory per operand buffer
+  static constexpr uint32_t kSumsAt = 4 * kOperandColumns;      // two operand buffers per set
   static constexpr uint32_t kUsedColumns = kSumsAt + 2 * kSlots * kAccs * kTokens;
   static constexpr uint32_t kTmemColumns = kUsedColumns <= 256 ? 256 : 512;
   static_assert(kUsedColumns <= 512, "tensor memory");
@@ -733,19 +746,35 @@ struct Shape {
   static constexpr uint32_t kQStageBytes = kPhase ? kQPhaseBytes : kQBytes;
   static constexpr uint32_t kStageBytes = kQStageBytes + kABytes;
   static constexpr int kStages = 192 * 1024 / kStageBytes < 6 ? static_cast<int>(192 * 1024 / kStageBytes) : 6;
-  // Behind the ring: barriers, then the place where the sums of the two sets meet.
-  static constexpr uint32_t kMeetBytes = kRows * kTokens * 4;
-  static constexpr uint32_t kSmemBytes = kStages * kStageBytes + 256 + kMeetBytes + 1024;
+  // Behind the ring: barriers, then a block's sums on their way to C.
+  static constexpr uint32_t kTileBytes = kRows * kTokens * 4;
+  static constexpr uint32_t kSmemBytes = kStages * kStageBytes + 256 + kTileBytes + 1024;
   static_assert(kStages >= 3 && kSmemBytes <= 227 * 1024, "shared memory of a CTA");
   static_assert(kStageBytes % 1024 == 0 && kQStageBytes % 1024 == 0, "swizzled boxes are 1 KiB aligned");
 };
 
-// Barriers of the expanding warps, and of the first set of them, which finishes a block.
-__device__ __forceinline__ void expanders_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kExpanders) : "memory"); }
-__device__ __forceinline__ void first_set_sync() { asm volatile("bar.sync 2, %0;" ::"n"(16 * kExpanders) : "memory"); }
+// Four columns of a row of C, as far as there are.
+__device__ __forceinline__ void store_four(const W4 &p, int row, long long column, const float4 &v) {
+  const long long at = row * p.ldc + column;
+  if (column + 3 < p.n && p.c_vector != 0) {
+    if (p.c_dtype == kCTypeF32)
+      *reinterpret_cast<float4 *>(static_cast<float *>(p.c) + at) = v;
+    else
+      *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.c) + at) =
+          make_uint2(pack_pair(v.x, v.y, p.c_dtype), pack_pair(v.z, v.w, p.c_dtype));
+    return;
+  }
+  const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (column + i < p.n)
+      store_c_element(p.c, at + i, e[i], p.c_dtype);
+}
+
+__device__ __forceinline__ void collectors_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kCollectors) : "memory"); }
 
 template <bool kBf16, int kTokens, bool kPhase, int kGroup>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Shape<kTokens, kPhase, kGroup>::kThreads, 1)
 gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_a, const W4 p,
                uint32_t idesc, int *status) {
   using S = Shape<kTokens, kPhase, kGroup>;
@@ -756,23 +785,22 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant
   const uint32_t bar_base = smem_base + S::kStages * S::kStageBytes;
   auto full_bar = [&](uint32_t s) { return bar_base + 8u * s; };                    // q and A have arrived
   auto empty_bar = [&](uint32_t s) { return bar_base + 8u * (S::kStages + s); };    // both have been read
-  auto order_bar = [&](uint32_t s) { return bar_base + 8u * (2 * S::kStages + s); };  // A is in order (arrangers)
-  auto operand_bar = [&](uint32_t set, uint32_t b) { return bar_base + 8u * (3 * S::kStages + 2 * set + b); };  // expanded
-  auto done_bar = [&](uint32_t set, uint32_t b) { return bar_base + 8u * (3 * S::kStages + 4 + 2 * set + b); };  // multiplied
-  constexpr uint32_t kMiscOff = S::kStages * S::kStageBytes + 8u * (3 * S::kStages + 8);
-  static_assert(8 * (3 * S::kStages + 8) + 12 <= 256, "barriers");
+  auto operand_bar = [&](uint32_t set, uint32_t b) { return bar_base + 8u * (2 * S::kStages + 2 * set + b); };  // expanded
+  // A step's products are done: its operand buffer is free, its sums are there.
+  auto done_bar = [&](uint32_t set, uint32_t b) { return bar_base + 8u * (2 * S::kStages + 4 + 2 * set + b); };
+  constexpr uint32_t kMiscOff = S::kStages * S::kStageBytes + 8u * (2 * S::kStages + 8);
+  static_assert(8 * (2 * S::kStages + 8) + 12 <= 256, "barriers");
   volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(smem_gen + kMiscOff);
   volatile uint32_t *last_flag = abort_flag + 1;
   volatile uint32_t *tmem_slot = abort_flag + 2;
   const int warp = static_cast<int>(threadIdx.x >> 5), lane = static_cast<int>(threadIdx.x & 31);
   if (threadIdx.x == 0) {
     for (uint32_t s = 0; s < S::kStages; ++s) {
-      mbar_init(full_bar(s), 1 + (kPhase ? 32 * kHelpers : 0));
-      mbar_init(empty_bar(s), kExpanders + 2);  // every expanding warp, and the products of each half
-      mbar_init(order_bar(s), kHelpers);
+      mbar_init(full_bar(s), 1 + (kPhase ? 32 * kCopiers : 0));
+      mbar_init(empty_bar(s), kExpanders + kCollectors);  // q has been read, and A (the products are done)
     }
     for (uint32_t i = 0; i < 4; ++i) {
-      mbar_init(operand_bar(i >> 1, i & 1), kExpanders / 2);
+      mbar_init(operand_bar(i >> 1, i & 1), kExpanders / 2 + kCollectors);  // expanded, and its place for sums is free
       mbar_init(done_bar(i >> 1, i & 1), 1);
     }
     *abort_flag = 0;
@@ -812,6 +840,8 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant
           tma_load_2d(a_dst + j * S::kABoxBytes, &tmap_a, full_bar(stage), ks * kStageK + j * 64, 0);
       }
       __syncwarp();
+      if (kPhase)
+        copy_stage(p, smem_base + stage * S::kStageBytes, full_bar(stage), block, ks, 0, kCopiers, lane);
       if (++stage == S::kStages) {
         stage = 0;
         phase ^= 1u;
@@ -821,62 +851,51 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant
         ++block;
       }
     }
-  } else if (warp == kMmaWarp) {
+    if (kPhase)
+      asm volatile("cp.async.wait_all;" ::: "memory");
+  } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
+    const uint32_t set = static_cast<uint32_t>(warp - kMmaWarp);
     // ------------------------------------------------------------ MMA issuer --------
-    uint32_t stage = 0, phase = 0, turn = 0;  // turn: stages done so far, modulo 2
+    // The whole warp walks along, so that the instructions' operands are known to be uniform; one lane issues.
+    uint32_t stage = 0, step = 0;  // step: of a set, counted from the start
     bool ok = true;
     for (int unit = unit_begin; ok && unit < unit_end; ++unit) {
       const uint32_t a_addr = smem_base + stage * S::kStageBytes + S::kQStageBytes;
-      const bool ready = mbar_wait(order_bar(stage), phase, abort_flag);
-      if (!__all_sync(0xffffffffu, ready))
-        break;
-      if (lane == 0) {
 #pragma unroll
-        for (uint32_t step = 0; step < 2; ++step) {
+      for (uint32_t part = 0; part < S::kSteps; ++part, ++step) {
+        const uint32_t buffer = step & 1u, slot = S::kSlots == 2 ? buffer : 0u;
+        // (The expanding warps have waited for the stage, A included.)
+        const bool ready = mbar_wait(operand_bar(set, buffer), (step >> 1) & 1u, abort_flag);
+        ok = __all_sync(0xffffffffu, ready);
+        if (!ok)
+          break;
+        tcgen05_fence_after_sync();
+        const uint32_t sums = tmem_base + S::kSumsAt + (set * S::kSlots + slot) * (S::kAccs * kTokens);
+        const uint32_t operand = tmem_base + (2 * set + buffer) * S::kOperandColumns;
+        // 64 of k are one box of A.
+        const uint64_t desc = make_smem_desc_sw128(a_addr + (set * kHalfK + part * S::kStepK) / 64 * S::kABoxBytes, 16, 1024);
+        if (elect_one()) {
 #pragma unroll
-          for (uint32_t set = 0; set < 2; ++set) {
-            if (ok && !mbar_wait(operand_bar(set, step), turn, abort_flag))
-              ok = false;
-            if (!ok)
-              continue;
-            tcgen05_fence_after_sync();
-            const uint32_t slot = kGroup == 128 ? turn : S::kSlots == 2 ? step : 0u;
-            const uint32_t sums = tmem_base + kSumsAt + (set * S::kSlots + slot) * (S::kAccs * kTokens);
-            const uint32_t operand = tmem_base + (2 * set + step) * kOperandColumns;
-            // 64 of k are one box of A.
-            const uint64_t desc = make_smem_desc_sw128(a_addr + (2 * set + step) * S::kABoxBytes, 16, 1024);
-#pragma unroll
-            for (uint32_t kk = 0; kk < kStepK / 16; ++kk) {
-              const bool first = kGroup == 128 ? step == 0 && kk == 0 : (kk * 16) % kGroup == 0;
-              umma_f16_ts(sums + (kGroup == 32 ? kk / 2 : 0) * kTokens, operand + kk * 8, desc + kk * 2, idesc, first ? 0u : 1u);
-            }
-            umma_commit(done_bar(set, step));
-            if (step == 1)
-              umma_commit(empty_bar(stage));  // this half of A's stage has been read
-          }
+          for (uint32_t kk = 0; kk < S::kStepK / 16; ++kk)
+            umma_f16_ts(sums + (kk * 16 / kGroup) * kTokens, operand + kk * 8,
+                        desc + (kk / 4) * (S::kABoxBytes >> 4) + (kk % 4) * 2, idesc, (kk * 16) % kGroup == 0 ? 0u : 1u);
+          umma_commit(done_bar(set, buffer));
         }
+        __syncwarp();
       }
-      ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-      turn ^= 1u;
-      if (++stage == S::kStages) {
+      if (++stage == S::kStages)
         stage = 0;
-        phase ^= 1u;
-      }
     }
-  } else if (warp >= kFirstHelper) {
-    // ------------------------------------------------------------ helpers -----------
-    const int helper = warp - kFirstHelper;
-    // A is put in order so many units behind the copies (fewer than the ring holds): by then they have mostly
-    // landed, and the copies stay ahead.
-    constexpr int kBehind = kPhase ? 2 : 0;
-    uint32_t stage = 0, phase = 0, arrange_stage = 0, arrange_phase = 0;
-    int block = unit_begin / stages_k, ks = unit_begin - block * stages_k;
-    for (int unit = unit_begin; unit < unit_end + kBehind; ++unit) {
-      if (kPhase && unit < unit_end) {
+  } else if (warp == kHelperWarp) {
+    // ------------------------------------------------------------ the other copier ---
+    if constexpr (kPhase) {
+      uint32_t stage = 0, phase = 0;
+      int block = unit_begin / stages_k, ks = unit_begin - block * stages_k;
+      for (int unit = unit_begin; unit < unit_end; ++unit) {
         const bool free = mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag);
         if (!__all_sync(0xffffffffu, free))
           break;
-        copy_stage(p, smem_base + stage * S::kStageBytes, full_bar(stage), block, ks, helper, kHelpers, lane);
+        copy_stage(p, smem_base + stage * S::kStageBytes, full_bar(stage), block, ks, 1, kCopiers, lane);
         if (++stage == S::kStages) {
           stage = 0;
           phase ^= 1u;
@@ -886,34 +905,139 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant
           ++block;
         }
       }
-      if (unit >= unit_begin + kBehind) {
-        const bool ready = mbar_wait(full_bar(arrange_stage), arrange_phase, abort_flag);
-        if (!__all_sync(0xffffffffu, ready))
-          break;
-        arrange_rows(smem_base + arrange_stage * S::kStageBytes + S::kQStageBytes, S::kABoxBytes, helper, kHelpers, p.m, lane);
-        __syncwarp();
-        if (lane == 0)
-          mbar_arrive(order_bar(arrange_stage));
-        if (++arrange_stage == S::kStages) {
-          arrange_stage = 0;
-          arrange_phase ^= 1u;
+      asm volatile("cp.async.wait_all;" ::: "memory");
+    }
+  } else if (warp >= kCollectors) {
+    // ------------------------------------------------------------ expanding warps ---
+    const uint32_t set = static_cast<uint32_t>(warp - kCollectors) >> 2;
+    const int local = (warp & 3) * 32 + lane;  // this lane's row of the block, and its tensor-memory lane
+    const uint32_t operands = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16) + 2 * set * S::kOperandColumns;
+    uint32_t stage = 0, phase = 0, step = 0;  // step: of this set, counted from the start
+    bool ok = true;
+    int block = unit_begin / stages_k, ks = unit_begin - block * stages_k;
+    uint32_t row_at = static_cast<uint32_t>(local) * 128, row_shift = 0;
+    // Zero points of this stage and the next two, a byte per group. (Rows past the end take the last row's; what
+    // becomes of them is not stored.)
+    uint32_t raw[2] = {0x08080808u, 0x08080808u};
+    auto fetch = [&](int unit, uint32_t &into) {
+      if (p.zeros == nullptr || unit >= unit_end)
+        return;
+      const int at_block = unit / stages_k, at_ks = unit - at_block * stages_k;
+      const long long row = min(static_cast<long long>(at_block) * kRows + local, static_cast<long long>(p.n) - 1);
+      const uint8_t *const zeros = p.zeros + row * p.ldz;
+      const int first = (at_ks * 2 + static_cast<int>(set)) * S::kGroupsPerHalf;
+      into = 0u;
+#pragma unroll
+      for (int j = 0; j < S::kGroupsPerHalf; ++j)  // (p.span: how many of the kernel's groups share a scale)
+        into |= static_cast<uint32_t>(zeros[min(p.span == 1 ? first + j : (first + j) / p.span, p.groups - 1)]) << (8 * j);
+    };
+    fetch(unit_begin, raw[0]);
+    fetch(unit_begin + 1, raw[1]);
+    for (int unit = unit_begin; ok && unit < unit_end; ++unit) {
+      if constexpr (kPhase) {
+        const uint32_t at = static_cast<uint32_t>(
+            (reinterpret_cast<uintptr_t>(p.q) + (static_cast<long long>(block) * kRows + local) * p.ldq) & 15);
+        row_at = static_cast<uint32_t>(local) * kPhasePitch + set * 64 + (at & ~3u);
+        row_shift = 8 * (at & 3u);
+      }
+      Zero<kBf16> zero[S::kGroupsPerHalf];
+#pragma unroll
+      for (int j = 0; j < S::kGroupsPerHalf; ++j)
+        zero[j].set(static_cast<int>((raw[0] >> (8 * j)) & 0xffu));
+      raw[0] = raw[1];
+      fetch(unit + 2, raw[1]);
+      const bool ready = mbar_wait(full_bar(stage), phase, abort_flag);
+      if (!__all_sync(0xffffffffu, ready))
+        break;
+      const uint32_t q_addr = smem_base + stage * S::kStageBytes + row_at;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {  // 64 of k at a time
+        const uint32_t buffer = step & 1u;
+        uint32_t w[8], r[32];
+        if constexpr (kPhase) {
+          uint32_t low = lds32(q_addr + half * 32);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t high = lds32(q_addr + half * 32 + i * 4 + 4);
+            w[i] = __funnelshift_r(low, high, row_shift);
+            low = high;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t piece = set * 4 + static_cast<uint32_t>(2 * half + i);
+            const uint4 v = lds128(q_addr + ((piece ^ (static_cast<uint32_t>(lane) & 7u)) << 4));
+            w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          expand_in_order(w[i], zero[(half * 8 + i) * 8 / kGroup], r + 4 * i);
+        if (half == 1) {
+          __syncwarp();
+          if (lane == 0)
+            mbar_arrive(empty_bar(stage));  // this warp's rows of q have been read
+        }
+        if ((S::kSteps == 2 || half == 0) && step >= 2) {  // the step that had this buffer must be done
+          const bool done = mbar_wait(done_bar(set, buffer), ((step >> 1) & 1u) ^ 1u, abort_flag);
+          if (!__all_sync(0xffffffffu, done)) {
+            ok = false;
+            break;
+          }
+          tcgen05_fence_after_sync();
+        }
+        tmem_store_x32(operands + buffer * S::kOperandColumns + (S::kSteps == 1 ? half * 32 : 0), r);
+        if (S::kSteps == 2 || half == 1) {
+          tmem_store_wait();
+          tcgen05_fence_before_sync();
+          __syncwarp();
+          if (lane == 0)
+            mbar_arrive(operand_bar(set, buffer));
+          ++step;
         }
       }
+      if (++stage == S::kStages) {
+        stage = 0;
+        phase ^= 1u;
+      }
+      if (++ks == stages_k) {
+        ks = 0;
+        ++block;
+      }
     }
-    if (kPhase)
-      asm volatile("cp.async.wait_all;" ::: "memory");
   } else {
-    // ------------------------------------------------------------ expanding warps ---
-    const uint32_t set = static_cast<uint32_t>(warp >> 2);
-    const int local = (warp & 3) * 32 + lane;  // this lane's row of the block, and its tensor-memory lane
-    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t operands = tmem_base + lanes + 2 * set * kOperandColumns;
-    const uint32_t sums = tmem_base + lanes + kSumsAt + set * (S::kSlots * S::kAccs * kTokens);
-    float *const meet = reinterpret_cast<float *>(smem_gen + S::kStages * S::kStageBytes + 256);
-    uint32_t stage = 0, phase = 0, turn = 0;
-    bool used = false;  // whether the operand buffers hold an earlier stage's steps
-    int unit = unit_begin;
+    // ------------------------------------------------------------ collecting warps --
+    const int local = warp * 32 + lane;  // this lane's row of the block, i.e. column of C
+    const uint32_t sums = tmem_base + (static_cast<uint32_t>(warp * 32) << 16) + S::kSumsAt;
+    constexpr int kGroups = kStageK / kGroup;  // of a stage: 2, 4 or 8
+    constexpr int kChunk = kTokens < 32 ? kTokens : 32;
+    uint32_t stage = 0, step = 0;
     bool ok = true;  // (a wait that ran out: the barriers below are still met)
+    int unit = unit_begin;
+    // Scales of this stage and the next two, two to a word. (A sector of them that is not in the cache yet takes
+    // longer to arrive than a stage takes to expand. Rows past the end take the last row's.)
+    uint32_t raw[2][kGroups / 2];
+    auto fetch = [&](int at_unit, uint32_t (&into)[kGroups / 2]) {
+      if (at_unit >= unit_end)
+        return;
+      const int at_block = at_unit / stages_k, first = (at_unit - at_block * stages_k) * kGroups;
+      const long long row = min(static_cast<long long>(at_block) * kRows + local, static_cast<long long>(p.n) - 1);
+      const uint16_t *const scales = p.scales + row * p.lds;
+      if (p.vector_scales) {
+        load_words(scales + first, into);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kGroups; ++j) {
+          const uint32_t v = scales[min(p.span == 1 ? first + j : (first + j) / p.span, p.groups - 1)];
+          into[j / 2] = j % 2 == 0 ? v : into[j / 2] | v << 16;
+        }
+      }
+    };
+    fetch(unit_begin, raw[0]);
+    fetch(unit_begin + 1, raw[1]);
+    if (lane == 0)
+      for (uint32_t i = 0; i < 2 * S::kSlots; ++i)  // at first every place is free
+        mbar_arrive(operand_bar(i & 1u, i >> 1));
     while (unit < unit_end) {
       const int block = unit / stages_k, ks_begin = unit - block * stages_k;
       const int ks_end = min(stages_k, ks_begin + (unit_end - unit));
@@ -921,201 +1045,117 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant
 #pragma unroll
       for (int t = 0; t < kTokens; ++t)
         total[t] = 0.0f;
-      // Adds the sums at `slot`, times their groups' scales.
-      auto collect = [&](uint32_t slot, const float *scale) {
+      for (int ks = ks_begin; ok && ks < ks_end; ++ks) {
+        uint32_t now[kGroups / 2];
 #pragma unroll
-        for (int j = 0; j < S::kAccs; ++j) {
-          const uint32_t at = sums + (slot * S::kAccs + j) * kTokens;
-#pragma unroll
-          for (int t0 = 0; t0 < kTokens; t0 += 16) {
-            uint32_t r[16];
-            tmem_load_32x32b_x16(at + t0, r);
-            tmem_load_wait();
-#pragma unroll
-            for (int t = 0; t < 16; ++t)
-              total[t0 + t] = fmaf(scale[j], __uint_as_float(r[t]), total[t0 + t]);
-          }
+        for (int j = 0; j < kGroups / 2; ++j) {
+          now[j] = raw[0][j];
+          raw[0][j] = raw[1][j];
         }
-      };
-      // Waits until the products of this set's step in buffer `b` of the stage with that turn are done.
-      auto wait_done = [&](uint32_t b, uint32_t of_turn) {
-        const bool done = mbar_wait(done_bar(set, b), of_turn, abort_flag);
-        if (!__all_sync(0xffffffffu, done))
-          ok = false;
-        tcgen05_fence_after_sync();
-      };
-      if (ok) {
-        // Rows past the end are computed on the last row's scales and not stored.
-        const long long row = static_cast<long long>(block) * kRows + local < p.n ? static_cast<long long>(block) * kRows + local : p.n - 1;
-        const uint16_t *const scales = p.scales + row * p.lds;
-        const uint8_t *const zeros = p.zeros != nullptr ? p.zeros + row * p.ldz : nullptr;
-        uint32_t row_at, row_shift = 0;
-        if constexpr (kPhase) {
-          const uint32_t at = static_cast<uint32_t>(
-              (reinterpret_cast<uintptr_t>(p.q) + (static_cast<long long>(block) * kRows + local) * p.ldq) & 15);
-          row_at = static_cast<uint32_t>(local) * kPhasePitch + set * 64 + (at & ~3u);
-          row_shift = 8 * (at & 3u);
-        } else {
-          row_at = static_cast<uint32_t>(local) * 128;
-        }
-        // Raw scales and zero points of this stage and the next two (a sector of them that is not in the cache
-        // yet takes longer to arrive than a stage takes to expand).
-        uint32_t raw[2][S::kGroupsPerHalf];
-        auto fetch = [&](int ks, uint32_t (&into)[S::kGroupsPerHalf]) {
-          // (p.span: how many of the kernel's groups share a scale, for groups of several times 128.)
-          const int first = (ks * 2 + static_cast<int>(set)) * S::kGroupsPerHalf;
+        fetch(unit + (ks - ks_begin) + 2, raw[1]);
 #pragma unroll
-          for (int j = 0; j < S::kGroupsPerHalf; ++j) {
-            const int group = min(p.span == 1 ? first + j : (first + j) / p.span, p.groups - 1);
-            into[j] = scales[group] | (zeros != nullptr ? zeros[group] : 8u) << 16;
-          }
-        };
-        fetch(ks_begin, raw[0]);
-        if (ks_begin + 1 < ks_end)
-          fetch(ks_begin + 1, raw[1]);
-        float before[S::kGroupsPerHalf];  // scales of the stage whose sums are not yet collected
-        bool pending = false;
-        for (int ks = ks_begin; ok && ks < ks_end; ++ks) {
-          float scale[S::kGroupsPerHalf];
-          Zero<kBf16> zero[S::kGroupsPerHalf];
+        for (int part = 0; part < S::kSteps; ++part, ++step) {
+          const uint32_t buffer = step & 1u, slot = S::kSlots == 2 ? buffer : 0u;
 #pragma unroll
-          for (int j = 0; j < S::kGroupsPerHalf; ++j) {
-            scale[j] = scale_value<kBf16>(static_cast<uint16_t>(raw[0][j]));
-            zero[j].set(static_cast<int>(raw[0][j] >> 16));
-            raw[0][j] = raw[1][j];
-          }
-          if (ks + 2 < ks_end)
-            fetch(ks + 2, raw[1]);
-          const bool ready = mbar_wait(full_bar(stage), phase, abort_flag);
-          if (!__all_sync(0xffffffffu, ready)) {
-            ok = false;
-            break;
-          }
-          const uint32_t q_addr = smem_base + stage * S::kStageBytes + row_at;
+          for (uint32_t set = 0; set < 2; ++set) {
+            const bool done = mbar_wait(done_bar(set, buffer), (step >> 1) & 1u, abort_flag);
+            if (!__all_sync(0xffffffffu, done))
+              ok = false;
+            tcgen05_fence_after_sync();
 #pragma unroll
-          for (int step = 0; step < 2; ++step) {
-            if (!ok)
-              break;
-            uint32_t w[8], r[32];
-            if constexpr (kPhase) {
-              uint32_t low = lds32(q_addr + step * 32);
+            for (int j = 0; j < S::kAccs; ++j) {
+              const int group = static_cast<int>(set) * (kGroups / 2) + part * S::kAccs + j;
+              const float scale = scale_value<kBf16>(
+                  static_cast<uint16_t>(group % 2 == 0 ? now[group / 2] & 0xffffu : now[group / 2] >> 16));
+              const uint32_t at = sums + ((set * S::kSlots + slot) * S::kAccs + j) * kTokens;
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const uint32_t high = lds32(q_addr + step * 32 + i * 4 + 4);
-                w[i] = __funnelshift_r(low, high, row_shift);
-                low = high;
-              }
-            } else {
+              for (int t0 = 0; t0 < kTokens; t0 += kChunk) {
+                uint32_t r[kChunk];
+                tmem_load_32x32b_x32(at + t0, r);
+                tmem_load_wait_for(r);
 #pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                const uint32_t piece = set * 4 + static_cast<uint32_t>(2 * step + i);
-                const uint4 v = lds128(q_addr + ((piece ^ (static_cast<uint32_t>(lane) & 7u)) << 4));
-                w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+                for (int t = 0; t < kChunk; ++t)
+                  total[t0 + t] = fmaf(scale, __uint_as_float(r[t]), total[t0 + t]);
               }
             }
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              expand(w[i], zero[(step * 8 + i) * 8 / kGroup], r + 4 * i);
-            if (step == 1) {
-              __syncwarp();
-              if (lane == 0)
-                mbar_arrive(empty_bar(stage));  // this warp's rows of q have been read
-            }
-            if (used)
-              wait_done(static_cast<uint32_t>(step), turn ^ 1u);  // the step that had this buffer a stage ago
-            tmem_store_x32(operands + static_cast<uint32_t>(step) * kOperandColumns, r);
-            // Sums that this step's products overwrite are collected first; they are done, by the wait above
-            // (with one place only, they are those of the step before, which are waited for here).
-            if constexpr (kGroup != 128 && S::kSlots == 2) {
-              if (pending)
-                collect(static_cast<uint32_t>(step), before + step * S::kAccs);
-            }
-            if constexpr (S::kSlots == 1) {
-              if (step == 0 ? pending : true) {
-                wait_done(static_cast<uint32_t>(step ^ 1), step == 0 ? turn ^ 1u : turn);
-                collect(0, step == 0 ? before + S::kAccs : scale);
-              }
-            }
-            tmem_store_wait();
             tcgen05_fence_before_sync();
             __syncwarp();
-            if (lane == 0)
-              mbar_arrive(operand_bar(set, static_cast<uint32_t>(step)));
-          }
-          // Groups of a whole stage half: the stage before is done, both its buffers having been waited for.
-          if constexpr (kGroup == 128) {
-            if (pending)
-              collect(turn ^ 1u, before);
-          }
-#pragma unroll
-          for (int j = 0; j < S::kGroupsPerHalf; ++j)
-            before[j] = scale[j];
-          pending = used = true;
-          turn ^= 1u;
-          if (++stage == S::kStages) {
-            stage = 0;
-            phase ^= 1u;
+            if (lane == 0)  // the step that will fill this place next has it
+              mbar_arrive(operand_bar(set, (step + S::kSlots) & 1u));
           }
         }
-        if (ok && pending) {  // the last stage of the segment
-          wait_done(0, turn ^ 1u);
-          wait_done(1, turn ^ 1u);
-          if constexpr (kGroup == 128) {
-            collect(turn ^ 1u, before);
-          } else if constexpr (S::kSlots == 2) {
-            collect(0, before);
-            collect(1, before + S::kAccs);
-          } else {
-            collect(0, before + S::kAccs);
-          }
-          tcgen05_fence_before_sync();
-        }
+        if (lane == 0)
+          mbar_arrive(empty_bar(stage));  // all products with this stage of A are done
+        if (++stage == S::kStages)
+          stage = 0;
       }
       unit += ks_end - ks_begin;
 
-      // The two sets meet in shared memory; a lane holds a row of q, i.e. a column of C.
-      if (set == 1) {
+      // The sums, one token's 128 columns after another's: into shared memory where the block is all this CTA's,
+      // else into its slot, from which the last of the CTAs that share it adds them up. Then warps take tokens and
+      // lanes four columns each. (This code runs once per block, mostly from a cold instruction cache: it is
+      // short, and all rows are kept, those past m being zeros.)
+      constexpr int kSlot = kRows * kTokens;
+      float *const tile = reinterpret_cast<float *>(smem_gen + S::kStages * S::kStageBytes + 256);
+      const bool whole = ks_begin == 0 && ks_end == stages_k;
+      int first = cta, last = cta;
+      if (whole) {
 #pragma unroll
         for (int t = 0; t < kTokens; ++t)
-          meet[t * kRows + local] = total[t];
+          tile[t * kRows + local] = total[t];
+        collectors_sync();
+      } else {
+        first = owner_of(p, block * stages_k);
+        last = owner_of(p, (block + 1) * stages_k - 1);
+        float *const mine = part_slot(p, cta, first, block, kSlot) + local;
+#pragma unroll
+        for (int t = 0; t < kTokens; ++t)
+          __stcg(mine + t * kRows, total[t]);
+        if (!count_part(p, block, last - first + 1, last_flag, [] { collectors_sync(); }))
+          continue;
       }
-      expanders_sync();
-      if (set == 0) {
+      const long long column = static_cast<long long>(block) * kRows + 4 * lane;
+      constexpr int kAtOnce = 4;  // tokens of a warp, and parts, whose loads are in flight together
+#pragma unroll 1
+      for (int t0 = warp; t0 < p.m; t0 += kCollectors * kAtOnce) {
+        float4 sum[kAtOnce];
+        if (whole) {
 #pragma unroll
-        for (int t = 0; t < kTokens; ++t)
-          total[t] += meet[t * kRows + local];
-        bool store = true;
-        if (ks_begin != 0 || ks_end != stages_k) {
-          constexpr int kSlot = kRows * kTokens;
-          const int first = owner_of(p, block * stages_k), last = owner_of(p, (block + 1) * stages_k - 1);
-          float *mine = part_slot(p, cta, first, block, kSlot) + local;
+          for (int u = 0; u < kAtOnce; ++u)
+            sum[u] = *reinterpret_cast<const float4 *>(tile + min(t0 + u * kCollectors, kTokens - 1) * kRows + 4 * lane);
+        } else {
 #pragma unroll
-          for (int t = 0; t < kTokens; ++t)
-            if (t < p.m)
-              __stcg(mine + t * kRows, total[t]);
-          store = count_part(p, block, last - first + 1, last_flag, [] { first_set_sync(); });
-          if (store) {
+          for (int u = 0; u < kAtOnce; ++u)
+            sum[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+          for (int part = first; part <= last; part += kAtOnce) {
+            float4 v[kAtOnce][kAtOnce];
 #pragma unroll
-            for (int t = 0; t < kTokens; ++t)
-              total[t] = 0.0f;
-            for (int part = first; part <= last; ++part) {
-              const float *from = part_slot(p, part, first, block, kSlot) + local;
+            for (int i = 0; i < kAtOnce; ++i) {
+              const float *const from = part_slot(p, min(part + i, last), first, block, kSlot) + 4 * lane;
 #pragma unroll
-              for (int t = 0; t < kTokens; ++t)
-                if (t < p.m)
-                  total[t] += __ldcg(from + t * kRows);
+              for (int u = 0; u < kAtOnce; ++u)
+                v[i][u] = __ldcg(reinterpret_cast<const float4 *>(from + min(t0 + u * kCollectors, kTokens - 1) * kRows));
             }
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i)
+              if (part + i <= last)
+#pragma unroll
+                for (int u = 0; u < kAtOnce; ++u) {
+                  sum[u].x += v[i][u].x;
+                  sum[u].y += v[i][u].y;
+                  sum[u].z += v[i][u].z;
+                  sum[u].w += v[i][u].w;
+                }
           }
         }
-        const long long column = static_cast<long long>(block) * kRows + local;
-        if (store && column < p.n) {
 #pragma unroll
-          for (int t = 0; t < kTokens; ++t)
-            if (t < p.m)
-              store_c_element(p.c, t * p.ldc + column, total[t], p.c_dtype);
-        }
+        for (int u = 0; u < kAtOnce; ++u)
+          if (t0 + u * kCollectors < p.m)
+            store_four(p, t0 + u * kCollectors, column, sum[u]);
       }
-      expanders_sync();  // `meet` is free again
+      if (whole)
+        collectors_sync();  // `tile` is free again
     }
   }
 
@@ -1167,7 +1207,7 @@ cudaError_t launch(const CUtensorMap &tmap_q, const CUtensorMap &tmap_a, const W
     if (err != cudaSuccess)
       return err;
     const uint32_t idesc = make_idesc_f16(kBf16 ? 1u : 0u, false, false, kRows, kTokens);
-    kernel<<<static_cast<unsigned>(p.grid), many::kThreads, S::kSmemBytes, stream>>>(tmap_q, tmap_a, p, idesc, status);
+    kernel<<<static_cast<unsigned>(p.grid), S::kThreads, S::kSmemBytes, stream>>>(tmap_q, tmap_a, p, idesc, status);
   }
   return cudaGetLastError();
 }

@@ -520,9 +520,10 @@ HC_CUDA_CAPI_EXPORTED int hcCudaLinearLossPlan(const HcCudaLinearLossArgs *args,
  * dloss hold,
  *   dh = g W,   dw = g^T H
  * both overwritten, in the type of h and w, each optional (NULL). lse is what hcCudaLinearLoss stored. The
- * logits are computed again, one piece of the vocabulary at a time; g is rounded to the operands' type for
- * the two products, whose sums are float32. For float16 a power of two found on the device keeps g inside
- * the type's normal range. A call gives the same bits every time. rows == 0 sets dw to zero. Uses context
+ * logits are computed again, one piece of the vocabulary at a time; g, with dloss as a fraction of its largest
+ * value among the rows that count (found on the device; for float16 times 2^14), is rounded to the operands'
+ * type for the two products, whose sums are float32 and take the factor back before they are rounded. A call
+ * gives the same bits every time. rows == 0 sets dw to zero. Uses context
  * scratch: a copy of h (for dw), g and its transpose for one piece of the vocabulary (together 512 MiB at
  * most, or 1 KiB per row where that is more), and float32 sums of dh when there is more than one piece. */
 typedef struct HcCudaLinearLossBackwardArgs {
