@@ -91,7 +91,7 @@ struct HcCudaEvent {
 };
 
 // One remembered cuTensorMapEncodeTiled result (see encode_map).
-constexpr unsigned kMapCacheEntries = 16;
+constexpr unsigned kMapCacheEntries = 48;
 struct MapCacheEntry {
   bool valid = false;
   int dtype = 0;
@@ -2653,7 +2653,7 @@ int hcCudaGemmW4(HcCudaContext *ctx, const HcCudaGemmW4Args *args) {
                (reinterpret_cast<uintptr_t>(args->c) & (args->c_dtype == HC_CUDA_C_F32 ? 15 : 7)) == 0;
   p.partials = reinterpret_cast<float *>(static_cast<char *>(ctx->scratch) + plan.partials);
   p.counters = ctx->counters;
-  CUtensorMap tmap_a, tmap_q;
+  CUtensorMap tmap_a, tmap_q[hc::sm100::w4_phases()];
   // Up to 16 rows: whole stages of k, as they lie in memory; more: boxes for the tensor cores.
   const bool few = m <= 16;
   if (int rc = encode_map(ctx, &tmap_a, args->dtype, a, static_cast<uint64_t>(k), static_cast<uint64_t>(m),
@@ -2661,11 +2661,23 @@ int hcCudaGemmW4(HcCudaContext *ctx, const HcCudaGemmW4Args *args) {
                           static_cast<uint32_t>(hc::sm100::w4_tokens(m)),
                           few ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B))
     return rc;
-  if (p.phase)
-    tmap_q = tmap_a;  // not used
-  else if (int rc = encode_map(ctx, &tmap_q, HC_CUDA_F8E4M3, args->q, static_cast<uint64_t>(p.row_bytes), static_cast<uint64_t>(n),
-                               static_cast<uint64_t>(args->ldq), 128, 128))
-    return rc;
+  if (!p.phase) {
+    if (int rc = encode_map(ctx, &tmap_q[0], HC_CUDA_F8E4M3, args->q, static_cast<uint64_t>(p.row_bytes), static_cast<uint64_t>(n),
+                            static_cast<uint64_t>(args->ldq), 128, 128))
+      return rc;
+  } else {
+    // Rows r, r + 16, ... start at the same place between two 16-byte boundaries, 16 pitches apart. (For an r past
+    // the last row any rows do: what is computed from them is not stored.)
+    constexpr int64_t phases = hc::sm100::w4_phases();
+    for (int64_t r = 0; r < phases; ++r) {
+      const int64_t row = r < n ? r : 0;
+      const uintptr_t first = reinterpret_cast<uintptr_t>(args->q) + static_cast<uintptr_t>(row * args->ldq), before = first & 15;
+      if (int rc = encode_map(ctx, &tmap_q[r], HC_CUDA_F8E4M3, reinterpret_cast<const void *>(first - before),
+                              before + static_cast<uint64_t>(p.row_bytes), static_cast<uint64_t>((n - row + phases - 1) / phases),
+                              static_cast<uint64_t>(phases * args->ldq), 128 + 16, 128 / phases, CU_TENSOR_MAP_SWIZZLE_NONE))
+        return rc;
+    }
+  }
   HC_TRY_CUDA(ctx, args->dtype == HC_CUDA_BF16
                        ? hc::sm100::launch_gemm_w4_bf16(tmap_q, tmap_a, p, ctx->status_dev, ctx->stream)
                        : hc::sm100::launch_gemm_w4_f16(tmap_q, tmap_a, p, ctx->status_dev, ctx->stream));

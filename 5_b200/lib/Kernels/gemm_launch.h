@@ -365,7 +365,7 @@ struct W4 {
   int group;      // 32, 64 or 128: the kernel's group ...
   int span;       // ... and how many of them share a scale
   int stages_k;   // w4_stages(k)
-  int phase;      // q's rows do not all start on 16-byte boundaries: tmap_q is not used
+  int phase;      // q's rows do not all start on 16-byte boundaries: tmap_q are w4_phases() maps
   int grid;       // CTAs, at most as many as there are (row block, stage of k) units
   int share;      // units of a CTA; the first `extra` CTAs have one more
   int extra;
@@ -390,16 +390,18 @@ inline long long w4_blocks(long long n) { return (n + 127) / 128; }
 inline long long w4_stages(long long k) { return (k + 255) / 256; }
 // CTAs of the kernel for up to 16 rows that fit on an SM.
 constexpr int w4_few_ctas() { return 3; }
+constexpr int w4_phases() { return 16; }
 inline int w4_grid(long long units, int m, int sm_count) {
   const long long slots = static_cast<long long>(sm_count) * (m <= 16 ? w4_few_ctas() : 1);
   return static_cast<int>(units < slots ? units : slots);
 }
 inline size_t w4_partials_bytes(int grid, int m) { return static_cast<size_t>(grid) * 2 * 128 * w4_tokens(m) * 4; }
-// tmap_q: q as bytes {row_bytes inner, n}, box {128, 128}, 128-byte swizzle; tmap_a: A as {k inner, m}, for
+// tmap_q: q as bytes {row_bytes inner, n}, box {128, 128}, 128-byte swizzle, or with `phase` map r of rows r, r + 16,
+// ... from the 16-byte boundary at or below the first one's start, box {144, 8}, without swizzle; tmap_a: A as {k inner, m}, for
 // more than 16 rows box {64, w4_tokens(m)} and 128-byte swizzle, else box {256, w4_tokens(m)} without swizzle.
-cudaError_t launch_gemm_w4_bf16(const CUtensorMap &tmap_q, const CUtensorMap &tmap_a, const W4 &p, int *status,
+cudaError_t launch_gemm_w4_bf16(const CUtensorMap *tmap_q, const CUtensorMap &tmap_a, const W4 &p, int *status,
                                 cudaStream_t stream);
-cudaError_t launch_gemm_w4_f16(const CUtensorMap &tmap_q, const CUtensorMap &tmap_a, const W4 &p, int *status,
+cudaError_t launch_gemm_w4_f16(const CUtensorMap *tmap_q, const CUtensorMap &tmap_a, const W4 &p, int *status,
                                cudaStream_t stream);
 
 } // namespace sm100

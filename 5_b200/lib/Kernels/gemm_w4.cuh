@@ -29,14 +29,19 @@
 // 17 to 64 rows: tcgen05.mma with M = 128 rows of q, N = 32 or 64. The expanded weights go to the tensor cores
 // through tensor memory, not through shared memory (the expanded form is four times q's bytes, which shared
 // memory would have to take and give back): a lane of an expanding warp owns a row of q, which is the lane its
-// operand has to lie in. Two sets of four warps take one half of a stage's k each, in steps of 64 of k. A set
-// has two operand buffers, so that a step's products run while the next step is expanded, and two places for
-// sums, so that a group's sums are read -- and added, times the group's scale, to the running ones -- only when
-// they are long done. A's pairs are formed by two helper warps.
+// operand has to lie in. Two sets of four warps take one half of a stage's k each; a set has two operand
+// buffers, so that a step's products run while the next is expanded. Four more warps collect: they read a
+// group's sums, add them, times the group's scale, to the running ones, and write C or join parts while the next
+// block is expanded already. The instructions are so small (N = 64 at most) that issuing them is what bounds
+// the kernel: one thread takes about 70 cycles for each, so each set has an issuing warp of its own
+// (64 x 18944 x 8192: 45.6 us with one, 39.1 with two, 37.9 with elect.sync in place of a lane's number). Here the
+// weights are expanded in the order of k, so that A is read as it lies.
 //
-// Rows of q that do not start on 16-byte boundaries (an odd k) cannot be addressed by a tensor map: warps of
-// their own then copy each row's 16-byte pieces from the boundary below its start with cp.async, and the
-// readers take words at the row's own phase with a funnel shift.
+// Rows of q that do not all start on 16-byte boundaries (an odd k) have a pitch that no tensor map takes, but every
+// sixteenth row lies at the same place between two boundaries: sixteen maps, of every sixteenth row from the
+// boundary at or below its start, bring such rows, 8 rows of 144 bytes each. In shared memory the rows of a block
+// then lie sorted by that place (position 8 r + i holds row 16 i + r), and the readers take words at a row's own
+// phase with a funnel shift. (1 x 18944 x 8190: 33.0 us; when warps copied the rows with cp.async, 57.5 us.)
 //
 // The (row block, stage of k) units are dealt out as one sequence, an equal share to every CTA, so that the GPU
 // is evenly loaded whatever n and k are; a CTA whose share begins or ends inside a row block leaves float32
@@ -56,9 +61,22 @@ namespace w4 {
 constexpr int kRows = 128;        // rows of q per block
 constexpr int kStageK = 256;      // of k per stage: 128 bytes of q
 constexpr uint32_t kQBytes = kRows * 128;
-constexpr int kPhasePieces = 9;   // 16-byte pieces of a row of a stage copied at its own phase
-constexpr uint32_t kPhasePitch = 16 * kPhasePieces;
+constexpr int kPhases = w4_phases();
+constexpr uint32_t kPhasePitch = 128 + 16;  // a row of a stage, with what precedes it to the boundary
 constexpr uint32_t kQPhaseBytes = kRows * kPhasePitch;
+
+// The row of a block at a position.
+template <bool kPhase>
+__device__ __forceinline__ int row_at_position(int position) {
+  return kPhase ? (position & (kRows / kPhases - 1)) * kPhases + position / (kRows / kPhases) : position;
+}
+
+// The maps of q: one, or one for every phase.
+template <bool kPhase>
+struct QMaps {
+  CUtensorMap map[kPhase ? kPhases : 1];
+};
+
 // (x & mask) | magic
 __device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t magic) {
   uint32_t r;
@@ -162,15 +180,6 @@ __device__ __forceinline__ void sts128(uint32_t addr, const uint4 &v) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" :: "r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
-// 16 bytes global -> shared, of which `bytes` are read and the rest are zeros.
-__device__ __forceinline__ void copy_16(uint32_t dst, const void *src, uint32_t bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-// One arrival on `bar` when this thread's copies so far have landed.
-__device__ __forceinline__ void copies_arrive(uint32_t bar) {
-  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" :: "r"(bar) : "memory");
-}
-
 // 32 columns of this warp's lanes of tensor memory.
 __device__ __forceinline__ void tmem_store_x32(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(
@@ -241,27 +250,17 @@ __device__ __forceinline__ bool count_part(const W4 &p, int block, int parts, vo
   return all;
 }
 
-// The work of the warps that bring rows of q from odd places: `warps` of them share a stage, 16-byte piece by
-// piece, from the boundary at or below each row's first byte.
-__device__ __forceinline__ void copy_stage(const W4 &p, uint32_t q_dst, uint32_t full, int block, int ks, int index,
-                                           int warps, int lane) {
-  const uint8_t *const q_end = p.q + (static_cast<long long>(p.n) - 1) * p.ldq + p.row_bytes;
-  const int wanted = min(128, p.row_bytes - ks * 128);  // bytes of a row in this stage, at least 1
-#pragma unroll 6
-  for (int i = index * 32 + lane; i < kRows * kPhasePieces; i += 32 * warps) {
-    const int local = i / kPhasePieces, piece = i - local * kPhasePieces;
-    const long long row = static_cast<long long>(block) * kRows + local;
-    if (row >= p.n)
-      break;
-    const uint8_t *begin = p.q + row * p.ldq + ks * 128ll;
-    const int at = static_cast<int>(reinterpret_cast<uintptr_t>(begin) & 15);
-    const uint8_t *src = begin - at + piece * 16;
-    // Nothing is read behind q; what precedes a row in its first piece belongs to the same allocation.
-    const long long inside = q_end - src;
-    if (piece * 16 < at + wanted && inside > 0)
-      copy_16(q_dst + static_cast<uint32_t>(i) * 16, src, inside < 16 ? static_cast<uint32_t>(inside) : 16u);
+// A stage of q; all lanes of a warp.
+template <bool kPhase>
+__device__ __forceinline__ void load_q(const QMaps<kPhase> &maps, uint32_t dst, uint32_t full, int block, int ks, int lane) {
+  if constexpr (kPhase) {
+    if (lane < kPhases)
+      tma_load_2d(dst + static_cast<uint32_t>(lane) * (kRows / kPhases * kPhasePitch), &maps.map[lane], full, ks * 128,
+                  block * (kRows / kPhases));
+  } else {
+    if (lane == 0)
+      tma_load_2d(dst, &maps.map[0], full, ks * 128, block * kRows);
   }
-  copies_arrive(full);
 }
 
 // 32-bit words, or bytes packed into words, from an address aligned to all of them.
@@ -293,7 +292,7 @@ __device__ __forceinline__ uint4 in_pairs(const uint4 &v) {
 // The scales and zero points on their way from memory to the stages, four rows of q per lane of the warp that
 // brings them: fetched as they lie in memory, kAhead stages early, and stored as pairs (the scale as a float,
 // what the zero point subtracts as two 16-bit floats), [group of the stage][row].
-template <bool kBf16, int kGroup>
+template <bool kBf16, bool kPhase, int kGroup>
 struct ScaleStream {
   static constexpr int kGroups = kStageK / kGroup;  // of a stage: 2, 4 or 8
   static constexpr int kAhead = 2;
@@ -317,7 +316,7 @@ struct ScaleStream {
 #pragma unroll
     for (int i = 0; i < kRows / 32; ++i) {
       // Rows past the end take the last row's scales; their results are not stored.
-      const long long at = block * kRows + i * 32 + lane, row = at < p.n ? at : p.n - 1;
+      const long long at = block * kRows + row_at_position<kPhase>(i * 32 + lane), row = at < p.n ? at : p.n - 1;
       scale_row[i] = p.scales + row * p.lds;
       zero_row[i] = p.zeros + row * p.ldz;
     }
@@ -441,7 +440,7 @@ __device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;
 
 template <bool kBf16, int kTiles, bool kPhase, int kGroup>
 __global__ void __launch_bounds__(kThreads, Shape<kTiles, kPhase, kGroup>::kCtasPerSm)
-gemm_w4_few_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_a, const W4 p,
+gemm_w4_few_kernel(const __grid_constant__ QMaps<kPhase> maps_q, const __grid_constant__ CUtensorMap tmap_a, const W4 p,
                    int *status) {
   using S = Shape<kTiles, kPhase, kGroup>;
   constexpr int kChunksPerGroup = kGroup / 32;
@@ -459,14 +458,14 @@ gemm_w4_few_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
   const int warp = static_cast<int>(threadIdx.x >> 5), lane = static_cast<int>(threadIdx.x & 31);
   if (threadIdx.x == 0) {
     for (uint32_t s = 0; s < S::kStages; ++s) {
-      mbar_init(full_bar(s), 1 + (kPhase ? 32 : 0));
+      mbar_init(full_bar(s), 1);
       mbar_init(empty_bar(s), kConsumers);
-      mbar_init(ready_bar(s), kPhase ? 1 : 2);
+      mbar_init(ready_bar(s), 2);
     }
     *abort_flag = 0;
     mbar_fence_init();
     if (!kPhase)
-      tma_prefetch_descriptor(&tmap_q);
+      tma_prefetch_descriptor(&maps_q.map[0]);
     tma_prefetch_descriptor(&tmap_a);
   }
   __syncthreads();
@@ -477,8 +476,8 @@ gemm_w4_few_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
 
   if (warp == kLoadWarp) {
     // ------------------------------------------------------------ loads -------------
-    // One lane issues the TMA loads. The others bring the scales, or the rows of q at odd places.
-    ScaleStream<kBf16, kGroup> scales(p, unit_begin, kPhase ? unit_begin : unit_end, lane);
+    // TMA loads, and the scales.
+    ScaleStream<kBf16, kPhase, kGroup> scales(p, unit_begin, unit_end, lane);
     uint32_t stage = 0, phase = 0;
     int block = unit_begin / stages_k, ks = unit_begin - block * stages_k;
     for (int unit = unit_begin; unit < unit_end; ++unit) {
@@ -487,20 +486,15 @@ gemm_w4_few_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         break;
       const uint32_t at = smem_base + stage * S::kStageBytes;
       if (lane == 0) {
-        mbar_arrive_expect_tx(full_bar(stage), kPhase ? S::kABytes : S::kStageBytes - S::kScaleBytes);
-        if (!kPhase)
-          tma_load_2d(at, &tmap_q, full_bar(stage), ks * 128, block * kRows);
+        mbar_arrive_expect_tx(full_bar(stage), S::kStageBytes - S::kScaleBytes);
         tma_load_2d(at + S::kQStageBytes, &tmap_a, full_bar(stage), ks * kStageK, 0);
       }
       __syncwarp();
-      if (kPhase) {
-        copy_stage(p, at, full_bar(stage), block, ks, 0, 1, lane);
-      } else {
-        scales.advance(p, at + S::kQStageBytes + S::kABytes, lane);
-        __syncwarp();
-        if (lane == 0)
-          mbar_arrive(ready_bar(stage));
-      }
+      load_q<kPhase>(maps_q, at, full_bar(stage), block, ks, lane);
+      scales.advance(p, at + S::kQStageBytes + S::kABytes, lane);
+      __syncwarp();
+      if (lane == 0)
+        mbar_arrive(ready_bar(stage));
       if (++stage == S::kStages) {
         stage = 0;
         phase ^= 1u;
@@ -510,21 +504,12 @@ gemm_w4_few_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         ++block;
       }
     }
-    if (kPhase)
-      asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp == kHelperWarp) {
     // ------------------------------------------------------------ helper ------------
-    // Forms A's pairs; brings the scales where the load warp copies q.
-    ScaleStream<kBf16, kGroup> scales(p, unit_begin, kPhase ? unit_end : unit_begin, lane);
+    // Forms A's pairs.
     uint32_t stage = 0, phase = 0;
     for (int unit = unit_begin; unit < unit_end; ++unit) {
       const uint32_t at = smem_base + stage * S::kStageBytes;
-      if (kPhase) {
-        const bool free = mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag);
-        if (!__all_sync(0xffffffffu, free))
-          break;
-        scales.advance(p, at + S::kQStageBytes + S::kABytes, lane);
-      }
       const bool arrived = mbar_wait(full_bar(stage), phase, abort_flag);
       if (!__all_sync(0xffffffffu, arrived))
         break;
@@ -543,6 +528,18 @@ gemm_w4_few_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     // Row g of A, of which odd rows have the halves of 128 bytes exchanged.
     const uint32_t a_lane = S::kQStageBytes + static_cast<uint32_t>(g) * 512 + static_cast<uint32_t>(q4) * 16;
     const uint32_t a_swap = (g & 1) != 0 ? 64u : 0u;
+    // This lane's four rows of q, two fragments, rows g and g + 8 of each: the word of the position, its phase.
+    uint32_t row_at[4], row_shift[4];
+    if constexpr (kPhase) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int position = warp * 32 + i * 8 + g;
+        const uint32_t shift = static_cast<uint32_t>(
+            (reinterpret_cast<uintptr_t>(p.q) + static_cast<long long>(row_at_position<kPhase>(position)) * p.ldq) & 15);
+        row_at[i] = static_cast<uint32_t>(position) * kPhasePitch + (shift & ~3u) + static_cast<uint32_t>(q4) * 4;
+        row_shift[i] = 8 * (shift & 3u);
+      }
+    }
     uint32_t stage = 0, phase = 0;
     int unit = unit_begin;
     while (unit < unit_end) {
@@ -556,18 +553,6 @@ gemm_w4_few_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             total[f][t][e] = 0.0f;
-      // This lane's four rows of q: two fragments, rows g and g + 8 of each.
-      uint32_t row_at[4], row_shift[4];
-      if constexpr (kPhase) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int local = warp * 32 + i * 8 + g;
-          const uint32_t shift = static_cast<uint32_t>(
-              (reinterpret_cast<uintptr_t>(p.q) + (static_cast<long long>(block) * kRows + local) * p.ldq) & 15);
-          row_at[i] = static_cast<uint32_t>(local) * kPhasePitch + (shift & ~3u) + static_cast<uint32_t>(q4) * 4;
-          row_shift[i] = 8 * (shift & 3u);
-        }
-      }
       const uint32_t q_lane = static_cast<uint32_t>(warp * 32 + g) * 128 + (static_cast<uint32_t>(g) << 4) + static_cast<uint32_t>(q4) * 4;
       const uint32_t scale_lane = S::kQStageBytes + S::kABytes + static_cast<uint32_t>(warp * 32 + g) * 8;
       for (int ks = ks_begin; ks < ks_end; ++ks) {
@@ -691,7 +676,7 @@ gemm_w4_few_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           for (int t = 0; t < kTiles; ++t)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const long long column = static_cast<long long>(block) * kRows + warp * 32 + i * 8 + g;
+              const long long column = static_cast<long long>(block) * kRows + row_at_position<kPhase>(warp * 32 + i * 8 + g);
               const int token = t * 8 + 2 * q4 + e;
               if (token < p.m && column < p.n)
                 store_c_element(p.c, token * p.ldc + column, total[i / 2][t][2 * (i % 2) + e], p.c_dtype);
@@ -719,19 +704,16 @@ namespace many {
 constexpr int kHalfK = 128;    // of a stage, for each of the two sets
 constexpr int kCollectors = 4;  // warps, one per quarter of the tensor-memory lanes; the first ones of the CTA
 constexpr int kExpanders = 8;   // warps: 2 sets x 4 quarters
-constexpr int kProducerWarp = kCollectors + kExpanders, kMmaWarp = kProducerWarp + 1, kHelperWarp = kMmaWarp + 2;
-// Rows of q at odd places are copied by the producer and one more warp.
-constexpr int kCopiers = 2;
+constexpr int kProducerWarp = kCollectors + kExpanders, kMmaWarp = kProducerWarp + 1, kThreads = 32 * (kMmaWarp + 2);
 
 // What follows from the rows of A a launch is made for (kTokens = 32 or 64, also N of the instruction), the group
 // and q's alignment.
 template <int kTokens, bool kPhase, int kGroup>
 struct Shape {
-  static constexpr int kThreads = 32 * (kCollectors + kExpanders + 3 + (kPhase ? kCopiers - 1 : 0));
   static constexpr int kGroupsPerHalf = kHalfK / kGroup;  // 1, 2 or 4
   // Of k between two hand-overs of a set. Every hand-over costs the issuing thread a wait and a commit, about as
   // much as four instructions of this size, so a half is handed over at once where tensor memory has room for
-  // the sums of all its groups (64 x 18944 x 8192: XX us, in halves of it YY us).
+  // the sums of all its groups (with one issuing warp, 64 x 18944 x 8192 took 49 us so and 60 us in steps of 64).
   static constexpr int kStepK = kGroupsPerHalf * kTokens <= 128 ? kHalfK : kHalfK / 2;
   static constexpr int kSteps = kHalfK / kStepK;
   static constexpr int kAccs = kStepK / kGroup;  // groups of a step, each with sums of its own
@@ -774,8 +756,8 @@ __device__ __forceinline__ void store_four(const W4 &p, int row, long long colum
 __device__ __forceinline__ void collectors_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kCollectors) : "memory"); }
 
 template <bool kBf16, int kTokens, bool kPhase, int kGroup>
-__global__ void __launch_bounds__(Shape<kTokens, kPhase, kGroup>::kThreads, 1)
-gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_a, const W4 p,
+__global__ void __launch_bounds__(kThreads, 1)
+gemm_w4_kernel(const __grid_constant__ QMaps<kPhase> maps_q, const __grid_constant__ CUtensorMap tmap_a, const W4 p,
                uint32_t idesc, int *status) {
   using S = Shape<kTokens, kPhase, kGroup>;
   extern __shared__ uint8_t smem_raw[];
@@ -796,7 +778,7 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant
   const int warp = static_cast<int>(threadIdx.x >> 5), lane = static_cast<int>(threadIdx.x & 31);
   if (threadIdx.x == 0) {
     for (uint32_t s = 0; s < S::kStages; ++s) {
-      mbar_init(full_bar(s), 1 + (kPhase ? 32 * kCopiers : 0));
+      mbar_init(full_bar(s), 1);
       mbar_init(empty_bar(s), kExpanders + kCollectors);  // q has been read, and A (the products are done)
     }
     for (uint32_t i = 0; i < 4; ++i) {
@@ -806,7 +788,7 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant
     *abort_flag = 0;
     mbar_fence_init();
     if (!kPhase)
-      tma_prefetch_descriptor(&tmap_q);
+      tma_prefetch_descriptor(&maps_q.map[0]);
     tma_prefetch_descriptor(&tmap_a);
   }
   if (warp == kMmaWarp) {
@@ -830,18 +812,15 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant
       const bool free = mbar_wait_asleep(empty_bar(stage), phase ^ 1u, abort_flag);
       if (!__all_sync(0xffffffffu, free))
         break;
+      const uint32_t q_dst = smem_base + stage * S::kStageBytes, a_dst = q_dst + S::kQStageBytes;
       if (lane == 0) {
-        const uint32_t q_dst = smem_base + stage * S::kStageBytes, a_dst = q_dst + S::kQStageBytes;
-        mbar_arrive_expect_tx(full_bar(stage), kPhase ? S::kABytes : S::kStageBytes);
-        if (!kPhase)
-          tma_load_2d(q_dst, &tmap_q, full_bar(stage), ks * 128, block * kRows);
+        mbar_arrive_expect_tx(full_bar(stage), S::kStageBytes);
 #pragma unroll
         for (int j = 0; j < kStageK / 64; ++j)
           tma_load_2d(a_dst + j * S::kABoxBytes, &tmap_a, full_bar(stage), ks * kStageK + j * 64, 0);
       }
       __syncwarp();
-      if (kPhase)
-        copy_stage(p, smem_base + stage * S::kStageBytes, full_bar(stage), block, ks, 0, kCopiers, lane);
+      load_q<kPhase>(maps_q, q_dst, full_bar(stage), block, ks, lane);
       if (++stage == S::kStages) {
         stage = 0;
         phase ^= 1u;
@@ -851,8 +830,6 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant
         ++block;
       }
     }
-    if (kPhase)
-      asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
     const uint32_t set = static_cast<uint32_t>(warp - kMmaWarp);
     // ------------------------------------------------------------ MMA issuer --------
@@ -886,36 +863,20 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant
       if (++stage == S::kStages)
         stage = 0;
     }
-  } else if (warp == kHelperWarp) {
-    // ------------------------------------------------------------ the other copier ---
-    if constexpr (kPhase) {
-      uint32_t stage = 0, phase = 0;
-      int block = unit_begin / stages_k, ks = unit_begin - block * stages_k;
-      for (int unit = unit_begin; unit < unit_end; ++unit) {
-        const bool free = mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag);
-        if (!__all_sync(0xffffffffu, free))
-          break;
-        copy_stage(p, smem_base + stage * S::kStageBytes, full_bar(stage), block, ks, 1, kCopiers, lane);
-        if (++stage == S::kStages) {
-          stage = 0;
-          phase ^= 1u;
-        }
-        if (++ks == stages_k) {
-          ks = 0;
-          ++block;
-        }
-      }
-      asm volatile("cp.async.wait_all;" ::: "memory");
-    }
   } else if (warp >= kCollectors) {
     // ------------------------------------------------------------ expanding warps ---
     const uint32_t set = static_cast<uint32_t>(warp - kCollectors) >> 2;
-    const int local = (warp & 3) * 32 + lane;  // this lane's row of the block, and its tensor-memory lane
+    const int position = (warp & 3) * 32 + lane;  // in the block, and this lane's tensor-memory lane
+    const int local = row_at_position<kPhase>(position);
     const uint32_t operands = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16) + 2 * set * S::kOperandColumns;
     uint32_t stage = 0, phase = 0, step = 0;  // step: of this set, counted from the start
     bool ok = true;
-    int block = unit_begin / stages_k, ks = unit_begin - block * stages_k;
-    uint32_t row_at = static_cast<uint32_t>(local) * 128, row_shift = 0;
+    uint32_t row_at = static_cast<uint32_t>(position) * 128, row_shift = 0;
+    if constexpr (kPhase) {
+      const uint32_t at = static_cast<uint32_t>((reinterpret_cast<uintptr_t>(p.q) + static_cast<long long>(local) * p.ldq) & 15);
+      row_at = static_cast<uint32_t>(position) * kPhasePitch + set * 64 + (at & ~3u);
+      row_shift = 8 * (at & 3u);
+    }
     // Zero points of this stage and the next two, a byte per group. (Rows past the end take the last row's; what
     // becomes of them is not stored.)
     uint32_t raw[2] = {0x08080808u, 0x08080808u};
@@ -934,12 +895,6 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant
     fetch(unit_begin, raw[0]);
     fetch(unit_begin + 1, raw[1]);
     for (int unit = unit_begin; ok && unit < unit_end; ++unit) {
-      if constexpr (kPhase) {
-        const uint32_t at = static_cast<uint32_t>(
-            (reinterpret_cast<uintptr_t>(p.q) + (static_cast<long long>(block) * kRows + local) * p.ldq) & 15);
-        row_at = static_cast<uint32_t>(local) * kPhasePitch + set * 64 + (at & ~3u);
-        row_shift = 8 * (at & 3u);
-      }
       Zero<kBf16> zero[S::kGroupsPerHalf];
 #pragma unroll
       for (int j = 0; j < S::kGroupsPerHalf; ++j)
@@ -1000,14 +955,10 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant
         stage = 0;
         phase ^= 1u;
       }
-      if (++ks == stages_k) {
-        ks = 0;
-        ++block;
-      }
     }
   } else {
     // ------------------------------------------------------------ collecting warps --
-    const int local = warp * 32 + lane;  // this lane's row of the block, i.e. column of C
+    const int local = row_at_position<kPhase>(warp * 32 + lane);  // this lane's row of the block, i.e. column of C
     const uint32_t sums = tmem_base + (static_cast<uint32_t>(warp * 32) << 16) + S::kSumsAt;
     constexpr int kGroups = kStageK / kGroup;  // of a stage: 2, 4 or 8
     constexpr int kChunk = kTokens < 32 ? kTokens : 32;
@@ -1191,15 +1142,18 @@ cudaError_t allow_shared(Kernel kernel, uint32_t bytes, int *configured_device) 
 }
 
 template <bool kBf16, int kTokens, bool kPhase, int kGroup>
-cudaError_t launch(const CUtensorMap &tmap_q, const CUtensorMap &tmap_a, const W4 &p, int *status, cudaStream_t stream) {
+cudaError_t launch(const CUtensorMap *tmap_q, const CUtensorMap &tmap_a, const W4 &p, int *status, cudaStream_t stream) {
   static thread_local int configured_device = -1;
+  QMaps<kPhase> maps;
+  for (int i = 0; i < (kPhase ? kPhases : 1); ++i)
+    maps.map[i] = tmap_q[i];
   if constexpr (kTokens <= 16) {
     using S = few::Shape<kTokens / 8, kPhase, kGroup>;
     auto kernel = few::gemm_w4_few_kernel<kBf16, kTokens / 8, kPhase, kGroup>;
     const cudaError_t err = allow_shared(kernel, S::kSmemBytes, &configured_device);
     if (err != cudaSuccess)
       return err;
-    kernel<<<static_cast<unsigned>(p.grid), few::kThreads, S::kSmemBytes, stream>>>(tmap_q, tmap_a, p, status);
+    kernel<<<static_cast<unsigned>(p.grid), few::kThreads, S::kSmemBytes, stream>>>(maps, tmap_a, p, status);
   } else {
     using S = many::Shape<kTokens, kPhase, kGroup>;
     auto kernel = many::gemm_w4_kernel<kBf16, kTokens, kPhase, kGroup>;
@@ -1207,13 +1161,13 @@ cudaError_t launch(const CUtensorMap &tmap_q, const CUtensorMap &tmap_a, const W
     if (err != cudaSuccess)
       return err;
     const uint32_t idesc = make_idesc_f16(kBf16 ? 1u : 0u, false, false, kRows, kTokens);
-    kernel<<<static_cast<unsigned>(p.grid), S::kThreads, S::kSmemBytes, stream>>>(tmap_q, tmap_a, p, idesc, status);
+    kernel<<<static_cast<unsigned>(p.grid), many::kThreads, S::kSmemBytes, stream>>>(maps, tmap_a, p, idesc, status);
   }
   return cudaGetLastError();
 }
 
 template <bool kBf16>
-cudaError_t launch_w4(const CUtensorMap &tmap_q, const CUtensorMap &tmap_a, const W4 &p, int *status, cudaStream_t stream) {
+cudaError_t launch_w4(const CUtensorMap *tmap_q, const CUtensorMap &tmap_a, const W4 &p, int *status, cudaStream_t stream) {
   const int tokens = w4_tokens(p.m);
   const bool phase = p.phase != 0;
 #define HC_W4(TOKENS, GROUP)                                                               \

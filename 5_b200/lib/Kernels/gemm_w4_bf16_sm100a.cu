@@ -4,7 +4,7 @@
 namespace hc {
 namespace sm100 {
 
-cudaError_t launch_gemm_w4_bf16(const CUtensorMap &tmap_q, const CUtensorMap &tmap_a, const W4 &p, int *status,
+cudaError_t launch_gemm_w4_bf16(const CUtensorMap *tmap_q, const CUtensorMap &tmap_a, const W4 &p, int *status,
                                cudaStream_t stream) {
   return w4::launch_w4<true>(tmap_q, tmap_a, p, status, stream);
 }
