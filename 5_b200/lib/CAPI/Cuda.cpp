@@ -2030,10 +2030,10 @@ int plan_layer_norm_backward(const HcCudaContext *ctx, const HcCudaLayerNormBack
   const int vec = hc::sm100::layer_norm_vector(args->dtype, args->cols, args->dy, args->lddy, args->x, args->ldx, args->dx, args->lddx);
   const bool params = args->dweight != nullptr || args->dbias != nullptr;
   plan->pieces = 1;
-  plan->kernel_launches = hc::sm100::layer_norm_backward_launches(args->rows, args->cols, vec, args->dtype, params);
+  plan->kernel_launches = hc::sm100::layer_norm_backward_launches(args->rows, args->cols, vec, args->dtype, args->param_dtype, params);
   if (params)
     plan->scratch_bytes =
-        static_cast<int64_t>(hc::sm100::layer_norm_backward_scratch(args->rows, args->cols, vec, args->dtype, sm_count));
+        static_cast<int64_t>(hc::sm100::layer_norm_backward_scratch(args->rows, args->cols, vec, args->dtype, args->param_dtype, sm_count));
   return HC_CUDA_OK;
 }
 

@@ -305,8 +305,8 @@ cudaError_t launch_map_f32(const float *x, const float *y, float *out, long long
 
 // ---- layer norm --------------------------------------------------------------------------------
 // dtype and param_dtype: kCTypeF32, kCTypeF16 or kCTypeBF16; param_dtype is float32 or dtype.
-// layer_norm_vector: elements per access for three matrices (16 bytes' worth, or 1 when a base, a pitch
-// or the number of columns rules that out).
+// layer_norm_vector: how three matrices lie: elements per access (16 bytes' worth) when all rows consist of whole
+// 16-byte pieces, 0 when they agree about where between two boundaries a row starts, else 1.
 int layer_norm_vector(int dtype, long long cols, const void *a, long long lda, const void *b, long long ldb, const void *c,
                       long long ldc);
 cudaError_t launch_layer_norm(const void *x, long long ldx, const void *weight, const void *bias, void *y,
@@ -314,8 +314,8 @@ cudaError_t launch_layer_norm(const void *x, long long ldx, const void *weight, 
                               int dtype, int param_dtype, int sm_count, int *status, cudaStream_t stream);
 // `partials`: layer_norm_backward_scratch bytes (with vec = layer_norm_vector of dy, x and dx), used when
 // dweight or dbias is wanted.
-int layer_norm_backward_launches(long long rows, long long cols, int vec, int dtype, bool params);
-size_t layer_norm_backward_scratch(long long rows, long long cols, int vec, int dtype, int sm_count);
+int layer_norm_backward_launches(long long rows, long long cols, int vec, int dtype, int param_dtype, bool params);
+size_t layer_norm_backward_scratch(long long rows, long long cols, int vec, int dtype, int param_dtype, int sm_count);
 cudaError_t launch_layer_norm_backward(const void *dy, long long lddy, const void *x, long long ldx, const void *weight,
                                        const float *mean, const float *rstd, void *dx, long long lddx, void *dweight,
                                        void *dbias, float *partials, long long rows, long long cols, int dtype,

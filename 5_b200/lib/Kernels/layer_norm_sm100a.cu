@@ -517,9 +517,13 @@ layer_norm_partials_kernel(const float *partials, int count, long long cols, P *
 // ---------------------------------------------------------------- rows through a ring in shared memory ------
 //
 // For many rows: a CTA is persistent and its rows arrive by cp.async.bulk a few rows ahead, so that the bytes
-// in flight depend neither on registers nor on how far the arithmetic has got. Rows at odd places are copied
-// from the 16-byte boundary below their first element to the one above their last (never behind the matrix:
-// there the last few elements are read where they stand) and read element by element.
+// in flight depend neither on registers nor on how far the arithmetic has got.
+//
+// Rows that do not all start on 16-byte boundaries (an odd number of columns): as long as the matrices agree about
+// where between two boundaries a row starts, that place is the same for every kVec-th row, and a CTA keeps to
+// rows of one place (kShift). Its packs are the 16-byte pieces as they lie in memory, `lead` elements of the first
+// one belonging to what precedes the row; rows are copied from the boundary below their first element to the one
+// above their last, though never behind the matrix: the few elements that leaves out are stored one by one.
 
 // How a thread's kPer elements lie: packs of kVec, a pack of every thread after another.
 template <int kVec>
@@ -550,93 +554,107 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, uintptr_t src, uint32_t 
                : "memory");
 }
 
-// A thread's elements of a row in the ring as floats, zeros past its end. `place`: the row's slot; only the
-// matrix's last row may have elements that were not copied. (Packs are whole: kVec > 1 divides cols.)
-template <typename T, int kVec, int kPer>
-__device__ __forceinline__ void read_row(float2 (&pairs)[kPer / 2], const uint8_t *place, const T *row, int cols, const RowCopy &copy,
-                                         bool last, int t, int threads) {
-  float v[kPer];
-  const int lead = kVec > 1 ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(row) - copy.low);  // bytes
-  if (kVec == 1 && last) {
+// The rows of a CTA: those of one place, ring.step rows apart, in tiles.
+struct Ring {
+  int stages;
+  uint32_t slot;    // bytes of one matrix's row in a stage, a multiple of 16
+  int rows, parts;  // backward: rows of a tile, warps that share one (rows x parts warps in all)
+  int step;         // 1, or with kShift kVec; the grid is a multiple of it
+};
+
+struct Place {
+  int first;   // the first row of this CTA's place
+  int lead;    // elements between the boundary and a row's start
+  __device__ __forceinline__ Place(const void *base, long long ld, int size, int step) {
+    first = static_cast<int>(blockIdx.x) % step;
+    lead = static_cast<int>((reinterpret_cast<uintptr_t>(base) + static_cast<uintptr_t>(first * ld * size)) & 15) / size;
+  }
+};
+
+// What the copy of the matrix's last row leaves out (at most 14 bytes), into the slot at `place`.
+template <typename T>
+__device__ __forceinline__ void store_rest(const RowCopy &copy, const T *row, long long cols, uint8_t *place) {
+  const uint8_t *const low = reinterpret_cast<const uint8_t *>(copy.low);
+  const int end = static_cast<int>(reinterpret_cast<const uint8_t *>(row + cols) - low);
+  for (int at = max(static_cast<int>(copy.bytes), static_cast<int>(reinterpret_cast<const uint8_t *>(row) - low)); at < end;
+       at += static_cast<int>(sizeof(T)))
+    *reinterpret_cast<T *>(place + at) = *reinterpret_cast<const T *>(low + at);
+}
+
+// kVec elements from column c on of a row that lies in the ring at `place`, as floats; zeros beyond its ends.
+template <typename T, int kVec, bool kShift>
+__device__ __forceinline__ void read_unit(float2 (&out)[kVec / 2], const uint8_t *place, int c, int lead, int cols) {
+  const Pack<T, kVec> p = *reinterpret_cast<const Pack<T, kVec> *>(place + (c + lead) * static_cast<int>(sizeof(T)));
+  float v[kVec];
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const int c = t + j * threads, at = lead + c * static_cast<int>(sizeof(T));
-      v[j] = c >= cols ? 0.0f
-             : at + static_cast<int>(sizeof(T)) <= static_cast<int>(copy.bytes) ? to_float(*reinterpret_cast<const T *>(place + at))
-                                                                                : to_float(row[c]);
-    }
-  } else {
+  for (int i = 0; i < kVec; ++i)
+    v[i] = to_float(p.v[i]);
+  if (kShift && (c < 0 || c + kVec > cols)) {
 #pragma unroll
-    for (int q = 0; q < kPer / kVec; ++q) {
-      const int c = (t + q * threads) * kVec;
-      Pack<T, kVec> p = zero_pack<T, kVec>();
-      if (c < cols)
-        p = *reinterpret_cast<const Pack<T, kVec> *>(place + lead + c * static_cast<int>(sizeof(T)));
-#pragma unroll
-      for (int i = 0; i < kVec; ++i)
-        v[q * kVec + i] = to_float(p.v[i]);
-    }
+    for (int i = 0; i < kVec; ++i)
+      if (c + i < 0 || c + i >= cols)
+        v[i] = 0.0f;
   }
 #pragma unroll
-  for (int j = 0; j < kPer / 2; ++j)
-    pairs[j] = make_float2(v[2 * j], v[2 * j + 1]);
+  for (int i = 0; i < kVec / 2; ++i)
+    out[i] = make_float2(v[2 * i], v[2 * i + 1]);
+}
+
+// kVec elements to column c on of a row, nothing beyond its ends.
+template <typename T, int kVec, bool kShift>
+__device__ __forceinline__ void store_unit(T *row, int c, int cols, const float2 (&v)[kVec / 2]) {
+  Pack<T, kVec> p;
+#pragma unroll
+  for (int i = 0; i < kVec / 2; ++i) {
+    p.v[2 * i] = from_float<T>(v[i].x);
+    p.v[2 * i + 1] = from_float<T>(v[i].y);
+  }
+  if (!kShift || (c >= 0 && c + kVec <= cols)) {
+    *reinterpret_cast<Pack<T, kVec> *>(row + c) = p;
+  } else {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i)
+      if (c + i >= 0 && c + i < cols)
+        row[c + i] = p.v[i];
+  }
 }
 
 // A thread's share of a weight or bias vector, kept for all rows as it lies in memory.
 template <typename P, int kVec, int kPer>
 struct Params {
   Pack<P, kVec> v[kPer / kVec];
-  __device__ __forceinline__ Params(const P *p, int cols, int t, int threads, float fallback) {
+  __device__ __forceinline__ Params(const P *p, int cols, int lead, int t, int threads, float fallback) {
 #pragma unroll
     for (int q = 0; q < kPer / kVec; ++q) {
-      const int c = (t + q * threads) * kVec;
+      const int c = (t + q * threads) * kVec - lead;
 #pragma unroll
       for (int i = 0; i < kVec; ++i)
-        v[q].v[i] = p != nullptr && c < cols ? p[c + i] : from_float<P>(fallback);
+        v[q].v[i] = p != nullptr && c + i >= 0 && c + i < cols ? p[c + i] : from_float<P>(fallback);
     }
   }
   __device__ __forceinline__ float operator[](int j) const { return to_float(v[j / kVec].v[j % kVec]); }
   __device__ __forceinline__ float2 pair(int j) const { return make_float2((*this)[2 * j], (*this)[2 * j + 1]); }
 };
 
-// kVec elements from column c of a row or, one by one, those at c and c + step; nothing past the end.
-template <typename T, int kVec>
-__device__ __forceinline__ void store_unit(T *row, int c, int step, int cols, const T (&v)[kVec > 1 ? kVec : 2]) {
-  if constexpr (kVec > 1) {
-    if (c < cols) {
-      Pack<T, kVec> p;
-#pragma unroll
-      for (int i = 0; i < kVec; ++i)
-        p.v[i] = v[i];
-      *reinterpret_cast<Pack<T, kVec> *>(row + c) = p;
-    }
-  } else {
-    if (c < cols)
-      row[c] = v[0];
-    if (c + step < cols)
-      row[c + step] = v[1];
-  }
-}
-
-struct Ring {
-  int stages;
-  uint32_t slot;    // bytes of one matrix's row in a stage, a multiple of 16
-  int rows, parts;  // backward: rows of a tile, warps that share one (rows x parts warps in all)
-};
-
-template <typename T, typename P, int kVec, int kPer, int kThreads, int kCtas>
+template <typename T, typename P, int kVec, int kPer, int kThreads, int kCtas, bool kShift>
 __global__ void __launch_bounds__(kThreads, kCtas)
 layer_norm_ring_kernel(const Forward f, const Ring ring, int *status) {
   extern __shared__ __align__(128) uint8_t shared[];
   __shared__ float sums[2][2][32];
   __shared__ uint32_t abort_word;
   volatile uint32_t *abort_flag = &abort_word;
+  constexpr int kUnits = kPer / kVec, kPairs = kVec / 2;
   const int t = threadIdx.x, threads = blockDim.x, cols = static_cast<int>(f.cols);
   const uint32_t bars = smem_u32(shared), slots = bars + 128;
   const uint8_t *const slots_gen = shared + 128;
   const T *x = static_cast<const T *>(f.x);
+  const Place place(x, f.ldx, sizeof(T), kShift ? ring.step : 1);
+  const int lead = kShift ? place.lead : 0;
+  // Rows blockIdx.x, blockIdx.x + gridDim.x, ...: all of one place, since the grid is a multiple of ring.step.
   auto load = [&](long long row, int stage) {
     const RowCopy copy(x, row, f.ldx, f.cols, f.rows, sizeof(T));
+    if (kShift && row == f.rows - 1)
+      store_rest(copy, x + row * f.ldx, f.cols, shared + 128 + stage * ring.slot);
     mbar_arrive_expect_tx(bars + 8u * stage, copy.bytes);
     if (copy.bytes != 0)
       bulk_load(slots + stage * ring.slot, copy.low, copy.bytes, bars + 8u * stage);
@@ -650,22 +668,28 @@ layer_norm_ring_kernel(const Forward f, const Ring ring, int *status) {
       if (blockIdx.x + static_cast<long long>(s) * gridDim.x < f.rows)
         load(blockIdx.x + static_cast<long long>(s) * gridDim.x, s);
   }
-  const Params<P, kVec, kPer> weight(static_cast<const P *>(f.weight), cols, t, threads, 1.0f);
-  const Params<P, kVec, kPer> bias(static_cast<const P *>(f.bias), cols, t, threads, 0.0f);
+  const Params<P, kVec, kPer> weight(static_cast<const P *>(f.weight), cols, lead, t, threads, 1.0f);
+  const Params<P, kVec, kPer> bias(static_cast<const P *>(f.bias), cols, lead, t, threads, 0.0f);
   __syncthreads();
   const float inv = 1.0f / static_cast<float>(cols);
   int stage = 0, turn = 0;
   uint32_t parity = 0;
   for (long long r = blockIdx.x; r < f.rows; r += gridDim.x, turn ^= 1) {
-    const T *row = x + r * f.ldx;
-    float2 v[kPer / 2];
+    float2 v[kUnits][kPairs];
     mbar_wait(bars + 8u * stage, parity, abort_flag);
-    read_row<T, kVec, kPer>(v, slots_gen + stage * ring.slot, row, cols,
-                            RowCopy(x, r, f.ldx, f.cols, f.rows, sizeof(T)), r == f.rows - 1, t, threads);
     float2 two = make_float2(0.0f, 0.0f);
 #pragma unroll
-    for (int j = 0; j < kPer / 2; ++j)
-      two = __fadd2_rn(two, v[j]);
+    for (int u = 0; u < kUnits; ++u) {
+      const int c = element_of<kVec>(t, u * kVec, threads) - lead;
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i)
+        v[u][i] = make_float2(0.0f, 0.0f);
+      if (c < cols)
+        read_unit<T, kVec, kShift>(v[u], slots_gen + stage * ring.slot, c, lead, cols);
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i)
+        two = __fadd2_rn(two, v[u][i]);
+    }
     const float sum = two.x + two.y;
     const float mean = row_sum<false>(sum, sums[turn][0]) * inv;
     if (t == 0 && r + static_cast<long long>(ring.stages) * gridDim.x < f.rows)
@@ -676,29 +700,39 @@ layer_norm_ring_kernel(const Forward f, const Ring ring, int *status) {
     }
     two = make_float2(0.0f, 0.0f);
 #pragma unroll
-    for (int j = 0; j < kPer / 2; ++j) {
-      if (element_of<kVec>(t, 2 * j, threads) < cols) {
-        v[j] = __fadd2_rn(v[j], splat(-mean));
-        if (kVec == 1 && element_of<kVec>(t, 2 * j + 1, threads) >= cols)
-          v[j].y = 0.0f;
-        two = __ffma2_rn(v[j], v[j], two);
+    for (int u = 0; u < kUnits; ++u) {
+      const int c = element_of<kVec>(t, u * kVec, threads) - lead;
+      if (c < cols) {
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i)
+          v[u][i] = __fadd2_rn(v[u][i], splat(-mean));
+        if (kShift && (c < 0 || c + kVec > cols)) {
+#pragma unroll
+          for (int i = 0; i < kPairs; ++i) {
+            if (c + 2 * i < 0 || c + 2 * i >= cols)
+              v[u][i].x = 0.0f;
+            if (c + 2 * i + 1 < 0 || c + 2 * i + 1 >= cols)
+              v[u][i].y = 0.0f;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i)
+          two = __ffma2_rn(v[u][i], v[u][i], two);
       }
     }
     const float square = two.x + two.y;
     const float rstd = rsqrtf(row_sum<false>(square, sums[turn][1]) * inv + f.eps);
     T *y = static_cast<T *>(f.y) + r * f.ldy;
-    constexpr int kUnit = kVec > 1 ? kVec : 2;
 #pragma unroll
-    for (int u = 0; u < kPer / kUnit; ++u) {
-      T out[kUnit];
+    for (int u = 0; u < kUnits; ++u) {
+      const int c = element_of<kVec>(t, u * kVec, threads) - lead;
+      if (c < cols) {
+        float2 out[kPairs];
 #pragma unroll
-      for (int i = 0; i < kUnit / 2; ++i) {
-        const int j = u * (kUnit / 2) + i;
-        const float2 o = __ffma2_rn(__fmul2_rn(v[j], splat(rstd)), weight.pair(j), bias.pair(j));
-        out[2 * i] = from_float<T>(o.x);
-        out[2 * i + 1] = from_float<T>(o.y);
+        for (int i = 0; i < kPairs; ++i)
+          out[i] = __ffma2_rn(__fmul2_rn(v[u][i], splat(rstd)), weight.pair(u * kPairs + i), bias.pair(u * kPairs + i));
+        store_unit<T, kVec, kShift>(y, c, cols, out);
       }
-      store_unit<T, kVec>(y, element_of<kVec>(t, u * kUnit, threads), threads, cols, out);
     }
     if (t == 0) {
       if (f.mean != nullptr)
@@ -716,29 +750,42 @@ layer_norm_ring_kernel(const Forward f, const Ring ring, int *status) {
 // share its rows, ring.parts warps a row, and find the two sums of each; then, with one barrier between, every
 // thread takes its own kPer columns of all rows, writes dx and adds to dw and db, which stay in registers. What
 // a row costs besides its elements (shuffles, barrier, addresses) is thus paid by few warps or for several
-// rows at once.
-template <typename T, typename P, int kVec, int kPer, int kThreads, int kCtas>
-__global__ void __launch_bounds__(kThreads, kCtas)
+// rows at once. With kShift the weights lie in shared memory behind the ring, as far from a boundary as the rows.
+template <typename T, typename P, int kVec, int kPer, int kThreads, bool kShift>
+__global__ void __launch_bounds__(kThreads, 1)
 layer_norm_backward_ring_kernel(const Backward g, const Ring ring, int *status) {
   extern __shared__ __align__(128) uint8_t shared[];
   __shared__ float4 sums[2][32];  // [row * parts + part]: sum a, sum a n, mean, rstd
   __shared__ uint32_t abort_word;
   volatile uint32_t *abort_flag = &abort_word;
+  constexpr int kUnits = kPer / kVec, kPairs = kVec / 2;
   const int t = threadIdx.x, threads = blockDim.x, cols = static_cast<int>(g.cols), lane = t & 31, warp = t >> 5;
-  const int rows = ring.rows, parts = ring.parts;
+  const int rows = ring.rows, parts = ring.parts, step = kShift ? ring.step : 1;
   const uint32_t bars = smem_u32(shared), slots = bars + 128, stage_bytes = 2u * rows * ring.slot;
   const uint8_t *const slots_gen = shared + 128;
   const T *x = static_cast<const T *>(g.x), *dy = static_cast<const T *>(g.dy);
-  const long long tiles = (g.rows + rows - 1) / rows;
+  const Place place(x, g.ldx, sizeof(T), step);
+  const int lead = kShift ? place.lead : 0;
+  const long long of_place = place.first < g.rows ? (g.rows - place.first + step - 1) / step : 0;  // rows
+  const long long tiles = (of_place + rows - 1) / rows;
+  const long long first_tile = blockIdx.x / step, tile_step = gridDim.x / step;
+  auto row_of = [&](long long tile, int r) { return place.first + step * (tile * rows + r); };
+  auto live_of = [&](long long tile) { return static_cast<int>(min(static_cast<long long>(rows), of_place - tile * rows)); };
   auto load = [&](long long tile, int stage) {
-    const int live = static_cast<int>(min(static_cast<long long>(rows), g.rows - tile * rows));
+    const int live = live_of(tile);
     uint32_t total = 0;
+    if (kShift && row_of(tile, live - 1) == g.rows - 1) {
+      uint8_t *const at = shared + 128 + stage * stage_bytes + 2u * (live - 1) * ring.slot;
+      store_rest(RowCopy(x, g.rows - 1, g.ldx, g.cols, g.rows, sizeof(T)), x + (g.rows - 1) * g.ldx, g.cols, at);
+      store_rest(RowCopy(dy, g.rows - 1, g.lddy, g.cols, g.rows, sizeof(T)), dy + (g.rows - 1) * g.lddy, g.cols, at + ring.slot);
+    }
     for (int r = 0; r < live; ++r)
-      total += RowCopy(x, tile * rows + r, g.ldx, g.cols, g.rows, sizeof(T)).bytes +
-               RowCopy(dy, tile * rows + r, g.lddy, g.cols, g.rows, sizeof(T)).bytes;
+      total += RowCopy(x, row_of(tile, r), g.ldx, g.cols, g.rows, sizeof(T)).bytes +
+               RowCopy(dy, row_of(tile, r), g.lddy, g.cols, g.rows, sizeof(T)).bytes;
     mbar_arrive_expect_tx(bars + 8u * stage, total);
     for (int r = 0; r < live; ++r) {
-      const RowCopy cx(x, tile * rows + r, g.ldx, g.cols, g.rows, sizeof(T)), cd(dy, tile * rows + r, g.lddy, g.cols, g.rows, sizeof(T));
+      const RowCopy cx(x, row_of(tile, r), g.ldx, g.cols, g.rows, sizeof(T)),
+          cd(dy, row_of(tile, r), g.lddy, g.cols, g.rows, sizeof(T));
       const uint32_t at = slots + stage * stage_bytes + 2u * r * ring.slot;
       if (cx.bytes != 0)
         bulk_load(at, cx.low, cx.bytes, bars + 8u * stage);
@@ -752,87 +799,75 @@ layer_norm_backward_ring_kernel(const Backward g, const Ring ring, int *status) 
     abort_word = 0;
     mbar_fence_init();
     for (int s = 0; s < ring.stages; ++s)
-      if (blockIdx.x + static_cast<long long>(s) * gridDim.x < tiles)
-        load(blockIdx.x + static_cast<long long>(s) * gridDim.x, s);
+      if (first_tile + s * tile_step < tiles)
+        load(first_tile + s * tile_step, s);
   }
-  constexpr int kUnit = kVec > 1 ? kVec : 2, kPairs = kUnit / 2;
-  constexpr bool kKeep = kPer <= 16;  // the weights stay in registers between the rows (else dw and db fill them)
   const P *const w = static_cast<const P *>(g.weight);
-  // The weights of the unit of elements at column c (with kVec == 1: at c and c + step).
-  auto weights = [&](float2 (&out)[kPairs], int c, int step) {
-    if constexpr (kVec > 1) {
-      float v[kVec];
-      load_params<P, kVec>(v, w, c, cols, g.params_aligned != 0, 1.0f);
+  P *const shifted = reinterpret_cast<P *>(shared + 128 + ring.stages * stage_bytes);
+  if constexpr (kShift) {
+    const int all = (lead + cols + kVec - 1) / kVec * kVec;
+    for (int i = t; i < all; i += threads)
+      shifted[i] = w != nullptr && i >= lead && i - lead < cols ? w[i - lead] : from_float<P>(1.0f);
+    __syncthreads();
+  }
+  auto weights = [&](float2 (&out)[kPairs], int c) {
+    float v[kVec];
+    if constexpr (kShift) {
+      const Pack<P, kVec> p = *reinterpret_cast<const Pack<P, kVec> *>(shifted + c + lead);
 #pragma unroll
-      for (int i = 0; i < kPairs; ++i)
-        out[i] = make_float2(v[2 * i], v[2 * i + 1]);
+      for (int i = 0; i < kVec; ++i)
+        v[i] = to_float(p.v[i]);
     } else {
-      out[0].x = w != nullptr && c < cols ? to_float(w[c]) : 1.0f;
-      out[0].y = w != nullptr && c + step < cols ? to_float(w[c + step]) : 1.0f;
+      load_params<P, kVec>(v, w, c, cols, g.params_aligned != 0, 1.0f);
     }
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i)
+      out[i] = make_float2(v[2 * i], v[2 * i + 1]);
   };
-  float2 dw[kPer / 2], db[kPer / 2], weight[kKeep ? kPer / kUnit : 1][kPairs];
+  constexpr bool kKeep = kPer <= 16;  // the weights stay in registers between the rows (else dw and db fill them)
+  float2 dw[kUnits][kPairs], db[kUnits][kPairs], weight[kKeep ? kUnits : 1][kPairs];
 #pragma unroll
-  for (int j = 0; j < kPer / 2; ++j)
-    dw[j] = db[j] = make_float2(0.0f, 0.0f);
-  if constexpr (kKeep) {
+  for (int u = 0; u < kUnits; ++u) {
+    const int c = element_of<kVec>(t, u * kVec, threads) - lead;
 #pragma unroll
-    for (int u = 0; u < kPer / kUnit; ++u)
-      weights(weight[u], element_of<kVec>(t, u * kUnit, threads), threads);
+    for (int i = 0; i < kPairs; ++i)
+      dw[u][i] = db[u][i] = make_float2(0.0f, 0.0f);
+    if (kKeep && c < cols)
+      weights(weight[kKeep ? u : 0], c);
   }
   __syncthreads();
   const float inv = 1.0f / static_cast<float>(cols);
   const int my_row = warp / parts, my_part = warp - my_row * parts;
   float next_mean = 0.0f, next_rstd = 0.0f;  // of this warp's row of the tile to come
   auto fetch_statistics = [&](long long tile) {
-    const long long r = tile * rows + my_row;
+    const long long r = row_of(tile, my_row);
     if (r < g.rows) {
       next_mean = g.mean[r];
       next_rstd = g.rstd[r];
     }
   };
-  fetch_statistics(blockIdx.x);
+  fetch_statistics(first_tile);
   int stage = 0, turn = 0, before = 0;
   uint32_t parity = 0;
-  for (long long tile = blockIdx.x; tile < tiles; tile += gridDim.x, turn ^= 1) {
-    const long long row0 = tile * rows;
-    const int live = static_cast<int>(min(static_cast<long long>(rows), g.rows - row0));
-    const uint8_t *const place = slots_gen + stage * stage_bytes;
-    // A unit of a row of the tile; at odd places, in the matrix's last row, what was not copied comes from memory.
-    auto unit = [&](float2 (&out)[kPairs], const T *base, long long ld, int r, int which, int c, int step) {
-      const uint8_t *const at = place + (2u * r + which) * ring.slot;
-      if constexpr (kVec > 1) {
-        const Pack<T, kVec> p = *reinterpret_cast<const Pack<T, kVec> *>(at + c * static_cast<int>(sizeof(T)));
-#pragma unroll
-        for (int i = 0; i < kPairs; ++i)
-          out[i] = make_float2(to_float(p.v[2 * i]), to_float(p.v[2 * i + 1]));
-      } else {
-        const T *const row = base + (row0 + r) * ld;
-        const int lead = static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15);
-        const int copied = row0 + r == g.rows - 1 ? static_cast<int>(RowCopy(base, row0 + r, ld, g.cols, g.rows, sizeof(T)).bytes)
-                                                  : static_cast<int>(ring.slot);
-        auto one = [&](int k) {
-          const int place_of = lead + k * static_cast<int>(sizeof(T));
-          return k >= cols ? 0.0f
-                 : place_of + static_cast<int>(sizeof(T)) <= copied ? to_float(*reinterpret_cast<const T *>(at + place_of))
-                                                                    : to_float(row[k]);
-        };
-        out[0] = make_float2(one(c), one(c + step));
-      }
+  for (long long tile = first_tile; tile < tiles; tile += tile_step, turn ^= 1) {
+    const int live = live_of(tile);
+    const uint8_t *const tile_at = slots_gen + stage * stage_bytes;
+    auto unit = [&](float2 (&out)[kPairs], int r, int which, int c) {
+      read_unit<T, kVec, kShift>(out, tile_at + (2u * r + which) * ring.slot, c, lead, cols);
     };
     const float mean = next_mean, rstd = next_rstd;
-    fetch_statistics(tile + gridDim.x);
+    fetch_statistics(tile + tile_step);
     mbar_wait(bars + 8u * stage, parity, abort_flag);
     if (my_row < live) {
       // sum of a, and of a (x - mean): rstd is multiplied in once at the end.
       float2 s = make_float2(0.0f, 0.0f), sn = s;
       const float2 minus = splat(-mean);
 #pragma unroll 4
-      for (int c = (my_part * 32 + lane) * kVec; c < cols; c += parts * 32 * kUnit) {
+      for (int c = (my_part * 32 + lane) * kVec - lead; c < cols; c += parts * 32 * kVec) {
         float2 vx[kPairs], vd[kPairs], vw[kPairs];
-        unit(vx, x, g.ldx, my_row, 0, c, parts * 32);
-        unit(vd, dy, g.lddy, my_row, 1, c, parts * 32);
-        weights(vw, c, parts * 32);
+        unit(vx, my_row, 0, c);
+        unit(vd, my_row, 1, c);
+        weights(vw, c);
 #pragma unroll
         for (int i = 0; i < kPairs; ++i) {
           const float2 a = __fmul2_rn(vd[i], vw[i]);
@@ -846,8 +881,8 @@ layer_norm_backward_ring_kernel(const Backward g, const Ring ring, int *status) 
     }
     __syncthreads();
     // Every thread is through with the tile before: its stage takes another.
-    const long long next = tile + static_cast<long long>(ring.stages - 1) * gridDim.x;
-    if (t == 0 && tile != blockIdx.x && next < tiles)
+    const long long next = tile + (ring.stages - 1) * tile_step;
+    if (t == 0 && tile != first_tile && next < tiles)
       load(next, before);
     for (int r = 0; r < live; ++r) {
       float4 total = sums[turn][r * parts];
@@ -863,28 +898,24 @@ layer_norm_backward_ring_kernel(const Backward g, const Ring ring, int *status) 
       }
       const float2 minus_ms = splat(-total.x * inv), minus_msn = splat(-total.y * inv), minus_mean = splat(-total.z),
                    rs = splat(total.w);
-      T *dx = static_cast<T *>(g.dx) + (row0 + r) * g.lddx;
+      T *dx = static_cast<T *>(g.dx) + row_of(tile, r) * g.lddx;
 #pragma unroll
-      for (int u = 0; u < kPer / kUnit; ++u) {
-        const int c = element_of<kVec>(t, u * kUnit, threads);
+      for (int u = 0; u < kUnits; ++u) {
+        const int c = element_of<kVec>(t, u * kVec, threads) - lead;
         if (c < cols) {
-          float2 vx[kPairs], vd[kPairs], vw[kPairs];
-          unit(vx, x, g.ldx, r, 0, c, threads);
-          unit(vd, dy, g.lddy, r, 1, c, threads);
+          float2 vx[kPairs], vd[kPairs], vw[kPairs], out[kPairs];
+          unit(vx, r, 0, c);
+          unit(vd, r, 1, c);
           if constexpr (!kKeep)
-            weights(vw, c, threads);
-          T out[kUnit];
+            weights(vw, c);
 #pragma unroll
           for (int i = 0; i < kPairs; ++i) {
-            const int j = u * kPairs + i;
             const float2 n = __fmul2_rn(__fadd2_rn(vx[i], minus_mean), rs), d = vd[i];
-            dw[j] = __ffma2_rn(d, n, dw[j]);
-            db[j] = __fadd2_rn(db[j], d);
-            const float2 o = __fmul2_rn(__ffma2_rn(n, minus_msn, __ffma2_rn(d, kKeep ? weight[kKeep ? u : 0][i] : vw[i], minus_ms)), rs);
-            out[2 * i] = from_float<T>(o.x);
-            out[2 * i + 1] = from_float<T>(o.y);
+            dw[u][i] = __ffma2_rn(d, n, dw[u][i]);
+            db[u][i] = __fadd2_rn(db[u][i], d);
+            out[i] = __fmul2_rn(__ffma2_rn(n, minus_msn, __ffma2_rn(d, kKeep ? weight[kKeep ? u : 0][i] : vw[i], minus_ms)), rs);
           }
-          store_unit<T, kVec>(dx, c, threads, cols, out);
+          store_unit<T, kVec, kShift>(dx, c, cols, out);
         }
       }
     }
@@ -896,22 +927,27 @@ layer_norm_backward_ring_kernel(const Backward g, const Ring ring, int *status) 
   }
   if (g.partials != nullptr) {
     float *mine = g.partials + static_cast<long long>(blockIdx.x) * 2 * cols;
-    if constexpr (kVec > 1) {  // four at a time: cols is a multiple of four, and so is every row of partials
 #pragma unroll
-      for (int j = 0; j < kPer; j += 4) {
-        const int c = element_of<kVec>(t, j, threads);
-        if (c < cols) {
-          *reinterpret_cast<float4 *>(mine + c) = make_float4(dw[j / 2].x, dw[j / 2].y, dw[j / 2 + 1].x, dw[j / 2 + 1].y);
-          *reinterpret_cast<float4 *>(mine + cols + c) = make_float4(db[j / 2].x, db[j / 2].y, db[j / 2 + 1].x, db[j / 2 + 1].y);
+    for (int u = 0; u < kUnits; ++u) {
+      const int c = element_of<kVec>(t, u * kVec, threads) - lead;
+      if (!kShift && c < cols) {  // four at a time: cols is a multiple of four, and so is every row of partials
+#pragma unroll
+        for (int i = 0; i < kPairs; i += 2) {
+          *reinterpret_cast<float4 *>(mine + c + 2 * i) = make_float4(dw[u][i].x, dw[u][i].y, dw[u][i + 1].x, dw[u][i + 1].y);
+          *reinterpret_cast<float4 *>(mine + cols + c + 2 * i) = make_float4(db[u][i].x, db[u][i].y, db[u][i + 1].x, db[u][i + 1].y);
         }
       }
-    } else {
+      if (kShift) {
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        const int c = element_of<kVec>(t, j, threads);
-        if (c < cols) {
-          mine[c] = j % 2 != 0 ? dw[j / 2].y : dw[j / 2].x;
-          mine[cols + c] = j % 2 != 0 ? db[j / 2].y : db[j / 2].x;
+        for (int i = 0; i < kPairs; ++i) {
+          if (c + 2 * i >= 0 && c + 2 * i < cols) {
+            mine[c + 2 * i] = dw[u][i].x;
+            mine[cols + c + 2 * i] = db[u][i].x;
+          }
+          if (c + 2 * i + 1 >= 0 && c + 2 * i + 1 < cols) {
+            mine[c + 2 * i + 1] = dw[u][i].y;
+            mine[cols + c + 2 * i + 1] = db[u][i].y;
+          }
         }
       }
     }
@@ -943,41 +979,48 @@ int ring_ctas(int threads_per_sm, int threads) {
   return ctas < 8 ? ctas : 8;
 }
 
+// How the matrices of a call lie: 16 / size where every row of every one consists of whole 16-byte pieces, kShifted
+// where they agree about where between two boundaries a row starts, else 1.
+constexpr int kShifted = 0;
+
 // Forward. What a row costs besides its elements is per warp, so few warps with 32 elements a thread (and the
 // registers of 512 threads) suit long rows: 16384 x 2048 bfloat16 takes 33.0 us so and 38.2 us with 8 elements
-// a thread; 16384 x 1024 takes 24.9 and 22.7 us. At odd places (vec == 1) 8 elements are better up to 2048
-// columns: 16384 x 1503 float16 takes 64 us, with 32 elements 84 us; beyond, a row is dearer to read from
-// shared memory element by element than it is worth (1024 x 4095: 18.7 us, without the ring 16.6 us).
+// a thread; 16384 x 1024 takes 24.9 and 22.7 us.
 bool forward_ring(Plan *plan, long long rows, long long cols, int vec, int size, int sm_count) {
-  if (cols > (vec > 1 ? kMostRingCols : 2048))
+  const int step = vec == kShifted ? 16 / size : 1;
+  if (vec == 1 || cols + step - 1 > kMostRingCols)
     return false;
   plan->kind = Plan::kRing;
-  plan->per = cols <= (vec > 1 ? 1024 : 2048) ? 8 : 32;
-  plan->threads = threads_for(cols, plan->per);
+  plan->per = cols <= 1024 ? 8 : 32;
+  plan->threads = threads_for(cols + step - 1, plan->per);
   plan->ring.slot = static_cast<uint32_t>((cols * size + 15) / 16 * 16 + 16);  // a row at an odd place needs 16 more
+  plan->ring.step = step;
   const int most = ring_ctas(plan->per == 8 ? 1024 : 512, plan->threads);
   const long long stages = (200 * 1024 / most - 256) / plan->ring.slot;
   if (stages < 2)
     return false;
   plan->ring.stages = static_cast<int>(stages < kMostStages ? stages : kMostStages);
   plan->shared = 128 + static_cast<size_t>(plan->ring.stages) * plan->ring.slot;
-  const long long ctas = static_cast<long long>(sm_count) * most;
-  plan->grid = static_cast<int>(rows < ctas ? rows : ctas);
+  const long long ctas = static_cast<long long>(sm_count) * most / step * step;
+  plan->grid = static_cast<int>(rows < ctas ? (rows + step - 1) / step * step : ctas);
   return true;
 }
 
 // Backward: 16 elements a thread up to 8192 columns (16384 x 4096 bfloat16 takes 115 us so, with 8 elements
 // 143 us, with 32 elements 136 us), 32 beyond, where dw and db of 512 threads fill the registers. Tiles of as
 // many rows as leave three stages and give every CTA four tiles, and warps to share them.
-bool backward_ring(Plan *plan, long long rows, long long cols, int vec, int size, int sm_count) {
-  if (cols > (vec > 1 ? kMostRingCols : 2048))
+bool backward_ring(Plan *plan, long long rows, long long cols, int vec, int size, int param_size, int sm_count) {
+  const int step = vec == kShifted ? 16 / size : 1;
+  if (vec == 1 || cols + step - 1 > kMostRingCols)
     return false;
   plan->kind = Plan::kRing;
-  plan->per = cols <= 8192 ? 16 : 32;
-  plan->threads = threads_for(cols, plan->per);
+  plan->per = cols + step - 1 <= 8192 ? 16 : 32;
+  plan->threads = threads_for(cols + step - 1, plan->per);
   plan->ring.slot = static_cast<uint32_t>((cols * size + 15) / 16 * 16 + 16);
+  plan->ring.step = step;
   const int most = ring_ctas(512, plan->threads);
-  const long long budget = 200 * 1024 / most - 256, pair = 2LL * plan->ring.slot;
+  const long long shifted = step > 1 ? (cols + 2 * step) * param_size : 0;  // the weights
+  const long long budget = 200 * 1024 / most - 256 - shifted, pair = 2LL * plan->ring.slot;
   const int warps = plan->threads / 32;
   int tile = 1;
   while (tile < 8 && warps % (2 * tile) == 0 && 3 * 2 * tile * pair <= budget && rows >= 4LL * tile * most * sm_count)
@@ -988,19 +1031,23 @@ bool backward_ring(Plan *plan, long long rows, long long cols, int vec, int size
   plan->ring.rows = tile;
   plan->ring.parts = warps / tile;
   plan->ring.stages = static_cast<int>(stages < kMostStages ? stages : kMostStages);
-  plan->shared = 128 + static_cast<size_t>(plan->ring.stages) * tile * pair;
-  const long long ctas = static_cast<long long>(sm_count) * most, tiles = (rows + tile - 1) / tile;
+  plan->shared = 128 + static_cast<size_t>(plan->ring.stages) * tile * pair + shifted;
+  const long long ctas = static_cast<long long>(sm_count) * most / step * step;
+  const long long tiles = ((rows + step - 1) / step + tile - 1) / tile * step;  // of all places
   plan->grid = static_cast<int>(tiles < ctas ? tiles : ctas);
   return true;
 }
 
 Plan forward_plan(long long rows, long long cols, int vec, int size, int sm_count) {
   Plan plan{};
-  const long long packs = (cols + vec - 1) / vec;
+  const long long packs = vec > 1 ? (cols + vec - 1) / vec : cols;  // outside the ring
   // The ring pays for rows of more than 1 KiB (16384 x 512 float32: 18.7 us either way; 65536 x 512 bfloat16
   // 53 us, without it 47 us) in matrices of 4 MiB and more, which give every CTA several rows (592 x 4096
   // bfloat16: 7.5 us, without it 7.9 us; 296 x 4096: 7.6 and 6.9 us).
-  if (cols * size > 1024 && rows * cols * size >= 4LL << 20 && forward_ring(&plan, rows, cols, vec, size, sm_count))
+  // At odd places, where the other kernels take one element at a time, it pays from 256 columns on (20000 x 259
+  // bfloat16: 31.0 us, without it 35.1 us; 16384 x 1503 float16 43 and 118 us, 4096 x 4095 bfloat16 32 and 55 us;
+  // but 20000 x 131 float32 24.8 and 20.7 us).
+  if ((vec == kShifted ? cols > 256 : cols * size > 1024) && rows * cols * size >= 4LL << 20 && forward_ring(&plan, rows, cols, vec, size, sm_count))
     return plan;
   if (packs <= 64) {  // a warp holds a row in at most two packs per lane
     plan.kind = Plan::kWarpRows;
@@ -1022,9 +1069,9 @@ Plan forward_plan(long long rows, long long cols, int vec, int size, int sm_coun
   return plan;
 }
 
-Plan backward_plan(long long rows, long long cols, int vec, int size, int sm_count) {
+Plan backward_plan(long long rows, long long cols, int vec, int size, int param_size, int sm_count) {
   Plan plan{};
-  const long long packs = (cols + vec - 1) / vec;
+  const long long packs = vec > 1 ? (cols + vec - 1) / vec : cols;  // outside the ring
   if (packs <= 32) {
     plan.kind = Plan::kWarpRows;
     plan.threads = 32 * kWarpRowWarps;
@@ -1036,7 +1083,11 @@ Plan backward_plan(long long rows, long long cols, int vec, int size, int sm_cou
   // Without the ring a thread holds one pack, which float32 rows of up to 1024 columns do with few enough
   // threads: 16384 x 512 takes 41.1 us, through the ring 45.2 us, 16384 x 1024 51.6 and 53.9 us (bfloat16: 65.7
   // and 43.3 us).
-  if (!(vec == 4 && cols <= 1024) && backward_ring(&plan, rows, cols, vec, size, sm_count))
+  // At odd places it takes more of a start, and pays for many rows that are not short: 16384 x 1503 float16 takes
+  // 80 us, without it 272 us, 2405 x 1503 bfloat16 30 and 49 us, but 200 x 16371 48 and 36 us, 2000 x 515 22 and
+  // 17 us, 20000 x 75 45 and 27 us.
+  const bool small = vec == kShifted && (cols * size <= 512 || rows * cols * size < 4LL << 20 || rows < 2LL * sm_count);
+  if (!(vec == 4 && cols <= 1024) && !small && backward_ring(&plan, rows, cols, vec, size, param_size, sm_count))
     return plan;
   if (packs <= kMaxThreads) {
     plan.kind = Plan::kDirect;
@@ -1065,8 +1116,10 @@ cudaError_t launch_ring(Kernel kernel, const Plan &plan, cudaStream_t stream, co
 }
 
 template <typename T, typename P, int kVec>
-cudaError_t launch_forward(const Forward &f, int sm_count, int *status, cudaStream_t stream) {
-  const Plan plan = forward_plan(f.rows, f.cols, kVec, sizeof(T), sm_count);
+cudaError_t launch_forward(const Forward &f, int vec, int sm_count, int *status, cudaStream_t stream) {
+  const Plan plan = forward_plan(f.rows, f.cols, vec, sizeof(T), sm_count);
+  constexpr bool kShift = kVec == 1;  // of the ring
+  constexpr int kFull = 16 / static_cast<int>(sizeof(T));
   switch (plan.kind) {
   case Plan::kWarpRows:
     if (plan.per == 1)
@@ -1076,10 +1129,8 @@ cudaError_t launch_forward(const Forward &f, int sm_count, int *status, cudaStre
     break;
   case Plan::kRing:
     if (plan.per == 8)
-      return launch_ring(layer_norm_ring_kernel<T, P, kVec, 8, 256, 4>, plan, stream, f, plan.ring, status);
-    if constexpr (kVec > 1)
-      return launch_ring(layer_norm_ring_kernel<T, P, kVec, 32, 512, 1>, plan, stream, f, plan.ring, status);
-    break;
+      return launch_ring(layer_norm_ring_kernel<T, P, kFull, 8, 256, 4, kShift>, plan, stream, f, plan.ring, status);
+    return launch_ring(layer_norm_ring_kernel<T, P, kFull, 32, 512, 1, kShift>, plan, stream, f, plan.ring, status);
   case Plan::kDirect:
     if (plan.per == 1)
       layer_norm_kernel<T, P, kVec, 1, false><<<plan.grid, plan.threads, 0, stream>>>(f);
@@ -1096,8 +1147,10 @@ cudaError_t launch_forward(const Forward &f, int sm_count, int *status, cudaStre
 }
 
 template <typename T, typename P, int kVec>
-cudaError_t launch_backward(const Backward &g, P *dweight, P *dbias, int sm_count, int *status, cudaStream_t stream) {
-  const Plan plan = backward_plan(g.rows, g.cols, kVec, sizeof(T), sm_count);
+cudaError_t launch_backward(const Backward &g, P *dweight, P *dbias, int vec, int sm_count, int *status, cudaStream_t stream) {
+  const Plan plan = backward_plan(g.rows, g.cols, vec, sizeof(T), sizeof(P), sm_count);
+  constexpr bool kShift = kVec == 1;  // of the ring
+  constexpr int kFull = 16 / static_cast<int>(sizeof(T));
   cudaError_t err = cudaSuccess;
   switch (plan.kind) {
   case Plan::kWarpRows:
@@ -1106,11 +1159,10 @@ cudaError_t launch_backward(const Backward &g, P *dweight, P *dbias, int sm_coun
     err = cudaGetLastError();
     break;
   case Plan::kRing:
-    if (plan.per == 16) {
-      err = launch_ring(layer_norm_backward_ring_kernel<T, P, kVec, 16, 512, 1>, plan, stream, g, plan.ring, status);
-    } else if constexpr (kVec > 1) {
-      err = launch_ring(layer_norm_backward_ring_kernel<T, P, kVec, 32, 512, 1>, plan, stream, g, plan.ring, status);
-    }
+    if (plan.per == 16)
+      err = launch_ring(layer_norm_backward_ring_kernel<T, P, kFull, 16, 512, kShift>, plan, stream, g, plan.ring, status);
+    else
+      err = launch_ring(layer_norm_backward_ring_kernel<T, P, kFull, 32, 512, kShift>, plan, stream, g, plan.ring, status);
     break;
   case Plan::kDirect:
     if (plan.threads <= 512)
@@ -1143,27 +1195,28 @@ bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 
 }  // namespace norm
 
-// Elements per access: 16 bytes' worth when every row of every matrix starts on a 16-byte boundary and consists
-// of whole 16-byte pieces.
+// See norm::kShifted.
 int layer_norm_vector(int dtype, long long cols, const void *a, long long lda, const void *b, long long ldb, const void *c,
                       long long ldc) {
   const int size = dtype == kCTypeF32 ? 4 : 2;
-  const bool ok = norm::aligned16(a) && norm::aligned16(b) && norm::aligned16(c) && (lda * size) % 16 == 0 &&
-                  (ldb * size) % 16 == 0 && (ldc * size) % 16 == 0 && (cols * size) % 16 == 0;
-  return ok ? 16 / size : 1;
+  auto place = [](const void *p) { return reinterpret_cast<uintptr_t>(p) & 15; };
+  auto pitch = [&](long long ld) { return static_cast<int>((ld * size) & 15); };
+  if (place(a) != place(b) || place(a) != place(c) || pitch(lda) != pitch(ldb) || pitch(lda) != pitch(ldc))
+    return 1;
+  return place(a) == 0 && pitch(lda) == 0 && pitch(cols) == 0 ? 16 / size : norm::kShifted;
 }
 
 #define HC_NORM_TYPES(CALL)                                                                          \
   if (dtype == kCTypeF32)                                                                            \
-    return vec == 1 ? CALL(float, float, 1) : CALL(float, float, 4);                                 \
+    return vec <= 1 ? CALL(float, float, 1) : CALL(float, float, 4);                                 \
   if (dtype == kCTypeF16) {                                                                          \
     if (param_dtype == kCTypeF32)                                                                    \
-      return vec == 1 ? CALL(__half, float, 1) : CALL(__half, float, 8);                             \
-    return vec == 1 ? CALL(__half, __half, 1) : CALL(__half, __half, 8);                             \
+      return vec <= 1 ? CALL(__half, float, 1) : CALL(__half, float, 8);                             \
+    return vec <= 1 ? CALL(__half, __half, 1) : CALL(__half, __half, 8);                             \
   }                                                                                                  \
   if (param_dtype == kCTypeF32)                                                                      \
-    return vec == 1 ? CALL(__nv_bfloat16, float, 1) : CALL(__nv_bfloat16, float, 8);                 \
-  return vec == 1 ? CALL(__nv_bfloat16, __nv_bfloat16, 1) : CALL(__nv_bfloat16, __nv_bfloat16, 8)
+    return vec <= 1 ? CALL(__nv_bfloat16, float, 1) : CALL(__nv_bfloat16, float, 8);                 \
+  return vec <= 1 ? CALL(__nv_bfloat16, __nv_bfloat16, 1) : CALL(__nv_bfloat16, __nv_bfloat16, 8)
 
 cudaError_t launch_layer_norm(const void *x, long long ldx, const void *weight, const void *bias, void *y,
                               long long ldy, float *mean, float *rstd, long long rows, long long cols, float eps,
@@ -1171,18 +1224,19 @@ cudaError_t launch_layer_norm(const void *x, long long ldx, const void *weight, 
   const int vec = layer_norm_vector(dtype, cols, x, ldx, y, ldy, y, ldy);
   norm::Forward f{x, weight, bias, y, mean, rstd, rows, cols, ldx, ldy, eps,
                   norm::aligned16(weight) && norm::aligned16(bias) ? 1 : 0};
-#define HC_NORM_FORWARD(T, P, V) norm::launch_forward<T, P, V>(f, sm_count, status, stream)
+#define HC_NORM_FORWARD(T, P, V) norm::launch_forward<T, P, V>(f, vec, sm_count, status, stream)
   HC_NORM_TYPES(HC_NORM_FORWARD);
 #undef HC_NORM_FORWARD
 }
 
-int layer_norm_backward_launches(long long rows, long long cols, int vec, int dtype, bool params) {
-  const norm::Plan plan = norm::backward_plan(rows, cols, vec, dtype == kCTypeF32 ? 4 : 2, 148);
+int layer_norm_backward_launches(long long rows, long long cols, int vec, int dtype, int param_dtype, bool params) {
+  const norm::Plan plan = norm::backward_plan(rows, cols, vec, dtype == kCTypeF32 ? 4 : 2, param_dtype == kCTypeF32 ? 4 : 2, 148);
   return 1 + (params ? (plan.kind == norm::Plan::kLong ? 2 : 1) : 0);
 }
 
-size_t layer_norm_backward_scratch(long long rows, long long cols, int vec, int dtype, int sm_count) {
-  const norm::Plan plan = norm::backward_plan(rows, cols, vec, dtype == kCTypeF32 ? 4 : 2, sm_count);
+size_t layer_norm_backward_scratch(long long rows, long long cols, int vec, int dtype, int param_dtype, int sm_count) {
+  const norm::Plan plan =
+      norm::backward_plan(rows, cols, vec, dtype == kCTypeF32 ? 4 : 2, param_dtype == kCTypeF32 ? 4 : 2, sm_count);
   return sizeof(float) * 2 * static_cast<size_t>(cols) * static_cast<size_t>(plan.grid);
 }
 
@@ -1194,7 +1248,7 @@ cudaError_t launch_layer_norm_backward(const void *dy, long long lddy, const voi
   norm::Backward g{dy, x, weight, mean, rstd, dx, dweight != nullptr || dbias != nullptr ? partials : nullptr,
                    rows, cols, lddy, ldx, lddx, norm::aligned16(weight) ? 1 : 0};
 #define HC_NORM_BACKWARD(T, P, V) \
-  norm::launch_backward<T, P, V>(g, static_cast<P *>(dweight), static_cast<P *>(dbias), sm_count, status, stream)
+  norm::launch_backward<T, P, V>(g, static_cast<P *>(dweight), static_cast<P *>(dbias), vec, sm_count, status, stream)
   HC_NORM_TYPES(HC_NORM_BACKWARD);
 #undef HC_NORM_BACKWARD
 }
