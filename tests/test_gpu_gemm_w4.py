@@ -155,6 +155,16 @@ def test_more_units_than_ctas_and_fewer(gpu_ctx) -> None:
         check(run(gpu_ctx, a, q, scales, z, 128, np.float32), a, q, scales, z, 128)
 
 
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("m, n, k", [(17, 20000, 1024), (64, 20001, 1024), (64, 20000, 999), (30, 9, 8000), (64, 1500, 5000)])
+def test_blocks_whole_and_shared(m, n, k, group, gpu_ctx) -> None:
+    """CTAs that begin and end inside row blocks with whole ones between, and blocks shared by many."""
+    a, q, scales, z = inputs(m, n, k, group, "bfloat16", seed=9)
+    got = run(gpu_ctx, a, q, scales, z, group, np_dtype("bfloat16"))
+    check(got, a, q, scales, z, group)
+    assert np.array_equal(got, run(gpu_ctx, a, q, scales, z, group, np_dtype("bfloat16")))
+
+
 def test_empty_products(gpu_ctx) -> None:
     c = empty(gpu_ctx, (3, 5), np.float32)
     gpu_ctx.gemm_w4(cuda.DeviceBuffer(gpu_ctx, (3, 0), np.float16), cuda.DeviceBuffer(gpu_ctx, (5, 0), np.uint8),

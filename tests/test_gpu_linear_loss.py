@@ -78,8 +78,8 @@ class Exact:
         self.dh, self.dw = self.g @ w, self.g.T @ h
 
     def bounds(self, dtype):
-        # float16: g is scaled so that the largest |dloss| becomes 2^13 to 2^14, and keeps that many times
-        # more below the type's smallest normal number.
+        # float16: g is scaled so that the largest |dloss| stands for 2^14, and keeps that many times more below
+        # the type's smallest normal number (2^13 leaves a factor of two).
         step = HALF_STEP[dtype]
         floor = 2.0**-25 * np.abs(self.scale).max() * 2.0**-13 if dtype == "float16" else 0.0
         g_err = np.abs(self.g) * step + np.abs(self.scale) * self.p * self.p_rel * (1 + step) + floor

@@ -1,7 +1,7 @@
 """Layer norm and its gradients on a B200 against the formula in 64 bits.
 
 Tolerances. u = 2^-24 is half a float32 step, h half a step of the stored type. A float32 sum of the kernel
-is a tree whose depth is at most 32 values per thread, 5 shuffles and 5 more for the warps, and longer only
+is a tree whose depth is at most 65 values per thread, 5 shuffles and 8 more for the warps, and longer only
 for rows of more than 32768 values (cols / 1024): DEPTH below bounds it, so a sum of s_i is off by at
 most DEPTH u sum|s_i|. Every product, difference and quotient adds u relative. What follows from that is
 written at each check; the factor 2 stands for the terms of second order.
@@ -218,6 +218,23 @@ def test_many_rows(rows, cols, pad, dtype, param, gpu_ctx) -> None:
     check_backward(dtype, param, dy, x, w, mean, rstd, *grads)
     for p, q in zip(grads, run_backward(gpu_ctx, dy, x, w, mean, rstd, pad, in_place="dy")):
         assert np.array_equal(p, q)
+
+
+@pytest.mark.parametrize("rows, cols, pad", [(1200, 1000, 0), (1200, 1001, 0), (2100, 1001, 4), (700, 3001, 0)])
+def test_many_rows_without_weight_bias_or_statistics(rows, cols, pad, gpu_ctx) -> None:
+    """Also with y's rows at other places than x's (pad)."""
+    x, dy, w, b = inputs(rows, cols, "float16", "float32", 10)
+    one, zero = np.ones(cols, np.float32), np.zeros(cols, np.float32)
+    bx, by = make(gpu_ctx, x), empty(gpu_ctx, x.shape, x.dtype, cols + pad)
+    gpu_ctx.layer_norm(bx, by, eps=EPS)
+    bm, br = empty(gpu_ctx, (rows,), np.float32), empty(gpu_ctx, (rows,), np.float32)
+    gpu_ctx.layer_norm(bx, empty(gpu_ctx, x.shape, x.dtype), mean=bm, rstd=br, eps=EPS)
+    bdy, bdx = make(gpu_ctx, dy), empty(gpu_ctx, x.shape, x.dtype, cols + pad)
+    gpu_ctx.layer_norm_backward(bdy, bx, bdx, mean=bm, rstd=br)
+    gpu_ctx.synchronize()
+    mean, rstd = bm.to_numpy(), br.to_numpy()
+    check_forward("float16", x, one, zero, by.to_numpy(), mean, rstd)
+    check_backward("float16", "float32", dy, x, one, mean, rstd, bdx.to_numpy(), None, None)
 
 
 @pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
