@@ -2164,6 +2164,7 @@ hc::sm100::LinearLoss loss_launch(const LossCall &c, int64_t first, int64_t coun
   p.rows = static_cast<int>(c.rows);
   p.vocab = static_cast<int>(count);
   p.width = static_cast<int>(c.width);
+  p.h_box = c.rows < 128 ? static_cast<int>(round_up(c.rows, 8)) : 128;
   p.first_column = first;
   p.vocab_total = c.vocab;
   p.targets = c.targets;
@@ -2197,7 +2198,7 @@ int enqueue_loss_copies(HcCudaContext *ctx, const LossWork &work, bool counting_
 int enqueue_loss_tiles(HcCudaContext *ctx, const LossCall &c, const hc::sm100::LinearLoss &p, bool grad) {
   CUtensorMap tmap_h, tmap_w;
   if (int rc = encode_map(ctx, &tmap_h, c.dtype, c.h, static_cast<uint64_t>(c.width), static_cast<uint64_t>(c.rows),
-                          static_cast<uint64_t>(c.ldh) * 2, 64, 128))
+                          static_cast<uint64_t>(c.ldh) * 2, 64, static_cast<uint32_t>(p.h_box)))
     return rc;
   const char *w = static_cast<const char *>(c.w) + static_cast<size_t>(p.first_column) * static_cast<size_t>(c.ldw) * 2;
   if (int rc = encode_map(ctx, &tmap_w, c.dtype, w, static_cast<uint64_t>(c.width), static_cast<uint64_t>(p.vocab),
@@ -2656,9 +2657,10 @@ int hcCudaGemmW4(HcCudaContext *ctx, const HcCudaGemmW4Args *args) {
   CUtensorMap tmap_a, tmap_q[hc::sm100::w4_phases()];
   // Up to 16 rows: whole stages of k, as they lie in memory; more: boxes for the tensor cores.
   const bool few = m <= 16;
+  p.a_box = few ? m : static_cast<int>(round_up(m, 8));
   if (int rc = encode_map(ctx, &tmap_a, args->dtype, a, static_cast<uint64_t>(k), static_cast<uint64_t>(m),
                           static_cast<uint64_t>(plan.a_ld) * 2, few ? 256 : 64,
-                          static_cast<uint32_t>(hc::sm100::w4_tokens(m)),
+                          static_cast<uint32_t>(p.a_box),
                           few ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B))
     return rc;
   if (!p.phase) {

@@ -327,6 +327,7 @@ cudaError_t launch_layer_norm_backward(const void *dy, long long lddy, const voi
 // columns first_column .. of a vocabulary of vocab_total.
 struct LinearLoss {
   int rows, vocab, width;
+  int h_box;  // rows of a box of H: 128, or the rows rounded up to a multiple of 8 when there are fewer
   long long first_column, vocab_total;
   const void *targets;  // rows int64 (targets_64) or int32
   int targets_64;
@@ -366,6 +367,7 @@ struct W4 {
   int span;       // ... and how many of them share a scale
   int stages_k;   // w4_stages(k)
   int phase;      // q's rows do not all start on 16-byte boundaries: tmap_q are w4_phases() maps
+  int a_box;      // rows of a box of A: m, or for more than 16 rows m rounded up to a multiple of 8
   int grid;       // CTAs, at most as many as there are (row block, stage of k) units
   int share;      // units of a CTA; the first `extra` CTAs have one more
   int extra;
@@ -398,7 +400,7 @@ inline int w4_grid(long long units, int m, int sm_count) {
 inline size_t w4_partials_bytes(int grid, int m) { return static_cast<size_t>(grid) * 2 * 128 * w4_tokens(m) * 4; }
 // tmap_q: q as bytes {row_bytes inner, n}, box {128, 128}, 128-byte swizzle, or with `phase` map r of rows r, r + 16,
 // ... from the 16-byte boundary at or below the first one's start, box {144, 8}, without swizzle; tmap_a: A as {k inner, m}, for
-// more than 16 rows box {64, w4_tokens(m)} and 128-byte swizzle, else box {256, w4_tokens(m)} without swizzle.
+// more than 16 rows box {64, a_box} and 128-byte swizzle, else box {256, a_box} without swizzle.
 cudaError_t launch_gemm_w4_bf16(const CUtensorMap *tmap_q, const CUtensorMap &tmap_a, const W4 &p, int *status,
                                 cudaStream_t stream);
 cudaError_t launch_gemm_w4_f16(const CUtensorMap *tmap_q, const CUtensorMap &tmap_a, const W4 &p, int *status,

@@ -43,6 +43,9 @@
 // then lie sorted by that place (position 8 r + i holds row 16 i + r), and the readers take words at a row's own
 // phase with a funnel shift. (1 x 18944 x 8190: 33.0 us; when warps copied the rows with cp.async, 57.5 us.)
 //
+// A's boxes have no more rows than A (for the tensor cores, whole groups of eight). What the ring holds in the places
+// of rows that are not there only reaches sums that nobody stores.
+//
 // The (row block, stage of k) units are dealt out as one sequence, an equal share to every CTA, so that the GPU
 // is evenly loaded whatever n and k are; a CTA whose share begins or ends inside a row block leaves float32
 // sums, and the last of the CTAs that share a block adds them in their order (no CTA waits).
@@ -486,7 +489,7 @@ gemm_w4_few_kernel(const __grid_constant__ QMaps<kPhase> maps_q, const __grid_co
         break;
       const uint32_t at = smem_base + stage * S::kStageBytes;
       if (lane == 0) {
-        mbar_arrive_expect_tx(full_bar(stage), S::kStageBytes - S::kScaleBytes);
+        mbar_arrive_expect_tx(full_bar(stage), S::kQStageBytes + static_cast<uint32_t>(p.a_box) * (kStageK * 2));
         tma_load_2d(at + S::kQStageBytes, &tmap_a, full_bar(stage), ks * kStageK, 0);
       }
       __syncwarp();
@@ -814,7 +817,7 @@ gemm_w4_kernel(const __grid_constant__ QMaps<kPhase> maps_q, const __grid_consta
         break;
       const uint32_t q_dst = smem_base + stage * S::kStageBytes, a_dst = q_dst + S::kQStageBytes;
       if (lane == 0) {
-        mbar_arrive_expect_tx(full_bar(stage), S::kStageBytes);
+        mbar_arrive_expect_tx(full_bar(stage), S::kQStageBytes + static_cast<uint32_t>(p.a_box) * (kStageK * 2));
 #pragma unroll
         for (int j = 0; j < kStageK / 64; ++j)
           tma_load_2d(a_dst + j * S::kABoxBytes, &tmap_a, full_bar(stage), ks * kStageK + j * 64, 0);

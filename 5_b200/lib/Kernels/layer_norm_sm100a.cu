@@ -985,13 +985,14 @@ constexpr int kShifted = 0;
 
 // Forward. What a row costs besides its elements is per warp, so few warps with 32 elements a thread (and the
 // registers of 512 threads) suit long rows: 16384 x 2048 bfloat16 takes 33.0 us so and 38.2 us with 8 elements
-// a thread; 16384 x 1024 takes 24.9 and 22.7 us.
+// a thread; 16384 x 1024 takes 24.9 and 22.7 us. A second warp that is mostly idle spoils it: 4095 x 1031 float32
+// takes 16.4 us so, 14.4 us with 8.
 bool forward_ring(Plan *plan, long long rows, long long cols, int vec, int size, int sm_count) {
   const int step = vec == kShifted ? 16 / size : 1;
   if (vec == 1 || cols + step - 1 > kMostRingCols)
     return false;
   plan->kind = Plan::kRing;
-  plan->per = cols <= 1024 ? 8 : 32;
+  plan->per = cols <= 1024 || (cols <= 2048 && threads_for(cols, 32) * 32 > 3 * cols / 2) ? 8 : 32;
   plan->threads = threads_for(cols + step - 1, plan->per);
   plan->ring.slot = static_cast<uint32_t>((cols * size + 15) / 16 * 16 + 16);  // a row at an odd place needs 16 more
   plan->ring.step = step;

@@ -187,6 +187,11 @@ linear_loss_kernel(const __grid_constant__ CUtensorMap tmap_h, const __grid_cons
         const int2 at = tile_of(tile, tiles_m, tiles_n, group_n);
         const int m0 = at.x * kTileM + static_cast<int>(cta_rank) * kCtaRows;
         const int n0 = at.y * kTileN + static_cast<int>(cta_rank) * kCtaRows;
+        // Rows past the end of H are not asked for where that can be helped: every SM's request for one goes to the
+        // same place of the L2 (53 x 44544 x 768: 28.6 us, with boxes of 128 rows for both CTAs 70 us; 1 x 131072 x
+        // 4096: 207 us and 1007 us). What is left in shared memory instead only reaches rows of l that nobody reads.
+        const uint32_t h_bytes = 2u * static_cast<uint32_t>(p.h_box) * 128u;
+        const uint32_t bytes = 2 * kOperandBytes + h_bytes + (at.x * kTileM + kCtaRows < p.rows ? h_bytes : 0u);
         if (!HC_CHECK(status, abort_flag, HC_CHECK_TILE_COORDINATES,
                       at.x >= 0 && at.x < tiles_m && at.y >= 0 && at.y < tiles_n))
           break;
@@ -198,11 +203,12 @@ linear_loss_kernel(const __grid_constant__ CUtensorMap tmap_h, const __grid_cons
           const uint32_t h_dst = smem_base + stage * kStageBytes, w_dst = h_dst + kOperandBytes;
           const uint32_t leader_full = map_to_cta(full_bar(stage), 0);
           if (cta_rank == 0)
-            mbar_arrive_expect_tx(full_bar(stage), 2 * kStageBytes);
+            mbar_arrive_expect_tx(full_bar(stage), bytes);
 #pragma unroll
           for (int sub = 0; sub < kBlockK / 64; ++sub) {
             const int k0 = kb * kBlockK + sub * 64;  // (past the width: zeros)
-            tma_load_2d_pair_hint(h_dst + sub * kBoxBytes, &tmap_h, leader_full, k0, m0, pol_h);
+            if (m0 < p.rows)
+              tma_load_2d_pair_hint(h_dst + sub * kBoxBytes, &tmap_h, leader_full, k0, m0, pol_h);
             tma_load_2d_pair_hint(w_dst + sub * kBoxBytes, &tmap_w, leader_full, k0, n0, pol_w);
           }
           if (++stage == kStages) {

@@ -128,6 +128,14 @@ def test_loss_and_gradients(rows, vocab, width, dtype, gpu_ctx) -> None:
     check(dtype, Exact(h, w, targets, dloss), *run(gpu_ctx, h, w, targets, dloss))
 
 
+@pytest.mark.parametrize("rows, vocab, width", [(1, 40000, 72), (8, 30001, 64), (53, 20000, 80), (127, 10000, 64), (385, 6000, 64)])
+def test_few_rows_and_a_large_vocabulary(rows, vocab, width, gpu_ctx) -> None:
+    """Several tiles per SM whose rows do not fill the tile."""
+    h, w, targets, dloss = inputs(rows, vocab, width, "bfloat16", 11)
+    targets[0] = vocab - 1
+    check("bfloat16", Exact(h, w, targets, dloss), *run(gpu_ctx, h, w, targets, dloss))
+
+
 @pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
 @pytest.mark.parametrize("piece", ["256", "512", "1024"])
 def test_pieces_of_the_vocabulary(piece, dtype, gpu_ctx, monkeypatch) -> None:
