@@ -2256,6 +2256,16 @@ struct LossBackwardPlan {
   int64_t scales = 0;
 };
 
+// A product whose results are multiplied by a factor on the device (Epilogue::device_factor, which the tiny kernel
+// does not read).
+void scale_by_factor(HcCudaGemmArgs *g) {
+  g->epilogue_count = 1;
+  g->epilogue_kind[0] = HC_CUDA_EPILOGUE_SCALE;
+  g->epilogue_value[0] = 1.0f;
+  if (hc::sm100::tiny_takes(g->m, g->n, g->k, g->dtype, kDefaultSmCount))
+    g->variant = HC_CUDA_GEMM_DENSE;
+}
+
 // The two products of a piece as GEMM arguments, their 16-bit results scaled by scales[1]; `c` is already aligned, `base` the start of `work`.
 HcCudaGemmArgs loss_dh_product(const LossCall &c, const LossBackwardPlan &plan, char *base, int64_t first, int64_t count,
                                const HcCudaLinearLossBackwardArgs &args) {
@@ -2278,9 +2288,7 @@ HcCudaGemmArgs loss_dh_product(const LossCall &c, const LossBackwardPlan &plan, 
     g.c = args.dh;
     g.ldc = args.lddh;
     g.c_dtype = c.dtype == HC_CUDA_BF16 ? HC_CUDA_C_BF16 : HC_CUDA_C_F16;
-    g.epilogue_count = 1;
-    g.epilogue_kind[0] = HC_CUDA_EPILOGUE_SCALE;
-    g.epilogue_value[0] = 1.0f;
+    scale_by_factor(&g);
   }
   return g;
 }
@@ -2300,9 +2308,7 @@ HcCudaGemmArgs loss_dw_product(const LossCall &c, const LossBackwardPlan &plan, 
   g.c = static_cast<char *>(args.dw) + static_cast<size_t>(first) * static_cast<size_t>(args.lddw) * 2;
   g.ldc = args.lddw;
   g.c_dtype = c.dtype == HC_CUDA_BF16 ? HC_CUDA_C_BF16 : HC_CUDA_C_F16;
-  g.epilogue_count = 1;
-  g.epilogue_kind[0] = HC_CUDA_EPILOGUE_SCALE;
-  g.epilogue_value[0] = 1.0f;
+  scale_by_factor(&g);
   return g;
 }
 

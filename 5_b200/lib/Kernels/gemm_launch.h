@@ -69,7 +69,7 @@ struct Epilogue {
   float op_value[kMaxEpilogueOps];
   const float *bias;
   // Where a launch's only operation is a scaling by a number that an earlier kernel finds: it is multiplied
-  // into op_value[0]. Null otherwise.
+  // into op_value[0]. Null otherwise. (Not read by the tiny kernel.)
   const float *device_factor;
   // Element type of C: 0 float32, 1 float16, 2 bfloat16 (the float32 value rounded to nearest
   // even). 16-bit output is written by the kernels that do not read C.

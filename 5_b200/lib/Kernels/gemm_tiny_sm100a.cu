@@ -194,7 +194,7 @@ gemm_tiny_kernel(const void *__restrict__ a, long long lda, const void *__restri
       float v = acc[i][j];
       for (int op = 0; op < ep.op_count; ++op) {
         const int kind = ep.op_kind[op];
-        const float x = kind == kEpilogueBiasColumn ? __ldg(ep.bias + col) : op_constant(ep, op);
+        const float x = kind == kEpilogueBiasColumn ? __ldg(ep.bias + col) : ep.op_value[op];
         // np.maximum / np.minimum as the simulator's NumPy computes them: a NaN stays, and of two
         // equal values (zeros of either sign) the constant is taken.
         v = kind == kEpilogueScale ? __fmul_rn(v, x)
