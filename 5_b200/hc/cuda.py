@@ -300,7 +300,20 @@ def device_count() -> int:
     return count.value
 
 
+# The types that have been looked up by name (building a dtype's name costs a microsecond).
+_DTYPE_CODES: dict[Any, int] = {}
+_C_DTYPE_CODES: dict[Any, int] = {}
+_FLOAT32, _UINT8, _INT64, _INT32 = (np.dtype(t) for t in ("float32", "uint8", "int64", "int32"))
+
+
 def dtype_code(dtype: Any) -> int:
+    code = _DTYPE_CODES.get(dtype)
+    if code is None:
+        code = _DTYPE_CODES[dtype] = _named_dtype_code(dtype)
+    return code
+
+
+def _named_dtype_code(dtype: Any) -> int:
     name = dtype if isinstance(dtype, str) else np.dtype(dtype).name
     codes = {"float16": F16, "bfloat16": BF16, "float8_e4m3fn": F8E4M3, "float8_e5m2": F8E5M2}
     if name not in codes:
@@ -312,6 +325,13 @@ C_F32, C_F16, C_BF16 = 0, 1, 2  # element type of C (HcCudaCType)
 
 
 def c_dtype_code(dtype: Any) -> int:
+    code = _C_DTYPE_CODES.get(dtype)
+    if code is None:
+        code = _C_DTYPE_CODES[dtype] = _named_c_dtype_code(dtype)
+    return code
+
+
+def _named_c_dtype_code(dtype: Any) -> int:
     name = dtype if isinstance(dtype, str) else np.dtype(dtype).name
     codes = {"float32": C_F32, "float16": C_F16, "bfloat16": C_BF16}
     if name not in codes:
@@ -333,7 +353,7 @@ def _vector(name: str, buf: "DeviceBuffer | None", length: int, *dtypes: Any) ->
     if buf is None:
         return None
     if buf.shape != (length,) or buf.dtype not in dtypes:
-        raise ValueError(f"{name} must be a vector of {length} elements of {' or '.join(np.dtype(d).name for d in dtypes)}, "
+        raise ValueError(f"{name} must be a vector of {length} elements of {' or '.join(d.name for d in dtypes)}, "
                          f"got {buf.shape} of {buf.dtype.name}")
     return buf.ptr
 
@@ -640,7 +660,7 @@ class Context:
         params = self._norm_params("layer_norm", x.dtype, weight, bias)
         args = _LayerNormArgs(rows, cols, c_dtype_code(x.dtype), c_dtype_code(params), x.ptr, x.ld,
                               _vector("weight", weight, cols, params), _vector("bias", bias, cols, params), y.ptr, y.ld,
-                              _vector("mean", mean, rows, np.float32), _vector("rstd", rstd, rows, np.float32), eps)
+                              _vector("mean", mean, rows, _FLOAT32), _vector("rstd", rstd, rows, _FLOAT32), eps)
         self._check(self._lib.hcCudaLayerNorm(self._handle, ctypes.byref(args)))
 
     def layer_norm_backward(self, dy: "DeviceBuffer", x: "DeviceBuffer", dx: "DeviceBuffer", *, mean: "DeviceBuffer",
@@ -652,8 +672,8 @@ class Context:
         rows, cols = self._norm_shape("layer_norm_backward", x, dy, dx)
         params = self._norm_params("layer_norm_backward", x.dtype, weight, dweight, dbias)
         args = _LayerNormBackwardArgs(rows, cols, c_dtype_code(x.dtype), c_dtype_code(params), dy.ptr, dy.ld, x.ptr, x.ld,
-                                      _vector("weight", weight, cols, params), _vector("mean", mean, rows, np.float32),
-                                      _vector("rstd", rstd, rows, np.float32), dx.ptr, dx.ld,
+                                      _vector("weight", weight, cols, params), _vector("mean", mean, rows, _FLOAT32),
+                                      _vector("rstd", rstd, rows, _FLOAT32), dx.ptr, dx.ld,
                                       _vector("dweight", dweight, cols, params), _vector("dbias", dbias, cols, params))
         self._check(self._lib.hcCudaLayerNormBackward(self._handle, ctypes.byref(args)))
 
@@ -667,10 +687,13 @@ class Context:
     @staticmethod
     def _norm_params(call: str, dtype: np.dtype, *vectors: "DeviceBuffer | None") -> np.dtype:
         """The type the weight and bias vectors share: float32, or that of the matrices."""
-        kinds = {v.dtype for v in vectors if v is not None}
-        if len(kinds) > 1:
-            raise ValueError(f"{call}() takes weight and bias vectors (and their gradients) of one type")
-        return kinds.pop() if kinds else np.dtype(np.float32)
+        kind = None
+        for v in vectors:
+            if v is not None:
+                if kind is not None and v.dtype != kind:
+                    raise ValueError(f"{call}() takes weight and bias vectors (and their gradients) of one type")
+                kind = v.dtype
+        return _FLOAT32 if kind is None else kind
 
     def linear_cross_entropy(self, h: "DeviceBuffer", w: "DeviceBuffer", targets: "DeviceBuffer", loss: "DeviceBuffer",
                              lse: "DeviceBuffer", *, ignore_index: int = -100) -> None:
@@ -680,7 +703,7 @@ class Context:
         type; `targets`: int64 or int32. Rows whose target is `ignore_index` have loss 0; any other target
         outside the vocabulary gives NaN. The logits are not stored."""
         args = _LinearLossArgs(*self._loss_call("linear_cross_entropy", h, w, targets, ignore_index),
-                               _vector("loss", loss, h.shape[0], np.float32), _vector("lse", lse, h.shape[0], np.float32))
+                               _vector("loss", loss, h.shape[0], _FLOAT32), _vector("lse", lse, h.shape[0], _FLOAT32))
         self._check(self._lib.hcCudaLinearLoss(self._handle, ctypes.byref(args)))
 
     def linear_cross_entropy_backward(self, h: "DeviceBuffer", w: "DeviceBuffer", targets: "DeviceBuffer",
@@ -695,7 +718,7 @@ class Context:
                 raise ValueError(f"{name} must have the shape and type of {name[1:]}")
         args = _LinearLossBackwardArgs(
             *self._loss_call("linear_cross_entropy_backward", h, w, targets, ignore_index),
-            _vector("lse", lse, h.shape[0], np.float32), _vector("dloss", dloss, h.shape[0], np.float32),
+            _vector("lse", lse, h.shape[0], _FLOAT32), _vector("dloss", dloss, h.shape[0], _FLOAT32),
             None if dh is None else dh.ptr, 0 if dh is None else dh.ld, None if dw is None else dw.ptr,
             0 if dw is None else dw.ld)
         self._check(self._lib.hcCudaLinearLossBackward(self._handle, ctypes.byref(args)))
@@ -705,8 +728,8 @@ class Context:
         if h.ndim != 2 or w.ndim != 2 or h.shape[1] != w.shape[1] or h.dtype != w.dtype:
             raise ValueError(f"{call}() takes h (rows, width) and w (vocab, width) of one type, got {h.shape} of "
                              f"{h.dtype.name} and {w.shape} of {w.dtype.name}")
-        return (h.shape[0], w.shape[0], h.shape[1], dtype_code(h.dtype), int(targets.dtype == np.int64), h.ptr, h.ld, w.ptr,
-                w.ld, _vector("targets", targets, h.shape[0], np.int64, np.int32), ignore_index)
+        return (h.shape[0], w.shape[0], h.shape[1], dtype_code(h.dtype), int(targets.dtype == _INT64), h.ptr, h.ld, w.ptr,
+                w.ld, _vector("targets", targets, h.shape[0], _INT64, _INT32), ignore_index)
 
     def gemm_w4(self, a: "DeviceBuffer", q: "DeviceBuffer", scales: "DeviceBuffer", c: "DeviceBuffer", *, group: int,
                 zeros: "DeviceBuffer | None" = None) -> None:
@@ -715,18 +738,17 @@ class Context:
         weights, uint8 (n, ceil(k / 2)) with the even k in the low half of a byte; `scales` (n, ceil(k / group))
         of A's type; `zeros`: uint8 of that shape, values 0..15, or 8 throughout; `group`: 32, 64 or a
         multiple of 128; `c` (m, n): float32 or A's type. Sums are float32, rounded once."""
-        for name, buf in (("a", a), ("q", q), ("scales", scales), ("c", c), ("zeros", zeros)):
-            if buf is not None and buf.ndim != 2:
-                raise ValueError(f"gemm_w4(): {name} must be a device matrix")
+        if a.ndim != 2 or q.ndim != 2 or scales.ndim != 2 or c.ndim != 2 or (zeros is not None and zeros.ndim != 2):
+            raise ValueError("gemm_w4(): a, q, scales, c and zeros must be device matrices")
         (m, k), n = a.shape, q.shape[0]
         groups = -(-k // group) if group > 0 else 0
-        if q.dtype != np.uint8 or q.shape != (n, (k + 1) // 2) or c.shape != (m, n):
+        if q.dtype != _UINT8 or q.shape != (n, (k + 1) // 2) or c.shape != (m, n):
             raise ValueError(f"gemm_w4(): a {a.shape} and c {c.shape} take q as uint8 of shape (n, {(k + 1) // 2}), got "
                              f"{q.shape} of {q.dtype.name}")
         if scales.dtype != a.dtype or (group > 0 and scales.shape != (n, groups)):
             raise ValueError(f"gemm_w4(): scales must be {a.dtype.name} of shape {(n, groups)}, got {scales.shape} of "
                              f"{scales.dtype.name}")
-        if zeros is not None and (zeros.dtype != np.uint8 or zeros.shape != scales.shape):
+        if zeros is not None and (zeros.dtype != _UINT8 or zeros.shape != scales.shape):
             raise ValueError("gemm_w4(): zeros must be uint8 with the shape of scales")
         args = _GemmW4Args(m, n, k, dtype_code(a.dtype), c_dtype_code(c.dtype), a.ptr, a.ld, q.ptr, q.ld, scales.ptr, scales.ld,
                            None if zeros is None else zeros.ptr, 0 if zeros is None else zeros.ld, group, c.ptr, c.ld)
