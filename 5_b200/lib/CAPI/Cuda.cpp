@@ -2253,6 +2253,10 @@ struct LossBackwardPlan {
   int64_t g = 0, gt = 0, ldg = 0, ldgt = 0;
   int64_t dh_sums = -1;  // float32, where dh is the sum of several products or their fastest form writes float32
   int64_t sums_ld = 0;
+  // 16-bit, where dw's rows do not all start on 16-byte boundaries: the product stores to it by TMA and a copy
+  // follows (16411 x 1001 x 1031: 41 and 12 us; 70 us when the product writes such rows itself).
+  int64_t dw_copy = -1;
+  int64_t dw_ld = 0;
   int64_t scales = 0;
 };
 
@@ -2305,8 +2309,13 @@ HcCudaGemmArgs loss_dw_product(const LossCall &c, const LossBackwardPlan &plan, 
   g.b = c.h;
   g.ldb = c.ldh;
   g.b_layout = HC_CUDA_B_KN;
-  g.c = static_cast<char *>(args.dw) + static_cast<size_t>(first) * static_cast<size_t>(args.lddw) * 2;
-  g.ldc = args.lddw;
+  if (plan.dw_copy >= 0) {
+    g.c = base + plan.dw_copy;
+    g.ldc = plan.dw_ld;
+  } else {
+    g.c = static_cast<char *>(args.dw) + static_cast<size_t>(first) * static_cast<size_t>(args.lddw) * 2;
+    g.ldc = args.lddw;
+  }
   g.c_dtype = c.dtype == HC_CUDA_BF16 ? HC_CUDA_C_BF16 : HC_CUDA_C_F16;
   scale_by_factor(&g);
   return g;
@@ -2358,6 +2367,10 @@ int plan_linear_loss_backward(const HcCudaContext *ctx, const HcCudaLinearLossBa
   plan->gt = plan->work.take(args->dw != nullptr ? columns * plan->ldgt * 2 : 0);
   plan->sums_ld = round_up(c.width, 4);
   plan->scales = plan->work.take(8);
+  if (args->dw != nullptr && needs_repack(args->dw, args->lddw)) {
+    plan->dw_ld = round_up(c.width, kRepackPitchBytes / 2);
+    plan->dw_copy = plan->work.take(columns * plan->dw_ld * 2);
+  }
 
   // Launches, and the scratch of the products.
   LossCall aligned = c;
@@ -2404,7 +2417,7 @@ int plan_linear_loss_backward(const HcCudaContext *ctx, const HcCudaLinearLossBa
       const HcCudaGemmArgs g = loss_dw_product(aligned, *plan, base, first, count, *args);
       if (int rc = plan_gemm(ctx, &g, sm_count, false, &product))
         return rc;
-      launches += product.kernel_launches;
+      launches += product.kernel_launches + (plan->dw_copy >= 0 ? 1 : 0);
       scratch = product.scratch_bytes > scratch ? product.scratch_bytes : scratch;
     }
   }
@@ -2520,6 +2533,10 @@ int hcCudaLinearLossBackward(HcCudaContext *ctx, const HcCudaLinearLossBackwardA
         return rc;
       if (int rc = enqueue_gemm(ctx, &g, product, scaled))
         return rc;
+      if (plan.dw_copy >= 0)
+        HC_TRY_CUDA(ctx, hc::sm100::launch_spread(base + plan.dw_copy, plan.dw_ld,
+                                                  static_cast<char *>(args->dw) + static_cast<size_t>(first) * args->lddw * 2,
+                                                  args->lddw, static_cast<int>(count), static_cast<int>(c.width), ctx->stream));
     }
   }
   if (plan.dh_sums >= 0)

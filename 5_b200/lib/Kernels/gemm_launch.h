@@ -354,6 +354,8 @@ cudaError_t launch_linear_loss_join(const LinearLoss &p, cudaStream_t stream);
 // that do not count.
 cudaError_t launch_linear_loss_prepare(const LinearLoss &p, float *scales, const void *h, long long ldh, void *copy,
                                        long long ldc, cudaStream_t stream);
+// dst[r, c] = src[r, c], 16 bits each; src 16-byte aligned with lds a multiple of 8, dst anywhere.
+cudaError_t launch_spread(const void *src, long long lds, void *dst, long long ldd, int rows, int cols, cudaStream_t stream);
 // dst[r, c] = src[r, c] * *factor, rounded to 16 bits; src 16-byte aligned with lds a multiple of 4.
 cudaError_t launch_narrow(const float *src, long long lds, void *dst, long long ldd, int rows, int cols,
                           const float *factor, int c_dtype, cudaStream_t stream);

@@ -472,6 +472,39 @@ prepare_kernel(const LinearLoss p, float *scales, const uint16_t *src, long long
   }
 }
 
+// A 16-bit matrix with aligned rows to one whose rows start anywhere: a thread writes eight elements from a 16-byte
+// boundary of dst, which begin at any even byte of src, or what there is of them at the ends of a row.
+__global__ void __launch_bounds__(256)
+spread_kernel(const uint16_t *src, long long lds, uint16_t *dst, long long ldd, int rows, int cols) {
+  const int pieces = (cols + 14) / 8;  // that can touch a row
+  const long long total = static_cast<long long>(rows) * pieces;
+  for (long long idx = blockIdx.x * 256LL + threadIdx.x; idx < total; idx += gridDim.x * 256LL) {
+    const int row = total <= 0x7fffffffLL ? static_cast<int>(static_cast<unsigned>(idx) / static_cast<unsigned>(pieces))
+                                          : static_cast<int>(idx / pieces);
+    uint16_t *const d = dst + row * ldd;
+    const int lead = static_cast<int>(reinterpret_cast<uintptr_t>(d) & 15) / 2;  // elements before the row's first boundary
+    const int col = static_cast<int>(idx - static_cast<long long>(row) * pieces) * 8 - lead;
+    const uint16_t *const s = src + row * lds + col;
+    if (col >= 0 && col + 8 <= cols) {
+      uint4 v;
+      if ((col & 1) == 0) {  // src's rows start on 16-byte boundaries
+        const uint32_t *w = reinterpret_cast<const uint32_t *>(s);
+        v = make_uint4(__ldg(w), __ldg(w + 1), __ldg(w + 2), __ldg(w + 3));
+      } else {
+        const uint32_t *w = reinterpret_cast<const uint32_t *>(s + 1);
+        const uint32_t first = __ldg(s), w0 = __ldg(w), w1 = __ldg(w + 1), w2 = __ldg(w + 2), last = __ldg(s + 7);
+        v = make_uint4(first | (w0 << 16), (w0 >> 16) | (w1 << 16), (w1 >> 16) | (w2 << 16), (w2 >> 16) | (last << 16));
+      }
+      *reinterpret_cast<uint4 *>(d + col) = v;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (col + i >= 0 && col + i < cols)
+          d[col + i] = s[i];
+    }
+  }
+}
+
 // dst = src * factor rounded to 16 bits, for a matrix of rows x cols.
 template <typename Pair>
 __global__ void __launch_bounds__(256)
@@ -547,6 +580,15 @@ cudaError_t launch_linear_loss_prepare(const LinearLoss &p, float *scales, const
     loss::prepare_kernel<uint4><<<grid, 256, 0, stream>>>(p, scales, src, ldh, dst, ldc);
   else
     loss::prepare_kernel<uint16_t><<<grid, 256, 0, stream>>>(p, scales, src, ldh, dst, ldc);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_spread(const void *src, long long lds, void *dst, long long ldd, int rows, int cols, cudaStream_t stream) {
+  if (rows == 0 || cols == 0)
+    return cudaSuccess;
+  const long long blocks = (static_cast<long long>(rows) * ((cols + 14) / 8) + 255) / 256;
+  loss::spread_kernel<<<static_cast<unsigned>(blocks < 148 * 16 ? blocks : 148 * 16), 256, 0, stream>>>(
+      static_cast<const uint16_t *>(src), lds, static_cast<uint16_t *>(dst), ldd, rows, cols);
   return cudaGetLastError();
 }
 

@@ -525,7 +525,8 @@ HC_CUDA_CAPI_EXPORTED int hcCudaLinearLossPlan(const HcCudaLinearLossArgs *args,
  * type for the two products, whose sums are float32 and take the factor back before they are rounded. A call
  * gives the same bits every time. rows == 0 sets dw to zero. Uses context
  * scratch: a copy of h (for dw), g and its transpose for one piece of the vocabulary (together 512 MiB at
- * most, or 1 KiB per row where that is more), and float32 sums of dh when there is more than one piece or few rows. */
+ * most, or 1 KiB per row where that is more), float32 sums of dh when there is more than one piece or few rows,
+ * and a copy of dw's piece when its rows do not all start on 16-byte boundaries. */
 typedef struct HcCudaLinearLossBackwardArgs {
   int64_t rows, vocab, width;
   int32_t dtype;
