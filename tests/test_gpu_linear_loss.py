@@ -148,6 +148,14 @@ def test_pieces_of_the_vocabulary(piece, dtype, gpu_ctx, monkeypatch) -> None:
         assert np.array_equal(a, b)  # the same bits every time
 
 
+@pytest.mark.parametrize("rows, width", [(150, 201), (33, 515)])
+def test_pieces_at_odd_places(rows, width, gpu_ctx, monkeypatch) -> None:
+    h, w, targets, dloss = inputs(rows, 1300, width, "float16", 12)
+    monkeypatch.setenv("HC_CUDA_LOSS_PIECE", "512")
+    check("float16", Exact(h, w, targets, dloss), *run(gpu_ctx, h, w, targets, dloss, 0, 0))
+    check("float16", Exact(h, w, targets, dloss), *run(gpu_ctx, h, w, targets, dloss, 2, 1))
+
+
 @pytest.mark.parametrize("pad_h, pad_w", [(8, 16), (1, 0), (0, 3), (5, 1)])
 def test_pitches(pad_h, pad_w, gpu_ctx) -> None:
     h, w, targets, dloss = inputs(70, 600, 96, "bfloat16", 3)
