@@ -1166,11 +1166,16 @@ cudaError_t launch_backward(const Backward &g, P *dweight, P *dbias, int vec, in
       err = launch_ring(layer_norm_backward_ring_kernel<T, P, kFull, 32, 512, kShift>, plan, stream, g, plan.ring, status);
     break;
   case Plan::kDirect:
-    if (plan.threads <= 512)
-      layer_norm_backward_kernel<T, P, kVec, 1, false, 512><<<plan.grid, plan.threads, 0, stream>>>(g);
-    else
-      layer_norm_backward_kernel<T, P, kVec, 1, false, kMaxThreads><<<plan.grid, plan.threads, 0, stream>>>(g);
-    err = cudaGetLastError();
+    // (The ring takes all 16-bit rows of whole packs that fit it, and float32 rows of more than 256 packs.)
+    if constexpr (kVec == 8) {
+      err = cudaErrorInvalidConfiguration;
+    } else {
+      if (kVec > 1 || plan.threads <= 512)
+        layer_norm_backward_kernel<T, P, kVec, 1, false, 512><<<plan.grid, plan.threads, 0, stream>>>(g);
+      else if constexpr (kVec == 1)
+        layer_norm_backward_kernel<T, P, kVec, 1, false, kMaxThreads><<<plan.grid, plan.threads, 0, stream>>>(g);
+      err = cudaGetLastError();
+    }
     break;
   case Plan::kLong:
     if (g.partials != nullptr) {  // before dx, which may be written over dy or x
