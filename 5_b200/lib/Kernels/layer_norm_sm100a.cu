@@ -489,12 +489,15 @@ layer_norm_columns_kernel(const Backward g) {
   }
 }
 
-// out[c] = sum over the partial rows, in their order within each of 32 interleaved chains that are then
-// added pairwise. A warp reads 32 neighbouring columns of a partial row.
-template <typename P>
-__global__ void __launch_bounds__(1024)
+// out[c] = sum over the partial rows, in their order within each of kChains interleaved chains that are then added.
+// A warp reads 32 neighbouring columns of a partial row. With 32 chains a column's sum is soon there but an SM holds
+// two CTAs only; with 8 all CTAs of wide rows run at once (backward of 1025 x 16384 float16: 49.9 us, with 32
+// chains 53.4 us; 16384 x 1024 bfloat16: 46.9 and 42.9 us).
+template <typename P, int kChains>
+__global__ void __launch_bounds__(32 * kChains)
 layer_norm_partials_kernel(const float *partials, int count, long long cols, P *dweight, P *dbias) {
-  __shared__ float part[32][33];
+  __shared__ float part[kChains][33];
+  constexpr int kAhead = 8;
   const int lane = threadIdx.x & 31, chain = threadIdx.x >> 5;
   const long long c = static_cast<long long>(blockIdx.x) * 32 + lane;
   const bool bias = blockIdx.y != 0;
@@ -502,16 +505,32 @@ layer_norm_partials_kernel(const float *partials, int count, long long cols, P *
   if (out == nullptr)
     return;
   float sum = 0.0f;
-  if (c < cols)
-    for (int k = chain; k < count; k += 32)
-      sum += partials[(static_cast<long long>(k) * 2 + (bias ? 1 : 0)) * cols + c];
+  if (c < cols) {
+    const float *from = partials + (static_cast<long long>(chain) * 2 + (bias ? 1 : 0)) * cols + c;
+    const long long step = 2LL * kChains * cols;
+    int left = (count - chain + kChains - 1) / kChains;
+    for (; left >= kAhead; left -= kAhead) {
+      float v[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        v[u] = from[u * step];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        sum += v[u];
+      from += kAhead * step;
+    }
+    for (; left > 0; --left, from += step)
+      sum += *from;
+  }
   part[chain][lane] = sum;
   __syncthreads();
-  // Warp `chain` now adds the 32 chains of column `chain` of the block.
-  const float total = warp_sum(part[lane][chain]);
-  const long long column = static_cast<long long>(blockIdx.x) * 32 + chain;
-  if (lane == 0 && column < cols)
-    out[column] = from_float<P>(total);
+  if (chain == 0 && c < cols) {
+    float total = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kChains; ++k)
+      total += part[k][lane];
+    out[c] = from_float<P>(total);
+  }
 }
 
 // ---------------------------------------------------------------- rows through a ring in shared memory ------
@@ -1193,7 +1212,10 @@ cudaError_t launch_backward(const Backward &g, P *dweight, P *dbias, int vec, in
   if (err != cudaSuccess || g.partials == nullptr)
     return err;
   const dim3 blocks(static_cast<unsigned>((g.cols + 31) / 32), 2);
-  layer_norm_partials_kernel<P><<<blocks, 1024, 0, stream>>>(g.partials, plan.grid, g.cols, dweight, dbias);
+  if (g.cols >= 8192)
+    layer_norm_partials_kernel<P, 8><<<blocks, 256, 0, stream>>>(g.partials, plan.grid, g.cols, dweight, dbias);
+  else
+    layer_norm_partials_kernel<P, 32><<<blocks, 1024, 0, stream>>>(g.partials, plan.grid, g.cols, dweight, dbias);
   return cudaGetLastError();
 }
 
