@@ -989,6 +989,7 @@ struct Plan {
 
 constexpr long long kMostRingCols = 16 * kMaxThreads;
 constexpr int kMostStages = 8;
+constexpr int kRingBytes = 200 * 1024;  // dynamic shared memory of an SM that the rings of its CTAs may take
 
 int threads_for(long long cols, int per) { return static_cast<int>((cols + per - 1) / per + 31) / 32 * 32; }
 
@@ -1016,7 +1017,7 @@ bool forward_ring(Plan *plan, long long rows, long long cols, int vec, int size,
   plan->ring.slot = static_cast<uint32_t>((cols * size + 15) / 16 * 16 + 16);  // a row at an odd place needs 16 more
   plan->ring.step = step;
   const int most = ring_ctas(plan->per == 8 ? 1024 : 512, plan->threads);
-  const long long stages = (200 * 1024 / most - 256) / plan->ring.slot;
+  const long long stages = (kRingBytes / most - 256) / plan->ring.slot;
   if (stages < 2)
     return false;
   plan->ring.stages = static_cast<int>(stages < kMostStages ? stages : kMostStages);
@@ -1040,7 +1041,7 @@ bool backward_ring(Plan *plan, long long rows, long long cols, int vec, int size
   plan->ring.step = step;
   const int most = ring_ctas(512, plan->threads);
   const long long shifted = step > 1 ? (cols + 2 * step) * param_size : 0;  // the weights
-  const long long budget = 200 * 1024 / most - 256 - shifted, pair = 2LL * plan->ring.slot;
+  const long long budget = kRingBytes / most - 256 - shifted, pair = 2LL * plan->ring.slot;
   const int warps = plan->threads / 32;
   int tile = 1;
   while (tile < 8 && warps % (2 * tile) == 0 && 3 * 2 * tile * pair <= budget && rows >= 4LL * tile * most * sm_count)
@@ -1125,13 +1126,22 @@ Plan backward_plan(long long rows, long long cols, int vec, int size, int param_
   return plan;
 }
 
-template <typename Kernel, typename... Args>
-cudaError_t launch_ring(Kernel kernel, const Plan &plan, cudaStream_t stream, const Args &...args) {
-  // (Set at every launch: the kernels are many and the call is cheap.)
-  const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(plan.shared));
+// The most shared memory a kernel may be launched with belongs to the kernel on its device, not to a launch: it is
+// set to what the largest ring takes, always the same number, so that threads whose contexts launch one kernel with
+// rings of different sizes cannot lower it for each other.
+template <auto kKernel, typename... Args>
+cudaError_t launch_ring(const Plan &plan, cudaStream_t stream, const Args &...args) {
+  static thread_local int configured_device = -1;
+  int device = 0;
+  cudaError_t err = cudaGetDevice(&device);
+  if (err == cudaSuccess && configured_device != device) {
+    err = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes);
+    if (err == cudaSuccess)
+      configured_device = device;
+  }
   if (err != cudaSuccess)
     return err;
-  kernel<<<plan.grid, plan.threads, plan.shared, stream>>>(args...);
+  kKernel<<<plan.grid, plan.threads, plan.shared, stream>>>(args...);
   return cudaGetLastError();
 }
 
@@ -1149,8 +1159,8 @@ cudaError_t launch_forward(const Forward &f, int vec, int sm_count, int *status,
     break;
   case Plan::kRing:
     if (plan.per == 8)
-      return launch_ring(layer_norm_ring_kernel<T, P, kFull, 8, 256, 4, kShift>, plan, stream, f, plan.ring, status);
-    return launch_ring(layer_norm_ring_kernel<T, P, kFull, 32, 512, 1, kShift>, plan, stream, f, plan.ring, status);
+      return launch_ring<layer_norm_ring_kernel<T, P, kFull, 8, 256, 4, kShift>>(plan, stream, f, plan.ring, status);
+    return launch_ring<layer_norm_ring_kernel<T, P, kFull, 32, 512, 1, kShift>>(plan, stream, f, plan.ring, status);
   case Plan::kDirect:
     if (plan.per == 1)
       layer_norm_kernel<T, P, kVec, 1, false><<<plan.grid, plan.threads, 0, stream>>>(f);
@@ -1180,9 +1190,9 @@ cudaError_t launch_backward(const Backward &g, P *dweight, P *dbias, int vec, in
     break;
   case Plan::kRing:
     if (plan.per == 16)
-      err = launch_ring(layer_norm_backward_ring_kernel<T, P, kFull, 16, 512, kShift>, plan, stream, g, plan.ring, status);
+      err = launch_ring<layer_norm_backward_ring_kernel<T, P, kFull, 16, 512, kShift>>(plan, stream, g, plan.ring, status);
     else
-      err = launch_ring(layer_norm_backward_ring_kernel<T, P, kFull, 32, 512, kShift>, plan, stream, g, plan.ring, status);
+      err = launch_ring<layer_norm_backward_ring_kernel<T, P, kFull, 32, 512, kShift>>(plan, stream, g, plan.ring, status);
     break;
   case Plan::kDirect:
     // (The ring takes all 16-bit rows of whole packs that fit it, and float32 rows of more than 256 packs.)

@@ -9,6 +9,9 @@ written at each check; the factor 2 stands for the terms of second order.
 
 from __future__ import annotations
 
+import ctypes
+import threading
+
 import numpy as np
 import pytest
 
@@ -319,3 +322,50 @@ def test_refusals_reach_python(gpu_ctx) -> None:
     ints = empty(gpu_ctx, (4, 8), np.int32)
     with pytest.raises(ValueError):
         gpu_ctx.layer_norm(ints, ints)
+
+
+def test_rings_of_different_sizes_from_several_contexts_at_once() -> None:
+    """The same kernels, launched by threads with a context each on rows of different widths, that is with rings of
+    different sizes: no launch changes what another may ask for. (Through the C ABI with the arguments made once,
+    for calls close enough together; waiting now and then, since launches that wait for room in the queue are not.)"""
+    lib = cuda.library()
+    programs, errors = [], []
+    for rows, cols in ((148, 16384), (300, 8200)) * 2:  # 4 MiB and more: through the ring
+        ctx = cuda.Context(0)
+        x, dy, w, b = inputs(rows, cols, "bfloat16", "bfloat16", 41)
+        bx, bdy, bw, bb = (make(ctx, v) for v in (x, dy, w, b))
+        by, bdx = empty(ctx, x.shape, x.dtype), empty(ctx, x.shape, x.dtype)
+        mean, rstd = empty(ctx, (rows,), np.float32), empty(ctx, (rows,), np.float32)
+        dw, db = empty(ctx, (cols,), w.dtype), empty(ctx, (cols,), w.dtype)
+        outputs = (by, mean, rstd, bdx, dw, db)
+        ctx.layer_norm(bx, by, weight=bw, bias=bb, eps=EPS, mean=mean, rstd=rstd)
+        ctx.layer_norm_backward(bdy, bx, bdx, mean=mean, rstd=rstd, weight=bw, dweight=dw, dbias=db)
+        ctx.synchronize()
+        alone = [out.to_numpy() for out in outputs]
+        check_forward("bfloat16", x, w, b, *alone[:3])
+        check_backward("bfloat16", "bfloat16", dy, x, w, alone[1], alone[2], *alone[3:])
+        args = (cuda._LayerNormArgs(rows, cols, cuda.C_BF16, cuda.C_BF16, bx.ptr, cols, bw.ptr, bb.ptr, by.ptr, cols, mean.ptr,
+                                    rstd.ptr, EPS),
+                cuda._LayerNormBackwardArgs(rows, cols, cuda.C_BF16, cuda.C_BF16, bdy.ptr, cols, bx.ptr, cols, bw.ptr, mean.ptr,
+                                            rstd.ptr, bdx.ptr, cols, dw.ptr, db.ptr))
+        programs.append((ctx, args, outputs, alone, (bx, bdy, bw, bb)))
+
+    def work(ctx, args):
+        forward, backward = (ctypes.byref(a) for a in args)
+        failed = 0
+        for _ in range(1500):
+            for _ in range(4):
+                failed += lib.hcCudaLayerNorm(ctx._handle, forward) != 0
+                failed += lib.hcCudaLayerNormBackward(ctx._handle, backward) != 0
+            ctx.synchronize()
+        errors.append(failed)
+
+    threads = [threading.Thread(target=work, args=program[:2]) for program in programs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert errors == [0] * len(programs)
+    for _, _, outputs, alone, _ in programs:
+        for out, before in zip(outputs, alone):
+            assert np.array_equal(out.to_numpy(), before)
