@@ -178,9 +178,10 @@ bool ranges_overlap(const void *p, size_t pbytes, const void *q, size_t qbytes) 
 
 // Validation + variant choice shared by hcCudaGemmPlan, hcCudaGemm and hcCudaGemmHost.
 // `host_buffers`: the pointers are host memory that will be staged with aligned pitches, so
-// no repack is ever needed.
+// no repack is ever needed. `apart`: the caller has made sure that c overlaps neither operand (its pointers may be
+// stand-ins that only have the alignment of the ones to come).
 int plan_gemm(const HcCudaContext *ctx, const HcCudaGemmArgs *args, int sm_count, bool host_buffers,
-              HcCudaGemmPlanInfo *plan) {
+              HcCudaGemmPlanInfo *plan, bool apart = false) {
   if (args == nullptr || plan == nullptr)
     return fail(ctx, HC_CUDA_ERR_INVALID_ARGUMENT, "args and plan must not be null");
   std::memset(plan, 0, sizeof(*plan));
@@ -266,8 +267,8 @@ int plan_gemm(const HcCudaContext *ctx, const HcCudaGemmArgs *args, int sm_count
     return fail(ctx, HC_CUDA_ERR_INVALID_ARGUMENT, "a and b must be aligned to their element size");
   const size_t a_bytes = (static_cast<size_t>(m - 1) * args->lda + k) * es;
   const size_t b_bytes = (static_cast<size_t>(b_rows - 1) * args->ldb + b_cols) * es;
-  if (ranges_overlap(args->c, c_bytes, args->a, a_bytes) ||
-      ranges_overlap(args->c, c_bytes, args->b, b_bytes))
+  if (!apart && (ranges_overlap(args->c, c_bytes, args->a, a_bytes) ||
+                 ranges_overlap(args->c, c_bytes, args->b, b_bytes)))
     return fail(ctx, HC_CUDA_ERR_INVALID_ARGUMENT, "c must not overlap a or b");
 
   int variant = args->variant;
@@ -2374,7 +2375,7 @@ int plan_linear_loss_backward(const HcCudaContext *ctx, const HcCudaLinearLossBa
 
   // Launches, and the scratch of the products.
   LossCall aligned = c;
-  char *const base = reinterpret_cast<char *>(uintptr_t(1) << 40);  // stands for `work`, which is aligned
+  char *const base = reinterpret_cast<char *>(uintptr_t(1) << 40);  // stands for `work`, which is aligned and apart from all others
   const bool counting_rows = args->dw != nullptr;
   const bool repacks = (plan->work.h_copy >= 0 && !counting_rows) || plan->work.w_copy >= 0;
   if (plan->work.h_copy >= 0) {
@@ -2393,7 +2394,7 @@ int plan_linear_loss_backward(const HcCudaContext *ctx, const HcCudaLinearLossBa
     plan->dh_sums = plan->work.take(c.rows * plan->sums_ld * 4);
     if (plan->pieces == 1) {
       const HcCudaGemmArgs g = loss_dh_product(aligned, *plan, base, 0, c.vocab, *args);
-      if (int rc = plan_gemm(ctx, &g, sm_count, false, &product))
+      if (int rc = plan_gemm(ctx, &g, sm_count, false, &product, /*apart=*/true))
         return rc;
       if (product.cluster_size <= 1) {
         plan->dh_sums = -1;
@@ -2408,14 +2409,14 @@ int plan_linear_loss_backward(const HcCudaContext *ctx, const HcCudaLinearLossBa
     ++launches;
     if (args->dh != nullptr) {
       const HcCudaGemmArgs g = loss_dh_product(aligned, *plan, base, first, count, *args);
-      if (int rc = plan_gemm(ctx, &g, sm_count, false, &product))
+      if (int rc = plan_gemm(ctx, &g, sm_count, false, &product, /*apart=*/true))
         return rc;
       launches += product.kernel_launches;
       scratch = product.scratch_bytes > scratch ? product.scratch_bytes : scratch;
     }
     if (args->dw != nullptr) {
       const HcCudaGemmArgs g = loss_dw_product(aligned, *plan, base, first, count, *args);
-      if (int rc = plan_gemm(ctx, &g, sm_count, false, &product))
+      if (int rc = plan_gemm(ctx, &g, sm_count, false, &product, /*apart=*/true))
         return rc;
       launches += product.kernel_launches + (plan->dw_copy >= 0 ? 1 : 0);
       scratch = product.scratch_bytes > scratch ? product.scratch_bytes : scratch;
@@ -2522,14 +2523,14 @@ int hcCudaLinearLossBackward(HcCudaContext *ctx, const HcCudaLinearLossBackwardA
     HcCudaGemmPlanInfo product;
     if (args->dh != nullptr) {
       const HcCudaGemmArgs g = loss_dh_product(c, plan, base, first, count, *args);
-      if (int rc = plan_gemm(ctx, &g, sm_count, false, &product))
+      if (int rc = plan_gemm(ctx, &g, sm_count, false, &product, /*apart=*/true))
         return rc;
       if (int rc = enqueue_gemm(ctx, &g, product, plan.dh_sums >= 0 ? hc::sm100::Epilogue{} : scaled))
         return rc;
     }
     if (args->dw != nullptr) {
       const HcCudaGemmArgs g = loss_dw_product(c, plan, base, first, count, *args);
-      if (int rc = plan_gemm(ctx, &g, sm_count, false, &product))
+      if (int rc = plan_gemm(ctx, &g, sm_count, false, &product, /*apart=*/true))
         return rc;
       if (int rc = enqueue_gemm(ctx, &g, product, scaled))
         return rc;

@@ -119,3 +119,12 @@ def test_null_arguments() -> None:
         assert getattr(lib, name)(None, None) == INVALID
         assert getattr(lib, name + "Plan")(None, 148, ctypes.byref(info)) == INVALID
         assert getattr(lib, name + "Plan")(None, 148, None) == INVALID
+
+
+@pytest.mark.parametrize("address", [1 << 40, (1 << 40) + 0x20000, (1 << 40) + 2, (1 << 40) - 0x1000])
+def test_gradients_may_lie_at_any_address(address) -> None:
+    """The plan is made before the scratch exists: no address of the caller's is mistaken for it."""
+    for change in ({"dw": address}, {"dh": address}, {"w": address}, {"h": address}):
+        status, info, message = backward(**change)
+        assert status == OK and info.kernel_launches > 0, message
+    assert backward(dw=address, dh=address)[0] == INVALID  # overlaps among the caller's own are still found
