@@ -2031,7 +2031,8 @@ int plan_layer_norm_backward(const HcCudaContext *ctx, const HcCudaLayerNormBack
   const int vec = hc::sm100::layer_norm_vector(args->dtype, args->cols, args->dy, args->lddy, args->x, args->ldx, args->dx, args->lddx);
   const bool params = args->dweight != nullptr || args->dbias != nullptr;
   plan->pieces = 1;
-  plan->kernel_launches = hc::sm100::layer_norm_backward_launches(args->rows, args->cols, vec, args->dtype, args->param_dtype, params);
+  plan->kernel_launches =
+      hc::sm100::layer_norm_backward_launches(args->rows, args->cols, vec, args->dtype, args->param_dtype, sm_count, params);
   if (params)
     plan->scratch_bytes =
         static_cast<int64_t>(hc::sm100::layer_norm_backward_scratch(args->rows, args->cols, vec, args->dtype, args->param_dtype, sm_count));
@@ -2537,7 +2538,7 @@ int hcCudaLinearLossBackward(HcCudaContext *ctx, const HcCudaLinearLossBackwardA
       if (plan.dw_copy >= 0)
         HC_TRY_CUDA(ctx, hc::sm100::launch_spread(base + plan.dw_copy, plan.dw_ld,
                                                   static_cast<char *>(args->dw) + static_cast<size_t>(first) * args->lddw * 2,
-                                                  args->lddw, static_cast<int>(count), static_cast<int>(c.width), ctx->stream));
+                                                  args->lddw, static_cast<int>(count), static_cast<int>(c.width), sm_count, ctx->stream));
     }
   }
   if (plan.dh_sums >= 0)

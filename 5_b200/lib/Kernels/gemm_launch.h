@@ -314,7 +314,7 @@ cudaError_t launch_layer_norm(const void *x, long long ldx, const void *weight, 
                               int dtype, int param_dtype, int sm_count, int *status, cudaStream_t stream);
 // `partials`: layer_norm_backward_scratch bytes (with vec = layer_norm_vector of dy, x and dx), used when
 // dweight or dbias is wanted.
-int layer_norm_backward_launches(long long rows, long long cols, int vec, int dtype, int param_dtype, bool params);
+int layer_norm_backward_launches(long long rows, long long cols, int vec, int dtype, int param_dtype, int sm_count, bool params);
 size_t layer_norm_backward_scratch(long long rows, long long cols, int vec, int dtype, int param_dtype, int sm_count);
 cudaError_t launch_layer_norm_backward(const void *dy, long long lddy, const void *x, long long ldx, const void *weight,
                                        const float *mean, const float *rstd, void *dx, long long lddx, void *dweight,
@@ -355,7 +355,8 @@ cudaError_t launch_linear_loss_join(const LinearLoss &p, cudaStream_t stream);
 cudaError_t launch_linear_loss_prepare(const LinearLoss &p, float *scales, const void *h, long long ldh, void *copy,
                                        long long ldc, cudaStream_t stream);
 // dst[r, c] = src[r, c], 16 bits each; src 16-byte aligned with lds a multiple of 8, dst anywhere.
-cudaError_t launch_spread(const void *src, long long lds, void *dst, long long ldd, int rows, int cols, cudaStream_t stream);
+cudaError_t launch_spread(const void *src, long long lds, void *dst, long long ldd, int rows, int cols, int sm_count,
+                          cudaStream_t stream);
 // dst[r, c] = src[r, c] * *factor, rounded to 16 bits; src 16-byte aligned with lds a multiple of 4.
 cudaError_t launch_narrow(const float *src, long long lds, void *dst, long long ldd, int rows, int cols,
                           const float *factor, int c_dtype, cudaStream_t stream);

@@ -1267,8 +1267,9 @@ cudaError_t launch_layer_norm(const void *x, long long ldx, const void *weight, 
 #undef HC_NORM_FORWARD
 }
 
-int layer_norm_backward_launches(long long rows, long long cols, int vec, int dtype, int param_dtype, bool params) {
-  const norm::Plan plan = norm::backward_plan(rows, cols, vec, dtype == kCTypeF32 ? 4 : 2, param_dtype == kCTypeF32 ? 4 : 2, 148);
+int layer_norm_backward_launches(long long rows, long long cols, int vec, int dtype, int param_dtype, int sm_count, bool params) {
+  const norm::Plan plan =
+      norm::backward_plan(rows, cols, vec, dtype == kCTypeF32 ? 4 : 2, param_dtype == kCTypeF32 ? 4 : 2, sm_count);
   return 1 + (params ? (plan.kind == norm::Plan::kLong ? 2 : 1) : 0);
 }
 

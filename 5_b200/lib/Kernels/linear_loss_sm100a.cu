@@ -618,11 +618,12 @@ cudaError_t launch_linear_loss_prepare(const LinearLoss &p, float *scales, const
   return cudaGetLastError();
 }
 
-cudaError_t launch_spread(const void *src, long long lds, void *dst, long long ldd, int rows, int cols, cudaStream_t stream) {
+cudaError_t launch_spread(const void *src, long long lds, void *dst, long long ldd, int rows, int cols, int sm_count,
+                          cudaStream_t stream) {
   if (rows == 0 || cols == 0)
     return cudaSuccess;
-  const long long blocks = (static_cast<long long>(rows) * ((cols + 14) / 8) + 255) / 256;
-  loss::spread_kernel<<<static_cast<unsigned>(blocks < 148 * 16 ? blocks : 148 * 16), 256, 0, stream>>>(
+  const long long blocks = (static_cast<long long>(rows) * ((cols + 14) / 8) + 255) / 256, most = 16LL * sm_count;
+  loss::spread_kernel<<<static_cast<unsigned>(blocks < most ? blocks : most), 256, 0, stream>>>(
       static_cast<const uint16_t *>(src), lds, static_cast<uint16_t *>(dst), ldd, rows, cols);
   return cudaGetLastError();
 }

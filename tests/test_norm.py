@@ -111,3 +111,21 @@ def test_null_arguments() -> None:
 def test_device_buffers_take_type_names() -> None:
     assert cuda.DeviceBuffer.wrap(None, 0, (3, 4), "bfloat16").dtype.name == "bfloat16"
     assert cuda.DeviceBuffer.wrap(None, 0, (3, 4), "float32").dtype == np.float32
+
+
+@pytest.mark.parametrize("sm_count", [132, 140, 148, 160])
+def test_a_plan_is_that_of_the_device_it_is_asked_for(sm_count) -> None:
+    """At odd places few rows (of 4 MiB and more) are walked three times and many go through the ring, with launches and scratch of
+    their own; where that changes depends on the device, and both change together."""
+    def plan(rows):
+        args = cuda._LayerNormBackwardArgs(rows, 8191, cuda.C_BF16, cuda.C_BF16, DY, 8191, X, 8191, W, MEAN, RSTD, DX, 8191,
+                                           DW, DB)
+        info = cuda._OperatorPlanInfo()
+        assert cuda.library().hcCudaLayerNormBackwardPlan(ctypes.byref(args), sm_count, ctypes.byref(info)) == OK
+        return info.kernel_launches, info.scratch_bytes
+
+    row = 2 * 4 * 8191  # of the partial sums of dweight and dbias
+    few, many = plan(2 * sm_count - 1), plan(2 * sm_count)
+    column_blocks = -(-8191 // 256)
+    assert few == (3, row * -(-8 * sm_count // column_blocks))  # chunks of rows: eight CTAs a multiprocessor
+    assert many == (2, row * (sm_count // 8 * 8))               # one CTA a multiprocessor, as many of each of eight places
