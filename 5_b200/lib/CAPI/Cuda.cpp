@@ -158,6 +158,7 @@ int fail(const HcCudaContext *ctx, int status, const char *fmt, ...) {
 }
 
 int fail_cuda(const HcCudaContext *ctx, cudaError_t err, const char *what) {
+  cudaGetLastError();  // reported here; left behind, it would read as the failure of this thread's next launch
   const int status = err == cudaErrorMemoryAllocation ? HC_CUDA_ERR_OUT_OF_MEMORY : HC_CUDA_ERR_CUDA;
   return fail(ctx, status, "%s: %s (%s)", what, cudaGetErrorName(err), cudaGetErrorString(err));
 }

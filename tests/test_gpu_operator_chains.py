@@ -14,6 +14,7 @@ import test_gpu_linear_loss as loss
 import test_gpu_norm as norm
 from conftest import np_dtype
 from hc import cuda
+from hc.errors import DeviceError
 
 pytestmark = pytest.mark.gpu
 
@@ -142,3 +143,21 @@ def test_two_contexts_at_once() -> None:
             after = p.results()
             assert all(np.array_equal(after[name], r[name]) for name in r)
             p.check(after)
+
+
+def test_a_call_that_finds_no_memory_leaves_the_next_one_alone(gpu_ctx) -> None:
+    """2^24 rows by 2^20 columns leave a partial pair per row and 128 columns: more than any GPU holds. The call is
+    refused before anything is launched, and its error is not read as the next launch's."""
+    h, w = cuda.DeviceBuffer(gpu_ctx, (1 << 24, 1), np.float16), cuda.DeviceBuffer(gpu_ctx, (1 << 20, 1), np.float16)
+    t = cuda.DeviceBuffer(gpu_ctx, (1 << 24,), np.int32)
+    f, g = (cuda.DeviceBuffer(gpu_ctx, (1 << 24,), np.float32) for _ in range(2))
+    x, _, weight, bias = norm.inputs(7, 300, "float32", "float32", 51)
+    bx, bw, bb = (norm.make(gpu_ctx, v) for v in (x, weight, bias))
+    y, mean, rstd = norm.empty(gpu_ctx, x.shape, np.float32), norm.empty(gpu_ctx, (7,), np.float32), norm.empty(gpu_ctx, (7,), np.float32)
+    with pytest.raises(DeviceError, match="OUT_OF_MEMORY"):
+        gpu_ctx.linear_cross_entropy(h, w, t, f, g)
+    gpu_ctx.layer_norm(bx, y, weight=bw, bias=bb, eps=norm.EPS, mean=mean, rstd=rstd)
+    gpu_ctx.synchronize()
+    norm.check_forward("float32", x, weight, bias, y.to_numpy(), mean.to_numpy(), rstd.to_numpy())
+    step = TrainingStep(gpu_ctx, 33, 300, 64, "bfloat16")
+    step.check(run(step))

@@ -115,8 +115,8 @@ def test_device_buffers_take_type_names() -> None:
 
 @pytest.mark.parametrize("sm_count", [132, 140, 148, 160])
 def test_a_plan_is_that_of_the_device_it_is_asked_for(sm_count) -> None:
-    """At odd places few rows (of 4 MiB and more) are walked three times and many go through the ring, with launches and scratch of
-    their own; where that changes depends on the device, and both change together."""
+    """At odd places few rows (of 4 MiB and more) are walked three times and many go through the ring, with launches
+    and scratch of their own; where that changes depends on the device, and both change together."""
     def plan(rows):
         args = cuda._LayerNormBackwardArgs(rows, 8191, cuda.C_BF16, cuda.C_BF16, DY, 8191, X, 8191, W, MEAN, RSTD, DX, 8191,
                                            DW, DB)
