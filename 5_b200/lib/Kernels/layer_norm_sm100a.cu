@@ -346,11 +346,13 @@ layer_norm_backward_kernel(const Backward g) {
 #pragma unroll
     for (int j = 0; j < kPacks; ++j) {
       const long long c = static_cast<long long>(t + j * step) * kVec;
+      if (c >= cols)  // (a row is whole packs; what lies past it is no 0 here: -mean * rstd may be infinite)
+        break;
       float w[kVec];
       load_params<P, kVec>(w, static_cast<const P *>(g.weight), c, cols, g.params_aligned != 0, 1.0f);
 #pragma unroll
       for (int i = 0; i < kVec; ++i) {
-        const float n = (to_float(px[j].v[i]) - mean) * rstd, d = to_float(pd[j].v[i]);  // (d is 0 past the end)
+        const float n = (to_float(px[j].v[i]) - mean) * rstd, d = to_float(pd[j].v[i]);
         const float a = d * w[i];
         s += a;
         sn = fmaf(a, n, sn);

@@ -369,3 +369,26 @@ def test_rings_of_different_sizes_from_several_contexts_at_once() -> None:
     for _, _, outputs, alone, _ in programs:
         for out, before in zip(outputs, alone):
             assert np.array_equal(out.to_numpy(), before)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("cols", [1, 8, 64, 512, 2048])
+def test_constant_rows_of_huge_values(cols, dtype, gpu_ctx) -> None:
+    """Rows of one value, 2^110, whose mean is exact (cols is a power of two): n is 0, although mean * rstd, with
+    rstd = 2^20 for eps = 2^-40, is beyond float32. Lanes and threads that hold nothing of the row add nothing."""
+    rng = np.random.default_rng(cols)
+    t, eps = np_dtype(dtype), 2.0**-40
+    x = np.full((5, cols), 2.0**110).astype(t)
+    dy = rng.standard_normal((5, cols)).astype(t)
+    w, b = rng.standard_normal(cols).astype(np.float32), rng.standard_normal(cols).astype(np.float32)
+    bx, bdy, bw, bb = (make(gpu_ctx, v) for v in (x, dy, w, b))
+    y, dx = empty(gpu_ctx, x.shape, t), empty(gpu_ctx, x.shape, t)
+    mean, rstd = empty(gpu_ctx, (5,), np.float32), empty(gpu_ctx, (5,), np.float32)
+    dw, db = empty(gpu_ctx, (cols,), np.float32), empty(gpu_ctx, (cols,), np.float32)
+    gpu_ctx.layer_norm(bx, y, weight=bw, bias=bb, eps=eps, mean=mean, rstd=rstd)
+    gpu_ctx.layer_norm_backward(bdy, bx, dx, mean=mean, rstd=rstd, weight=bw, dweight=dw, dbias=db)
+    gpu_ctx.synchronize()
+    m, r = mean.to_numpy(), rstd.to_numpy()
+    assert (m == 2.0**110).all() and (np.abs(r - 2.0**20) <= 8 * U * 2.0**20).all()
+    assert (np.abs(y.to_numpy().astype(np.float64) - b.astype(np.float64)) <= HALF_STEP[dtype] * np.abs(b)).all()
+    check_backward(dtype, "float32", dy, x, w, m, r, dx.to_numpy(), dw.to_numpy(), db.to_numpy())
