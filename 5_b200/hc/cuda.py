@@ -736,8 +736,8 @@ class Context:
         """Enqueues C = A @ W.T for W[j, k] = scales[j, k // group] * (q[j, k] - zeros[j, k // group])
         (asynchronous; see `synchronize`). `a`: up to 64 rows (m, k) of float16 or bfloat16; `q`: 4-bit
         weights, uint8 (n, ceil(k / 2)) with the even k in the low half of a byte; `scales` (n, ceil(k / group))
-        of A's type; `zeros`: uint8 of that shape, values 0..15, or 8 throughout; `group`: 32, 64 or a
-        multiple of 128; `c` (m, n): float32 or A's type. Sums are float32, rounded once."""
+        of A's type; `zeros`: uint8 of that shape, values 0..63 (the low six bits count), or 8 throughout;
+        `group`: 32, 64 or a multiple of 128; `c` (m, n): float32 or A's type. Sums are float32, rounded once."""
         if a.ndim != 2 or q.ndim != 2 or scales.ndim != 2 or c.ndim != 2 or (zeros is not None and zeros.ndim != 2):
             raise ValueError("gemm_w4(): a, q, scales, c and zeros must be device matrices")
         (m, k), n = a.shape, q.shape[0]

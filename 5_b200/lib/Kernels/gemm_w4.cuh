@@ -3,7 +3,7 @@
 //   C[i, j] = sum_groups s[j, g] sum_{k in group g} (q[j, k] - z[j, g]) A[i, k]
 //
 // q: 0..15, two to a byte (even k in the low half), rows of ceil(k / 2) bytes; s: one scale per row of q and
-// group of 32, 64 or a multiple of 128 consecutive k, in A's type; z: one byte each, or 8 throughout. A:
+// group of 32, 64 or a multiple of 128 consecutive k, in A's type; z: the low six bits of a byte each, or 8 throughout. A:
 // m <= 64 rows of float16 or bfloat16.
 //
 // Bound: HBM reads of q, half a byte per weight. At the copy bandwidth an SM receives 45 weights per cycle, and
@@ -87,7 +87,9 @@ __device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t m
   return r;
 }
 
-// What a row's zero point subtracts from the expanded nibbles.
+// What a row's zero point subtracts from the expanded nibbles. Six bits of it, for all numbers of rows of A alike: that
+// is what 64 + z leaves in float16 four bits further up (set_pair), and all of it is exact in both types.
+constexpr uint32_t kZeroBits = 0x3fu;
 template <bool kBf16>
 struct Zero {
   __nv_bfloat162 low;  // 128 + z
@@ -106,7 +108,7 @@ struct Zero<false> {
   }
   __device__ void set_pair(uint32_t pair) {
     low = *reinterpret_cast<const __half2 *>(&pair);
-    const uint32_t up = and_or(pair << 4, 0x00f000f0u, 0xd400d400u);
+    const uint32_t up = and_or(pair << 4, 0x03f003f0u, 0xd400d400u);
     high = *reinterpret_cast<const __half2 *>(&up);
   }
 };
@@ -363,7 +365,8 @@ struct ScaleStream {
 #pragma unroll
       for (int i = 0; i < kRows / 32; ++i) {
         const uint32_t bits = j % 2 == 0 ? scale[0][i][j / 2] & 0xffffu : scale[0][i][j / 2] >> 16;
-        const uint32_t pair = __byte_perm(zero[0][i][j / 4], kBf16 ? 0x43434343u : 0x64646464u, 0x4040u | (0x101u * (j % 4)));
+        const uint32_t pair = __byte_perm(zero[0][i][j / 4] & (kZeroBits * 0x01010101u), kBf16 ? 0x43434343u : 0x64646464u,
+                                          0x4040u | (0x101u * (j % 4)));
         asm volatile("st.shared.v2.u32 [%0], {%1, %2};"
                      :: "r"(at + static_cast<uint32_t>((j * kRows + i * 32 + lane) * 8)),
                         "r"(__float_as_uint(scale_value<kBf16>(static_cast<uint16_t>(bits)))), "r"(pair)
@@ -901,7 +904,7 @@ gemm_w4_kernel(const __grid_constant__ QMaps<kPhase> maps_q, const __grid_consta
       Zero<kBf16> zero[S::kGroupsPerHalf];
 #pragma unroll
       for (int j = 0; j < S::kGroupsPerHalf; ++j)
-        zero[j].set(static_cast<int>((raw[0] >> (8 * j)) & 0xffu));
+        zero[j].set(static_cast<int>((raw[0] >> (8 * j)) & kZeroBits));
       raw[0] = raw[1];
       fetch(unit + 2, raw[1]);
       const bool ready = mbar_wait(full_bar(stage), phase, abort_flag);

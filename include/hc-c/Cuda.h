@@ -556,8 +556,8 @@ HC_CUDA_CAPI_EXPORTED int hcCudaLinearLossBackwardPlan(const HcCudaLinearLossBac
 /* C[i, j] = sum over groups g of scales[j, g] * sum over k in g of (q[j, k] - zeros[j, g]) * A[i, k]
  * for m <= 64 rows of A (float16 or bfloat16) and n rows of 4-bit weights: q holds two to a byte, the even k
  * in the low half, rows of ceil(k / 2) bytes at a pitch of ldq bytes; scales, n x ceil(k / group), in A's type;
- * zeros, n x ceil(k / group) bytes of 0..15 each, or NULL for 8 throughout. group: 32, 64 or a multiple of
- * 128; the last group of a row may be shorter. Everything is summed in float32 (the weights enter as integers,
+ * zeros, n x ceil(k / group) bytes, 0..63 each (the low six bits of a byte count), or NULL for 8 throughout. group:
+ * 32, 64 or a multiple of 128; the last group of a row may be shorter. Everything is summed in float32 (the weights enter as integers,
  * the scales multiply the sums of their groups) and rounded once into C: float32, or A's type. The same bits
  * every call. It is to a matrix of 4-bit weights what the skinny variant of hcCudaGemm is to one of 16 bits:
  * HBM bound for few rows. An A of several rows whose base or pitch is not a multiple of 16 bytes costs a

@@ -190,3 +190,17 @@ def test_refusals_reach_python(gpu_ctx) -> None:
         gpu_ctx.gemm_w4(a, q, empty(gpu_ctx, (9, 4), np.float16), c, group=16)
     with pytest.raises(DeviceError, match="m <= 64"):
         gpu_ctx.gemm_w4(empty(gpu_ctx, (65, 64), np.float16), q, s, empty(gpu_ctx, (65, 9), np.float32), group=32)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("pad_q", [0, 1])
+def test_zero_points_beyond_fifteen(pad_q, group, dtype, gpu_ctx) -> None:
+    """0..63 are zero points, of a larger byte the low six bits, whatever the number of rows of A."""
+    for m in (1, 9, 16, 17, 40):
+        a, q, scales, _ = inputs(m, 150, 640, group, dtype, seed=10)
+        z = np.random.default_rng(group).integers(0, 64, (150, 640 // group), dtype=np.uint8)
+        z[:, 0] = np.arange(150) % 64
+        got = run(gpu_ctx, a, q, scales, z, group, np.float32, pad_q=pad_q)
+        check(got, a, q, scales, z, group)
+        assert np.array_equal(got, run(gpu_ctx, a, q, scales, z + np.uint8(64 * (m % 4)), group, np.float32, pad_q=pad_q))
