@@ -559,9 +559,11 @@ int encode_map(HcCudaContext *ctx, CUtensorMap *map, int dtype, const void *base
 // Enqueues the GEMM on device-resident buffers. The caller holds ctx->mu and has made the
 // context's device current.
 int enqueue_gemm(HcCudaContext *ctx, const HcCudaGemmArgs *args, const HcCudaGemmPlanInfo &plan,
-                 const hc::sm100::Epilogue &push = hc::sm100::Epilogue{}) {
+                 const hc::sm100::Epilogue &push = hc::sm100::Epilogue{}, const float *device_factor = nullptr) {
   if (plan.variant == HC_CUDA_GEMM_NOOP)
     return HC_CUDA_OK;
+  if (device_factor != nullptr && (plan.variant != HC_CUDA_GEMM_DENSE || plan.cluster_size > 1))
+    return fail(ctx, HC_CUDA_ERR_UNSUPPORTED, "a factor on the device needs a dense product of whole tiles");
   const int m = static_cast<int>(args->m), n = static_cast<int>(args->n), k = static_cast<int>(args->k);
   hc::sm100::Epilogue ep = push;  // the push targets, if any; the fused work comes from args
   ep.accumulate = args->accumulate;
@@ -737,7 +739,7 @@ int enqueue_gemm(HcCudaContext *ctx, const HcCudaGemmArgs *args, const HcCudaGem
     if (wide) {
       HC_TRY_CUDA(ctx, hc::sm100::launch_gemm_dense_wide(tmap_a, tmap_b, args->c, m, n, k, args->ldc, args->dtype,
                                                          ctx->group_n_wide, plan.grid, b_layout, ep, c_map,
-                                                         ctx->status_dev, ctx->stream));
+                                                         ctx->status_dev, ctx->stream, device_factor));
     } else if (pairs) {
       // Push targets as tensor maps (they are shaped and pitched like C): the epilogue then stores
       // every staged chunk to C and to each target through the TMA store engine instead of with
@@ -759,12 +761,12 @@ int enqueue_gemm(HcCudaContext *ctx, const HcCudaGemmArgs *args, const HcCudaGem
       HC_TRY_CUDA(ctx, hc::sm100::launch_gemm_dense_pair(tmap_a, tmap_b, args->c, m, n, k, args->ldc,
                                                          args->dtype, ctx->group_n, plan.grid, b_layout, ep,
                                                          c_map, split, &tmap_p, ctx->status_dev, ctx->stream,
-                                                         push_maps.count > 0 ? &push_maps : nullptr));
+                                                         push_maps.count > 0 ? &push_maps : nullptr, device_factor));
     } else {
       HC_TRY_CUDA(ctx, hc::sm100::launch_gemm_dense(tmap_a, tmap_b, args->c, m, n, k, args->ldc,
                                                     args->dtype, ctx->group_n, plan.grid, b_layout, ep,
                                                     c_map, split, &tmap_p, ctx->status_dev, ctx->stream,
-                                                    narrow ? hc::sm100::dense_narrow_block_n() : t.block_n));
+                                                    narrow ? hc::sm100::dense_narrow_block_n() : t.block_n, device_factor));
     }
     return HC_CUDA_OK;
   }
@@ -2263,14 +2265,13 @@ struct LossBackwardPlan {
   int64_t scales = 0;
 };
 
-// A product whose results are multiplied by a factor on the device (Epilogue::device_factor, which the tiny kernel
-// does not read).
+// A product whose 16-bit results are multiplied by a factor on the device, which the dense kernels can do
+// (hc::sm100::ScaledEpilogue).
 void scale_by_factor(HcCudaGemmArgs *g) {
   g->epilogue_count = 1;
   g->epilogue_kind[0] = HC_CUDA_EPILOGUE_SCALE;
   g->epilogue_value[0] = 1.0f;
-  if (hc::sm100::tiny_takes(g->m, g->n, g->k, g->dtype, kDefaultSmCount))
-    g->variant = HC_CUDA_GEMM_DENSE;
+  g->variant = HC_CUDA_GEMM_DENSE;
 }
 
 // The two products of a piece as GEMM arguments, their 16-bit results scaled by scales[1]; `c` is already aligned, `base` the start of `work`.
@@ -2390,15 +2391,15 @@ int plan_linear_loss_backward(const HcCudaContext *ctx, const HcCudaLinearLossBa
   }
   HcCudaGemmPlanInfo product;
   if (args->dh != nullptr) {
-    // The sums are float32 where there are several products, and where the form that shares one product's k
-    // among clusters, which writes float32, would be taken for it: 128 x 512 x 4099 takes 38 us without it.
+    // The sums are float32 where there are several products, and where one would run as the form that shares its k
+    // among clusters, which writes float32 (128 x 512 x 4099 takes 38 us without it), or outside the dense kernels.
     const int64_t bytes = plan->work.bytes;
     plan->dh_sums = plan->work.take(c.rows * plan->sums_ld * 4);
     if (plan->pieces == 1) {
       const HcCudaGemmArgs g = loss_dh_product(aligned, *plan, base, 0, c.vocab, *args);
       if (int rc = plan_gemm(ctx, &g, sm_count, false, &product, /*apart=*/true))
         return rc;
-      if (product.cluster_size <= 1) {
+      if (product.variant == HC_CUDA_GEMM_DENSE && product.cluster_size <= 1) {
         plan->dh_sums = -1;
         plan->work.bytes = bytes;
       }
@@ -2504,8 +2505,7 @@ int hcCudaLinearLossBackward(HcCudaContext *ctx, const HcCudaLinearLossBackwardA
   if (int rc = enqueue_loss_copies(ctx, plan.work, copy_h, &c))
     return rc;
   const int narrow_type = c.dtype == HC_CUDA_BF16 ? hc::sm100::kCTypeBF16 : hc::sm100::kCTypeF16;
-  hc::sm100::Epilogue scaled{};
-  scaled.device_factor = scales + 1;
+  const float *const factor = scales + 1;
   for (int64_t first = 0; first < c.vocab; first += plan.piece) {
     const int64_t count = c.vocab - first < plan.piece ? c.vocab - first : plan.piece;
     hc::sm100::LinearLoss p = loss_launch(c, first, count);
@@ -2527,14 +2527,14 @@ int hcCudaLinearLossBackward(HcCudaContext *ctx, const HcCudaLinearLossBackwardA
       const HcCudaGemmArgs g = loss_dh_product(c, plan, base, first, count, *args);
       if (int rc = plan_gemm(ctx, &g, sm_count, false, &product, /*apart=*/true))
         return rc;
-      if (int rc = enqueue_gemm(ctx, &g, product, plan.dh_sums >= 0 ? hc::sm100::Epilogue{} : scaled))
+      if (int rc = enqueue_gemm(ctx, &g, product, hc::sm100::Epilogue{}, plan.dh_sums >= 0 ? nullptr : factor))
         return rc;
     }
     if (args->dw != nullptr) {
       const HcCudaGemmArgs g = loss_dw_product(c, plan, base, first, count, *args);
       if (int rc = plan_gemm(ctx, &g, sm_count, false, &product, /*apart=*/true))
         return rc;
-      if (int rc = enqueue_gemm(ctx, &g, product, scaled))
+      if (int rc = enqueue_gemm(ctx, &g, product, hc::sm100::Epilogue{}, factor))
         return rc;
       if (plan.dw_copy >= 0)
         HC_TRY_CUDA(ctx, hc::sm100::launch_spread(base + plan.dw_copy, plan.dw_ld,
@@ -2544,7 +2544,7 @@ int hcCudaLinearLossBackward(HcCudaContext *ctx, const HcCudaLinearLossBackwardA
   }
   if (plan.dh_sums >= 0)
     HC_TRY_CUDA(ctx, hc::sm100::launch_narrow(reinterpret_cast<const float *>(base + plan.dh_sums), plan.sums_ld, args->dh,
-                                              args->lddh, static_cast<int>(c.rows), static_cast<int>(c.width), scales + 1,
+                                              args->lddh, static_cast<int>(c.rows), static_cast<int>(c.width), factor,
                                               narrow_type, ctx->stream));
   return HC_CUDA_OK;
 }

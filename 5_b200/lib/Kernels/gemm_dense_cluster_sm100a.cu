@@ -165,7 +165,7 @@ __device__ __forceinline__ void reduce_rows(const ReduceArgs &ra, int block, int
     if (op >= ep.op_count)
       break;
     const int kind = ep.op_kind[op];
-    const float x = op_constant(ep, op);
+    const float x = ep.op_value[op];
 #pragma unroll
     for (int i = 0; i < kVectors; ++i) {
       float4 y = make_float4(x, x, x, x);

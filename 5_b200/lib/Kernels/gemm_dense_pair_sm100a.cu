@@ -98,7 +98,7 @@ __device__ __forceinline__ TileCoord tile_coord(int tile, int tiles_m, int tiles
 // cannot do the addition themselves: operations follow it, C's pitch rules out TMA, or there are
 // push targets). Every other launch -- the plain product, element-wise operations, accumulation
 // by TMA additions -- runs the other instantiation, which never reads C.
-template <bool kReadsC>
+template <bool kReadsC, typename Ep = Epilogue>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Roles<kReadsC>::kThreads, 1)
 gemm_dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_a,
                        const __grid_constant__ CUtensorMap tmap_b,
@@ -106,7 +106,7 @@ gemm_dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_a,
                        const __grid_constant__ CUtensorMap tmap_partials,
                        const __grid_constant__ PushMaps push_maps, void *c, int m, int n,
                        int k, long long ldc, uint32_t idesc, int tiles_m, int tiles_n, int group_n,
-                       int l2_hints, int b_layout, int elem8, Epilogue ep, SplitK split, int *status) {
+                       int l2_hints, int b_layout, int elem8, Ep ep, SplitK split, int *status) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   const uint32_t smem_base = (raw_addr + 1023u) & ~1023u;
@@ -377,7 +377,7 @@ cudaError_t launch_gemm_dense_pair(const CUtensorMap &tmap_a, const CUtensorMap 
                                    int m, int n, int k, long long ldc, int dtype, int group_n,
                                    int max_ctas, int b_layout, const Epilogue &ep, const CUtensorMap *tmap_c,
                                    const SplitK &split, const CUtensorMap *tmap_partials, int *status,
-                                   cudaStream_t stream, const PushMaps *push_maps) {
+                                   cudaStream_t stream, const PushMaps *push_maps, const float *device_factor) {
   using namespace dense_pair;
   static thread_local int configured_device = -1;
   int device = 0;
@@ -389,6 +389,9 @@ cudaError_t launch_gemm_dense_pair(const CUtensorMap &tmap_a, const CUtensorMap 
                                static_cast<int>(kSmemBytes));
     if (err == cudaSuccess)
       err = cudaFuncSetAttribute(gemm_dense_pair_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 static_cast<int>(kSmemBytes));
+    if (err == cudaSuccess)
+      err = cudaFuncSetAttribute(gemm_dense_pair_kernel<false, ScaledEpilogue>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  static_cast<int>(kSmemBytes));
     if (err != cudaSuccess)
       return err;
@@ -425,6 +428,8 @@ cudaError_t launch_gemm_dense_pair(const CUtensorMap &tmap_a, const CUtensorMap 
   // reads C with ordinary loads, in the other instantiation.
   if (ep.c_dtype != kCTypeF32 && (ep.accumulate != 0 || ep.push_count != 0))
     return cudaErrorInvalidValue;  // rejected with a message by the caller's validation
+  if (device_factor != nullptr && ep.c_dtype == kCTypeF32)
+    return cudaErrorInvalidValue;
   Epilogue launch_ep = ep;
   // With push targets the tiles leave through TMA stores too when the caller supplies the targets'
   // tensor maps and the launch is the plain or element-wise product on whole tiles (an accumulating
@@ -448,7 +453,11 @@ cudaError_t launch_gemm_dense_pair(const CUtensorMap &tmap_a, const CUtensorMap 
   if (const char *h = std::getenv("HC_CUDA_L2_HINTS"))  // tuning aid
     l2_hints = std::atoi(h);
   const unsigned grid = static_cast<unsigned>(clusters * 2);
-  if (reads_c)
+  if (device_factor != nullptr)
+    gemm_dense_pair_kernel<false, ScaledEpilogue><<<grid, Roles<false>::kThreads, kSmemBytes, stream>>>(
+        tmap_a, tmap_b, c_map, c_tma, p_map, push_arg, c, m, n, k, ldc, idesc, tiles_m, tiles_n, group_n, l2_hints, b_layout, elem8,
+        ScaledEpilogue{launch_ep, device_factor}, split, status);
+  else if (reads_c)
     gemm_dense_pair_kernel<true><<<grid, Roles<true>::kThreads, kSmemBytes, stream>>>(
         tmap_a, tmap_b, c_map, c_tma, p_map, push_arg, c, m, n, k, ldc, idesc, tiles_m, tiles_n, group_n, l2_hints, b_layout, elem8, launch_ep, split, status);
   else

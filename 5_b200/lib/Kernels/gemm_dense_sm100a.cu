@@ -89,14 +89,14 @@ __device__ __forceinline__ TileCoord tile_coord(int tile, int tiles_m, int tiles
 }
 
 // kReadsC: the epilogue has to read C's previous contents (see gemm_dense_pair_kernel).
-template <bool kReadsC, int kBlockN>
+template <bool kReadsC, int kBlockN, typename Ep = Epilogue>
 __global__ void __launch_bounds__(Roles<kReadsC>::kThreads, 1)
 gemm_dense_kernel(const __grid_constant__ CUtensorMap tmap_a,
                   const __grid_constant__ CUtensorMap tmap_b,
                        const __grid_constant__ CUtensorMap tmap_c, int c_tma,
                        const __grid_constant__ CUtensorMap tmap_partials, void *c, int m, int n,
                   int k, long long ldc, uint32_t idesc, int tiles_m, int tiles_n, int group_n,
-                  int b_layout, int elem8, Epilogue ep, SplitK split, int *status) {
+                  int b_layout, int elem8, Ep ep, SplitK split, int *status) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   const uint32_t smem_base = (raw_addr + 1023u) & ~1023u;  // swizzled tiles need 1 KiB alignment
@@ -346,7 +346,7 @@ cudaError_t launch_gemm_dense(const CUtensorMap &tmap_a, const CUtensorMap &tmap
                               int m, int n, int k, long long ldc, int dtype, int group_n,
                               int max_ctas, int b_layout, const Epilogue &ep, const CUtensorMap *tmap_c,
                               const SplitK &split, const CUtensorMap *tmap_partials, int *status,
-                                   cudaStream_t stream, int block_n) {
+                                   cudaStream_t stream, int block_n, const float *device_factor) {
   using namespace dense;
   if (block_n != kWideBlockN && block_n != kNarrowBlockN)
     return cudaErrorInvalidValue;
@@ -370,6 +370,12 @@ cudaError_t launch_gemm_dense(const CUtensorMap &tmap_a, const CUtensorMap &tmap
     if (err == cudaSuccess)
       err = cudaFuncSetAttribute(gemm_dense_kernel<true, kNarrowBlockN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  static_cast<int>(Tile<kNarrowBlockN>::kSmemBytes));
+    if (err == cudaSuccess)
+      err = cudaFuncSetAttribute(gemm_dense_kernel<false, kWideBlockN, ScaledEpilogue>,
+                                 cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Tile<kWideBlockN>::kSmemBytes));
+    if (err == cudaSuccess)
+      err = cudaFuncSetAttribute(gemm_dense_kernel<false, kNarrowBlockN, ScaledEpilogue>,
+                                 cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Tile<kNarrowBlockN>::kSmemBytes));
     if (err != cudaSuccess)
       return err;
     configured_device = device;
@@ -401,6 +407,8 @@ cudaError_t launch_gemm_dense(const CUtensorMap &tmap_a, const CUtensorMap &tmap
   // reads C with ordinary loads, in the other instantiation.
   if (ep.c_dtype != kCTypeF32 && (ep.accumulate != 0 || ep.push_count != 0))
     return cudaErrorInvalidValue;  // rejected with a message by the caller's validation
+  if (device_factor != nullptr && ep.c_dtype == kCTypeF32)
+    return cudaErrorInvalidValue;
   Epilogue launch_ep = ep;
   const bool tma_possible = tmap_c != nullptr && ep.push_count == 0;
   launch_ep.accumulate_by_tma = (tma_possible && ep.accumulate != 0 && ep.op_count == 0) ? 1 : 0;
@@ -411,18 +419,23 @@ cudaError_t launch_gemm_dense(const CUtensorMap &tmap_a, const CUtensorMap &tmap
   const int c_tma = (tma_possible && !reads_c) ? 1 : 0;
   const CUtensorMap c_map = c_tma ? *tmap_c : tmap_a;  // unused unless c_tma
   const CUtensorMap p_map = split.splits > 1 ? *tmap_partials : tmap_a;  // unused unless split
-#define HC_DENSE_LAUNCH(READS_C, BLOCK_N)                                                                       \
+#define HC_DENSE_LAUNCH(READS_C, BLOCK_N, EP)                                                                   \
   gemm_dense_kernel<READS_C, BLOCK_N><<<grid, Roles<READS_C>::kThreads, Tile<BLOCK_N>::kSmemBytes, stream>>>(      \
       tmap_a, tmap_b, c_map, c_tma, p_map, c, m, n, k, ldc, idesc, tiles_m, tiles_n, group_n, b_layout, elem8,  \
-      launch_ep, split, status)
-  if (reads_c && narrow)
-    HC_DENSE_LAUNCH(true, kNarrowBlockN);
+      EP, split, status)
+  const ScaledEpilogue scaled{launch_ep, device_factor};
+  if (device_factor != nullptr && narrow)
+    HC_DENSE_LAUNCH(false, kNarrowBlockN, scaled);
+  else if (device_factor != nullptr)
+    HC_DENSE_LAUNCH(false, kWideBlockN, scaled);
+  else if (reads_c && narrow)
+    HC_DENSE_LAUNCH(true, kNarrowBlockN, launch_ep);
   else if (reads_c)
-    HC_DENSE_LAUNCH(true, kWideBlockN);
+    HC_DENSE_LAUNCH(true, kWideBlockN, launch_ep);
   else if (narrow)
-    HC_DENSE_LAUNCH(false, kNarrowBlockN);
+    HC_DENSE_LAUNCH(false, kNarrowBlockN, launch_ep);
   else
-    HC_DENSE_LAUNCH(false, kWideBlockN);
+    HC_DENSE_LAUNCH(false, kWideBlockN, launch_ep);
 #undef HC_DENSE_LAUNCH
   return cudaGetLastError();
 }

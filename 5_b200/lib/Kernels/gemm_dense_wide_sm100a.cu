@@ -78,12 +78,13 @@ __device__ __forceinline__ TileCoord tile_coord(int tile, int tiles_m, int tiles
   return tc;
 }
 
+template <typename Ep>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 gemm_dense_wide_kernel(const __grid_constant__ CUtensorMap tmap_a,
                        const __grid_constant__ CUtensorMap tmap_b,
                        const __grid_constant__ CUtensorMap tmap_c, int c_tma, void *c, int m, int n,
                        int k, long long ldc, uint32_t idesc, int tiles_m, int tiles_n, int group_n,
-                       int l2_hints, int b_layout, int elem8, Epilogue ep, int *status) {
+                       int l2_hints, int b_layout, int elem8, Ep ep, int *status) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   const uint32_t smem_base = (raw_addr + 1023u) & ~1023u;
@@ -331,7 +332,8 @@ bool dense_uses_wide(long long m, long long n, long long k, int sm_count) {
 
 cudaError_t launch_gemm_dense_wide(const CUtensorMap &tmap_a, const CUtensorMap &tmap_b, void *c, int m, int n,
                                    int k, long long ldc, int dtype, int group_n, int max_ctas, int b_layout,
-                                   const Epilogue &ep, const CUtensorMap *tmap_c, int *status, cudaStream_t stream) {
+                                   const Epilogue &ep, const CUtensorMap *tmap_c, int *status, cudaStream_t stream,
+                                   const float *device_factor) {
   using namespace dense_wide;
   static thread_local int configured_device = -1;
   int device = 0;
@@ -339,8 +341,11 @@ cudaError_t launch_gemm_dense_wide(const CUtensorMap &tmap_a, const CUtensorMap 
   if (err != cudaSuccess)
     return err;
   if (configured_device != device) {
-    err = cudaFuncSetAttribute(gemm_dense_wide_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    err = cudaFuncSetAttribute(gemm_dense_wide_kernel<Epilogue>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                static_cast<int>(kSmemBytes));
+    if (err == cudaSuccess)
+      err = cudaFuncSetAttribute(gemm_dense_wide_kernel<ScaledEpilogue>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 static_cast<int>(kSmemBytes));
     if (err != cudaSuccess)
       return err;
     configured_device = device;
@@ -357,6 +362,8 @@ cudaError_t launch_gemm_dense_wide(const CUtensorMap &tmap_a, const CUtensorMap 
   if (ep.push_count != 0 || (ep.accumulate != 0 && !(tma_possible && ep.op_count == 0)))
     return cudaErrorInvalidValue;
   if (ep.c_dtype != kCTypeF32 && ep.accumulate != 0)
+    return cudaErrorInvalidValue;
+  if (device_factor != nullptr && ep.c_dtype == kCTypeF32)
     return cudaErrorInvalidValue;
   const int elem8 = dtype_is_8bit(dtype) ? 1 : 0;
   if (elem8 && b_layout != kBLayoutNK)
@@ -379,9 +386,15 @@ cudaError_t launch_gemm_dense_wide(const CUtensorMap &tmap_a, const CUtensorMap 
   if (const char *h = std::getenv("HC_CUDA_L2_HINTS"))  // tuning aid
     l2_hints = std::atoi(h);
   const unsigned grid = static_cast<unsigned>(clusters * 2);
-  gemm_dense_wide_kernel<<<grid, kThreads, kSmemBytes, stream>>>(tmap_a, tmap_b, c_map, c_tma, c, m, n, k, ldc, idesc,
-                                                                 tiles_m, tiles_n, group_n, l2_hints, b_layout, elem8,
-                                                                 launch_ep, status);
+  auto launch = [&](const auto &with) {
+    gemm_dense_wide_kernel<<<grid, kThreads, kSmemBytes, stream>>>(tmap_a, tmap_b, c_map, c_tma, c, m, n, k, ldc, idesc,
+                                                                   tiles_m, tiles_n, group_n, l2_hints, b_layout, elem8,
+                                                                   with, status);
+  };
+  if (device_factor != nullptr)
+    launch(ScaledEpilogue{launch_ep, device_factor});
+  else
+    launch(launch_ep);
   return cudaGetLastError();
 }
 

@@ -58,8 +58,9 @@ __device__ __forceinline__ void store_c_element(void *c, long long index, float 
 }
 
 // The constant of operation `op`.
-__device__ __forceinline__ float op_constant(const Epilogue &ep, int op) {
-  return ep.device_factor != nullptr ? ep.op_value[op] * __ldg(ep.device_factor) : ep.op_value[op];
+__device__ __forceinline__ float op_constant(const Epilogue &ep, int op) { return ep.op_value[op]; }
+__device__ __forceinline__ float op_constant(const ScaledEpilogue &ep, int op) {
+  return ep.op_value[op] * __ldg(ep.device_factor);
 }
 
 // The fused element-wise work on one value that is about to be stored at `dst` (column `col`).
@@ -70,7 +71,7 @@ __device__ __forceinline__ float finish_value(float v, const float *dst, int col
   for (int i = 0; i < kMaxEpilogueOps; ++i) {
     if (i < ep.op_count) {
       const int kind = ep.op_kind[i];
-      const float x = kind == kEpilogueBiasColumn ? __ldg(ep.bias + col) : op_constant(ep, i);
+      const float x = kind == kEpilogueBiasColumn ? __ldg(ep.bias + col) : ep.op_value[i];
       v = kind == kEpilogueScale ? v * x
         : kind == kEpilogueMax   ? max_nan(v, x)
         : kind == kEpilogueMin   ? min_nan(v, x)
@@ -90,7 +91,7 @@ __device__ __forceinline__ void apply_ops_to_groups(float4 (&v)[8], const Epilog
     if (op >= ep.op_count)
       break;
     const int kind = ep.op_kind[op];
-    const float x = op_constant(ep, op);
+    const float x = ep.op_value[op];
     if (kind == kEpilogueScale) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -142,7 +143,7 @@ __device__ __forceinline__ void apply_ops_to_column(float (&v)[N], float bias, c
     if (op >= ep.op_count)
       break;
     const int kind = ep.op_kind[op];
-    const float x = kind == kEpilogueBiasColumn ? bias : op_constant(ep, op);
+    const float x = kind == kEpilogueBiasColumn ? bias : ep.op_value[op];
     if (kind == kEpilogueScale) {
 #pragma unroll
       for (int j = 0; j < N; ++j)
@@ -167,7 +168,8 @@ __device__ __forceinline__ void apply_ops_to_column(float (&v)[N], float bias, c
 // col0 + j): one instruction per value and operation, the kind branched on once per chunk. Used
 // whenever C's previous contents are not needed, so that the chunk can then leave like a plain one
 // (TMA store, or the coalesced writers for an odd pitch).
-__device__ __forceinline__ void apply_ops_lane_row(uint32_t (&r)[32], int col0, int n, int lane, const Epilogue &ep) {
+template <typename Ep>
+__device__ __forceinline__ void apply_ops_lane_row(uint32_t (&r)[32], int col0, int n, int lane, const Ep &ep) {
   float bias_lane = 0.0f;
   if (ep.bias != nullptr && col0 + lane < n)
     bias_lane = __ldg(ep.bias + col0 + lane);
@@ -221,7 +223,7 @@ __device__ __forceinline__ float finish_loaded(float v, float previous, float bi
   for (int i = 0; i < kMaxEpilogueOps; ++i) {
     if (i < ep.op_count) {
       const int kind = ep.op_kind[i];
-      const float x = kind == kEpilogueBiasColumn ? bias : op_constant(ep, i);
+      const float x = kind == kEpilogueBiasColumn ? bias : ep.op_value[i];
       v = kind == kEpilogueScale ? v * x
         : kind == kEpilogueMax   ? max_nan(v, x)
         : kind == kEpilogueMin   ? min_nan(v, x)
@@ -689,11 +691,11 @@ __device__ __forceinline__ void store_block16_plain(const uint32_t (&w)[32], int
 
 // The accumulator drain for a 16-bit C: two 32-column chunks make one 64-column block of packed
 // pairs; element-wise operations run on the float32 values first.
-template <int kColumns>
+template <int kColumns, typename Ep>
 __device__ __forceinline__ void drain_accumulator_rows16(uint32_t taddr, float *stage, void *c, long long ldc, int m,
                                                          int n, int row_base, int col_base, int lane,
                                                          uint32_t release_bar, bool release_remote,
-                                                         const Epilogue &ep, const CUtensorMap *tmap_c) {
+                                                         const Ep &ep, const CUtensorMap *tmap_c) {
   constexpr int kChunks = kColumns / 32;
   static_assert(kChunks % 2 == 0, "chunks are processed in pairs");
   uint32_t ra[32], rb[32], w[32];
@@ -739,12 +741,12 @@ __device__ __forceinline__ void drain_accumulator_rows16(uint32_t taddr, float *
 //
 // The TMEM load of the next chunk is in flight while the current chunk is transposed and
 // stored (two register sets alternate), so the TMEM latency is hidden behind the stores.
-template <int kColumns, bool kReadsC>
+template <int kColumns, bool kReadsC, typename Ep>
 __device__ __forceinline__ void drain_accumulator_rows(uint32_t taddr, float *stage, void *c_any,
                                                        long long ldc, int m, int n, int row_base,
                                                        int col_base, bool vec_ok, int lane,
                                                        uint32_t release_bar, bool release_remote,
-                                                       const Epilogue &ep, const CUtensorMap *tmap_c,
+                                                       const Ep &ep, const CUtensorMap *tmap_c,
                                                        uint32_t c_load_bar = 0, uint32_t *c_load_phase = nullptr,
                                                        volatile uint32_t *abort_flag = nullptr,
                                                        const PushMaps *push_maps = nullptr) {
@@ -825,11 +827,11 @@ namespace sm100 {
 // instruction fetches four full lines.
 // (Not inlined: it runs once per tile, and kept apart it cannot raise the register demand of the
 // chunk loop that every tile goes through.)
-template <int kColumns, bool kReadsC>
+template <int kColumns, bool kReadsC, typename Ep>
 __device__ __noinline__ void reduce_partials_rows(const float *partial_rows, int partial_ld, size_t split_stride,
                                                   int splits, float *stage, void *c_any, long long ldc,
                                                   int m, int n, int row_base, int col_base, bool vec_ok, int lane,
-                                                  const Epilogue &ep, const CUtensorMap *tmap_c) {
+                                                  const Ep &ep, const CUtensorMap *tmap_c) {
   constexpr int kChunks = kColumns / 32;
   float carry[6] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
   float *__restrict__ c = static_cast<float *>(c_any);

@@ -68,9 +68,6 @@ struct Epilogue {
   int op_kind[kMaxEpilogueOps];
   float op_value[kMaxEpilogueOps];
   const float *bias;
-  // Where a launch's only operation is a scaling by a number that an earlier kernel finds: it is multiplied
-  // into op_value[0]. Null otherwise. (Not read by the tiny kernel.)
-  const float *device_factor;
   // Element type of C: 0 float32, 1 float16, 2 bfloat16 (the float32 value rounded to nearest
   // even). 16-bit output is written by the kernels that do not read C.
   int c_dtype;
@@ -81,6 +78,13 @@ struct Epilogue {
   // address: each chunk of C's previous contents comes in by a TMA load, is added in registers,
   // the operations run, and the chunk leaves by a TMA store.
   int accumulate_by_tma_load;
+};
+
+// The same for a 16-bit C whose operations take a number that an earlier kernel finds: it is multiplied into their
+// constants. Launches without one run kernels of their own, which know nothing of it (a test and a load per operation
+// cost products with fused operations 2 to 10 %: 256 x 256 x 4096 scaled 14.9 and 16.4 us).
+struct ScaledEpilogue : Epilogue {
+  const float *device_factor;
 };
 
 // Splitting dense tiles over k. Tiles [0, first_split_tile) are computed whole; each later tile
@@ -125,8 +129,8 @@ cudaError_t launch_gemm_dense(const CUtensorMap &tmap_a, const CUtensorMap &tmap
                               int m, int n, int k, long long ldc, int dtype, int group_n,
                               int max_ctas, int b_layout, const Epilogue &ep, const CUtensorMap *tmap_c,
                               const SplitK &split, const CUtensorMap *tmap_partials, int *status,
-                                   cudaStream_t stream, int block_n = 256);
-// `block_n`: 256, or 128 (dense_narrow_block_n) for tiles of 128 x 128 -- never split over k; tmap_b of a
+                                   cudaStream_t stream, int block_n = 256, const float *device_factor = nullptr);
+// `device_factor` (here and in the launchers below; a 16-bit C): see ScaledEpilogue. `block_n`: 256, or 128 (dense_narrow_block_n) for tiles of 128 x 128 -- never split over k; tmap_b of a
 // B stored [N, K] then has boxes of 128 rows. dense_uses_narrow: whether the 256-wide tiles (or CTA pairs)
 // of an m x n product with a short k would keep at most a quarter of the SMs busy while 128-wide tiles fit
 // one round; such a product is not split over k.
@@ -165,7 +169,8 @@ cudaError_t launch_gemm_dense_pair(const CUtensorMap &tmap_a, const CUtensorMap 
                                    int m, int n, int k, long long ldc, int dtype, int group_n,
                                    int max_ctas, int b_layout, const Epilogue &ep, const CUtensorMap *tmap_c,
                                    const SplitK &split, const CUtensorMap *tmap_partials, int *status,
-                                   cudaStream_t stream, const PushMaps *push_maps = nullptr);
+                                   cudaStream_t stream, const PushMaps *push_maps = nullptr,
+                                   const float *device_factor = nullptr);
 
 // The pair kernel's big brother: 512x256 tiles per pair (a 256x256 accumulator per CTA, all of its
 // tensor memory), a quarter fewer operand bytes per flop, no overlap of epilogue and next k-loop.
@@ -173,7 +178,8 @@ cudaError_t launch_gemm_dense_pair(const CUtensorMap &tmap_a, const CUtensorMap 
 // C, accumulation by TMA additions), without split-k and without push targets.
 cudaError_t launch_gemm_dense_wide(const CUtensorMap &tmap_a, const CUtensorMap &tmap_b, void *c, int m, int n,
                                    int k, long long ldc, int dtype, int group_n, int max_ctas, int b_layout,
-                                   const Epilogue &ep, const CUtensorMap *tmap_c, int *status, cudaStream_t stream);
+                                   const Epilogue &ep, const CUtensorMap *tmap_c, int *status, cudaStream_t stream,
+                                   const float *device_factor = nullptr);
 // Whether a product of this shape is large enough for the 512x256 tiles to pay.
 bool dense_uses_wide(long long m, long long n, long long k, int sm_count);
 constexpr int kDenseWideTileM = 512;
