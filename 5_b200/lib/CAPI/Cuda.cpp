@@ -2256,7 +2256,7 @@ struct LossBackwardPlan {
   int64_t piece = 0;  // columns of the vocabulary per piece, a multiple of 256
   int64_t pieces = 0;
   int64_t g = 0, gt = 0, ldg = 0, ldgt = 0;
-  int64_t dh_sums = -1;  // float32, where dh is the sum of several products or their fastest form writes float32
+  int64_t dh_sums = -1;  // float32 sums of dh without the rows' dloss (g_plain), rounded at the end; -1: dh is written at once
   int64_t sums_ld = 0;
   // 16-bit, where dw's rows do not all start on 16-byte boundaries: the product stores to it by TMA and a copy
   // follows (16411 x 1001 x 1031: 41 and 12 us; 70 us when the product writes such rows itself).
@@ -2392,10 +2392,11 @@ int plan_linear_loss_backward(const HcCudaContext *ctx, const HcCudaLinearLossBa
   HcCudaGemmPlanInfo product;
   if (args->dh != nullptr) {
     // The sums are float32 where there are several products, and where one would run as the form that shares its k
-    // among clusters, which writes float32 (128 x 512 x 4099 takes 38 us without it), or outside the dense kernels.
+    // among clusters, which writes float32 (128 x 512 x 4099 takes 38 us without it), or outside the dense kernels;
+    // and for float16, whose rows take their own factors after the product.
     const int64_t bytes = plan->work.bytes;
     plan->dh_sums = plan->work.take(c.rows * plan->sums_ld * 4);
-    if (plan->pieces == 1) {
+    if (plan->pieces == 1 && c.dtype == HC_CUDA_BF16) {
       const HcCudaGemmArgs g = loss_dh_product(aligned, *plan, base, 0, c.vocab, *args);
       if (int rc = plan_gemm(ctx, &g, sm_count, false, &product, /*apart=*/true))
         return rc;
@@ -2504,7 +2505,6 @@ int hcCudaLinearLossBackward(HcCudaContext *ctx, const HcCudaLinearLossBackwardA
                                                          plan.work.copy_ld, ctx->stream));
   if (int rc = enqueue_loss_copies(ctx, plan.work, copy_h, &c))
     return rc;
-  const int narrow_type = c.dtype == HC_CUDA_BF16 ? hc::sm100::kCTypeBF16 : hc::sm100::kCTypeF16;
   const float *const factor = scales + 1;
   for (int64_t first = 0; first < c.vocab; first += plan.piece) {
     const int64_t count = c.vocab - first < plan.piece ? c.vocab - first : plan.piece;
@@ -2515,6 +2515,7 @@ int hcCudaLinearLossBackward(HcCudaContext *ctx, const HcCudaLinearLossBackwardA
     if (args->dh != nullptr) {
       p.g = base + plan.g;
       p.ldg = plan.ldg;
+      p.g_plain = plan.dh_sums >= 0 ? 1 : 0;
     }
     if (args->dw != nullptr) {
       p.gt = base + plan.gt;
@@ -2543,9 +2544,8 @@ int hcCudaLinearLossBackward(HcCudaContext *ctx, const HcCudaLinearLossBackwardA
     }
   }
   if (plan.dh_sums >= 0)
-    HC_TRY_CUDA(ctx, hc::sm100::launch_narrow(reinterpret_cast<const float *>(base + plan.dh_sums), plan.sums_ld, args->dh,
-                                              args->lddh, static_cast<int>(c.rows), static_cast<int>(c.width), factor,
-                                              narrow_type, ctx->stream));
+    HC_TRY_CUDA(ctx, hc::sm100::launch_linear_loss_narrow(all, reinterpret_cast<const float *>(base + plan.dh_sums), plan.sums_ld,
+                                                          args->dh, args->lddh, static_cast<int>(c.width), ctx->stream));
   return HC_CUDA_OK;
 }
 

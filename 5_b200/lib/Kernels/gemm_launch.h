@@ -343,8 +343,10 @@ struct LinearLoss {
   float2 *partials;
   float *target_logit, *loss_out, *lse_out;
   // Gradient: the upstream factors as fractions of scales[0]; g [rows, ldg] with ldg a multiple of
-  // 32 not below vocab, and its transpose gt [vocab, ldgt]; either may be null.
+  // 32 not below vocab, and its transpose gt [vocab, ldgt]; either may be null. With g_plain g is formed without
+  // the upstream factors (0 in the rows that do not count or whose factor is 0).
   const float *lse, *dloss, *scales;
+  int g_plain;
   void *g;
   long long ldg;
   void *gt;
@@ -363,9 +365,10 @@ cudaError_t launch_linear_loss_prepare(const LinearLoss &p, float *scales, const
 // dst[r, c] = src[r, c], 16 bits each; src 16-byte aligned with lds a multiple of 8, dst anywhere.
 cudaError_t launch_spread(const void *src, long long lds, void *dst, long long ldd, int rows, int cols, int sm_count,
                           cudaStream_t stream);
-// dst[r, c] = src[r, c] * *factor, rounded to 16 bits; src 16-byte aligned with lds a multiple of 4.
-cudaError_t launch_narrow(const float *src, long long lds, void *dst, long long ldd, int rows, int cols,
-                          const float *factor, int c_dtype, cudaStream_t stream);
+// dst[r, c] = src[r, c] times the row's upstream factor, what g was multiplied by taken back, rounded to 16 bits; 0 in the
+// rows that do not count. src [p.rows, cols] 16-byte aligned with lds a multiple of 4: the product of a g made with g_plain.
+cudaError_t launch_linear_loss_narrow(const LinearLoss &p, const float *src, long long lds, void *dst, long long ldd, int cols,
+                                      cudaStream_t stream);
 
 // ---- products with 4-bit weights -------------------------------------------------------------------
 struct W4 {

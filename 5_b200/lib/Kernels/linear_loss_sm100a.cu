@@ -30,6 +30,10 @@
 // therefore finds the largest |dloss| of the rows that count, uses dloss as a fraction of it, so that g is
 // (p - 1) or p to the type's precision, and the products take the factor back in float32 before they are
 // rounded. float16 also multiplies g by 2^14, because p may lie below the type's normal range.
+// For dw, a sum over rows, one factor for all rows is right: next to the largest a row of a small dloss is small. A row
+// of dh is that row's alone, and 2^-25 of the largest dloss may be more than all of it, in float16. Where dh goes
+// through float32 sums, which it always does in float16, its g is therefore formed without dloss, and each row of the
+// sums is multiplied by its own. (bfloat16 has float32's exponents.)
 #include "gemm_epilogue.cuh"
 #include "device_checks.cuh"
 #include "gemm_launch.h"
@@ -286,16 +290,21 @@ linear_loss_kernel(const __grid_constant__ CUtensorMap tmap_h, const __grid_cons
       // What the row needs is fetched while its products are still running.
       long long target = -1;
       float scale = 0.0f, lse2 = 0.0f;
+      bool nothing = true;  // of this row is in the gradient
       if (live) {
         target = target_of(p, row);
         if (kGrad) {
           // A row that does not count has no gradient, whatever its dloss and lse hold.
           const bool counts = counts_row(p, target);
-          scale = counts ? p.dloss[row] / p.scales[0] * g_scale(p.c_dtype) : 0.0f;
+          const float dloss = counts ? p.dloss[row] : 0.0f;
+          nothing = dloss == 0.0f;
+          scale = dloss / p.scales[0] * g_scale(p.c_dtype);
           lse2 = counts ? p.lse[row] * kLog2e : INFINITY;
         }
         target = target == p.ignore_index ? -1 : target - p.first_column;
       }
+      // Whether g differs from what its transpose holds: not where dloss is the largest one, in all rows mostly.
+      const bool plain = kGrad && p.g_plain != 0 && __any_sync(0xffffffffu, !nothing && scale != g_scale(p.c_dtype));
       const int target_col =
           target >= 0 && target < p.vocab ? static_cast<int>(target) - col_base : -1;  // within this warp's columns
       const bool ready = mbar_wait(tmem_full_bar(acc), (iter >> 1) & 1u, abort_flag);
@@ -314,22 +323,25 @@ linear_loss_kernel(const __grid_constant__ CUtensorMap tmap_h, const __grid_cons
           take_chunk(r, col0, p.vocab, run);
           take_target(r, live ? target_col - chunk * 32 : -1, p.target_logit + row);
         } else {
-          // g, rounded to the operands' type; two neighbouring columns per word.
+          // p - [v == target], then g, rounded to the operands' type; two neighbouring columns per word.
           uint32_t w[16];
           const int hit = target_col - chunk * 32;
 #pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            float a = exp2_fast(fmaf(__uint_as_float(r[j]), kLog2e, -lse2));
-            float b = exp2_fast(fmaf(__uint_as_float(r[j + 1]), kLog2e, -lse2));
-            a = (j == hit ? a - 1.0f : a) * scale;
-            b = (j + 1 == hit ? b - 1.0f : b) * scale;
-            w[j / 2] = pack_pair(a, b, p.c_dtype);
+          for (int j = 0; j < 32; ++j) {
+            const float a = exp2_fast(fmaf(__uint_as_float(r[j]), kLog2e, -lse2));
+            r[j] = __float_as_uint(j == hit ? a - 1.0f : a);
           }
-          if (scale == 0.0f) {  // exactly nothing, also where the logits are not finite
+          auto scaled_by = [&](float by) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-              w[j] = 0u;
-          }
+            for (int j = 0; j < 32; j += 2)
+              w[j / 2] = pack_pair(__uint_as_float(r[j]) * by, __uint_as_float(r[j + 1]) * by, p.c_dtype);
+            if (nothing) {  // exactly, also where the logits are not finite
+#pragma unroll
+              for (int j = 0; j < 16; ++j)
+                w[j] = 0u;
+            }
+          };
+          scaled_by(scale);
           // Transposed: two neighbouring lanes share their words, so that each writes two neighbouring rows of every
           // other column. (The pitch holds whole groups of 32 rows; what rows past the end get is not read.)
           const int row0 = row - lane;
@@ -348,6 +360,8 @@ linear_loss_kernel(const __grid_constant__ CUtensorMap tmap_h, const __grid_cons
           // As it stands: four lanes exchange their 16-byte pieces, so that together they write the 64 bytes of one row
           // after another (the pitch holds whole chunks of 32 columns).
           if (p.g != nullptr && row0 < p.rows) {
+            if (plain)
+              scaled_by(g_scale(p.c_dtype));
             uint4 piece[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j)
@@ -540,26 +554,29 @@ spread_kernel(const uint16_t *src, long long lds, uint16_t *dst, long long ldd, 
   }
 }
 
-// dst = src * factor rounded to 16 bits, for a matrix of rows x cols.
+// dh = (float32 sums of g W) * dloss / g_scale, rounded to 16 bits, for a g formed without dloss.
 template <typename Pair>
 __global__ void __launch_bounds__(256)
-narrow_kernel(const float *src, long long lds, void *dst, long long ldd, int rows, int cols, const float *factor, int c_dtype) {
-  const float f = *factor;
-  for (int row = blockIdx.y; row < rows; row += gridDim.y) {
+narrow_kernel(const LinearLoss p, const float *src, long long lds, void *dst, long long ldd, int cols) {
+  const float back = 1.0f / g_scale(p.c_dtype);  // (a power of two)
+  for (int row = blockIdx.y; row < p.rows; row += gridDim.y) {
     const float *s = src + static_cast<long long>(row) * lds;
     uint16_t *d = static_cast<uint16_t *>(dst) + static_cast<long long>(row) * ldd;
     const int c = (blockIdx.x * 256 + threadIdx.x) * 4;
     if (c >= cols)
       continue;
+    const bool counts = counts_row(p, target_of(p, row));
+    const float f = counts ? p.dloss[row] : 0.0f;
     const float4 v = *reinterpret_cast<const float4 *>(s + c);  // (lds is a multiple of 4)
+    auto of = [&](float x) { return f == 0.0f ? 0.0f : x * back * f; };
     if (sizeof(Pair) == 8 && c + 4 <= cols) {
-      *reinterpret_cast<uint2 *>(d + c) = make_uint2(pack_pair(v.x * f, v.y * f, c_dtype), pack_pair(v.z * f, v.w * f, c_dtype));
+      *reinterpret_cast<uint2 *>(d + c) = make_uint2(pack_pair(of(v.x), of(v.y), p.c_dtype), pack_pair(of(v.z), of(v.w), p.c_dtype));
     } else {
       const float e[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         if (c + i < cols)
-          d[c + i] = round_to_16(e[i] * f, c_dtype);
+          d[c + i] = round_to_16(of(e[i]), p.c_dtype);
     }
   }
 }
@@ -628,15 +645,15 @@ cudaError_t launch_spread(const void *src, long long lds, void *dst, long long l
   return cudaGetLastError();
 }
 
-cudaError_t launch_narrow(const float *src, long long lds, void *dst, long long ldd, int rows, int cols,
-                          const float *factor, int c_dtype, cudaStream_t stream) {
-  if (rows == 0 || cols == 0)
+cudaError_t launch_linear_loss_narrow(const LinearLoss &p, const float *src, long long lds, void *dst, long long ldd, int cols,
+                                      cudaStream_t stream) {
+  if (p.rows == 0 || cols == 0)
     return cudaSuccess;
-  const dim3 grid(static_cast<unsigned>((cols + 1023) / 1024), static_cast<unsigned>(rows < 65535 ? rows : 65535));
+  const dim3 grid(static_cast<unsigned>((cols + 1023) / 1024), static_cast<unsigned>(p.rows < 65535 ? p.rows : 65535));
   if ((ldd & 3) == 0 && (reinterpret_cast<uintptr_t>(dst) & 7) == 0)
-    loss::narrow_kernel<uint2><<<grid, 256, 0, stream>>>(src, lds, dst, ldd, rows, cols, factor, c_dtype);
+    loss::narrow_kernel<uint2><<<grid, 256, 0, stream>>>(p, src, lds, dst, ldd, cols);
   else
-    loss::narrow_kernel<uint16_t><<<grid, 256, 0, stream>>>(src, lds, dst, ldd, rows, cols, factor, c_dtype);
+    loss::narrow_kernel<uint16_t><<<grid, 256, 0, stream>>>(p, src, lds, dst, ldd, cols);
   return cudaGetLastError();
 }
 

@@ -520,13 +520,15 @@ HC_CUDA_CAPI_EXPORTED int hcCudaLinearLossPlan(const HcCudaLinearLossArgs *args,
  * dloss hold,
  *   dh = g W,   dw = g^T H
  * both overwritten, in the type of h and w, each optional (NULL). lse is what hcCudaLinearLoss stored. The
- * logits are computed again, one piece of the vocabulary at a time; g, with dloss as a fraction of its largest
- * value among the rows that count (found on the device; for float16 times 2^14), is rounded to the operands'
- * type for the two products, whose sums are float32 and take the factor back before they are rounded. A call
- * gives the same bits every time. rows == 0 sets dw to zero. Uses context
- * scratch: a copy of h (for dw), g and its transpose for one piece of the vocabulary (together 512 MiB at
- * most, or 1 KiB per row where that is more), float32 sums of dh when there is more than one piece or few rows,
- * and a copy of dw's piece when its rows do not all start on 16-byte boundaries. */
+ * logits are computed again, one piece of the vocabulary at a time; g is rounded to the operands' type for the two
+ * products, whose sums are float32. For dw, dloss enters g as a fraction of its largest value among the rows that
+ * count (found on the device; for float16 times 2^14) and the product takes the factor back before it is rounded: an
+ * entry of g is off by half a step of its type, in float16 at least 2^-39 of that largest value. For dh the same with
+ * bfloat16 and one piece; else, and always with float16, each row of the float32 sums is multiplied by its own
+ * dloss, so that a row is as exact however small its dloss is. A call gives the same bits every time. rows == 0 sets dw
+ * to zero. Uses context scratch: a copy of h (for dw), g and its transpose for one piece of the vocabulary (together
+ * 512 MiB at most, or 1 KiB per row where that is more), the float32 sums of dh, and a copy of dw's piece when its
+ * rows do not all start on 16-byte boundaries. */
 typedef struct HcCudaLinearLossBackwardArgs {
   int64_t rows, vocab, width;
   int32_t dtype;

@@ -277,3 +277,34 @@ def test_refusals_reach_python(gpu_ctx) -> None:
     with pytest.raises(ValueError, match="multiplies"):
         single = empty(gpu_ctx, (4, 8), np.float32)
         gpu_ctx.linear_cross_entropy(single, single, t, f, g)
+
+
+@pytest.mark.parametrize("rows, vocab, width", [(48, 3000, 64), (300, 900, 40), (31, 700, 33)])
+@pytest.mark.parametrize("piece", [None, "512"])
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+def test_rows_of_very_different_upstream_factors(dtype, piece, rows, vocab, width, gpu_ctx, monkeypatch) -> None:
+    """dloss from 1e5 down to 1e-5 of it and less in one batch, flat distributions (p near 1 / vocab): every row of dh is
+    as exact as if it were alone. In float16 an entry of its g is off by half a step, at least 2^-25 below the 2^14
+    that stands for 1 (2^13 leaves a factor of two): nothing of another row's dloss."""
+    if piece is not None:
+        monkeypatch.setenv("HC_CUDA_LOSS_PIECE", piece)
+    h, w, targets, _ = inputs(rows, vocab, width, dtype, 13, sure=0.0)
+    h = (h.astype(np.float64) / 8).astype(h.dtype)
+    w = (w.astype(np.float64) * 4).astype(w.dtype)
+    dloss = (1e5 * 10.0 ** -np.linspace(0, 9, rows)).astype(np.float32) * np.where(np.arange(rows) % 3, 1, -1).astype(np.float32)
+    targets[[0, rows // 2]] = IGNORE, 1
+    loss, lse, dh, dw = run(gpu_ctx, h, w, targets, dloss)
+    exact = Exact(h, w, targets, dloss)
+    step = HALF_STEP[dtype]
+    size = np.abs(exact.scale)
+    floor = 2.0**-38 * size if dtype == "float16" else 0.0
+    g_err = np.where(size == 0, 0.0, np.abs(exact.g) * step + size * exact.p * exact.p_rel * (1 + step) + floor)
+    sums = (np.abs(exact.g) + g_err) @ np.abs(exact.w)
+    bound = (g_err @ np.abs(exact.w) + (vocab / 16 + 64) * 2.0**-22 * sums) * (1 + step) + step * np.abs(exact.dh) + TINY[dtype]
+    # (What lies beyond float16's 65504 is infinite there; below 6e4 the bound cannot reach it.)
+    fits_h, fits_w = np.abs(exact.dh) < 6e4, np.abs(exact.dw) < 6e4
+    assert (np.abs(dh.astype(np.float64) - exact.dh) <= bound)[fits_h].all()
+    # dw is a sum over the rows: exact next to the largest dloss.
+    assert (np.abs(dw.astype(np.float64) - exact.dw) <= exact.bounds(dtype)[1])[fits_w].all()
+    if dtype == "float16":
+        assert np.array_equal(dh[np.abs(exact.dh) > 7e4], np.copysign(np.inf, exact.dh[np.abs(exact.dh) > 7e4]))
