@@ -14,8 +14,14 @@
 // rounded to the operands' type, for one piece of the vocabulary at a time -- stored both as it stands and
 // transposed, so that both products with it, dH += g W_piece and dW_piece = g^T H, read it along their
 // inner dimension. Those products are the dense kernels' (lib/CAPI/Cuda.cpp enqueues them).
-// Accuracy: a logit is a float32 sum whose additions the tensor cores cut instead of rounding them, so that lse and
-// loss are off by 1e-6 to 2e-6 of their size at a width of 4096 (3e-7 with sums that are rounded).
+//
+// Accuracy: the tensor cores cut what they add to a float32 accumulator instead of rounding it, so that its error grows
+// with the number of additions. An accumulator therefore takes a run of 1024 of the width (64 additions), and the
+// epilogue adds the runs in registers, with rounding. lse is off by 1.7e-7 of its size whatever the width, by 2.9e-6
+// where all products have one sign; with one accumulator 6.4e-7 and 1.7e-5 at a width of 4096, 4.9e-6 and 1.6e-4 at
+// 32768. (4096 x 32768 x 4096: 690 us, with one accumulator 680; runs of 512: 714 us, 1.0e-7 and 1.0e-6.) Both passes
+// add alike, so that the gradient's logits are those of lse. A width of one run keeps to one accumulator and, in the
+// epilogue, two alternating sets of 32 registers.
 //
 // g's stores: a lane holds a row, so lanes exchange words first, and what a warp writes at once covers whole
 // sectors of both forms (1031 x 16411 x 1001: 49.5 us, when every lane stored its own values 57 us).
@@ -56,6 +62,9 @@ constexpr int kEpilogueWarps = 8;  // two per quarter of the tensor-memory lanes
 constexpr int kThreads = 64 + 32 * kEpilogueWarps;
 constexpr int kTmemColumns = 512;  // two accumulators
 constexpr int kColumnsPerWarp = kTileN / 2;
+constexpr int kChunks = kColumnsPerWarp / 32;
+// k blocks whose products are summed in an accumulator before the epilogue adds them to the logits ("a run").
+constexpr int kRunBlocks = 8;
 constexpr uint32_t kBoxBytes = kCtaRows * 64 * 2;
 constexpr uint32_t kOperandBytes = 2 * kBoxBytes;
 constexpr uint32_t kStageBytes = 2 * kOperandBytes;  // per CTA
@@ -99,28 +108,19 @@ struct Running {
   float sum;  // sum exp2(l * log2(e) - top)
 };
 
-// 32 logits of this lane's row, the first at column `col0` of `vocab`.
-__device__ __forceinline__ void take_chunk(const uint32_t (&r)[32], int col0, int vocab, Running &run) {
+// 32 logits of this lane's row.
+__device__ __forceinline__ void take_chunk(const uint32_t (&r)[32], Running &run) {
   float top = -INFINITY;
-  if (col0 + 32 <= vocab) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
-      top = fmaxf(top, __uint_as_float(r[j]));
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (col0 + j < vocab)
-        top = fmaxf(top, __uint_as_float(r[j]));
-  }
+  for (int j = 0; j < 32; ++j)
+    top = fmaxf(top, __uint_as_float(r[j]));
   top = fmaxf(run.top, top * kLog2e);
   const float base = top == -INFINITY ? 0.0f : top;  // nothing finite yet: exp2(-inf - 0) = 0
   float sum = run.sum * exp2_fast(run.top - base);
   float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-  for (int j = 0; j < 32; ++j) {
-    const float e = exp2_fast(fmaf(__uint_as_float(r[j]), kLog2e, -base));
-    part[j & 3] += (col0 + 32 <= vocab || col0 + j < vocab) ? e : 0.0f;
-  }
+  for (int j = 0; j < 32; ++j)
+    part[j & 3] += exp2_fast(fmaf(__uint_as_float(r[j]), kLog2e, -base));
   run.top = top;
   run.sum = sum + ((part[0] + part[1]) + (part[2] + part[3]));
 }
@@ -148,7 +148,8 @@ __device__ __forceinline__ void swap_pieces(uint4 &a, uint4 &b, int lane, int bi
     b = got;
 }
 
-template <bool kGrad>
+// kRuns: the width is more than one run.
+template <bool kGrad, bool kRuns>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 linear_loss_kernel(const __grid_constant__ CUtensorMap tmap_h, const __grid_constant__ CUtensorMap tmap_w,
                    const LinearLoss p, uint32_t idesc, int tiles_m, int tiles_n, int group_n, int *status) {
@@ -242,38 +243,43 @@ linear_loss_kernel(const __grid_constant__ CUtensorMap tmap_h, const __grid_cons
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer (CTA 0) -
     if (lane == 0 && cta_rank == 0) {
-      uint32_t stage = 0, phase = 0, iter = 0;
+      uint32_t stage = 0, phase = 0, iter = 0;  // iter: accumulators filled
       bool ok = true;
-      for (int tile = first_tile; ok && tile < num_tiles; tile += tile_step, ++iter) {
-        const uint32_t acc = iter & 1u;
-        if (!mbar_wait(tmem_empty_bar(acc), ((iter >> 1) & 1u) ^ 1u, abort_flag))
-          break;
-        tcgen05_fence_after_sync();
-        for (int kb = 0; kb < num_kb; ++kb) {
-          if (!mbar_wait(full_bar(stage), phase, abort_flag)) {
+      for (int tile = first_tile; ok && tile < num_tiles; tile += tile_step) {
+        for (int kb = 0; ok && kb < num_kb; ++iter) {
+          const uint32_t acc = iter & 1u;
+          if (!mbar_wait(tmem_empty_bar(acc), ((iter >> 1) & 1u) ^ 1u, abort_flag)) {
             ok = false;
             break;
           }
           tcgen05_fence_after_sync();
-          const uint32_t h_addr = smem_base + stage * kStageBytes, w_addr = h_addr + kOperandBytes;
+          const int run_begin = kb, run_end = kRuns ? min(kb + kRunBlocks, num_kb) : num_kb;
+          for (; kb < run_end; ++kb) {
+            if (!mbar_wait(full_bar(stage), phase, abort_flag)) {
+              ok = false;
+              break;
+            }
+            tcgen05_fence_after_sync();
+            const uint32_t h_addr = smem_base + stage * kStageBytes, w_addr = h_addr + kOperandBytes;
 #pragma unroll
-          for (int kk = 0; kk < kBlockK / kUmmaK; ++kk) {
-            const uint64_t advance = static_cast<uint64_t>((kk % 4) * 2);  // 32 bytes inside the swizzle row
-            umma_ss_pair<false>(tmem_base + acc * kTileN,
-                                make_smem_desc_sw128(h_addr + (kk / 4) * kBoxBytes, 16, 1024) + advance,
-                                make_smem_desc_sw128(w_addr + (kk / 4) * kBoxBytes, 16, 1024) + advance, idesc,
-                                (kb != 0 || kk != 0) ? 1u : 0u);
+            for (int kk = 0; kk < kBlockK / kUmmaK; ++kk) {
+              const uint64_t advance = static_cast<uint64_t>((kk % 4) * 2);  // 32 bytes inside the swizzle row
+              umma_ss_pair<false>(tmem_base + acc * kTileN,
+                                  make_smem_desc_sw128(h_addr + (kk / 4) * kBoxBytes, 16, 1024) + advance,
+                                  make_smem_desc_sw128(w_addr + (kk / 4) * kBoxBytes, 16, 1024) + advance, idesc,
+                                  (kb != run_begin || kk != 0) ? 1u : 0u);
+            }
+            umma_commit_pair(map_to_cta(empty_bar(stage), 0));
+            umma_commit_pair(map_to_cta(empty_bar(stage), 1));
+            if (++stage == kStages) {
+              stage = 0;
+              phase ^= 1u;
+            }
           }
-          umma_commit_pair(map_to_cta(empty_bar(stage), 0));
-          umma_commit_pair(map_to_cta(empty_bar(stage), 1));
-          if (++stage == kStages) {
-            stage = 0;
-            phase ^= 1u;
+          if (ok) {
+            umma_commit_pair(map_to_cta(tmem_full_bar(acc), 0));
+            umma_commit_pair(map_to_cta(tmem_full_bar(acc), 1));
           }
-        }
-        if (ok) {
-          umma_commit_pair(map_to_cta(tmem_full_bar(acc), 0));
-          umma_commit_pair(map_to_cta(tmem_full_bar(acc), 1));
         }
       }
     }
@@ -281,9 +287,9 @@ linear_loss_kernel(const __grid_constant__ CUtensorMap tmap_h, const __grid_cons
     // ------------------------------------------------------------ epilogue ----------
     const int quarter = warp & 3, part = (warp - 2) >> 2;
     uint32_t iter = 0;
-    for (int tile = first_tile; tile < num_tiles; tile += tile_step, ++iter) {
+    bool ok = true;
+    for (int tile = first_tile; ok && tile < num_tiles; tile += tile_step) {
       const int2 at = tile_of(tile, tiles_m, tiles_n, group_n);
-      const uint32_t acc = iter & 1u;
       const int row = at.x * kTileM + static_cast<int>(cta_rank) * kCtaRows + quarter * 32 + lane;
       const int col_base = at.y * kTileN + part * kColumnsPerWarp;
       const bool live = row < p.rows;
@@ -307,12 +313,20 @@ linear_loss_kernel(const __grid_constant__ CUtensorMap tmap_h, const __grid_cons
       const bool plain = kGrad && p.g_plain != 0 && __any_sync(0xffffffffu, !nothing && scale != g_scale(p.c_dtype));
       const int target_col =
           target >= 0 && target < p.vocab ? static_cast<int>(target) - col_base : -1;  // within this warp's columns
-      const bool ready = mbar_wait(tmem_full_bar(acc), (iter >> 1) & 1u, abort_flag);
-      if (!__all_sync(0xffffffffu, ready))
-        break;
-      tcgen05_fence_after_sync();
-      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * kTileN + part * kColumnsPerWarp;
-      uint32_t ra[32], rb[32];
+      const uint32_t lanes = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + part * kColumnsPerWarp;
+      auto wait_for_sums = [&](uint32_t acc) {
+        const bool ready = mbar_wait(tmem_full_bar(acc), (iter >> 1) & 1u, abort_flag);
+        if (!__all_sync(0xffffffffu, ready))
+          return false;
+        tcgen05_fence_after_sync();
+        return true;
+      };
+      auto release = [&](uint32_t acc) {  // the accumulator has been read: back to the MMA issuer
+        tcgen05_fence_before_sync();
+        __syncwarp();
+        if (lane == 0)
+          mbar_arrive_cluster(map_to_cta(tmem_empty_bar(acc), 0));
+      };
       Running run{-INFINITY, 0.0f};
 
       auto finish = [&](uint32_t (&r)[32], int chunk) {
@@ -320,8 +334,14 @@ linear_loss_kernel(const __grid_constant__ CUtensorMap tmap_h, const __grid_cons
         if (col0 >= p.vocab)
           return;  // the same for the whole warp
         if constexpr (!kGrad) {
-          take_chunk(r, col0, p.vocab, run);
           take_target(r, live ? target_col - chunk * 32 : -1, p.target_logit + row);
+          if (col0 + 32 > p.vocab) {  // columns past the vocabulary add nothing
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (col0 + j >= p.vocab)
+                r[j] = __float_as_uint(-INFINITY);
+          }
+          take_chunk(r, run);
         } else {
           // p - [v == target], then g, rounded to the operands' type; two neighbouring columns per word.
           uint32_t w[16];
@@ -380,22 +400,61 @@ linear_loss_kernel(const __grid_constant__ CUtensorMap tmap_h, const __grid_cons
         }
       };
 
-      tmem_load_32x32b_x32(taddr, ra);
+      if constexpr (!kRuns) {
+        const uint32_t acc = iter & 1u;
+        if (!wait_for_sums(acc))
+          break;
+        const uint32_t taddr = lanes + acc * kTileN;
+        uint32_t ra[32], rb[32];
+        tmem_load_32x32b_x32(taddr, ra);
 #pragma unroll 1
-      for (int chunk = 0; chunk < kColumnsPerWarp / 32; chunk += 2) {
-        tmem_load_wait_for(ra);
-        tmem_load_32x32b_x32(taddr + (chunk + 1) * 32, rb);
-        finish(ra, chunk);
-        tmem_load_wait_for(rb);
-        if (chunk + 2 < kColumnsPerWarp / 32) {
-          tmem_load_32x32b_x32(taddr + (chunk + 2) * 32, ra);
-        } else {  // the accumulator has been read: back to the MMA issuer
-          tcgen05_fence_before_sync();
-          __syncwarp();
-          if (lane == 0)
-            mbar_arrive_cluster(map_to_cta(tmem_empty_bar(acc), 0));
+        for (int chunk = 0; chunk < kChunks; chunk += 2) {
+          tmem_load_wait_for(ra);
+          tmem_load_32x32b_x32(taddr + (chunk + 1) * 32, rb);
+          finish(ra, chunk);
+          tmem_load_wait_for(rb);
+          if (chunk + 2 < kChunks)
+            tmem_load_32x32b_x32(taddr + (chunk + 2) * 32, ra);
+          else
+            release(acc);
+          finish(rb, chunk + 1);
         }
-        finish(rb, chunk + 1);
+        ++iter;
+      } else {
+        uint32_t l[kChunks][32];  // the runs' sums, added in their order
+        for (int kb = 0; kb < num_kb; kb += kRunBlocks, ++iter) {
+          const uint32_t acc = iter & 1u;
+          ok = wait_for_sums(acc);
+          if (!ok)
+            break;
+          const uint32_t taddr = lanes + acc * kTileN;
+          if (kb == 0) {
+#pragma unroll
+            for (int chunk = 0; chunk < kChunks; ++chunk)
+              tmem_load_32x32b_x32(taddr + chunk * 32, l[chunk]);
+#pragma unroll
+            for (int chunk = 0; chunk < kChunks; ++chunk)
+              tmem_load_wait_for(l[chunk]);
+          } else {
+#pragma unroll
+            for (int half = 0; half < 2 * kChunks; ++half) {
+              uint32_t r[16];
+              tmem_load_32x32b_x16(taddr + half * 16, r);
+              tmem_load_wait_for(r);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                uint32_t &to = l[half / 2][half % 2 * 16 + j];
+                to = __float_as_uint(__uint_as_float(to) + __uint_as_float(r[j]));
+              }
+            }
+          }
+          release(acc);
+        }
+        if (!ok)
+          break;
+#pragma unroll
+        for (int chunk = 0; chunk < kChunks; ++chunk)
+          finish(l[chunk], chunk);
       }
       if (!kGrad && live)
         p.partials[static_cast<long long>(at.y * 2 + part) * p.rows + row] = make_float2(run.top, run.sum);
@@ -594,11 +653,12 @@ cudaError_t launch_linear_loss(const CUtensorMap &tmap_h, const CUtensorMap &tma
   if (err != cudaSuccess)
     return err;
   if (configured_device != device) {
-    err = cudaFuncSetAttribute(linear_loss_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
-    if (err == cudaSuccess)
-      err = cudaFuncSetAttribute(linear_loss_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
-    if (err != cudaSuccess)
-      return err;
+    for (const auto kernel : {linear_loss_kernel<false, false>, linear_loss_kernel<false, true>, linear_loss_kernel<true, false>,
+                              linear_loss_kernel<true, true>}) {
+      err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+      if (err != cudaSuccess)
+        return err;
+    }
     configured_device = device;
   }
   const int tiles_m = (p.rows + kTileM - 1) / kTileM, tiles_n = (p.vocab + kTileN - 1) / kTileN;
@@ -608,10 +668,10 @@ cudaError_t launch_linear_loss(const CUtensorMap &tmap_h, const CUtensorMap &tma
   const long long clusters = tiles < sm_count / 2 ? tiles : sm_count / 2;
   const uint32_t idesc = make_idesc_f16(p.c_dtype == kCTypeBF16 ? 1u : 0u, false, false, kTileM, kTileN);
   const unsigned grid = static_cast<unsigned>(2 * clusters);
-  if (grad)
-    linear_loss_kernel<true><<<grid, kThreads, kSmemBytes, stream>>>(tmap_h, tmap_w, p, idesc, tiles_m, tiles_n, 8, status);
-  else
-    linear_loss_kernel<false><<<grid, kThreads, kSmemBytes, stream>>>(tmap_h, tmap_w, p, idesc, tiles_m, tiles_n, 8, status);
+  const bool runs = p.width > kRunBlocks * kBlockK;
+  const auto kernel = grad ? (runs ? linear_loss_kernel<true, true> : linear_loss_kernel<true, false>)
+                           : (runs ? linear_loss_kernel<false, true> : linear_loss_kernel<false, false>);
+  kernel<<<grid, kThreads, kSmemBytes, stream>>>(tmap_h, tmap_w, p, idesc, tiles_m, tiles_n, 8, status);
   return cudaGetLastError();
 }
 

@@ -308,3 +308,24 @@ def test_rows_of_very_different_upstream_factors(dtype, piece, rows, vocab, widt
     assert (np.abs(dw.astype(np.float64) - exact.dw) <= exact.bounds(dtype)[1])[fits_w].all()
     if dtype == "float16":
         assert np.array_equal(dh[np.abs(exact.dh) > 7e4], np.copysign(np.inf, exact.dh[np.abs(exact.dh) > 7e4]))
+
+
+@pytest.mark.parametrize("width", [500, 1024, 1025, 2049, 4096, 9000, 20000])
+def test_long_sums_of_one_sign(width, gpu_ctx) -> None:
+    """Products that are all positive, so that whatever an addition cuts off is cut off every time. The tensor cores
+    add 1024 of the width (64 additions, and the 8 of the other tests' bound), these sums are added with rounding."""
+    rows, vocab = 64, 600
+    rng = np.random.default_rng(width)
+    h = (0.5 + 0.5 * rng.random((rows, width))).astype(np.float16)
+    w = ((0.5 + 0.5 * rng.random((vocab, width))) * (20 / (0.5625 * width))).astype(np.float16)
+    targets = rng.integers(0, vocab, rows)
+    dloss = (rng.standard_normal(rows) / rows).astype(np.float32)
+    loss, lse, dh, dw = run(gpu_ctx, h, w, targets, dloss)
+    exact = Exact(h, w, targets, dloss)
+    size = np.abs(exact.h) @ np.abs(exact.w).T
+    e_logit = (min(width, 1024) / 16 + 8 + width / 4096) * 2.0**-22 * size
+    own = 8 * U * (1 + np.abs(exact.lse))
+    exact.lse_bound = e_logit.max(axis=1) + (vocab / 256 + 64) * U + 2.0**-21 + own
+    exact.loss_bound = exact.lse_bound + e_logit[np.arange(rows), targets] + U * np.abs(exact.loss)
+    exact.p_rel = e_logit + (exact.lse_bound + 2.0**-20 + own)[:, None]
+    check("float16", exact, loss, lse, dh, dw)
