@@ -728,6 +728,8 @@ class Context:
         if h.ndim != 2 or w.ndim != 2 or h.shape[1] != w.shape[1] or h.dtype != w.dtype:
             raise ValueError(f"{call}() takes h (rows, width) and w (vocab, width) of one type, got {h.shape} of "
                              f"{h.dtype.name} and {w.shape} of {w.dtype.name}")
+        if not -(1 << 63) <= ignore_index < 1 << 63:
+            raise ValueError(f"{call}(): ignore_index must be a 64-bit integer, got {ignore_index}")
         return (h.shape[0], w.shape[0], h.shape[1], dtype_code(h.dtype), int(targets.dtype == _INT64), h.ptr, h.ld, w.ptr,
                 w.ld, _vector("targets", targets, h.shape[0], _INT64, _INT32), ignore_index)
 

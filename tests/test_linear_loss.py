@@ -128,3 +128,15 @@ def test_gradients_may_lie_at_any_address(address) -> None:
         status, info, message = backward(**change)
         assert status == OK and info.kernel_launches > 0, message
     assert backward(dw=address, dh=address)[0] == INVALID  # overlaps among the caller's own are still found
+
+
+def test_an_ignore_index_is_passed_on_as_it_is_or_refused() -> None:
+    """The C ABI takes 64 bits; a larger number would arrive as another, possibly a token's."""
+    h, w = cuda.DeviceBuffer.wrap(None, H, (4, 8), "bfloat16"), cuda.DeviceBuffer.wrap(None, W, (9, 8), "bfloat16")
+    targets = cuda.DeviceBuffer.wrap(None, T, (4,), "int64")
+    for index in (-100, 0, 8, -(1 << 63), (1 << 63) - 1):
+        args = cuda._LinearLossArgs(*cuda.Context._loss_call("linear_cross_entropy", h, w, targets, index), LOSS, LSE)
+        assert args.ignore_index == index
+    for index in ((1 << 64) + 5, 1 << 63, -(1 << 63) - 1):
+        with pytest.raises(ValueError, match="64-bit"):
+            cuda.Context._loss_call("linear_cross_entropy", h, w, targets, index)
