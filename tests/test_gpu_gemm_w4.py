@@ -204,3 +204,32 @@ def test_zero_points_beyond_fifteen(pad_q, group, dtype, gpu_ctx) -> None:
         got = run(gpu_ctx, a, q, scales, z, group, np.float32, pad_q=pad_q)
         check(got, a, q, scales, z, group)
         assert np.array_equal(got, run(gpu_ctx, a, q, scales, z + np.uint8(64 * (m % 4)), group, np.float32, pad_q=pad_q))
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("m, group, k", [(1, 128, 8192), (3, 64, 8192), (8, 64, 8192), (16, 32, 8192), (8, 128, 8191), (32, 64, 8192),
+                                         (64, 128, 8192)])
+def test_long_products_stay_right_in_every_column(m, group, k, dtype, gpu_ctx) -> None:
+    """Rings that are refilled some hundred times by every CTA: no stage is overwritten while its last words are being
+    read. The weights are one block of rows a hundred times over, so that the definition is computed once."""
+    block, copies = 1000, 100
+    a, q, scales, z = inputs(m, block, k, group, dtype, seed=11)
+    many = [empty(gpu_ctx, (block * copies, v.shape[1]), v.dtype) for v in (q, scales, z)]
+    for buf, v in zip(many, (q, scales, z)):
+        for i in range(copies):
+            buf.window(i * block, (i + 1) * block, 0, v.shape[1]).copy_from_host(v)
+    ba, c = make(gpu_ctx, a), empty(gpu_ctx, (m, block * copies), np.float32)
+    first = None
+    for _ in range(3):
+        c.fill_bytes(0xFF)
+        gpu_ctx.gemm_w4(ba, many[0], many[1], c, group=group, zeros=many[2])
+        gpu_ctx.synchronize()
+        got = c.to_numpy()
+        assert first is None or np.array_equal(got, first)
+        first = got
+    w = weights(q, scales, z, k, group)
+    a64 = a.astype(np.float64)
+    want, size = a64 @ w.T, np.abs(a64) @ np.abs(w).T
+    bound = HALF_STEP["float32"] * np.abs(want) + (k / 16 + scales.shape[1] + 64) * 2.0**-22 * size
+    # (A stage's last words taken from the next stage are off by 1e-4 to 1e-3 of the sum of sizes; the bound is 2e-4.)
+    assert (np.abs(got.reshape(m, copies, block) - want[:, None]) <= bound[:, None]).all()
