@@ -711,6 +711,7 @@ layer_norm_ring_kernel(const Forward f, const Ring ring, int *status) {
       for (int i = 0; i < kPairs; ++i)
         two = __fadd2_rn(two, v[u][i]);
     }
+    fence_proxy_async_smem();  // the slot has been read before a bulk copy, another proxy's write, refills it
     const float sum = two.x + two.y;
     const float mean = row_sum<false>(sum, sums[turn][0]) * inv;
     if (t == 0 && r + static_cast<long long>(ring.stages) * gridDim.x < f.rows)
@@ -940,6 +941,7 @@ layer_norm_backward_ring_kernel(const Backward g, const Ring ring, int *status) 
         }
       }
     }
+    fence_proxy_async_smem();  // this thread's reads of the stage come before its refill, after the next barrier
     before = stage;
     if (++stage == ring.stages) {
       stage = 0;

@@ -392,3 +392,49 @@ def test_constant_rows_of_huge_values(cols, dtype, gpu_ctx) -> None:
     assert (m == 2.0**110).all() and (np.abs(r - 2.0**20) <= 8 * U * 2.0**20).all()
     assert (np.abs(y.to_numpy().astype(np.float64) - b.astype(np.float64)) <= HALF_STEP[dtype] * np.abs(b)).all()
     check_backward(dtype, "float32", dy, x, w, m, r, dx.to_numpy(), dw.to_numpy(), db.to_numpy())
+
+
+@pytest.mark.parametrize("dtype, cols", [("bfloat16", 4096), ("float16", 1032), ("float32", 2048), ("bfloat16", 16384)])
+def test_a_row_gives_the_same_bits_wherever_it_stands(dtype, cols, gpu_ctx) -> None:
+    """The same rows many times over: rings that every CTA refills again and again, each row's y and dx as the first
+    time, and so in every run. (Rows on 16-byte boundaries: a row's sums do not depend on where it lies.)"""
+    block, copies = 96, (1 << 25) // (96 * cols)
+    x, dy, w, b = inputs(block, cols, dtype, "float32", 61)
+    t = np_dtype(dtype)
+    big = [empty(gpu_ctx, (block * copies, cols), t) for _ in range(4)]
+    for buf, v in zip(big, (x, dy)):
+        for i in range(copies):
+            buf.window(i * block, (i + 1) * block, 0, cols).copy_from_host(v)
+    bx, bdy, by, bdx = big
+    bw, bb = make(gpu_ctx, w), make(gpu_ctx, b)
+    mean, rstd = (empty(gpu_ctx, (block * copies,), np.float32) for _ in range(2))
+    dw, db = (empty(gpu_ctx, (cols,), np.float32) for _ in range(2))
+    sums = None
+    for _ in range(3):
+        for buf in (by, bdx, mean, rstd, dw, db):
+            buf.fill_bytes(0xFF)
+        gpu_ctx.layer_norm(bx, by, weight=bw, bias=bb, eps=EPS, mean=mean, rstd=rstd)
+        gpu_ctx.layer_norm_backward(bdy, bx, bdx, mean=mean, rstd=rstd, weight=bw, dweight=dw, dbias=db)
+        gpu_ctx.synchronize()
+        y, dx = (buf.to_numpy().reshape(copies, block, cols) for buf in (by, bdx))
+        assert (y == y[0]).all() and (dx == dx[0]).all()
+        again = dw.to_numpy(), db.to_numpy()
+        assert sums is None or all(np.array_equal(p, q) for p, q in zip(sums, again))
+        sums = again
+    m, r = mean.to_numpy()[:block], rstd.to_numpy()[:block]
+    check_forward(dtype, x, w, b, y[0], m, r)
+    check_backward(dtype, "float32", dy, x, w, m, r, dx[0], None, None)
+
+
+@pytest.mark.parametrize("rows, cols, pad", [(1200, 4096, 0), (1200, 4095, 0), (700, 8200, 0), (900, 5001, 3)])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_many_rows_in_place(dtype, rows, cols, pad, gpu_ctx) -> None:
+    """y written over x, and dx over x and over dy, where rows are read some rows ahead."""
+    x, dy, w, b = inputs(rows, cols, dtype, "float32", 62)
+    apart = run_forward(gpu_ctx, x, w, b, pad)
+    for p, q in zip(apart, run_forward(gpu_ctx, x, w, b, pad, in_place=True)):
+        assert np.array_equal(p, q)
+    grads = run_backward(gpu_ctx, dy, x, w, apart[1], apart[2], pad)
+    for which in ("x", "dy"):
+        for p, q in zip(grads, run_backward(gpu_ctx, dy, x, w, apart[1], apart[2], pad, in_place=which)):
+            assert np.array_equal(p, q)
