@@ -236,6 +236,21 @@ __device__ __forceinline__ int owner_of(const W4 &p, int unit) {
   return unit < long_ones ? unit / (p.share + 1) : p.extra + (unit - long_ones) / p.share;
 }
 
+// Index checks of the checked build: a unit a CTA is about to load, and a block whose parts lie in first .. last.
+__device__ __forceinline__ bool unit_ok(const W4 &p, uint32_t stage, int stages, int block, int ks, int *status,
+                                        volatile uint32_t *abort_flag) {
+  return HC_CHECK(status, abort_flag, HC_CHECK_RING_STAGE, stage < static_cast<uint32_t>(stages)) &&
+         HC_CHECK(status, abort_flag, HC_CHECK_TILE_COORDINATES,
+                  block >= 0 && static_cast<long long>(block) * kRows < p.n && ks >= 0 && ks < p.stages_k) &&
+         HC_CHECK(status, abort_flag, HC_CHECK_TMA_COORDINATES, ks * 128 < p.row_bytes);
+}
+__device__ __forceinline__ bool parts_ok(const W4 &p, int cta, int first, int last, int block, int *status,
+                                         volatile uint32_t *abort_flag) {
+  return HC_CHECK(status, abort_flag, HC_CHECK_PARTIAL_SLOT,
+                  first >= 0 && first <= cta && cta <= last && last < p.grid && block >= 0 &&
+                      first_unit(p, first) < (block + 1) * p.stages_k && first_unit(p, last + 1) >= (block + 1) * p.stages_k);
+}
+
 // A CTA that did part of a row block leaves its sums in a slot of its own: its first if the block is the first
 // it touches, else its second. Of the CTAs `first` .. that share a block only `first` may have begun before it.
 __device__ __forceinline__ float *part_slot(const W4 &p, int cta, int first, int block, int slot_floats) {
@@ -496,7 +511,7 @@ gemm_w4_few_kernel(const __grid_constant__ QMaps<kPhase> maps_q, const __grid_co
     int block = unit_begin / stages_k, ks = unit_begin - block * stages_k;
     for (int unit = unit_begin; unit < unit_end; ++unit) {
       const bool free = mbar_wait_asleep(empty_bar(stage), phase ^ 1u, abort_flag);
-      if (!__all_sync(0xffffffffu, free))
+      if (!__all_sync(0xffffffffu, free) || !unit_ok(p, stage, S::kStages, block, ks, status, abort_flag))
         break;
       const uint32_t at = smem_base + stage * S::kStageBytes;
       if (lane == 0) {
@@ -642,6 +657,8 @@ gemm_w4_few_kernel(const __grid_constant__ QMaps<kPhase> maps_q, const __grid_co
       if (ks_begin != 0 || ks_end != stages_k) {
         constexpr int kSlot = kRows * S::kTokens;
         const int first = owner_of(p, block * stages_k), last = owner_of(p, (block + 1) * stages_k - 1);
+        if (!parts_ok(p, cta, first, last, block, status, abort_flag))
+          break;  // (the same for all consumers)
         float *mine = part_slot(p, cta, first, block, kSlot);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -824,7 +841,7 @@ gemm_w4_kernel(const __grid_constant__ QMaps<kPhase> maps_q, const __grid_consta
     int block = unit_begin / stages_k, ks = unit_begin - block * stages_k;
     for (int unit = unit_begin; unit < unit_end; ++unit) {
       const bool free = mbar_wait_asleep(empty_bar(stage), phase ^ 1u, abort_flag);
-      if (!__all_sync(0xffffffffu, free))
+      if (!__all_sync(0xffffffffu, free) || !unit_ok(p, stage, S::kStages, block, ks, status, abort_flag))
         break;
       const uint32_t q_dst = smem_base + stage * S::kStageBytes, a_dst = q_dst + S::kQStageBytes;
       if (lane == 0) {
@@ -1072,6 +1089,8 @@ gemm_w4_kernel(const __grid_constant__ QMaps<kPhase> maps_q, const __grid_consta
       } else {
         first = owner_of(p, block * stages_k);
         last = owner_of(p, (block + 1) * stages_k - 1);
+        if (!parts_ok(p, cta, first, last, block, status, abort_flag))
+          break;  // (the same for all collectors)
         float *const mine = part_slot(p, cta, first, block, kSlot) + local;
 #pragma unroll
         for (int t = 0; t < kTokens; ++t)

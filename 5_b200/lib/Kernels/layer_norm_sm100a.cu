@@ -27,6 +27,7 @@
 // 8192 float32 49.4 us (5.3 TB/s) and 91 us (4.3 TB/s). What holds the 16-bit ones back is no longer memory
 // but arithmetic and its latency (0.6 instructions a cycle and scheduler with four warps, the registers being
 // full), which is why the sums and the scaling work on pairs of floats in one instruction.
+#include "device_checks.cuh"
 #include "gemm_launch.h"
 #include "sm100_ptx.cuh"
 
@@ -674,6 +675,9 @@ layer_norm_ring_kernel(const Forward f, const Ring ring, int *status) {
   // Rows blockIdx.x, blockIdx.x + gridDim.x, ...: all of one place, since the grid is a multiple of ring.step.
   auto load = [&](long long row, int stage) {
     const RowCopy copy(x, row, f.ldx, f.cols, f.rows, sizeof(T));
+    if (!HC_CHECK(status, abort_flag, HC_CHECK_RING_STAGE, stage >= 0 && stage < ring.stages && copy.bytes <= ring.slot) ||
+        !HC_CHECK(status, abort_flag, HC_CHECK_TILE_COORDINATES, row >= 0 && row < f.rows))
+      return;
     if (kShift && row == f.rows - 1)
       store_rest(copy, x + row * f.ldx, f.cols, shared + 128 + stage * ring.slot);
     mbar_arrive_expect_tx(bars + 8u * stage, copy.bytes);
@@ -796,6 +800,13 @@ layer_norm_backward_ring_kernel(const Backward g, const Ring ring, int *status) 
   auto load = [&](long long tile, int stage) {
     const int live = live_of(tile);
     uint32_t total = 0;
+    if (!HC_CHECK(status, abort_flag, HC_CHECK_RING_STAGE, stage >= 0 && stage < ring.stages) ||
+        !HC_CHECK(status, abort_flag, HC_CHECK_TILE_COORDINATES,
+                  tile >= 0 && tile < tiles && live >= 1 && live <= rows && row_of(tile, live - 1) < g.rows) ||
+        !HC_CHECK(status, abort_flag, HC_CHECK_TMA_COORDINATES,
+                  RowCopy(x, row_of(tile, 0), g.ldx, g.cols, g.rows, sizeof(T)).bytes <= ring.slot &&
+                      RowCopy(dy, row_of(tile, 0), g.lddy, g.cols, g.rows, sizeof(T)).bytes <= ring.slot))
+      return;
     if (kShift && row_of(tile, live - 1) == g.rows - 1) {
       uint8_t *const at = shared + 128 + stage * stage_bytes + 2u * (live - 1) * ring.slot;
       store_rest(RowCopy(x, g.rows - 1, g.ldx, g.cols, g.rows, sizeof(T)), x + (g.rows - 1) * g.ldx, g.cols, at);

@@ -218,7 +218,8 @@ linear_loss_kernel(const __grid_constant__ CUtensorMap tmap_h, const __grid_cons
                       at.x >= 0 && at.x < tiles_m && at.y >= 0 && at.y < tiles_n))
           break;
         for (int kb = 0; kb < num_kb; ++kb) {
-          if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag)) {
+          if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag) ||
+              !HC_CHECK(status, abort_flag, HC_CHECK_RING_STAGE, stage < static_cast<uint32_t>(kStages))) {
             ok = false;
             break;
           }
@@ -293,6 +294,9 @@ linear_loss_kernel(const __grid_constant__ CUtensorMap tmap_h, const __grid_cons
       const int row = at.x * kTileM + static_cast<int>(cta_rank) * kCtaRows + quarter * 32 + lane;
       const int col_base = at.y * kTileN + part * kColumnsPerWarp;
       const bool live = row < p.rows;
+      if (!HC_CHECK(status, abort_flag, HC_CHECK_OUTPUT_RANGE,
+                    row >= lane && row - lane < tiles_m * kTileM && col_base >= 0 && col_base < tiles_n * kTileN))  // (per warp)
+        break;
       // What the row needs is fetched while its products are still running.
       long long target = -1;
       float scale = 0.0f, lse2 = 0.0f;
