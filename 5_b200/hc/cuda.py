@@ -712,7 +712,8 @@ class Context:
         """Enqueues the gradients of sum(loss * dloss) (asynchronous): `dh` and `dw`, shaped and typed like `h` and
         `w`, each optional and overwritten. `lse` is what `linear_cross_entropy` stored, `dloss` a float32
         vector. Rows that `linear_cross_entropy` leaves out have no gradient. The logits are computed
-        again, a piece of the vocabulary at a time."""
+        again, a piece of the vocabulary at a time; their gradient is rounded to the type of `h` and `w`
+        for the two products."""
         for name, grad, like in (("dh", dh, h), ("dw", dw, w)):
             if grad is not None and (grad.shape != like.shape or grad.dtype != like.dtype):
                 raise ValueError(f"{name} must have the shape and type of {name[1:]}")

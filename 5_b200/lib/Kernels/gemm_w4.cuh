@@ -11,7 +11,8 @@
 // instructions per 8 weights leave little room for anything else.
 //
 // The weights enter the product as integers: a nibble becomes a float by being put under the exponent of 1024
-// (128 for bfloat16), and one subtraction of 1024 + z, exact, serves two of them. The group's scale
+// (128 for bfloat16), and one subtraction of 1024 + z, exact, serves two of them (Kim, Henry, Fahim, Hassan Awadalla,
+// "Who Says Elephants Can't Run", 2022, describe it for weights of 8 and 4 bits). The group's scale
 // multiplies the float32 sums of the group. So nothing is lost to a 16-bit product of scale and weight: the
 // only roundings are those of float32 sums and of the result.
 //
@@ -992,7 +993,6 @@ gemm_w4_kernel(const __grid_constant__ QMaps<kPhase> maps_q, const __grid_consta
     const int local = row_at_position<kPhase>(warp * 32 + lane);  // this lane's row of the block, i.e. column of C
     const uint32_t sums = tmem_base + (static_cast<uint32_t>(warp * 32) << 16) + S::kSumsAt;
     constexpr int kGroups = kStageK / kGroup;  // of a stage: 2, 4 or 8
-    constexpr int kChunk = kTokens < 32 ? kTokens : 32;
     uint32_t stage = 0, step = 0;
     bool ok = true;  // (a wait that ran out: the barriers below are still met)
     int unit = unit_begin;
@@ -1051,12 +1051,12 @@ gemm_w4_kernel(const __grid_constant__ QMaps<kPhase> maps_q, const __grid_consta
                   static_cast<uint16_t>(group % 2 == 0 ? now[group / 2] & 0xffffu : now[group / 2] >> 16));
               const uint32_t at = sums + ((set * S::kSlots + slot) * S::kAccs + j) * kTokens;
 #pragma unroll
-              for (int t0 = 0; t0 < kTokens; t0 += kChunk) {
-                uint32_t r[kChunk];
+              for (int t0 = 0; t0 < kTokens; t0 += 32) {
+                uint32_t r[32];
                 tmem_load_32x32b_x32(at + t0, r);
                 tmem_load_wait_for(r);
 #pragma unroll
-                for (int t = 0; t < kChunk; ++t)
+                for (int t = 0; t < 32; ++t)
                   total[t0 + t] = fmaf(scale, __uint_as_float(r[t]), total[t0 + t]);
               }
             }

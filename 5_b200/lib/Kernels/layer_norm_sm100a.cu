@@ -494,8 +494,9 @@ layer_norm_columns_kernel(const Backward g) {
 
 // out[c] = sum over the partial rows, in their order within each of kChains interleaved chains that are then added.
 // A warp reads 32 neighbouring columns of a partial row. With 32 chains a column's sum is soon there but an SM holds
-// two CTAs only; with 8 all CTAs of wide rows run at once (backward of 1025 x 16384 float16: 49.9 us, with 32
-// chains 53.4 us; 16384 x 1024 bfloat16: 46.9 and 42.9 us).
+// two CTAs only; with 8 all CTAs of wide rows run at once. Backward passes with 8 and 32 chains: 16384 x 1024 bfloat16
+// 46.5 and 42.6 us, x 2048 67.5 and 65.9, x 4096 120.9 and 121.0; 4000 x 6144 float16 61.6 and 61.7, x 8192 69.7 and
+// 71.0; 2000 x 12288 67.8 and 69.9, 1025 x 16384 49.8 and 53.4: 8 from 8192 columns on.
 template <typename P, int kChains>
 __global__ void __launch_bounds__(32 * kChains)
 layer_norm_partials_kernel(const float *partials, int count, long long cols, P *dweight, P *dbias) {
