@@ -233,3 +233,29 @@ def test_long_products_stay_right_in_every_column(m, group, k, dtype, gpu_ctx) -
     bound = HALF_STEP["float32"] * np.abs(want) + (k / 16 + scales.shape[1] + 64) * 2.0**-22 * size
     # (A stage's last words taken from the next stage are off by 1e-4 to 1e-3 of the sum of sizes; the bound is 2e-4.)
     assert (np.abs(got.reshape(m, copies, block) - want[:, None]) <= bound[:, None]).all()
+
+
+@pytest.mark.parametrize("dtype, out", [("float16", "float16"), ("bfloat16", "float32")])
+@pytest.mark.parametrize("m", [1, 7, 16, 40])
+def test_everything_at_odd_places(m, dtype, out, gpu_ctx) -> None:
+    """All matrices as windows that begin inside a row of a larger buffer, whose other columns stay as they are."""
+    n, k, group = 261, 1100, 64
+    a, q, scales, z = inputs(m, n, k, group, dtype, seed=12)
+    whole_buffers = []  # (a window does not keep the buffer it lies in)
+
+    def window(values, left, pad):
+        host = np.zeros((values.shape[0], left + values.shape[1] + pad), values.dtype)
+        host.view(np.uint8)[:] = 0x5A
+        host[:, left:left + values.shape[1]] = values
+        whole_buffers.append(make(gpu_ctx, host))
+        return whole_buffers[-1].window(0, values.shape[0], left, left + values.shape[1])
+
+    guard = empty(gpu_ctx, (m, n + 5), np_dtype(out))
+    guard.fill_bytes(0x5A)
+    parts = [window(v, left, pad) for v, left, pad in ((a, 3, 2), (q, 5, 1), (scales, 1, 1), (z, 3, 4))]
+    gpu_ctx.gemm_w4(parts[0], parts[1], parts[2], guard.window(0, m, 3, n + 3), group=group, zeros=parts[3])
+    gpu_ctx.synchronize()
+    whole = guard.to_numpy()
+    check(np.ascontiguousarray(whole[:, 3:n + 3]), a, q, scales, z, group)
+    for beside in (whole[:, :3], whole[:, n + 3:]):
+        assert (np.ascontiguousarray(beside).view(np.uint8) == 0x5A).all()

@@ -329,3 +329,32 @@ def test_long_sums_of_one_sign(width, gpu_ctx) -> None:
     exact.loss_bound = exact.lse_bound + e_logit[np.arange(rows), targets] + U * np.abs(exact.loss)
     exact.p_rel = e_logit + (exact.lse_bound + 2.0**-20 + own)[:, None]
     check("float16", exact, loss, lse, dh, dw)
+
+
+@pytest.mark.parametrize("rows, vocab, width", [(70, 600, 96), (300, 2051, 129), (5, 300, 64)])
+@pytest.mark.parametrize("left", [1, 4, 8])
+def test_windows_of_larger_matrices(left, rows, vocab, width, gpu_ctx) -> None:
+    """h, w and both gradients inside rows of larger buffers, whose other columns stay as they are."""
+    for dtype in ("bfloat16", "float16"):
+        h, w, targets, dloss = inputs(rows, vocab, width, dtype, 14)
+
+        def window(values, fill=0x5A):
+            host = np.zeros((values.shape[0], left + width + 3), values.dtype)
+            host.view(np.uint8)[:] = fill
+            host[:, left:left + width] = values
+            buf = make(gpu_ctx, host)
+            return buf, buf.window(0, values.shape[0], left, left + width)
+
+        (bh, vh), (bw, vw), (gh, dh), (gw, dw) = window(h), window(w), window(h), window(w)
+        bt, bd = make(gpu_ctx, targets), make(gpu_ctx, dloss)
+        loss, lse = empty(gpu_ctx, (rows,), np.float32), empty(gpu_ctx, (rows,), np.float32)
+        gpu_ctx.linear_cross_entropy(vh, vw, bt, loss, lse)
+        gpu_ctx.linear_cross_entropy_backward(vh, vw, bt, lse, bd, dh=dh, dw=dw)
+        gpu_ctx.synchronize()
+        got = [buf.to_numpy() for buf in (gh, gw)]
+        assert bh.ptr and bw.ptr  # (a window does not keep the buffer it lies in)
+        check(dtype, Exact(h, w, targets, dloss), loss.to_numpy(), lse.to_numpy(),
+              *(np.ascontiguousarray(v[:, left:left + width]) for v in got))
+        for v in got:
+            for beside in (v[:, :left], v[:, left + width:]):
+                assert (np.ascontiguousarray(beside).view(np.uint8) == 0x5A).all()

@@ -438,3 +438,34 @@ def test_many_rows_in_place(dtype, rows, cols, pad, gpu_ctx) -> None:
     for which in ("x", "dy"):
         for p, q in zip(grads, run_backward(gpu_ctx, dy, x, w, apart[1], apart[2], pad, in_place=which)):
             assert np.array_equal(p, q)
+
+
+@pytest.mark.parametrize("rows, cols", [(5, 64), (300, 1000), (700, 4096), (700, 4095)])
+@pytest.mark.parametrize("param", ["bfloat16", "float32"])
+def test_vectors_at_any_address(param, rows, cols, gpu_ctx) -> None:
+    """Weight, bias, their gradients and the statistics at addresses that are multiples of their element alone."""
+    x, dy, w, b = inputs(rows, cols, "bfloat16", param, 71)
+    keep = []
+
+    def odd(values, length, dtype):
+        dtype = np.dtype(dtype)
+        raw = empty(gpu_ctx, (length + 2,), dtype)
+        keep.append(raw)
+        if values is not None:
+            raw.copy_from_host(np.concatenate([np.full(1, np.nan, dtype), values, np.full(1, np.nan, dtype)]))
+        return raw, cuda.DeviceBuffer.wrap(gpu_ctx, raw.ptr + dtype.itemsize, (length,), dtype)
+
+    (_, vw), (_, vb) = odd(w, cols, w.dtype), odd(b, cols, b.dtype)
+    outs = [odd(None, rows, np.float32), odd(None, rows, np.float32), odd(None, cols, w.dtype), odd(None, cols, w.dtype)]
+    (_, mean), (_, rstd), (_, dw), (_, db) = outs
+    bx, bdy = make(gpu_ctx, x), make(gpu_ctx, dy)
+    y, dx = empty(gpu_ctx, x.shape, x.dtype), empty(gpu_ctx, x.shape, x.dtype)
+    gpu_ctx.layer_norm(bx, y, weight=vw, bias=vb, eps=EPS, mean=mean, rstd=rstd)
+    gpu_ctx.layer_norm_backward(bdy, bx, dx, mean=mean, rstd=rstd, weight=vw, dweight=dw, dbias=db)
+    gpu_ctx.synchronize()
+    got = [raw.to_numpy() for raw, _ in outs]
+    for v in got:  # nothing beside a vector is written
+        assert (v[[0, -1]].view(np.uint8) == 0xFF).all()
+    m, r, gw, gb = (v[1:-1] for v in got)
+    check_forward("bfloat16", x, w, b, y.to_numpy(), m, r)
+    check_backward("bfloat16", param, dy, x, w, m, r, dx.to_numpy(), gw, gb)
