@@ -675,12 +675,14 @@ int enqueue_gemm(HcCudaContext *ctx, const HcCudaGemmArgs *args, const HcCudaGem
                           : encode_map(ctx, &tmap_b, args->dtype, b, n, k, static_cast<uint64_t>(ldb) * 2, 64,
                                        t.block_k))
       return rc;
-    // C leaves through TMA stores when its rows start on 16-byte boundaries (the launcher falls
-    // back to ordinary stores for fused work and push targets).
+    // C leaves through TMA stores when its rows start on 16-byte boundaries and consist of whole 32-bit words: of a
+    // 16-bit row that ends inside a word TMA stores all of the word, the element behind the row with it. (The launcher
+    // falls back to ordinary stores for fused work and push targets.)
     CUtensorMap tmap_c;
     const CUtensorMap *c_map = nullptr;
     const bool c_rows_aligned = (static_cast<size_t>(args->ldc) * c_elem) % 16 == 0 &&
-                                (reinterpret_cast<uintptr_t>(args->c) & 15) == 0;
+                                (reinterpret_cast<uintptr_t>(args->c) & 15) == 0 &&
+                                (static_cast<size_t>(n) * c_elem) % 4 == 0;
     if (c_rows_aligned && ctx->c_tma_store) {
       // float32: 32 x 32 boxes; 16-bit: 64 columns x 32 rows (128-byte rows either way).
       const int map_type = args->c_dtype == HC_CUDA_C_F32 ? kMapFloat32
@@ -2258,8 +2260,9 @@ struct LossBackwardPlan {
   int64_t g = 0, gt = 0, ldg = 0, ldgt = 0;
   int64_t dh_sums = -1;  // float32 sums of dh without the rows' dloss (g_plain), rounded at the end; -1: dh is written at once
   int64_t sums_ld = 0;
-  // 16-bit, where dw's rows do not all start on 16-byte boundaries: the product stores to it by TMA and a copy
-  // follows (16411 x 1001 x 1031: 41 and 12 us; 70 us when the product writes such rows itself).
+  // 16-bit, where dw's rows do not all start on 16-byte boundaries or end inside a 32-bit word: the product, of an even
+  // width, stores to it by TMA and a copy follows (16411 x 1001 x 1031: 41 and 12 us; 70 us when the product writes
+  // such rows itself).
   int64_t dw_copy = -1;
   int64_t dw_ld = 0;
   int64_t scales = 0;
@@ -2314,6 +2317,7 @@ HcCudaGemmArgs loss_dw_product(const LossCall &c, const LossBackwardPlan &plan, 
   g.ldb = c.ldh;
   g.b_layout = HC_CUDA_B_KN;
   if (plan.dw_copy >= 0) {
+    g.n = round_up(c.width, 2);  // (the copy of h, like this one, has a longer pitch; the column more is not copied)
     g.c = base + plan.dw_copy;
     g.ldc = plan.dw_ld;
   } else {
@@ -2371,7 +2375,7 @@ int plan_linear_loss_backward(const HcCudaContext *ctx, const HcCudaLinearLossBa
   plan->gt = plan->work.take(args->dw != nullptr ? columns * plan->ldgt * 2 : 0);
   plan->sums_ld = round_up(c.width, 4);
   plan->scales = plan->work.take(8);
-  if (args->dw != nullptr && needs_repack(args->dw, args->lddw)) {
+  if (args->dw != nullptr && (needs_repack(args->dw, args->lddw) || c.width % 2 != 0)) {
     plan->dw_ld = round_up(c.width, kRepackPitchBytes / 2);
     plan->dw_copy = plan->work.take(columns * plan->dw_ld * 2);
   }

@@ -358,3 +358,22 @@ def test_windows_of_larger_matrices(left, rows, vocab, width, gpu_ctx) -> None:
         for v in got:
             for beside in (v[:, :left], v[:, left + width:]):
                 assert (np.ascontiguousarray(beside).view(np.uint8) == 0x5A).all()
+
+
+@pytest.mark.parametrize("rows, vocab, width", [(1, 37, 7), (70, 600, 95), (300, 2051, 129), (700, 300, 1001), (640, 2500, 513)])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_odd_widths_in_rows_of_whole_pieces(dtype, rows, vocab, width, gpu_ctx) -> None:
+    """Rows that start on 16-byte boundaries and end inside a 32-bit word: the elements behind them stay."""
+    h, w, targets, dloss = inputs(rows, vocab, width, dtype, 15)
+    ld = (width + 7) // 8 * 8
+    bh, bw, bt, bd = make(gpu_ctx, h, ld), make(gpu_ctx, w, ld), make(gpu_ctx, targets), make(gpu_ctx, dloss)
+    gh, gw = empty(gpu_ctx, (rows, ld), h.dtype), empty(gpu_ctx, (vocab, ld), h.dtype)
+    loss, lse = empty(gpu_ctx, (rows,), np.float32), empty(gpu_ctx, (rows,), np.float32)
+    gpu_ctx.linear_cross_entropy(bh, bw, bt, loss, lse)
+    gpu_ctx.linear_cross_entropy_backward(bh, bw, bt, lse, bd, dh=gh.window(0, rows, 0, width), dw=gw.window(0, vocab, 0, width))
+    gpu_ctx.synchronize()
+    dh, dw = gh.to_numpy(), gw.to_numpy()
+    for out in (dh, dw):
+        assert (np.ascontiguousarray(out[:, width:]).view(np.uint8) == 0xFF).all()
+    check(dtype, Exact(h, w, targets, dloss), loss.to_numpy(), lse.to_numpy(), np.ascontiguousarray(dh[:, :width]),
+          np.ascontiguousarray(dw[:, :width]))
