@@ -179,10 +179,19 @@ bool ranges_overlap(const void *p, size_t pbytes, const void *q, size_t qbytes) 
 
 // Validation + variant choice shared by hcCudaGemmPlan, hcCudaGemm and hcCudaGemmHost.
 // `host_buffers`: the pointers are host memory that will be staged with aligned pitches, so
-// no repack is ever needed. `apart`: the caller has made sure that c overlaps neither operand (its pointers may be
-// stand-ins that only have the alignment of the ones to come).
+// no repack is ever needed. `known`: what the caller answers for.
+constexpr int kCApart = 1;    // c overlaps neither operand (pointers may be stand-ins with the alignment of the ones to come)
+constexpr int kCPadding = 2;  // c is the library's own, and its rows may be written up to the next 16-byte boundary
+
+// Whether TMA may store C: its rows start on 16-byte boundaries and consist of whole 16-byte pieces. (Of a row that ends
+// inside a piece a TMA store writes all of the piece, what lies behind the row with it.)
+bool c_takes_tma(const HcCudaGemmArgs *args, size_t c_elem, int known) {
+  return (static_cast<size_t>(args->ldc) * c_elem) % 16 == 0 && (reinterpret_cast<uintptr_t>(args->c) & 15) == 0 &&
+         ((static_cast<size_t>(args->n) * c_elem) % 16 == 0 || (known & kCPadding) != 0);
+}
+
 int plan_gemm(const HcCudaContext *ctx, const HcCudaGemmArgs *args, int sm_count, bool host_buffers,
-              HcCudaGemmPlanInfo *plan, bool apart = false) {
+              HcCudaGemmPlanInfo *plan, int known = 0) {
   if (args == nullptr || plan == nullptr)
     return fail(ctx, HC_CUDA_ERR_INVALID_ARGUMENT, "args and plan must not be null");
   std::memset(plan, 0, sizeof(*plan));
@@ -268,8 +277,8 @@ int plan_gemm(const HcCudaContext *ctx, const HcCudaGemmArgs *args, int sm_count
     return fail(ctx, HC_CUDA_ERR_INVALID_ARGUMENT, "a and b must be aligned to their element size");
   const size_t a_bytes = (static_cast<size_t>(m - 1) * args->lda + k) * es;
   const size_t b_bytes = (static_cast<size_t>(b_rows - 1) * args->ldb + b_cols) * es;
-  if (!apart && (ranges_overlap(args->c, c_bytes, args->a, a_bytes) ||
-                 ranges_overlap(args->c, c_bytes, args->b, b_bytes)))
+  if ((known & kCApart) == 0 && (ranges_overlap(args->c, c_bytes, args->a, a_bytes) ||
+                                 ranges_overlap(args->c, c_bytes, args->b, b_bytes)))
     return fail(ctx, HC_CUDA_ERR_INVALID_ARGUMENT, "c must not overlap a or b");
 
   int variant = args->variant;
@@ -303,7 +312,7 @@ int plan_gemm(const HcCudaContext *ctx, const HcCudaGemmArgs *args, int sm_count
     // 8192 x 8192: m = 64: 30.7 against 39.0 us, m = 32: 28.7 against 32.9; 64 x 2048 x 16384: 18.5
     // against 38.9; m = 8: no difference).
     if (variant == HC_CUDA_GEMM_SKINNY && m > 8 && !host_buffers && args->c_dtype == HC_CUDA_C_F32 &&
-        (static_cast<size_t>(args->ldc) * c_elem) % 16 == 0 && (reinterpret_cast<uintptr_t>(args->c) & 15) == 0 &&
+        c_takes_tma(args, c_elem, known) &&
         (ctx == nullptr || (ctx->c_tma_store && !ctx->planning_push && !ctx->planning_host_panels)) &&
         std::getenv("HC_CUDA_DENSE_SPLITS") == nullptr && std::getenv("HC_CUDA_SKINNY_SPLITS") == nullptr &&
         hc::sm100::skinny_choose_splits(static_cast<int>(n), static_cast<int>((k * es + 1) / 2), sm_count) > 1) {
@@ -341,8 +350,7 @@ int plan_gemm(const HcCudaContext *ctx, const HcCudaGemmArgs *args, int sm_count
     // 512x256 tiles for products that fill the GPU with them, when the epilogue never has to read C
     // with ordinary loads (an accumulation must be one the TMA stores can perform) and the tiles go
     // nowhere but C. Decided again below if tiles turn out to be split over k.
-    const bool c_tma_ok = (static_cast<size_t>(args->ldc) * c_elem) % 16 == 0 &&
-                          (reinterpret_cast<uintptr_t>(args->c) & 15) == 0 && (ctx == nullptr || ctx->c_tma_store);
+    const bool c_tma_ok = c_takes_tma(args, c_elem, known) && (ctx == nullptr || ctx->c_tma_store);
     bool wide = pairs && hc::sm100::dense_uses_wide(m, n, k, sm_count) &&
                 (args->accumulate == 0 || (c_tma_ok && args->epilogue_count == 0)) &&
                 !(ctx != nullptr && ctx->planning_push);
@@ -559,7 +567,8 @@ int encode_map(HcCudaContext *ctx, CUtensorMap *map, int dtype, const void *base
 // Enqueues the GEMM on device-resident buffers. The caller holds ctx->mu and has made the
 // context's device current.
 int enqueue_gemm(HcCudaContext *ctx, const HcCudaGemmArgs *args, const HcCudaGemmPlanInfo &plan,
-                 const hc::sm100::Epilogue &push = hc::sm100::Epilogue{}, const float *device_factor = nullptr) {
+                 const hc::sm100::Epilogue &push = hc::sm100::Epilogue{}, const float *device_factor = nullptr,
+                 int known = 0) {
   if (plan.variant == HC_CUDA_GEMM_NOOP)
     return HC_CUDA_OK;
   if (device_factor != nullptr && (plan.variant != HC_CUDA_GEMM_DENSE || plan.cluster_size > 1))
@@ -675,15 +684,11 @@ int enqueue_gemm(HcCudaContext *ctx, const HcCudaGemmArgs *args, const HcCudaGem
                           : encode_map(ctx, &tmap_b, args->dtype, b, n, k, static_cast<uint64_t>(ldb) * 2, 64,
                                        t.block_k))
       return rc;
-    // C leaves through TMA stores when its rows start on 16-byte boundaries and consist of whole 32-bit words: of a
-    // 16-bit row that ends inside a word TMA stores all of the word, the element behind the row with it. (The launcher
-    // falls back to ordinary stores for fused work and push targets.)
+    // C leaves through TMA stores when they can address its rows (the launcher falls back to ordinary stores for fused
+    // work and push targets).
     CUtensorMap tmap_c;
     const CUtensorMap *c_map = nullptr;
-    const bool c_rows_aligned = (static_cast<size_t>(args->ldc) * c_elem) % 16 == 0 &&
-                                (reinterpret_cast<uintptr_t>(args->c) & 15) == 0 &&
-                                (static_cast<size_t>(n) * c_elem) % 4 == 0;
-    if (c_rows_aligned && ctx->c_tma_store) {
+    if (c_takes_tma(args, c_elem, known) && ctx->c_tma_store) {
       // float32: 32 x 32 boxes; 16-bit: 64 columns x 32 rows (128-byte rows either way).
       const int map_type = args->c_dtype == HC_CUDA_C_F32 ? kMapFloat32
                            : args->c_dtype == HC_CUDA_C_BF16 ? HC_CUDA_BF16 : HC_CUDA_F16;
@@ -1222,7 +1227,7 @@ int hcCudaGemmHost(HcCudaContext *ctx, const HcCudaGemmArgs *args) {
     return fail(ctx, HC_CUDA_ERR_INVALID_ARGUMENT, "ctx must not be null");
   std::lock_guard<std::mutex> lock(ctx->mu);
   HcCudaGemmPlanInfo plan;
-  if (int rc = plan_gemm(ctx, args, ctx->prop.multiProcessorCount, true, &plan))
+  if (int rc = plan_gemm(ctx, args, ctx->prop.multiProcessorCount, true, &plan, kCPadding))
     return rc;
   if (plan.variant == HC_CUDA_GEMM_NOOP)
     return HC_CUDA_OK;
@@ -1273,9 +1278,9 @@ int hcCudaGemmHost(HcCudaContext *ctx, const HcCudaGemmArgs *args) {
     if (args->accumulate)
       HC_TRY_CUDA(ctx, cudaMemcpy2DAsync(dev_c, ldc * ce, host_c, host_c_pitch, n * ce, m, cudaMemcpyHostToDevice,
                                          ctx->stream));
-    if (int rc = plan_gemm(ctx, &dev, ctx->prop.multiProcessorCount, false, &plan))
+    if (int rc = plan_gemm(ctx, &dev, ctx->prop.multiProcessorCount, false, &plan, kCPadding))
       return rc;
-    if (int rc = enqueue_gemm(ctx, &dev, plan))
+    if (int rc = enqueue_gemm(ctx, &dev, plan, {}, nullptr, kCPadding))
       return rc;
     HC_TRY_CUDA(ctx, cudaMemcpy2DAsync(host_c, host_c_pitch, dev_c, ldc * ce, n * ce, m, cudaMemcpyDeviceToHost,
                                        ctx->stream));
@@ -1293,9 +1298,9 @@ int hcCudaGemmHost(HcCudaContext *ctx, const HcCudaGemmArgs *args) {
     if (args->accumulate)
       HC_TRY_CUDA(ctx, cudaMemcpy2DAsync(dev_c, ldc * ce, host_c, host_c_pitch, n * ce, m, cudaMemcpyHostToDevice,
                                          ctx->stream));
-    if (int rc = plan_gemm(ctx, &dev, ctx->prop.multiProcessorCount, false, &plan))
+    if (int rc = plan_gemm(ctx, &dev, ctx->prop.multiProcessorCount, false, &plan, kCPadding))
       return rc;
-    if (int rc = enqueue_gemm(ctx, &dev, plan))
+    if (int rc = enqueue_gemm(ctx, &dev, plan, {}, nullptr, kCPadding))
       return rc;
     HC_TRY_CUDA(ctx, cudaMemcpy2DAsync(host_c, host_c_pitch, dev_c, ldc * ce, n * ce, m, cudaMemcpyDeviceToHost,
                                        ctx->stream));
@@ -1341,9 +1346,9 @@ int hcCudaGemmHost(HcCudaContext *ctx, const HcCudaGemmArgs *args) {
     if (has_bias)
       part.bias = dev.bias + col0;
     HcCudaGemmPlanInfo part_plan;
-    if (int rc = plan_gemm(ctx, &part, ctx->prop.multiProcessorCount, false, &part_plan))
+    if (int rc = plan_gemm(ctx, &part, ctx->prop.multiProcessorCount, false, &part_plan, kCPadding))
       return rc;
-    if (int rc = enqueue_gemm(ctx, &part, part_plan))
+    if (int rc = enqueue_gemm(ctx, &part, part_plan, {}, nullptr, kCPadding))
       return rc;
     cudaEvent_t done = ctx->panel_done[done_events++];
     HC_TRY_CUDA(ctx, cudaEventRecord(done, ctx->stream));
@@ -1464,7 +1469,7 @@ int hcCudaGemmHostDeviceA(HcCudaContext *ctx, const HcCudaGemmArgs *args) {
     return fail(ctx, HC_CUDA_ERR_INVALID_ARGUMENT, "ctx must not be null");
   std::lock_guard<std::mutex> lock(ctx->mu);
   HcCudaGemmPlanInfo plan;
-  if (int rc = plan_gemm(ctx, args, ctx->prop.multiProcessorCount, true, &plan))
+  if (int rc = plan_gemm(ctx, args, ctx->prop.multiProcessorCount, true, &plan, kCPadding))
     return rc;
   if (plan.variant == HC_CUDA_GEMM_NOOP)
     return HC_CUDA_OK;
@@ -1546,9 +1551,9 @@ int hcCudaGemmHostDeviceA(HcCudaContext *ctx, const HcCudaGemmArgs *args) {
     if (has_bias)
       part.bias = dev.bias + col0;
     HcCudaGemmPlanInfo part_plan;
-    if (int rc = plan_gemm(ctx, &part, ctx->prop.multiProcessorCount, false, &part_plan))
+    if (int rc = plan_gemm(ctx, &part, ctx->prop.multiProcessorCount, false, &part_plan, kCPadding))
       return rc;
-    if (int rc = enqueue_gemm(ctx, &part, part_plan))
+    if (int rc = enqueue_gemm(ctx, &part, part_plan, {}, nullptr, kCPadding))
       return rc;
     HC_TRY_CUDA(ctx, cudaEventRecord(ctx->panel_done[panel], ctx->stream));
     HC_TRY_CUDA(ctx, cudaStreamWaitEvent(ctx->copy_out, ctx->panel_done[panel], 0));
@@ -2260,9 +2265,8 @@ struct LossBackwardPlan {
   int64_t g = 0, gt = 0, ldg = 0, ldgt = 0;
   int64_t dh_sums = -1;  // float32 sums of dh without the rows' dloss (g_plain), rounded at the end; -1: dh is written at once
   int64_t sums_ld = 0;
-  // 16-bit, where dw's rows do not all start on 16-byte boundaries or end inside a 32-bit word: the product, of an even
-  // width, stores to it by TMA and a copy follows (16411 x 1001 x 1031: 41 and 12 us; 70 us when the product writes
-  // such rows itself).
+  // 16-bit, where dw's rows do not all consist of whole 16-byte pieces: the product stores to it by TMA and a copy
+  // follows (16411 x 1001 x 1031: 41 and 12 us; 70 us when the product writes such rows itself).
   int64_t dw_copy = -1;
   int64_t dw_ld = 0;
   int64_t scales = 0;
@@ -2276,6 +2280,11 @@ void scale_by_factor(HcCudaGemmArgs *g) {
   g->epilogue_value[0] = 1.0f;
   g->variant = HC_CUDA_GEMM_DENSE;
 }
+
+// What the products' planning may rely on: the caller's matrices do not overlap each other, scratch overlaps none, and
+// scratch has pitches of whole 16-byte pieces.
+int known_of_dh(const LossBackwardPlan &plan) { return kCApart | (plan.dh_sums >= 0 ? kCPadding : 0); }
+int known_of_dw(const LossBackwardPlan &plan) { return kCApart | (plan.dw_copy >= 0 ? kCPadding : 0); }
 
 // The two products of a piece as GEMM arguments, their 16-bit results scaled by scales[1]; `c` is already aligned, `base` the start of `work`.
 HcCudaGemmArgs loss_dh_product(const LossCall &c, const LossBackwardPlan &plan, char *base, int64_t first, int64_t count,
@@ -2317,7 +2326,6 @@ HcCudaGemmArgs loss_dw_product(const LossCall &c, const LossBackwardPlan &plan, 
   g.ldb = c.ldh;
   g.b_layout = HC_CUDA_B_KN;
   if (plan.dw_copy >= 0) {
-    g.n = round_up(c.width, 2);  // (the copy of h, like this one, has a longer pitch; the column more is not copied)
     g.c = base + plan.dw_copy;
     g.ldc = plan.dw_ld;
   } else {
@@ -2375,7 +2383,7 @@ int plan_linear_loss_backward(const HcCudaContext *ctx, const HcCudaLinearLossBa
   plan->gt = plan->work.take(args->dw != nullptr ? columns * plan->ldgt * 2 : 0);
   plan->sums_ld = round_up(c.width, 4);
   plan->scales = plan->work.take(8);
-  if (args->dw != nullptr && (needs_repack(args->dw, args->lddw) || c.width % 2 != 0)) {
+  if (args->dw != nullptr && (needs_repack(args->dw, args->lddw) || c.width % 8 != 0)) {
     plan->dw_ld = round_up(c.width, kRepackPitchBytes / 2);
     plan->dw_copy = plan->work.take(columns * plan->dw_ld * 2);
   }
@@ -2402,7 +2410,7 @@ int plan_linear_loss_backward(const HcCudaContext *ctx, const HcCudaLinearLossBa
     plan->dh_sums = plan->work.take(c.rows * plan->sums_ld * 4);
     if (plan->pieces == 1 && c.dtype == HC_CUDA_BF16) {
       const HcCudaGemmArgs g = loss_dh_product(aligned, *plan, base, 0, c.vocab, *args);
-      if (int rc = plan_gemm(ctx, &g, sm_count, false, &product, /*apart=*/true))
+      if (int rc = plan_gemm(ctx, &g, sm_count, false, &product, known_of_dh(*plan)))
         return rc;
       if (product.variant == HC_CUDA_GEMM_DENSE && product.cluster_size <= 1) {
         plan->dh_sums = -1;
@@ -2417,14 +2425,14 @@ int plan_linear_loss_backward(const HcCudaContext *ctx, const HcCudaLinearLossBa
     ++launches;
     if (args->dh != nullptr) {
       const HcCudaGemmArgs g = loss_dh_product(aligned, *plan, base, first, count, *args);
-      if (int rc = plan_gemm(ctx, &g, sm_count, false, &product, /*apart=*/true))
+      if (int rc = plan_gemm(ctx, &g, sm_count, false, &product, known_of_dh(*plan)))
         return rc;
       launches += product.kernel_launches;
       scratch = product.scratch_bytes > scratch ? product.scratch_bytes : scratch;
     }
     if (args->dw != nullptr) {
       const HcCudaGemmArgs g = loss_dw_product(aligned, *plan, base, first, count, *args);
-      if (int rc = plan_gemm(ctx, &g, sm_count, false, &product, /*apart=*/true))
+      if (int rc = plan_gemm(ctx, &g, sm_count, false, &product, known_of_dw(*plan)))
         return rc;
       launches += product.kernel_launches + (plan->dw_copy >= 0 ? 1 : 0);
       scratch = product.scratch_bytes > scratch ? product.scratch_bytes : scratch;
@@ -2530,16 +2538,16 @@ int hcCudaLinearLossBackward(HcCudaContext *ctx, const HcCudaLinearLossBackwardA
     HcCudaGemmPlanInfo product;
     if (args->dh != nullptr) {
       const HcCudaGemmArgs g = loss_dh_product(c, plan, base, first, count, *args);
-      if (int rc = plan_gemm(ctx, &g, sm_count, false, &product, /*apart=*/true))
+      if (int rc = plan_gemm(ctx, &g, sm_count, false, &product, known_of_dh(plan)))
         return rc;
-      if (int rc = enqueue_gemm(ctx, &g, product, hc::sm100::Epilogue{}, plan.dh_sums >= 0 ? nullptr : factor))
+      if (int rc = enqueue_gemm(ctx, &g, product, hc::sm100::Epilogue{}, plan.dh_sums >= 0 ? nullptr : factor, known_of_dh(plan)))
         return rc;
     }
     if (args->dw != nullptr) {
       const HcCudaGemmArgs g = loss_dw_product(c, plan, base, first, count, *args);
-      if (int rc = plan_gemm(ctx, &g, sm_count, false, &product, /*apart=*/true))
+      if (int rc = plan_gemm(ctx, &g, sm_count, false, &product, known_of_dw(plan)))
         return rc;
-      if (int rc = enqueue_gemm(ctx, &g, product, hc::sm100::Epilogue{}, factor))
+      if (int rc = enqueue_gemm(ctx, &g, product, hc::sm100::Epilogue{}, factor, known_of_dw(plan)))
         return rc;
       if (plan.dw_copy >= 0)
         HC_TRY_CUDA(ctx, hc::sm100::launch_spread(base + plan.dw_copy, plan.dw_ld,

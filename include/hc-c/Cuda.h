@@ -528,7 +528,7 @@ HC_CUDA_CAPI_EXPORTED int hcCudaLinearLossPlan(const HcCudaLinearLossArgs *args,
  * dloss, so that a row is as exact however small its dloss is. A call gives the same bits every time. rows == 0 sets dw
  * to zero. Uses context scratch: a copy of h (for dw), g and its transpose for one piece of the vocabulary (together
  * 512 MiB at most, or 1 KiB per row where that is more), the float32 sums of dh, and a copy of dw's piece when its
- * rows do not all start on 16-byte boundaries or the width is odd. */
+ * rows do not all consist of whole 16-byte pieces. */
 typedef struct HcCudaLinearLossBackwardArgs {
   int64_t rows, vocab, width;
   int32_t dtype;

@@ -360,10 +360,11 @@ def test_windows_of_larger_matrices(left, rows, vocab, width, gpu_ctx) -> None:
                 assert (np.ascontiguousarray(beside).view(np.uint8) == 0x5A).all()
 
 
-@pytest.mark.parametrize("rows, vocab, width", [(1, 37, 7), (70, 600, 95), (300, 2051, 129), (700, 300, 1001), (640, 2500, 513)])
+@pytest.mark.parametrize("rows, vocab, width", [(1, 37, 7), (70, 600, 95), (300, 2051, 130), (700, 300, 1001), (640, 2500, 516),
+                                               (2500, 900, 1030)])
 @pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
-def test_odd_widths_in_rows_of_whole_pieces(dtype, rows, vocab, width, gpu_ctx) -> None:
-    """Rows that start on 16-byte boundaries and end inside a 32-bit word: the elements behind them stay."""
+def test_widths_that_end_inside_a_piece(dtype, rows, vocab, width, gpu_ctx) -> None:
+    """Rows that start on 16-byte boundaries and end inside a 16-byte piece: the elements behind them stay."""
     h, w, targets, dloss = inputs(rows, vocab, width, dtype, 15)
     ld = (width + 7) // 8 * 8
     bh, bw, bt, bd = make(gpu_ctx, h, ld), make(gpu_ctx, w, ld), make(gpu_ctx, targets), make(gpu_ctx, dloss)
